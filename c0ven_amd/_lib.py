@@ -15,6 +15,7 @@ if not os.path.exists(LIB_PATH):
     raise ImportError("c0ven_amd: %s is not built; run __graft_entry__.build()" % LIB_PATH)
 lib = C.CDLL(LIB_PATH)
 
+QT_F32, QT_F16, QT_BF16 = 0, 1, 30
 QT_Q8_0, QT_Q4_K, QT_Q8_K, QT_IQ3_XXS, QT_IQ4_NL, QT_IQ3_S, QT_IQ2_S, QT_Q2_0 = 8, 12, 15, 18, 20, 21, 22, 42
 QT_Q5_K, QT_Q6_K, QT_IQ4_XS = 13, 14, 23
 TYPE_NAMES = {QT_Q8_0: "Q8_0", QT_Q4_K: "Q4_K", QT_Q5_K: "Q5_K", QT_Q6_K: "Q6_K", QT_IQ3_S: "IQ3_S",
@@ -30,6 +31,7 @@ Q8_FAMILY = (QT_Q8_0, QT_IQ4_NL, QT_Q2_0)  # the weight types whose dot products
 MOE_OK, MOE_ERROR, MOE_BAD_ARGUMENT, MOE_BUSY, MOE_TIMEOUT = 0, 1, 2, 3, 4
 MOE_FLAG_EXACT_ROUTER = 1
 MOE_FLAG_HC_FIXED_ORDER = 2
+MOE_SCORE_SOFTMAX, MOE_SCORE_SIGMOID = 0, 1
 
 
 class MoeConfig(C.Structure):
@@ -69,6 +71,23 @@ class MoeTile(C.Structure):
 
 class MoeGroup(C.Structure):
     _fields_ = [("slot", C.c_int32), ("n", C.c_uint32), ("asg", C.c_uint32 * 8)]
+
+
+class MoeRouteConfig(C.Structure):
+    _fields_ = [("n_expert", C.c_uint32), ("n_used", C.c_uint32), ("score", C.c_uint32), ("n_group", C.c_uint32),
+                ("top_group", C.c_uint32), ("group_top", C.c_uint32), ("renorm", C.c_uint32), ("scale", C.c_float),
+                ("type", C.c_uint32), ("device", C.c_int32)]
+
+
+class Mx4Matrix(C.Structure):
+    """A matrix in microscaled 4-bit floats: Mx4Matrix(codes, scales, rows, cols), the first two device pointers."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_uint32), ("cols", C.c_uint32)]
+
+
+class MoeMx4Experts(C.Structure):
+    _fields_ = [("n_embd", C.c_uint32), ("n_ff", C.c_uint32), ("n_expert", C.c_uint32), ("n_used", C.c_uint32),
+                ("gate", Mx4Matrix), ("up", Mx4Matrix), ("down", Mx4Matrix), ("x_type", C.c_uint32),
+                ("y_type", C.c_uint32), ("swiglu_limit", C.c_float), ("device", C.c_int32)]
 
 
 class GgufTensorInfo(C.Structure):
@@ -116,6 +135,17 @@ _SIGS = {
     "moe_synth_set_codebooks": (_i32, [_P, _u64]),
     "moe_zipf_bias": (None, [_u64, _u32, _f32, _P]),
     "moe_row_bytes": (_u64, [_u32, _u32]),
+    "moe_route_async": (_i32, [C.POINTER(MoeRouteConfig), _P, _u64, _P, _u32, _P, _P, _P, _P]),
+    "moe_mx4_code_bytes": (_u64, [_u32, _u32]),
+    "moe_mx4_scale_bytes": (_u64, [_u32, _u32]),
+    "moe_mx4_quantize_async": (_i32, [_i32, _u32, _P, _u64, C.POINTER(Mx4Matrix), _P]),
+    "moe_mx4_dequantize_async": (_i32, [_i32, C.POINTER(Mx4Matrix), _u32, _P, _u64, _P]),
+    "moe_mx4_matmul_work_bytes": (_u64, [C.POINTER(Mx4Matrix), _u32]),
+    "moe_mx4_matmul_async": (_i32, [_i32, C.POINTER(Mx4Matrix), C.POINTER(Mx4Matrix), _u32, _P, _u64, _P, _u64, _P]),
+    "moe_mx4_linear_work_bytes": (_u64, [C.POINTER(Mx4Matrix), _u32]),
+    "moe_mx4_linear_async": (_i32, [_i32, _u32, _P, _u64, _u32, C.POINTER(Mx4Matrix), _u32, _P, _u64, _P, _u64, _P]),
+    "moe_mx4_experts_work_bytes": (_u64, [C.POINTER(MoeMx4Experts), _u32]),
+    "moe_mx4_experts_async": (_i32, [C.POINTER(MoeMx4Experts), _P, _u64, _u32, _P, _P, _P, _u64, _P, _u64, _P]),
     "moe_abi_layout": (_u32, [C.POINTER(MoeAbiRow), _u32]),
     "moe_load_layer_gguf": (_i32, [_P, _u32, _P, _u32]),
     "moe_load_hc": (_i32, [_P, _u32, _P, _P, _P, _P]),
@@ -502,3 +532,80 @@ class MoeBlock:
 
     def device_bytes(self):
         return int(lib.moe_device_bytes(self.h))
+
+
+# The operators on device buffers. Pointers are device addresses (integers), strides elements (None: the rows follow one
+# another), stream a hipStream_t (None: the device's null stream). Nothing is copied and nothing waits.
+
+def _op(st):
+    if st != MOE_OK:
+        raise MoeError(st, lib.moe_last_error(None).decode())
+
+
+class Router:
+    """The routing of logits to experts (moe_route_async)."""
+
+    def __init__(self, n_expert, n_used, score=MOE_SCORE_SOFTMAX, n_group=0, top_group=0, group_top=1, renorm=True,
+                 scale=1.0, type=QT_F32, device=0):
+        self.cfg = MoeRouteConfig(n_expert, n_used, score, n_group, top_group, group_top, 1 if renorm else 0, scale, type,
+                                  device)
+        self._cfg = C.byref(self.cfg)
+
+    def route_async(self, logits, ntok, ids, w, load=None, bias=None, stride=None, stream=None):
+        _op(lib.moe_route_async(self._cfg, logits, self.cfg.n_expert if stride is None else stride, bias, ntok, ids, w,
+                                load, stream))
+
+
+def mx4_code_bytes(rows, cols):
+    return int(lib.moe_mx4_code_bytes(rows, cols))
+
+
+def mx4_scale_bytes(rows, cols):
+    return int(lib.moe_mx4_scale_bytes(rows, cols))
+
+
+def mx4_quantize_async(type, x, m, stride=None, device=0, stream=None):
+    """x (m.rows x m.cols of type) into the Mx4Matrix m."""
+    _op(lib.moe_mx4_quantize_async(device, type, x, m.cols if stride is None else stride, m, stream))
+
+
+def mx4_dequantize_async(m, type, out, stride=None, device=0, stream=None):
+    _op(lib.moe_mx4_dequantize_async(device, m, type, out, m.cols if stride is None else stride, stream))
+
+
+def mx4_matmul_work_bytes(w, ntok):
+    return int(lib.moe_mx4_matmul_work_bytes(w, ntok))
+
+
+def mx4_matmul_async(x, w, y_type, y, work=None, work_bytes=0, y_stride=None, device=0, stream=None):
+    """y = x w^T of two Mx4Matrix."""
+    _op(lib.moe_mx4_matmul_async(device, x, w, y_type, y, w.rows if y_stride is None else y_stride, work, work_bytes,
+                                 stream))
+
+
+def mx4_linear_work_bytes(w, ntok):
+    return int(lib.moe_mx4_linear_work_bytes(w, ntok))
+
+
+def mx4_linear_async(x_type, x, ntok, w, y_type, y, work, work_bytes, x_stride=None, y_stride=None, device=0, stream=None):
+    """y = mx4(x) w^T of ntok rows of floats."""
+    _op(lib.moe_mx4_linear_async(device, x_type, x, w.cols if x_stride is None else x_stride, ntok, w, y_type, y,
+                                 w.rows if y_stride is None else y_stride, work, work_bytes, stream))
+
+
+class Mx4Experts:
+    """The experts of routed tokens in MX4 (moe_mx4_experts_async): gate, up and down describe one expert's matrix and
+    point to n_expert of them."""
+
+    def __init__(self, n_embd, n_ff, n_expert, n_used, gate, up, down, x_type=QT_BF16, y_type=QT_BF16, swiglu_limit=0.0,
+                 device=0):
+        self.cfg = MoeMx4Experts(n_embd, n_ff, n_expert, n_used, gate, up, down, x_type, y_type, swiglu_limit, device)
+        self._cfg = C.byref(self.cfg)
+
+    def work_bytes(self, ntok):
+        return int(lib.moe_mx4_experts_work_bytes(self._cfg, ntok))
+
+    def forward_async(self, x, ntok, ids, w, y, work, work_bytes, x_stride=None, y_stride=None, stream=None):
+        H = self.cfg.n_embd
+        _op(lib.moe_mx4_experts_async(self._cfg, x, H if x_stride is None else x_stride, ntok, ids, w, y,
+                                      H if y_stride is None else y_stride, work, work_bytes, stream))

@@ -19,6 +19,7 @@
 #include "gguf_index.h"
 #include "iq3s_grid.h"
 #include "layout.h"
+#include "ops.h"
 #include "prefill.h"
 #include "prefill_hc.h"
 #include "repack.h"
@@ -283,6 +284,14 @@ moe_status fail(moe_ctx *c, const Error &e) {
 }
 
 thread_local std::string g_open_error;
+
+}  // namespace
+
+namespace c0ven {
+std::string &open_error() { return g_open_error; }
+}  // namespace c0ven
+
+namespace {
 
 template <typename F>
 moe_status guarded(moe_ctx *c, F f) {
@@ -1652,6 +1661,16 @@ MOE_API uint32_t moe_abi_layout(moe_abi_row *table, uint32_t cap) {
       STRUCT(MoeTile),               ROW(MoeGroup, slot),           ROW(MoeGroup, n),
       ROW(MoeGroup, asg),            STRUCT(MoeGroup),              ROW(moe_abi_row, name),
       ROW(moe_abi_row, offset),      ROW(moe_abi_row, size),        STRUCT(moe_abi_row),
+      ROW(moe_route_config, n_expert), ROW(moe_route_config, n_used), ROW(moe_route_config, score),
+      ROW(moe_route_config, n_group), ROW(moe_route_config, top_group), ROW(moe_route_config, group_top),
+      ROW(moe_route_config, renorm), ROW(moe_route_config, scale),  ROW(moe_route_config, type),
+      ROW(moe_route_config, device), STRUCT(moe_route_config),      ROW(moe_mx4_matrix, codes),
+      ROW(moe_mx4_matrix, scales),   ROW(moe_mx4_matrix, rows),     ROW(moe_mx4_matrix, cols),
+      STRUCT(moe_mx4_matrix),        ROW(moe_mx4_experts, n_embd),  ROW(moe_mx4_experts, n_ff),
+      ROW(moe_mx4_experts, n_expert), ROW(moe_mx4_experts, n_used), ROW(moe_mx4_experts, gate),
+      ROW(moe_mx4_experts, up),      ROW(moe_mx4_experts, down),    ROW(moe_mx4_experts, x_type),
+      ROW(moe_mx4_experts, y_type),  ROW(moe_mx4_experts, swiglu_limit), ROW(moe_mx4_experts, device),
+      STRUCT(moe_mx4_experts),
   };
   const uint32_t n = sizeof rows / sizeof rows[0];
   if (table)

@@ -305,6 +305,102 @@ MOE_API void moe_zipf_bias(uint64_t seed, uint32_t n_expert, float s, float *out
 /* Bytes of rows x cols values of type in the file's layout. */
 MOE_API uint64_t moe_row_bytes(uint32_t type, uint32_t cols);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * Operators on device buffers: routing to experts, microscaled 4-bit floats (MX4) and the experts' products in them. No
+ * counterpart in the reference, whose router is the block's and whose weights are integer grids.
+ *
+ * They take no context: every buffer is the caller's (device memory of the description's device), nothing is allocated,
+ * copied to the host or waited for, and a call may be captured into a graph. Each is enqueued on stream (a hipStream_t of
+ * that device; null: the device's null stream); the host's current device is left as it was. Calls that share a work
+ * buffer share its contents: order them (one stream, or event waits), graphs that were captured with it among them. A
+ * refused call enqueues nothing; its message is moe_last_error(null) on the calling thread. Any number of host threads
+ * may call. Element types are QT_F32, QT_F16 or QT_BF16; strides count elements from row to row and are at least a row's
+ * values. ntok 0 is accepted and writes nothing (moe_route_async: load, if given, is cleared). Inputs and outputs do not
+ * overlap. */
+
+/* The routing of logits, per token: the scores s_e (over the experts whose logit is neither -inf nor NaN), selection
+ * values v_e = s_e + bias_e, the experts of the best groups, of those the n_used largest v_e (the lower id first among
+ * equals), and their weights w = s, divided by max(their sum, 1e-20) if renorm, times scale. The order is decided in 64
+ * bits: without a bias and with a group's worth from one value it is the logits' own, otherwise that of s + bias in fp64.
+ * A -inf or NaN logit or bias leaves its expert out; ranks without an expert have id -1 and weight 0 (a token whose
+ * logits are all -inf has no other). +inf logits share a softmax evenly. */
+enum { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID = 1 };
+typedef struct {
+  uint32_t n_expert;  /* at most 512 */
+  uint32_t n_used;    /* at most 16 and at most the experts of the groups kept */
+  uint32_t score;     /* MOE_SCORE_* */
+  uint32_t n_group;   /* 0 or 1: no groups; else divides n_expert, at most 64: group g has the experts g n_expert /
+                       * n_group and on */
+  uint32_t top_group; /* the groups kept: those of the largest worth, the lower group first among equals */
+  uint32_t group_top; /* 1 or 2: a group's worth is the sum of its group_top largest v_e */
+  uint32_t renorm;    /* 1: the weights are divided by their sum */
+  float scale;        /* of the weights (0: 1) */
+  uint32_t type;      /* of the logits */
+  int32_t device;
+} moe_route_config;
+/* logits ntok x n_expert (rows stride apart); bias n_expert fp32 or null; ids and w ntok x n_used; load (n_expert, or
+ * null) receives the number of tokens that use each expert. */
+MOE_API moe_status moe_route_async(const moe_route_config *cfg, const void *logits, uint64_t stride, const float *bias,
+                                   uint32_t ntok, int32_t *ids, float *w, uint32_t *load, void *stream);
+
+/* A matrix in microscaled 4-bit floats (the OCP MX format MXFP4: E2M1 values, E8M0 scales), in device memory. A row is
+ * padded to C = cols rounded up to 128 values: C / 2 bytes of codes (value 2 i in the low half of byte i: a sign bit and
+ * the index into 0, 0.5, 1, 1.5, 2, 3, 4, 6) and C / 32 bytes of scales, one per 32 values (2^(s - 127); 255 makes the
+ * block's values NaN). Codes past cols are 0. Rows follow one another; both pointers are 16-byte aligned. */
+typedef struct {
+  uint8_t *codes;
+  uint8_t *scales;
+  uint32_t rows;
+  uint32_t cols;
+} moe_mx4_matrix;
+MOE_API uint64_t moe_mx4_code_bytes(uint32_t rows, uint32_t cols);
+MOE_API uint64_t moe_mx4_scale_bytes(uint32_t rows, uint32_t cols);
+/* x (m->rows x m->cols of type, rows stride apart) into m: a block's scale is 2^max(floor(log2 of its largest |x|) - 2,
+ * -127), its values the nearest of the format's under it (halves to the even code, the largest at most 6). A block with
+ * an infinity or a NaN gets scale 255 and codes 0. */
+MOE_API moe_status moe_mx4_quantize_async(int32_t device, uint32_t type, const void *x, uint64_t stride,
+                                          const moe_mx4_matrix *m, void *stream);
+/* m's values, rounded to type, into out (rows stride apart). */
+MOE_API moe_status moe_mx4_dequantize_async(int32_t device, const moe_mx4_matrix *m, uint32_t type, void *out,
+                                            uint64_t stride, void *stream);
+
+/* y = x w^T (y x->rows x w->rows of y_type, rows y_stride apart): the MX4 values' products summed in fp32 on the matrix
+ * cores and rounded once. x->cols == w->cols. work: at least moe_mx4_matmul_work_bytes(w, x->rows) bytes, 16-byte
+ * aligned (may be null where that is 0). */
+MOE_API uint64_t moe_mx4_matmul_work_bytes(const moe_mx4_matrix *w, uint32_t ntok);
+MOE_API moe_status moe_mx4_matmul_async(int32_t device, const moe_mx4_matrix *x, const moe_mx4_matrix *w,
+                                        uint32_t y_type, void *y, uint64_t y_stride, void *work, uint64_t work_bytes,
+                                        void *stream);
+/* The same for x of floats (ntok x w->cols of x_type, rows x_stride apart), quantised as by moe_mx4_quantize_async. */
+MOE_API uint64_t moe_mx4_linear_work_bytes(const moe_mx4_matrix *w, uint32_t ntok);
+MOE_API moe_status moe_mx4_linear_async(int32_t device, uint32_t x_type, const void *x, uint64_t x_stride,
+                                        uint32_t ntok, const moe_mx4_matrix *w, uint32_t y_type, void *y,
+                                        uint64_t y_stride, void *work, uint64_t work_bytes, void *stream);
+
+/* The experts of routed tokens in MX4, the counterpart of moe_forward_experts: for each token y = sum over its ranks of
+ * w o, in rank order in fp32, rounded once, with o = down(mx4(h)), h = silu(gate(mx4(x))) * up(mx4(x)), mx4() the
+ * quantisation above (of fp32 h). gate and up are n_expert matrices of n_ff x n_embd one after the other, down of
+ * n_embd x n_ff: the descriptions' rows are one expert's. An id outside 0 .. n_expert - 1 (moe_route_async's -1) adds
+ * nothing, a repeated one adds each time; a shared expert is one more expert and rank. */
+typedef struct {
+  uint32_t n_embd;      /* at most 16384 */
+  uint32_t n_ff;        /* at most 16384 */
+  uint32_t n_expert;    /* at most 512 */
+  uint32_t n_used;      /* at most 16 */
+  moe_mx4_matrix gate, up, down;
+  uint32_t x_type;
+  uint32_t y_type;
+  float swiglu_limit;   /* as moe_config's: > 0: gate at most L, up within -L .. L before the SiLU; 0: off */
+  int32_t device;
+} moe_mx4_experts;
+/* Bytes of work a call of ntok tokens takes (0 for a description that the call refuses). */
+MOE_API uint64_t moe_mx4_experts_work_bytes(const moe_mx4_experts *e, uint32_t ntok);
+/* x ntok x n_embd of x_type, ids and w ntok x n_used, y ntok x n_embd of y_type; ntok at most 16384; work 16-byte
+ * aligned. */
+MOE_API moe_status moe_mx4_experts_async(const moe_mx4_experts *e, const void *x, uint64_t x_stride, uint32_t ntok,
+                                         const int32_t *ids, const float *w, void *y, uint64_t y_stride, void *work,
+                                         uint64_t work_bytes, void *stream);
+
 /* For the ABI test: one row per field of every struct above, "struct.field" with its offset and size, then one row
  * per struct, "struct", offset 0 and its size. Returns the number of rows; table may be null. */
 typedef struct {

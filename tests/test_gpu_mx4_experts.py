@@ -1,0 +1,186 @@
+"""The experts of routed tokens in microscaled 4-bit floats, against the plain form in 64 bits within the bound that
+tests/ops_ref.py derives (and one rounding to the result's type), alone and behind the routing."""
+import numpy as np
+import pytest
+
+from tests import ops_ref as ref
+from tests.harness import moe
+from tests.ops_dev import TYPES, Raw, decode, encode, hip
+from tests.test_gpu_mx4 import matrix, room, say
+
+pytestmark = pytest.mark.gpu
+
+
+class Model:
+    def __init__(self, E, H, F, seed, sigma=0.05):
+        r = np.random.default_rng(seed)
+        self.E, self.H, self.F, self.hold = E, H, F, []
+        self.m, self.v = [], []
+        for rows, cols in ((F, H), (F, H), (H, F)):
+            codes, scales = ref.mx4_quantize(r.normal(size=(E * rows, cols)) * sigma)
+            m, c, s = matrix(E * rows, cols, codes, scales)
+            self.hold += [(codes, c), (scales, s)]
+            self.m.append(moe.Mx4Matrix(m.codes, m.scales, rows, cols))
+            self.v.append(ref.mx4_values(codes, scales, cols).reshape(E, rows, cols))
+
+    def op(self, K, x="f32", y="f32", limit=0.0):
+        return moe.Mx4Experts(self.H, self.F, self.E, K, *self.m, x_type=TYPES[x], y_type=TYPES[y], swiglu_limit=limit)
+
+
+def run(model, x, ids, w, type="f32", out="f32", limit=0.0, extra=0):
+    T, K = ids.shape
+    H = model.H
+    xb, values = hip.rows(x, type, extra)
+    idb, wb = hip.put(ids.astype(np.int32)), hip.put(w.astype(np.float32))
+    y, _ = hip.rows(np.full((T, H), 7.0), out, extra, 1, 7.0)
+    op = model.op(K, type, out, limit)
+    n = op.work_bytes(T)
+    work = room(n + 64)
+    op.forward_async(xb.ptr, T, idb.ptr, wb.ptr, y.ptr, work.ptr, n, x_stride=H + extra, y_stride=H + extra)
+    got = decode(y.get(), out)
+    assert (got[T:] == 7.0).all() and (got[:, H:] == 7.0).all() and (work.get()[n:] == 0xA5).all()
+    return got[:T, :H], values
+
+
+def check(model, x, ids, w, type="f32", out="f32", limit=0.0, extra=0):
+    got, values = run(model, x, ids, w, type, out, limit, extra)
+    y, off = ref.experts(values, ids, w.astype(np.float32).astype(np.float64), *model.v, limit=limit)
+    off = off + ref.EPS[out] * (np.abs(y) + off) + 2.0 ** -126
+    assert np.all(np.abs(got - y) <= off), float((np.abs(got - y) / off).max())
+    return got
+
+
+def tokens(T, H, E, K, seed, dropped=0.0, repeat=False):
+    r = np.random.default_rng(seed)
+    x = r.normal(size=(T, H)).astype(np.float32)
+    ids = r.integers(0, E, size=(T, K)) if repeat else np.array([r.permutation(E)[:K] for _ in range(T)]).reshape(T, K)
+    ids = np.where(r.random((T, K)) < dropped, -1, ids)
+    return x, ids, r.random((T, K))
+
+
+@pytest.mark.parametrize("T,H,F,E,K", [(1, 128, 32, 4, 2), (1, 1000, 200, 8, 3), (1, 512, 256, 16, 10), (2, 33, 7, 3, 1),
+                                       (5, 640, 96, 32, 6), (8, 256, 160, 64, 8), (16, 512, 128, 8, 4), (17, 256, 96, 16, 4),
+                                       (33, 1, 1, 2, 2), (40, 384, 128, 4, 4), (70, 320, 260, 5, 2), (150, 256, 64, 3, 2),
+                                       (9, 2560, 640, 6, 4), (300, 130, 129, 40, 5)])
+def test_experts(T, H, F, E, K):
+    say("experts", T, H, F, E, K)
+    model = Model(E, H, F, T + H)
+    check(model, *tokens(T, H, E, K, T))
+    check(model, *tokens(T, H, E, K, T + 1, 0.3, True), limit=0.05, extra=3)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("T", [1, 6, 50])
+def test_types(T, type, out):
+    say("types", T, type, out)
+    check(Model(8, 512, 160, 3), *tokens(T, 512, 8, 3, T, 0.1), type=type, out=out, extra=8)
+
+
+@pytest.mark.parametrize("T", [1, 7, 64, 200])
+def test_ids(T):
+    """Every token on one expert; none at all; ids out of range; the same expert in each rank."""
+    say("ids", T)
+    model = Model(6, 256, 96, 8)
+    x, ids, w = tokens(T, 256, 6, 4, 5)
+    check(model, x, np.full((T, 1), 5), w[:, :1])
+    got = check(model, x, np.full((T, 4), -1), w)
+    assert not got.any()
+    far = ids.copy()
+    far[:, 0], far[:, 1], far[::2, 2] = 6, -(1 << 31), (1 << 31) - 1
+    check(model, x, far, w)
+    check(model, x, np.repeat(ids[:, :1], 4, 1), w)
+    check(model, x, ids, np.where(w < 0.5, 0.0, -w))
+
+
+@pytest.mark.parametrize("T", [1, 20, 130])
+def test_nans_stay_with_their_token(T):
+    say("nans", T)
+    model = Model(6, 256, 96, 8)
+    x, ids, w = tokens(T, 256, 6, 2, 5)
+    clean, _ = run(model, x, ids, w)
+    x[T // 2, 200] = np.nan
+    got, _ = run(model, x, ids, w)
+    assert np.isnan(got[T // 2]).all()
+    rest = np.arange(T) != T // 2
+    assert np.array_equal(got[rest], clean[rest])
+    # A dropped rank's weight is not read as one.
+    x[T // 2, 200] = 0
+    ids[0, 1], w[0, 1] = -1, np.nan
+    got, _ = run(model, x, ids, w)
+    assert not np.isnan(got).any()
+
+
+@pytest.mark.parametrize("T", [1, 12, 100])
+def test_twice_the_same(T):
+    """The sums' order is fixed: equal calls give equal bits, whatever the work buffer held, and a token's result does not
+    depend on the others where the batch runs the same kernels."""
+    say("twice", T)
+    model = Model(12, 512, 128, 4)
+    a = tokens(T, 512, 12, 4, 6, 0.2)
+    assert np.array_equal(run(model, *a)[0], run(model, *a)[0])
+
+
+def chain(model, x, T, wr, K, work, out, stream):
+    """Logits by the dense product, the routing, the experts: as a layer calls them."""
+    E = model.E
+    logits, ids, w, load, y = out
+    moe.mx4_linear_async(moe.QT_BF16, x.ptr, T, wr, moe.QT_F32, logits.ptr, work[0].ptr, work[0].nbytes, stream=stream)
+    moe.Router(E, K, moe.MOE_SCORE_SIGMOID, 4, 2, 2).route_async(logits.ptr, T, ids.ptr, w.ptr, load.ptr, stream=stream)
+    model.op(K, "bf16", "bf16").forward_async(x.ptr, T, ids.ptr, w.ptr, y.ptr, work[1].ptr, work[1].nbytes, stream=stream)
+
+
+@pytest.mark.parametrize("T", [1, 8, 90])
+def test_chain_and_graph(T):
+    """The operators together, eager against the plain forms, then captured and replayed on new tokens between eager calls."""
+    say("chain", T)
+    E, H, F, K = 16, 512, 96, 4
+    model = Model(E, H, F, 21)
+    r = np.random.default_rng(T)
+    wf = hip.put((r.normal(size=(E, H)) * 0.1).astype(np.float32))
+    wr, c, s = matrix(E, H)
+    moe.mx4_quantize_async(moe.QT_F32, wf.ptr, wr)
+    x = hip.full((T, H), 0, np.uint16)
+    work = [[room(moe.mx4_linear_work_bytes(wr, T) + 16), room(model.op(K).work_bytes(T))] for _ in range(2)]
+
+    def outputs():
+        return [hip.full((T, E), 0), hip.full((T, K), 0, np.int32), hip.full((T, K), 0), hip.full(E, 0, np.int32),
+                hip.full((T, H), 0, np.uint16)]
+
+    a, b = outputs(), outputs()
+    s1, s2 = hip.stream(), hip.stream()
+    x.get()  # (the quantisation is done)
+    launch = hip.capture(s1, lambda: chain(model, x, T, wr, K, work[0], a, s1))
+    for i in range(4):
+        x.put(encode(r.normal(size=(T, H)), "bf16"))
+        launch()
+        chain(model, x, T, wr, K, work[1], b, s2)
+        for u, v in zip(a, b):
+            assert np.array_equal(u.get(), v.get())
+        ids, w, load = ref.route(b[0].get(), K, True, None, 4, 2, 2)
+        assert np.array_equal(b[1].get(), ids) and np.array_equal(b[3].get(), load)
+        y, off = ref.experts(decode(x.get(), "bf16"), ids, b[2].get().astype(np.float64), *model.v)
+        off = off + ref.EPS["bf16"] * (np.abs(y) + off) + 2.0 ** -126
+        assert np.all(np.abs(decode(b[4].get(), "bf16") - y) <= off)
+
+
+def test_far_experts():
+    """Matrices past 2^32 bytes: the last expert's."""
+    say("far experts")
+    E, H, F = 512, 16384, 1280  # 512 x 1280 x 16384 / 2 bytes: 5.4 GB a matrix
+    model = Model(1, H, F, 2)
+    far = Model.__new__(Model)
+    far.E, far.H, far.F, far.m, far.hold = E, H, F, [], []
+    for i, (rows, cols) in enumerate(((F, H), (F, H), (H, F))):
+        parts = []
+        for host, _ in model.hold[2 * i:2 * i + 2]:
+            b = Raw(hip, E * host.nbytes)
+            b.put(host.ravel(), (E - 1) * host.nbytes)
+            parts.append(b)
+        far.hold += parts
+        far.m.append(moe.Mx4Matrix(parts[0].ptr, parts[1].ptr, rows, cols))
+    for T in (1, 20):
+        x, _, w = tokens(T, H, 2, 1, 3)
+        got, values = run(far, x, np.full((T, 1), E - 1), w)
+        y, off = ref.experts(values, np.zeros((T, 1), int), w.astype(np.float32).astype(np.float64), *model.v)
+        assert np.all(np.abs(got - y) <= off + 2.0 ** -24 * (np.abs(y) + off))
