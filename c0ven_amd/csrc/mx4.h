@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "../../include/c0ven_quant.h"
+#include "device_math.h"
 
 namespace c0ven {
 
@@ -57,6 +58,62 @@ __device__ __forceinline__ uint32_t mx_codes8(const float v[8], uint32_t s) {
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], scale, 2);
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], scale, 3);
   return c;
+}
+
+// The values of a word of eight codes under a power of two (a float: mx_pow2), exactly, unless it leaves fp32's range.
+__device__ __forceinline__ void mx_values8(uint32_t codes, float pow2, float v[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const uint32_t q = codes >> (4 * j) & 15, m = q & 7;
+    const float a = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126) << 23 | (m & 1) << 22);
+    v[j] = (q & 8 ? -a : a) * pow2;
+  }
+}
+
+// Eight neighbours of a row, from column c on: as one (two for fp32) 16-byte access where the caller knows the rows to
+// be aligned for it (kVec) and all eight are there.
+template <uint32_t kType, bool kVec>
+__device__ __forceinline__ void load8(const typename Elem<kType>::T *row, uint32_t c, uint32_t cols, float v[8]) {
+  typedef typename Elem<kType>::T T;
+  struct alignas(16) Pack {
+    T e[8];
+  };
+  if (kVec && c + 8 <= cols) {
+    const Pack p = *(const Pack *)(row + c);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = (float)p.e[j];
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; j++) v[j] = c + j < cols ? (float)row[c + j] : 0.0f;
+  }
+}
+template <uint32_t kType, bool kVec>
+__device__ __forceinline__ void store8(typename Elem<kType>::T *row, uint32_t c, uint32_t cols, const float v[8]) {
+  typedef typename Elem<kType>::T T;
+  struct alignas(16) Pack {
+    T e[8];
+  };
+  if (kVec && c + 8 <= cols) {
+    Pack p;
+#pragma unroll
+    for (int j = 0; j < 8; j++) p.e[j] = (T)v[j];
+    *(Pack *)(row + c) = p;
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; j++)
+      if (c + j < cols) row[c + j] = (T)v[j];
+  }
+}
+
+// A block of 32 values held eight a lane by four neighbouring lanes: this lane's word of codes and the block's scale.
+__device__ __forceinline__ uint32_t mx_quantize8(const float v[8], uint32_t &scale) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+  most = max(most, dpp_u32<kDppXor1>(most));
+  most = max(most, dpp_u32<kDppXor2>(most));
+  scale = mx_scale_of(most);
+  return scale == 255 ? 0u : mx_codes8(v, scale);
 }
 
 __device__ __forceinline__ mx_i8 mx_wide(mx_i4 a) { return mx_i8{a[0], a[1], a[2], a[3], 0, 0, 0, 0}; }

@@ -5,46 +5,55 @@
 
 namespace c0ven {
 
-// One block of 32 values a thread.
-template <uint32_t kType>
-__global__ void mx4_quantize(const typename Elem<kType>::T *x, uint64_t stride, uint32_t rows, uint32_t cols,
-                             uint8_t *codes, uint8_t *scales) {
-  const uint32_t nb = mx_steps(cols) * 4;
-  const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (uint64_t)rows * nb) return;
-  const uint64_t r = i / nb;
-  const uint32_t b = (uint32_t)(i - r * nb);
-  float v[32];
-  uint32_t most = 0;
+// Both kernels take eight values a thread and kMxAhead such groups, all loaded before the first is used: bound by memory,
+// they need the bytes in flight. A work-group has 256 / 2^shift rows of 2^shift threads (whole rows where they are short),
+// each 2^shift kMxAhead groups wide.
+constexpr int kMxAhead = 4;
+
+struct MxRows {
+  uint32_t rows, cols, shift, wide;  // wide: work-groups a row takes
+};
+
+template <uint32_t kType, bool kVec>
+__global__ void __launch_bounds__(256) mx4_quantize(const typename Elem<kType>::T *x, uint64_t stride, MxRows a,
+                                                    uint8_t *codes, uint8_t *scales) {
+  const uint32_t ng = mx_steps(a.cols) * 16;
+  const uint32_t r = (blockIdx.x / a.wide << (8 - a.shift)) + (threadIdx.x >> a.shift);
+  const uint32_t g0 = (blockIdx.x % a.wide * kMxAhead << a.shift) + (threadIdx.x & ((1u << a.shift) - 1));
+  if (r >= a.rows) return;  // (four neighbours of a block are in one row)
+  const typename Elem<kType>::T *row = x + r * stride;
+  float v[kMxAhead][8];
 #pragma unroll
-  for (uint32_t j = 0; j < 32; j++) {
-    v[j] = b * 32 + j < cols ? (float)x[r * stride + b * 32 + j] : 0.0f;
-    most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+  for (int i = 0; i < kMxAhead; i++) load8<kType, kVec>(row, (g0 + (i << a.shift)) * 8, a.cols, v[i]);
+#pragma unroll
+  for (int i = 0; i < kMxAhead; i++) {
+    const uint32_t g = g0 + (i << a.shift);
+    uint32_t s;
+    const uint32_t c = mx_quantize8(v[i], s);
+    if (g >= ng) break;
+    ((uint32_t *)codes)[(uint64_t)r * ng + g] = c;
+    if (g % 4 == 0) scales[((uint64_t)r * ng + g) / 4] = (uint8_t)s;
   }
-  const uint32_t s = mx_scale_of(most);
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; j++) w[j] = s == 255 ? 0u : mx_codes8(v + 8 * j, s);
-  *(uint4 *)(codes + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-  scales[i] = (uint8_t)s;
 }
 
-// Eight values a thread.
-template <uint32_t kType>
-__global__ void mx4_dequantize(const uint8_t *codes, const uint8_t *scales, uint32_t rows, uint32_t cols,
-                               typename Elem<kType>::T *out, uint64_t stride) {
-  const uint32_t nw = mx_steps(cols) * 16;
-  const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (uint64_t)rows * nw) return;
-  const uint64_t r = i / nw;
-  const uint32_t c = (uint32_t)(i - r * nw) * 8;
-  const uint32_t w = ((const uint32_t *)codes)[i];
-  const float s = mx_pow2(scales[i / 4]);
+template <uint32_t kType, bool kVec>
+__global__ void __launch_bounds__(256) mx4_dequantize(const uint8_t *codes, const uint8_t *scales, MxRows a,
+                                                      typename Elem<kType>::T *out, uint64_t stride) {
+  const uint32_t ng = mx_steps(a.cols) * 16;
+  const uint32_t r = (blockIdx.x / a.wide << (8 - a.shift)) + (threadIdx.x >> a.shift);
+  const uint32_t g0 = (blockIdx.x % a.wide * kMxAhead << a.shift) + (threadIdx.x & ((1u << a.shift) - 1));
+  if (r >= a.rows) return;
+  uint32_t c[kMxAhead], s[kMxAhead];
 #pragma unroll
-  for (uint32_t j = 0; j < 8; j++) {
-    const uint32_t q = w >> (4 * j) & 15, m = q & 7;
-    const float a = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126) << 23 | (m & 1) << 22);
-    if (c + j < cols) out[r * stride + c + j] = (typename Elem<kType>::T)((q & 8 ? -a : a) * s);
+  for (int i = 0; i < kMxAhead; i++) {
+    const uint64_t at = (uint64_t)r * ng + min(g0 + (i << a.shift), ng - 1);
+    c[i] = ((const uint32_t *)codes)[at], s[i] = scales[at / 4];
+  }
+#pragma unroll
+  for (int i = 0; i < kMxAhead; i++) {
+    float v[8];
+    mx_values8(c[i], mx_pow2(s[i]), v);
+    store8<kType, kVec>(out + r * stride, (g0 + (i << a.shift)) * 8, a.cols, v);
   }
 }
 
@@ -52,12 +61,35 @@ __global__ void mx4_dequantize(const uint8_t *codes, const uint8_t *scales, uint
 
 using namespace c0ven;
 
+namespace {
+
+MxRows rows_of(uint32_t rows, uint32_t cols, uint64_t &blocks) {
+  const uint32_t ng = mx_steps(cols) * 16;
+  uint32_t shift = 4;
+  while (shift < 8 && (uint32_t)kMxAhead << shift < ng) shift++;
+  const uint32_t wide = (ng + (kMxAhead << shift) - 1) / (kMxAhead << shift);
+  blocks = (((uint64_t)rows + (256 >> shift) - 1) / (256 >> shift)) * wide;
+  return MxRows{rows, cols, shift, wide};
+}
+bool vectors(const void *p, uint64_t stride, uint32_t type) {
+  return op_aligned(p, 16) && stride * op_size(type) % 16 == 0;
+}
+
+}  // namespace
+
 void c0ven::mx4_quantize_launch(uint32_t type, const void *x, uint64_t stride, const moe_mx4_matrix &m, void *stream) {
-  const uint64_t n = ((uint64_t)m.rows * mx_steps(m.cols) * 4 + 255) / 256;
-  const auto run = [&](auto kernel, auto *p) { op_launch(kernel, n, 256, stream, p, stride, m.rows, m.cols, m.codes, m.scales); };
-  if (type == QT_F32) run(mx4_quantize<QT_F32>, (const float *)x);
-  if (type == QT_F16) run(mx4_quantize<QT_F16>, (const _Float16 *)x);
-  if (type == QT_BF16) run(mx4_quantize<QT_BF16>, (const __bf16 *)x);
+  uint64_t n;
+  const MxRows a = rows_of(m.rows, m.cols, n);
+  const auto run = [&](auto kernel, auto *p) { op_launch(kernel, n, 256, stream, p, stride, a, m.codes, m.scales); };
+  if (vectors(x, stride, type)) {
+    if (type == QT_F32) run(mx4_quantize<QT_F32, true>, (const float *)x);
+    if (type == QT_F16) run(mx4_quantize<QT_F16, true>, (const _Float16 *)x);
+    if (type == QT_BF16) run(mx4_quantize<QT_BF16, true>, (const __bf16 *)x);
+  } else {
+    if (type == QT_F32) run(mx4_quantize<QT_F32, false>, (const float *)x);
+    if (type == QT_F16) run(mx4_quantize<QT_F16, false>, (const _Float16 *)x);
+    if (type == QT_BF16) run(mx4_quantize<QT_BF16, false>, (const __bf16 *)x);
+  }
 }
 
 extern "C" {
@@ -81,13 +113,20 @@ MOE_API moe_status moe_mx4_dequantize_async(int32_t device, const moe_mx4_matrix
     op_mx4(m);
     op_rows(out, stride, m->cols, type);
     OnDevice on(device);
-    const uint64_t n = ((uint64_t)m->rows * mx_steps(m->cols) * 16 + 255) / 256;
+    uint64_t n;
+    const MxRows a = rows_of(m->rows, m->cols, n);
     const auto run = [&](auto kernel, auto *p) {
-      op_launch(kernel, n, 256, stream, (const uint8_t *)m->codes, (const uint8_t *)m->scales, m->rows, m->cols, p, stride);
+      op_launch(kernel, n, 256, stream, (const uint8_t *)m->codes, (const uint8_t *)m->scales, a, p, stride);
     };
-    if (type == QT_F32) run(mx4_dequantize<QT_F32>, (float *)out);
-    if (type == QT_F16) run(mx4_dequantize<QT_F16>, (_Float16 *)out);
-    if (type == QT_BF16) run(mx4_dequantize<QT_BF16>, (__bf16 *)out);
+    if (vectors(out, stride, type)) {
+      if (type == QT_F32) run(mx4_dequantize<QT_F32, true>, (float *)out);
+      if (type == QT_F16) run(mx4_dequantize<QT_F16, true>, (_Float16 *)out);
+      if (type == QT_BF16) run(mx4_dequantize<QT_BF16, true>, (__bf16 *)out);
+    } else {
+      if (type == QT_F32) run(mx4_dequantize<QT_F32, false>, (float *)out);
+      if (type == QT_F16) run(mx4_dequantize<QT_F16, false>, (_Float16 *)out);
+      if (type == QT_BF16) run(mx4_dequantize<QT_BF16, false>, (__bf16 *)out);
+    }
   });
 }
 

@@ -346,7 +346,8 @@ MOE_API moe_status moe_route_async(const moe_route_config *cfg, const void *logi
 /* A matrix in microscaled 4-bit floats (the OCP MX format MXFP4: E2M1 values, E8M0 scales), in device memory. A row is
  * padded to C = cols rounded up to 128 values: C / 2 bytes of codes (value 2 i in the low half of byte i: a sign bit and
  * the index into 0, 0.5, 1, 1.5, 2, 3, 4, 6) and C / 32 bytes of scales, one per 32 values (2^(s - 127); 255 makes the
- * block's values NaN). Codes past cols are 0. Rows follow one another; both pointers are 16-byte aligned. */
+ * block's values NaN). Codes past cols are 0. Rows follow one another; both pointers are 16-byte aligned. At most
+ * 2^30 rows of 1 to 2^20 cols. */
 typedef struct {
   uint8_t *codes;
   uint8_t *scales;
