@@ -4,28 +4,98 @@
 #include "mx4_gemm.h"
 #include "ops.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace c0ven {
 
-// One wave a 16 x 16 tile of y: w's rows are the instruction's first operand, so that a lane holds four neighbours of a
-// row of y.
-template <uint32_t kType>
-__global__ void __launch_bounds__(64) mx4_matmul(const uint8_t *xc, const uint8_t *xs, const uint8_t *wc,
-                                                 const uint8_t *ws, uint32_t M, uint32_t N, uint32_t steps,
-                                                 typename Elem<kType>::T *y, uint64_t stride) {
-  const uint32_t lane = threadIdx.x, q = lane / 16, nt = (N + 15) / 16;
-  const uint32_t n0 = blockIdx.x % nt * 16, m0 = blockIdx.x / nt * 16;
-  const uint64_t wr = (uint64_t)min(n0 + lane % 16, N - 1) * steps, xr = (uint64_t)min(m0 + lane % 16, M - 1) * steps;
-  mx_f4 c = {0, 0, 0, 0};
-  for (uint32_t k = 0; k < steps; k++) {
-    const mx_i4 a = *(const mx_i4 *)(wc + (wr + k) * 64 + q * 16), b = *(const mx_i4 *)(xc + (xr + k) * 64 + q * 16);
-    c = mx_mfma16<0, 0>(a, b, c, ws[(wr + k) * 4 + q], xs[(xr + k) * 4 + q]);
-  }
-  const uint32_t m = m0 + lane % 16;
+// Few rows of x (at most 16): y = x w^T is bound by reading w. A work-group has 16 rows of w, its kWaves waves each a run
+// of their k, four steps of 128 in flight a wave; the waves' sums are added in their order. kX kQuantised: x is quantised
+// already (xc, xs); else x are floats of that type (QT_F32 is 0), which the work-group quantises into LDS while its first loads of w are on
+// their way.
+constexpr uint32_t kQuantised = ~0u;
+constexpr uint32_t kFewRows = 16, kFewLds = 16384;  // the most values of x that a work-group quantises for itself
+
+template <uint32_t kX, uint32_t kType, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves)
+    mx4_few(const void *x, uint64_t x_stride, const uint8_t *xc, const uint8_t *xs, const uint8_t *wc, const uint8_t *ws,
+            uint32_t M, uint32_t N, uint32_t cols, typename Elem<kType>::T *y, uint64_t stride) {
+  constexpr bool kFloats = kX != kQuantised;
+  constexpr uint32_t kCodes = kFloats ? kFewLds / 2 + 16 * kFewRows : 16;
+  __shared__ __align__(16) uint8_t lc[kCodes];
+  __shared__ __align__(16) uint8_t ls[kFloats ? kFewLds / 32 : 16];
+  __shared__ float sums[kWaves][16][17];
+  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 16, r = lane % 16, steps = mx_steps(cols);
+  const uint32_t n0 = blockIdx.x * 16, per = (steps + kWaves - 1) / kWaves;
+  const uint32_t k0 = min(wave * per, steps), k1 = min(k0 + per, steps);
+  const uint64_t row = (uint64_t)min(n0 + r, N - 1) * steps;
+  const uint32_t m = min(r, M - 1);
+  constexpr int kAhead = 4;
+  mx_i4 a[kAhead], b[kAhead];
+  uint32_t sa[kAhead], sb[kAhead];
+  const auto load = [&](uint32_t k) {
 #pragma unroll
-  for (uint32_t i = 0; i < 4; i++) {
-    const uint32_t n = n0 + 4 * q + i;
-    if (m < M && n < N) y[(uint64_t)m * stride + n] = (typename Elem<kType>::T)c[i];
+    for (int j = 0; j < kAhead; j++) {
+      const uint64_t at = row + min(k + j, steps - 1);
+      a[j] = *(const mx_i4 *)(wc + at * 64 + q * 16), sa[j] = *(const uint32_t *)(ws + at * 4);
+      if constexpr (!kFloats) {
+        const uint64_t ax = (uint64_t)m * steps + min(k + j, steps - 1);
+        b[j] = *(const mx_i4 *)(xc + ax * 64 + q * 16), sb[j] = *(const uint32_t *)(xs + ax * 4);
+      }
+    }
+  };
+  load(k0);
+  const uint32_t pitch = steps * 64 + 16;
+  if constexpr (kFloats) {
+    typedef typename Elem<kX>::T X;
+    const bool vec = ((uintptr_t)x & 15) == 0 && x_stride * sizeof(X) % 16 == 0;
+    for (uint32_t i = threadIdx.x; i < M * steps * 16; i += 64 * kWaves) {
+      const uint32_t xr = i / (steps * 16), g = i - xr * (steps * 16);
+      const X *from = (const X *)x + xr * x_stride;
+      float v[8];
+      if (vec)
+        load8<kX, true>(from, g * 8, cols, v);
+      else
+        load8<kX, false>(from, g * 8, cols, v);
+      uint32_t s;
+      *(uint32_t *)(lc + xr * pitch + g * 4) = mx_quantize8(v, s);
+      if (g % 4 == 0) ls[xr * steps * 4 + g / 4] = (uint8_t)s;
+    }
+    __syncthreads();
   }
+  mx_f4 c = {0, 0, 0, 0};
+  for (uint32_t k = k0; k < k1; k += kAhead) {
+    if (k != k0) load(k);
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      if (k + j >= k1) break;
+      if constexpr (kFloats) {
+        b[j] = *(const mx_i4 *)(lc + m * pitch + (k + j) * 64 + q * 16);
+        sb[j] = *(const uint32_t *)(ls + (m * steps + k + j) * 4);
+      }
+      c = mx_mfma16<0, 0>(a[j], b[j], c, sa[j] >> (8 * q), sb[j] >> (8 * q));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) sums[wave][r][4 * q + i] = c[i];
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < M * 16; i += 64 * kWaves) {
+    float s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kWaves; v++) s += sums[v][i / 16][i % 16];
+    if (n0 + i % 16 < N) y[(uint64_t)(i / 16) * stride + n0 + i % 16] = (typename Elem<kType>::T)s;
+  }
+}
+
+// The sums of `parts` parts of y, each M x N, in their order.
+template <uint32_t kType>
+__global__ void __launch_bounds__(256) mx4_join(const float *sums, uint32_t parts, uint32_t M, uint32_t N,
+                                                typename Elem<kType>::T *y, uint64_t stride) {
+  const uint64_t n = (uint64_t)M * N, i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.0f;
+  for (uint32_t p = 0; p < parts; p++) s += sums[p * n + i];
+  y[i / N * stride + i % N] = (typename Elem<kType>::T)s;
 }
 
 // A tile of y a work-group, k split into parts of `span` stages (256 each); part p's sums go to y + p * part.
@@ -116,37 +186,98 @@ using namespace c0ven;
 
 namespace {
 
-void launch_matmul(const uint8_t *xc, const uint8_t *xs, uint32_t M, const moe_mx4_matrix *w, uint32_t y_type, void *y,
-                   uint64_t stride, void *stream) {
-  const uint32_t N = w->rows, steps = mx_steps(w->cols);
-  if (M >= 256 && N >= 256) {
-    const uint64_t blocks = ((uint64_t)((M + 255) / 256) * ((N + 255) / 256) + 7) / 8 * 8;
-    const auto gemm = [&](auto kernel, auto *p) {
-      op_launch(kernel, blocks, 256, stream, xc, xs, (const uint8_t *)w->codes, (const uint8_t *)w->scales, M, N, steps,
-                (steps + 1) / 2, p, stride, (uint64_t)0);
-    };
-    if (y_type == QT_F32) gemm(mx4_gemm<QT_F32, 4, 4>, (float *)y);
-    if (y_type == QT_F16) gemm(mx4_gemm<QT_F16, 4, 4>, (_Float16 *)y);
-    if (y_type == QT_BF16) gemm(mx4_gemm<QT_BF16, 4, 4>, (__bf16 *)y);
-    return;
+// How a product of M rows with N rows runs: tiles of 64 t by 64 t, k in parts of span stages of 256. The largest tile that
+// still gives every CU one (a 256 tile moves a quarter of the bytes of a 64 tile through LDS per product, but a product
+// bound by latency wants work-groups); if even the smallest leaves CUs without one, the k axis is split.
+struct Plan {
+  uint32_t tile = 1, span, parts = 1;
+  uint64_t tiles;
+  Plan(uint32_t M, uint32_t N, uint32_t steps) {
+    const auto count = [&](uint64_t t) { return ((M + 64 * t - 1) / (64 * t)) * ((N + 64 * t - 1) / (64 * t)); };
+    for (uint32_t t : {4u, 2u})
+      if (count(t) >= 200) {
+        tile = t;
+        break;
+      }
+    tiles = count(tile);
+    const uint32_t stages = (steps + 1) / 2;
+    span = stages;
+    if (tile == 1 && tiles < 200) {
+      const uint32_t want = (uint32_t)std::min<uint64_t>(400 / tiles, stages / 2);
+      if (want > 1) span = (stages + want - 1) / want;
+    }
+    parts = (stages + span - 1) / span;
   }
-  const uint64_t n = (uint64_t)((M + 15) / 16) * ((w->rows + 15) / 16);
-  const auto run = [&](auto kernel, auto *p) {
-    op_launch(kernel, n, 64, stream, xc, xs, (const uint8_t *)w->codes, (const uint8_t *)w->scales, M, w->rows,
-              mx_steps(w->cols), p, stride);
-  };
-  if (y_type == QT_F32) run(mx4_matmul<QT_F32>, (float *)y);
-  if (y_type == QT_F16) run(mx4_matmul<QT_F16>, (_Float16 *)y);
-  if (y_type == QT_BF16) run(mx4_matmul<QT_BF16>, (__bf16 *)y);
+  uint64_t bytes(uint32_t M, uint32_t N) const { return parts > 1 ? (uint64_t)parts * M * N * 4 : 0; }
+};
+
+template <typename F>
+void by_type(uint32_t type, F f) {
+  if (type == QT_F32) f(std::integral_constant<uint32_t, QT_F32>());
+  if (type == QT_F16) f(std::integral_constant<uint32_t, QT_F16>());
+  if (type == QT_BF16) f(std::integral_constant<uint32_t, QT_BF16>());
 }
 
-uint64_t quantised_bytes(uint32_t rows, uint32_t cols) { return moe_mx4_code_bytes(rows, cols) + (moe_mx4_scale_bytes(rows, cols) + 15) / 16 * 16; }
+template <uint32_t kX>
+void launch_few(const void *x, uint64_t x_stride, const uint8_t *xc, const uint8_t *xs, uint32_t M, const moe_mx4_matrix *w,
+                uint32_t y_type, void *y, uint64_t stride, void *stream) {
+  const uint32_t N = w->rows, blocks = (N + 15) / 16;
+  by_type(y_type, [&](auto t) {
+    constexpr uint32_t kType = decltype(t)::value;
+    const auto run = [&](auto kernel, uint32_t waves) {
+      op_launch(kernel, blocks, 64 * waves, stream, x, x_stride, xc, xs, (const uint8_t *)w->codes,
+                (const uint8_t *)w->scales, M, N, w->cols, (typename Elem<kType>::T *)y, stride);
+    };
+    // Sixteen waves a work-group where there are too few work-groups of four to fill the CUs.
+    if (blocks >= 512 || mx_steps(w->cols) <= 8)
+      run(mx4_few<kX, kType, 4>, 4);
+    else
+      run(mx4_few<kX, kType, 16>, 16);
+  });
+}
+
+void launch_matmul(const uint8_t *xc, const uint8_t *xs, uint32_t M, const moe_mx4_matrix *w, uint32_t y_type, void *y,
+                   uint64_t stride, void *work, void *stream) {
+  const uint32_t N = w->rows, steps = mx_steps(w->cols);
+  if (M <= kFewRows) return launch_few<kQuantised>(nullptr, 0, xc, xs, M, w, y_type, y, stride, stream);
+  const Plan p(M, N, steps);
+  const auto tiles = [&](auto t, void *to, uint64_t to_stride) {
+    constexpr uint32_t kType = decltype(t)::value;
+    const auto run = [&](auto kernel) {
+      op_launch(kernel, (p.tiles * p.parts + 7) / 8 * 8, 256, stream, xc, xs, (const uint8_t *)w->codes,
+                (const uint8_t *)w->scales, M, N, steps, p.span, (typename Elem<kType>::T *)to, to_stride,
+                (uint64_t)M * N);
+    };
+    if (p.tile == 4) run(mx4_gemm<kType, 4, 4>);
+    if (p.tile == 2) run(mx4_gemm<kType, 2, 2>);
+    if (p.tile == 1) run(mx4_gemm<kType, 1, 1>);
+  };
+  if (p.parts == 1) return by_type(y_type, [&](auto t) { tiles(t, y, stride); });
+  tiles(std::integral_constant<uint32_t, QT_F32>(), work, N);
+  by_type(y_type, [&](auto t) {
+    constexpr uint32_t kType = decltype(t)::value;
+    op_launch(mx4_join<kType>, ((uint64_t)M * N + 255) / 256, 256, stream, (const float *)work, p.parts, M, N,
+              (typename Elem<kType>::T *)y, stride);
+  });
+}
+
+// x's rows quantised, in a work buffer.
+uint64_t quantised_bytes(uint32_t rows, uint32_t cols) {
+  return moe_mx4_code_bytes(rows, cols) + (moe_mx4_scale_bytes(rows, cols) + 15) / 16 * 16;
+}
+// The rows that the few-rows kernel quantises for itself: another launch costs more than M cols / 2048 rounds of it.
+bool quantises_itself(uint32_t M, uint32_t cols) {
+  return M <= kFewRows && (uint64_t)M * mx_steps(cols) * kMxRow <= kFewLds;
+}
 
 }  // namespace
 
 extern "C" {
 
-MOE_API uint64_t moe_mx4_matmul_work_bytes(const moe_mx4_matrix *, uint32_t) { return 0; }
+MOE_API uint64_t moe_mx4_matmul_work_bytes(const moe_mx4_matrix *w, uint32_t ntok) {
+  if (!w || !w->cols || ntok <= kFewRows || !w->rows) return 0;
+  return Plan(ntok, w->rows, mx_steps(w->cols)).bytes(ntok, w->rows);
+}
 
 MOE_API moe_status moe_mx4_matmul_async(int32_t device, const moe_mx4_matrix *x, const moe_mx4_matrix *w,
                                         uint32_t y_type, void *y, uint64_t y_stride, void *work, uint64_t work_bytes,
@@ -157,13 +288,15 @@ MOE_API moe_status moe_mx4_matmul_async(int32_t device, const moe_mx4_matrix *x,
     op_require(x->cols == w->cols, "x and w must have the same cols");
     op_rows(y, y_stride, w->rows, y_type);
     op_work(work, work_bytes, moe_mx4_matmul_work_bytes(w, x->rows));
+    if (!x->rows || !w->rows) return;
     OnDevice on(device);
-    launch_matmul(x->codes, x->scales, x->rows, w, y_type, y, y_stride, stream);
+    launch_matmul(x->codes, x->scales, x->rows, w, y_type, y, y_stride, work, stream);
   });
 }
 
 MOE_API uint64_t moe_mx4_linear_work_bytes(const moe_mx4_matrix *w, uint32_t ntok) {
-  return w ? quantised_bytes(ntok, w->cols) : 0;
+  if (!w || !w->cols || quantises_itself(ntok, w->cols)) return 0;
+  return quantised_bytes(ntok, w->cols) + moe_mx4_matmul_work_bytes(w, ntok);
 }
 
 MOE_API moe_status moe_mx4_linear_async(int32_t device, uint32_t x_type, const void *x, uint64_t x_stride,
@@ -175,12 +308,16 @@ MOE_API moe_status moe_mx4_linear_async(int32_t device, uint32_t x_type, const v
     op_rows(y, y_stride, w->rows, y_type);
     op_require(ntok <= 1u << 30, "too many tokens");
     op_work(work, work_bytes, moe_mx4_linear_work_bytes(w, ntok));
-    if (!ntok) return;
+    if (!ntok || !w->rows) return;
     OnDevice on(device);
+    if (quantises_itself(ntok, w->cols))
+      return by_type(x_type, [&](auto t) {
+        launch_few<decltype(t)::value>(x, x_stride, nullptr, nullptr, ntok, w, y_type, y, y_stride, stream);
+      });
     uint8_t *xc = (uint8_t *)work, *xs = xc + moe_mx4_code_bytes(ntok, w->cols);
     const moe_mx4_matrix xm{xc, xs, ntok, w->cols};
     mx4_quantize_launch(x_type, x, x_stride, xm, stream);
-    launch_matmul(xc, xs, ntok, w, y_type, y, y_stride, stream);
+    launch_matmul(xc, xs, ntok, w, y_type, y, y_stride, (uint8_t *)work + quantised_bytes(ntok, w->cols), stream);
   });
 }
 
