@@ -70,15 +70,24 @@ __device__ __forceinline__ void mx_values8(uint32_t codes, float pow2, float v[8
   }
 }
 
-// Eight neighbours of a row, from column c on: as one (two for fp32) 16-byte access where the caller knows the rows to
-// be aligned for it (kVec) and all eight are there.
-template <uint32_t kType, bool kVec>
+// exp(x) to about one unit of the last place: 2^(x log2 e) with the product's low part (v_exp_f32 is good to a unit; the
+// product alone would lose |x| units). 0 below -104, infinite above 89; NaN stays.
+__device__ __forceinline__ float exp_f32(float x) {
+  x = x < -104.0f ? -104.0f : x > 89.0f ? 89.0f : x;
+  const float hi = x * 1.4426950216e+0f;
+  const float lo = __builtin_fmaf(x, 1.9259629911e-8f, __builtin_fmaf(x, 1.4426950216e+0f, -hi));
+  return __builtin_amdgcn_exp2f(hi) * __builtin_fmaf(lo, 0.69314718f, 1.0f);
+}
+
+// Eight neighbours of a row, from column c on: one (two for fp32) 16-byte access where all eight are there, at whatever
+// address (global memory takes it at any; rows of odd strides lose a little to the lines they share).
+template <uint32_t kType>
 __device__ __forceinline__ void load8(const typename Elem<kType>::T *row, uint32_t c, uint32_t cols, float v[8]) {
   typedef typename Elem<kType>::T T;
-  struct alignas(16) Pack {
+  struct __attribute__((packed)) Pack {
     T e[8];
   };
-  if (kVec && c + 8 <= cols) {
+  if (c + 8 <= cols) {
     const Pack p = *(const Pack *)(row + c);
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = (float)p.e[j];
@@ -87,13 +96,13 @@ __device__ __forceinline__ void load8(const typename Elem<kType>::T *row, uint32
     for (uint32_t j = 0; j < 8; j++) v[j] = c + j < cols ? (float)row[c + j] : 0.0f;
   }
 }
-template <uint32_t kType, bool kVec>
+template <uint32_t kType>
 __device__ __forceinline__ void store8(typename Elem<kType>::T *row, uint32_t c, uint32_t cols, const float v[8]) {
   typedef typename Elem<kType>::T T;
-  struct alignas(16) Pack {
+  struct __attribute__((packed)) Pack {
     T e[8];
   };
-  if (kVec && c + 8 <= cols) {
+  if (c + 8 <= cols) {
     Pack p;
 #pragma unroll
     for (int j = 0; j < 8; j++) p.e[j] = (T)v[j];

@@ -14,7 +14,7 @@ struct MxRows {
   uint32_t rows, cols, shift, wide;  // wide: work-groups a row takes
 };
 
-template <uint32_t kType, bool kVec>
+template <uint32_t kType>
 __global__ void __launch_bounds__(256) mx4_quantize(const typename Elem<kType>::T *x, uint64_t stride, MxRows a,
                                                     uint8_t *codes, uint8_t *scales) {
   const uint32_t ng = mx_steps(a.cols) * 16;
@@ -24,7 +24,7 @@ __global__ void __launch_bounds__(256) mx4_quantize(const typename Elem<kType>::
   const typename Elem<kType>::T *row = x + r * stride;
   float v[kMxAhead][8];
 #pragma unroll
-  for (int i = 0; i < kMxAhead; i++) load8<kType, kVec>(row, (g0 + (i << a.shift)) * 8, a.cols, v[i]);
+  for (int i = 0; i < kMxAhead; i++) load8<kType>(row, (g0 + (i << a.shift)) * 8, a.cols, v[i]);
 #pragma unroll
   for (int i = 0; i < kMxAhead; i++) {
     const uint32_t g = g0 + (i << a.shift);
@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(256) mx4_quantize(const typename Elem<kType>::
   }
 }
 
-template <uint32_t kType, bool kVec>
+template <uint32_t kType>
 __global__ void __launch_bounds__(256) mx4_dequantize(const uint8_t *codes, const uint8_t *scales, MxRows a,
                                                       typename Elem<kType>::T *out, uint64_t stride) {
   const uint32_t ng = mx_steps(a.cols) * 16;
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(256) mx4_dequantize(const uint8_t *codes, cons
   for (int i = 0; i < kMxAhead; i++) {
     float v[8];
     mx_values8(c[i], mx_pow2(s[i]), v);
-    store8<kType, kVec>(out + r * stride, (g0 + (i << a.shift)) * 8, a.cols, v);
+    store8<kType>(out + r * stride, (g0 + (i << a.shift)) * 8, a.cols, v);
   }
 }
 
@@ -71,9 +71,6 @@ MxRows rows_of(uint32_t rows, uint32_t cols, uint64_t &blocks) {
   blocks = (((uint64_t)rows + (256 >> shift) - 1) / (256 >> shift)) * wide;
   return MxRows{rows, cols, shift, wide};
 }
-bool vectors(const void *p, uint64_t stride, uint32_t type) {
-  return op_aligned(p, 16) && stride * op_size(type) % 16 == 0;
-}
 
 }  // namespace
 
@@ -81,15 +78,9 @@ void c0ven::mx4_quantize_launch(uint32_t type, const void *x, uint64_t stride, c
   uint64_t n;
   const MxRows a = rows_of(m.rows, m.cols, n);
   const auto run = [&](auto kernel, auto *p) { op_launch(kernel, n, 256, stream, p, stride, a, m.codes, m.scales); };
-  if (vectors(x, stride, type)) {
-    if (type == QT_F32) run(mx4_quantize<QT_F32, true>, (const float *)x);
-    if (type == QT_F16) run(mx4_quantize<QT_F16, true>, (const _Float16 *)x);
-    if (type == QT_BF16) run(mx4_quantize<QT_BF16, true>, (const __bf16 *)x);
-  } else {
-    if (type == QT_F32) run(mx4_quantize<QT_F32, false>, (const float *)x);
-    if (type == QT_F16) run(mx4_quantize<QT_F16, false>, (const _Float16 *)x);
-    if (type == QT_BF16) run(mx4_quantize<QT_BF16, false>, (const __bf16 *)x);
-  }
+  if (type == QT_F32) run(mx4_quantize<QT_F32>, (const float *)x);
+  if (type == QT_F16) run(mx4_quantize<QT_F16>, (const _Float16 *)x);
+  if (type == QT_BF16) run(mx4_quantize<QT_BF16>, (const __bf16 *)x);
 }
 
 extern "C" {
@@ -118,15 +109,9 @@ MOE_API moe_status moe_mx4_dequantize_async(int32_t device, const moe_mx4_matrix
     const auto run = [&](auto kernel, auto *p) {
       op_launch(kernel, n, 256, stream, (const uint8_t *)m->codes, (const uint8_t *)m->scales, a, p, stride);
     };
-    if (vectors(out, stride, type)) {
-      if (type == QT_F32) run(mx4_dequantize<QT_F32, true>, (float *)out);
-      if (type == QT_F16) run(mx4_dequantize<QT_F16, true>, (_Float16 *)out);
-      if (type == QT_BF16) run(mx4_dequantize<QT_BF16, true>, (__bf16 *)out);
-    } else {
-      if (type == QT_F32) run(mx4_dequantize<QT_F32, false>, (float *)out);
-      if (type == QT_F16) run(mx4_dequantize<QT_F16, false>, (_Float16 *)out);
-      if (type == QT_BF16) run(mx4_dequantize<QT_BF16, false>, (__bf16 *)out);
-    }
+    if (type == QT_F32) run(mx4_dequantize<QT_F32>, (float *)out);
+    if (type == QT_F16) run(mx4_dequantize<QT_F16>, (_Float16 *)out);
+    if (type == QT_BF16) run(mx4_dequantize<QT_BF16>, (__bf16 *)out);
   });
 }
 

@@ -48,15 +48,11 @@ __global__ void __launch_bounds__(64 * kWaves)
   const uint32_t pitch = steps * 64 + 16;
   if constexpr (kFloats) {
     typedef typename Elem<kX>::T X;
-    const bool vec = ((uintptr_t)x & 15) == 0 && x_stride * sizeof(X) % 16 == 0;
     for (uint32_t i = threadIdx.x; i < M * steps * 16; i += 64 * kWaves) {
       const uint32_t xr = i / (steps * 16), g = i - xr * (steps * 16);
       const X *from = (const X *)x + xr * x_stride;
       float v[8];
-      if (vec)
-        load8<kX, true>(from, g * 8, cols, v);
-      else
-        load8<kX, false>(from, g * 8, cols, v);
+      load8<kX>(from, g * 8, cols, v);
       uint32_t s;
       *(uint32_t *)(lc + xr * pitch + g * 4) = mx_quantize8(v, s);
       if (g % 4 == 0) ls[xr * steps * 4 + g / 4] = (uint8_t)s;

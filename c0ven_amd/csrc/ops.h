@@ -67,15 +67,20 @@ class OnDevice {
 
 // A launch that reports its own error and no earlier one's.
 template <typename... P, typename... A>
-void op_launch(void (*kernel)(P...), uint64_t blocks, uint32_t threads, void *stream, A... args) {
+void op_launch_lds(void (*kernel)(P...), uint64_t blocks, uint32_t threads, uint32_t lds, void *stream, A... args) {
   op_require(blocks <= 0x7fffffffull, "too many rows");
   if (!blocks) return;
   static_assert(sizeof...(P) == sizeof...(A), "a kernel's arguments");
   [&](P... a) {
     void *list[] = {(void *)&a...};
-    op_check(hipLaunchKernel((const void *)kernel, dim3((uint32_t)blocks), dim3(threads), list, 0, (hipStream_t)stream),
+    op_check(hipLaunchKernel((const void *)kernel, dim3((uint32_t)blocks), dim3(threads), list, lds, (hipStream_t)stream),
              "launch");
   }(args...);
+}
+
+template <typename... P, typename... A>
+void op_launch(void (*kernel)(P...), uint64_t blocks, uint32_t threads, void *stream, A... args) {
+  op_launch_lds(kernel, blocks, threads, 0, stream, args...);
 }
 
 inline bool op_float(uint32_t t) { return t == QT_F32 || t == QT_F16 || t == QT_BF16; }
