@@ -7,7 +7,7 @@
 // Where the order is that of the logits (no bias, a group's worth from one value) it is exact in fp32 and only the chosen
 // need an exponential. Otherwise the order is that of s + bias in fp64: it is formed in fp32 within a bound, and where two
 // neighbours of the order (the k-th and the next among them), or the last group kept and the next, are nearer than their
-// bounds, the wave does that token again in fp64 (exact_token). Equal logits under equal biases need no bound: their order
+// bounds, the wave decides that in fp64: among the candidates, or among all where too many are near. Equal logits under equal biases need no bound: their order
 // is by id either way.
 //
 // Bound by memory (the logits read once) where tokens are many, by the launch where they are few. 16384 x 512 fp32, top
@@ -30,6 +30,7 @@ struct RouteArgs {
 struct RouteScratch {
   union {
     float v[512];       // the selection values, for the groups
+    double d[512];      // the same in fp64
     uint2 cand[64];     // the candidates
   };
 };
@@ -49,11 +50,15 @@ __device__ __forceinline__ void wave_best(double &v, uint32_t &id) {
 __device__ __forceinline__ float lane_f32(float v, uint32_t l) {
   return __uint_as_float(readlane_u32(__float_as_uint(v), (int)l));
 }
+template <int kCtrl>
+__device__ __forceinline__ float dpp_f32(float v) {
+  return __uint_as_float(dpp_u32<kCtrl>(__float_as_uint(v)));
+}
 __device__ __forceinline__ float wave_sum_f32(float v) {
-  v += __uint_as_float(dpp_u32<kDppXor1>(__float_as_uint(v)));
-  v += __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(v)));
-  v += __uint_as_float(dpp_u32<kDppHalfMirror>(__float_as_uint(v)));
-  v += __uint_as_float(dpp_u32<kDppMirror>(__float_as_uint(v)));
+  v += dpp_f32<kDppXor1>(v);
+  v += dpp_f32<kDppXor2>(v);
+  v += dpp_f32<kDppHalfMirror>(v);
+  v += dpp_f32<kDppMirror>(v);
   return (lane_f32(v, 0) + lane_f32(v, 16)) + (lane_f32(v, 32) + lane_f32(v, 48));
 }
 __device__ __forceinline__ void lds_done() {  // this wave's LDS accesses
@@ -61,88 +66,106 @@ __device__ __forceinline__ void lds_done() {  // this wave's LDS accesses
   __builtin_amdgcn_wave_barrier();
 }
 
-struct Ranked {
-  uint32_t id;
-  float s;
+// The scores in fp64 of the lanes' logits (minus infinity: no score): a softmax's largest logit and sum (1 for a sigmoid).
+struct Exact {
+  double top = -INFINITY, sum = 1.0;
+
+  template <int kPer>
+  __device__ __forceinline__ Exact(const RouteArgs &a, const float (&x)[kPer]) {
+    if (a.sigmoid) return;
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < kPer; i++) m = fmaxf(m, x[i]);
+    top = (double)key_float(wave_max_u32(float_key(m)));
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) sum += part(a, x[i]);
+    sum = wave_sum_f64(sum);
+  }
+  __device__ __forceinline__ double part(const RouteArgs &a, float xf) const {
+    const double x = (double)xf;
+    return xf == -INFINITY ? 0.0 : a.sigmoid ? 1.0 / (1.0 + exp(-x)) : x == top ? 1.0 : exp(x - top);
+  }
+  __device__ __forceinline__ double score(const RouteArgs &a, float x) const { return sum > 0.0 ? part(a, x) / sum : 0.0; }
+  // The values that select, into LDS (minus infinity: not to be selected).
+  template <int kPer>
+  __device__ __forceinline__ void keys(const RouteArgs &a, const float (&x)[kPer], const float (&b)[kPer], double *d) const {
+    const uint32_t e0 = (threadIdx.x & 63) * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; i++)
+      if (e0 + i < a.E) d[e0 + i] = x[i] > -INFINITY && b[i] > -INFINITY ? score(a, x[i]) + (double)b[i] : -INFINITY;
+    lds_done();
+  }
 };
-// A token in fp64 throughout: lane r < K receives rank r's id (~0 for none) and score.
-template <uint32_t kType, int kPer>
-__device__ __noinline__ Ranked exact_token(RouteArgs a, const typename Elem<kType>::T *row, const float *bias) {
-  uint32_t my_id = ~0u;
-  float my_s = 0.0f;
-  const uint32_t lane = threadIdx.x & 63, e0 = lane * kPer;
-  const double kNone = -INFINITY;
-  double x[kPer], s[kPer], key[kPer], top = kNone, sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < kPer; i++) {
-    const double v = e0 + i < a.E ? (double)(float)row[e0 + i] : kNone;
-    x[i] = v > kNone ? v : kNone;  // (no NaN)
-    top = fmax(top, x[i]);
-  }
-  top = wave_max_d(top);
-#pragma unroll
-  for (int i = 0; i < kPer; i++) {
-    s[i] = x[i] == kNone ? 0.0 : a.sigmoid ? 1.0 / (1.0 + exp(-x[i])) : x[i] == top ? 1.0 : exp(x[i] - top);
-    sum += s[i];
-  }
-  if (!a.sigmoid) {
-    sum = wave_sum_d(sum);
-#pragma unroll
-    for (int i = 0; i < kPer; i++) s[i] = sum > 0.0 ? s[i] / sum : 0.0;
-  }
-#pragma unroll
-  for (int i = 0; i < kPer; i++) {
-    const float b = bias && e0 + i < a.E ? bias[e0 + i] : 0.0f;
-    key[i] = x[i] > kNone && b > -INFINITY ? s[i] + (double)b : kNone;
-  }
-  if (a.groups > 1) {
-    const uint32_t n = a.E / a.groups;
-    double mine = kNone;  // lane g: group g's worth
-    for (uint32_t g = 0; g < a.groups; g++) {
-      double b1 = kNone, b2 = kNone;
-      uint32_t i1 = ~0u, i2 = ~0u;
-#pragma unroll
-      for (int i = 0; i < kPer; i++)
-        if (e0 + i < a.E && (e0 + i) / n == g && key[i] > b1) b1 = key[i], i1 = e0 + i;
-      wave_best(b1, i1);
-#pragma unroll
-      for (int i = 0; i < kPer; i++)
-        if (e0 + i < a.E && (e0 + i) / n == g && e0 + i != i1 && key[i] > b2) b2 = key[i], i2 = e0 + i;
-      wave_best(b2, i2);
-      if (lane == g) mine = a.best > 1 && b2 > kNone ? b1 + b2 : b1;
+
+// The groups that stay, decided on the values in d.
+__device__ __forceinline__ uint64_t exact_groups(const RouteArgs &a, const double *d) {
+  const uint32_t lane = threadIdx.x & 63, n = a.E / a.groups;
+  double b1 = -INFINITY, b2 = -INFINITY;
+  if (lane < a.groups)
+    for (uint32_t j = 0; j < n; j++) {
+      const double o = d[lane * n + j];
+      b2 = o > b1 ? b1 : fmax(b2, o), b1 = fmax(b1, o);
     }
-    uint32_t place = 0;
-    for (uint32_t g = 0; g < a.groups; g++) {
-      const double o = __shfl(mine, (int)g, 64);
-      place += o > mine || (o == mine && g < lane);
-    }
-    const uint64_t stays = __ballot(lane < a.groups && place < a.kept);
-#pragma unroll
-    for (int i = 0; i < kPer; i++)
-      if (e0 + i >= a.E || !(stays >> ((e0 + i) / n) & 1)) key[i] = kNone;
+  lds_done();
+  const double mine = a.best > 1 && b2 > -INFINITY ? b1 + b2 : b1;
+  uint32_t place = 0;
+  for (uint32_t g = 0; g < a.groups; g++) {
+    const double o = readlane_f64(mine, (int)g);
+    place += o > mine || (o == mine && g < lane);
   }
-  for (uint32_t k = 0; k < a.K; k++) {
-    double b = kNone;
-    uint32_t id = ~0u;
-#pragma unroll
-    for (int i = 0; i < kPer; i++)
-      if (key[i] > b) b = key[i], id = e0 + i;
-    wave_best(b, id);
-    float v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; i++)
-      if (id == e0 + i) v = (float)s[i], key[i] = kNone;
-    v = __shfl(v, id == ~0u ? 0 : (int)(id / kPer), 64);
-    if (lane == k) my_id = id, my_s = id == ~0u ? 0.0f : v;
-  }
-  return Ranked{my_id, my_s};
+  return __ballot(lane < a.groups && place < a.kept);
 }
 
-// The n largest keys of the wave (0: no key), the lower id first among equals: lane r < n receives the r-th one's key and
-// id (key 0 where there are fewer).
+struct Ranked {
+  uint32_t id;  // ~0: none
+  float s;
+};
+// The ranks in fp64 among the candidates that lanes 0 .. total - 1 hold (id, logit, bias): lane r receives rank r.
+__device__ __forceinline__ Ranked exact_ranks(const RouteArgs &a, const Exact &e, uint32_t total, uint32_t id, float x, float b) {
+  const uint32_t lane = threadIdx.x & 63;
+  const double s = e.score(a, x), key = s + (double)b;
+  uint32_t rank = 0;
+  for (uint32_t i = 0; i < total; i++) {
+    const double o = readlane_f64(key, (int)i);
+    rank += o > key || (o == key && readlane_u32(id, (int)i) < id);
+  }
+  const int to = 4 * (int)(lane < total ? rank : lane);
+  const uint32_t ri = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)id);
+  const float rs = __uint_as_float((uint32_t)__builtin_amdgcn_ds_permute(to, (int)__float_as_uint((float)s)));
+  return lane < total ? Ranked{ri, rs} : Ranked{~0u, 0.0f};
+}
+// The ranks of the values in d (changed) among the experts of the groups that stay, one after the other.
+template <uint32_t kType, int kPer>
+__device__ __forceinline__ Ranked exact_all(const RouteArgs &a, const Exact &e, const typename Elem<kType>::T *row,
+                                            uint64_t stays, double *d) {
+  const uint32_t lane = threadIdx.x & 63, e0 = lane * kPer, n = a.groups > 1 ? a.E / a.groups : a.E;
+  Ranked mine{~0u, 0.0f};
+  for (uint32_t k = 0; k < a.K; k++) {
+    double b = -INFINITY;
+    uint32_t id = ~0u;
+#pragma unroll 1
+    for (int i = 0; i < kPer; i++) {
+      if (e0 + i >= a.E) break;
+      const double v = d[e0 + i];
+      if (v > b && (stays >> ((e0 + i) / n) & 1)) b = v, id = e0 + i;
+    }
+    wave_best(b, id);
+    if (id == ~0u) break;
+    if (id / kPer == lane) d[id] = -INFINITY;
+    if (lane == k) mine.id = id;
+  }
+  lds_done();
+  if (mine.id != ~0u) mine.s = (float)e.score(a, (float)row[mine.id]);
+  return mine;
+}
+
+// The n largest keys of the wave (0: no key), the lower id first among equals: lane r receives the r-th one's key and id
+// (key 0 where there are fewer), for r below the number returned, at least n where there are so many; every other expert's
+// key is at most floor (0: there is no other).
 template <int kPer>
-__device__ __forceinline__ void select_ranks(const uint32_t (&key)[kPer], uint32_t n, RouteScratch &lds, uint32_t &my_key,
-                                             uint32_t &my_id) {
+__device__ __forceinline__ uint32_t select_ranks(const uint32_t (&key)[kPer], uint32_t n, RouteScratch &lds, uint32_t &my_key,
+                                                 uint32_t &my_id, uint32_t &floor) {
   const uint32_t lane = threadIdx.x & 63, e0 = lane * kPer;
   uint32_t m = key[0];
 #pragma unroll
@@ -150,8 +173,11 @@ __device__ __forceinline__ void select_ranks(const uint32_t (&key)[kPer], uint32
   uint32_t tau = 0;
   for (int b = 31; b >= 0; b--) {
     const uint32_t c = tau | (1u << b);
-    if ((uint32_t)__popcll(__ballot(m >= c)) >= n) tau = c;
+    const uint32_t reach = (uint32_t)__popcll(__ballot(m >= c));
+    if (reach >= n) tau = c;
+    if (reach == n) break;  // (no lower bit changes who reaches it)
   }
+  floor = tau;
   tau = max(tau, 1u);
   uint32_t cnt = 0, pos = 0, total = 0;  // this lane's candidates, those of the lanes below, all
 #pragma unroll
@@ -178,27 +204,30 @@ __device__ __forceinline__ void select_ranks(const uint32_t (&key)[kPer], uint32
     my_key = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)me.x);
     my_id = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)me.y);
     if (lane >= total) my_key = 0u;
-    return;
+    return total;
   }
   // (Many equal values.) One after the other: the largest, its lowest lane, that lane's first one.
   uint32_t gone = 0;
   my_key = 0u, my_id = 0u;
-  for (uint32_t k = 0; k < n; k++) {
+  uint32_t k = 0;
+  for (; k < n; k++) {
     uint32_t b = 0, at = 0;
 #pragma unroll
     for (int i = kPer - 1; i >= 0; i--)
       if (!(gone >> i & 1) && key[i] >= b) b = key[i], at = i;
     const uint32_t top = wave_max_u32(b);
+    floor = top;
     if (!top) break;
     const uint32_t who = (uint32_t)__ffsll(__ballot(b == top)) - 1;
     if (lane == who) gone |= 1u << at;
     const uint32_t id = who * kPer + readlane_u32(at, (int)who);
     if (lane == k) my_key = top, my_id = id;
   }
+  return k;
 }
 
-// kScores: the order is that of s + bias. Tokens go round the grid's waves; load (or null) is counted in LDS and added at
-// the end, or stored where one work-group does it all.
+// kScores: the order is that of s + bias. Tokens go round the grid's waves. load (or null): one work-group counts it; of
+// several the first clears it for route_count.
 template <uint32_t kType, bool kScores, int kPer>
 __global__ void __launch_bounds__(512) moe_route(RouteArgs a, const typename Elem<kType>::T *logits, uint64_t stride,
                                                  const float *bias, uint32_t ntok, int32_t *ids, float *w, uint32_t *load) {
@@ -207,131 +236,196 @@ __global__ void __launch_bounds__(512) moe_route(RouteArgs a, const typename Ele
   RouteScratch *all = (RouteScratch *)(count + 512);
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x / 64, e0 = lane * kPer;
   RouteScratch &lds = all[wave];
-  if (load) {
+  const bool counts = load && gridDim.x == 1;
+  if (counts) {
     for (uint32_t e = threadIdx.x; e < a.E; e += blockDim.x) count[e] = 0;
     __syncthreads();
+  } else if (load && blockIdx.x == 0) {
+    for (uint32_t e = threadIdx.x; e < a.E; e += blockDim.x) load[e] = 0;
   }
-  const uint32_t n = a.groups > 1 ? a.E / a.groups : a.E;
-  uint32_t group[kPer];
+  const uint32_t step = gridDim.x * waves, n = a.groups > 1 ? a.E / a.groups : a.E;
+  const auto finish = [&](uint32_t t, uint32_t id, float score) {  // lane r < K: rank r's expert (~0: none)
+    if (id == ~0u || lane >= a.K) score = 0.0f;
+    float all_s = 0.0f;
+    for (uint32_t k = 0; k < a.K; k++) all_s += lane_f32(score, k);
+    if (lane >= a.K) return;
+    const uint64_t at = (uint64_t)t * a.K + lane;
+    ids[at] = (int32_t)id;
+    w[at] = (a.renorm ? score / fmaxf(all_s, 1e-20f) : score) * a.scale;
+    if (counts && id != ~0u) atomicAdd(count + id, 1u);
+  };
+  // The tokens whose order fp32 decides, one after the other; at one that it leaves open the loop is left and entered
+  // again, so that what only it needs (the next token's logits, the biases) is in no register beside fp64's.
+  const uint32_t per_group = ((1u << 20) + n - 1) / n;  // e per_group >> 20 = e / n for e < 512
+  // A group of a power of two lanes is compared lane by lane.
+  const uint32_t run = a.groups > 1 && n % kPer == 0 && (n / kPer & (n / kPer - 1)) == 0 ? n / kPer : 0;
+  uint64_t stays = ~0ull;
+  bool decided = false;  // stays, for token t, in fp64
+  for (uint32_t t = blockIdx.x * waves + wave; t < ntok;) {
+    float b[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; i++) group[i] = (e0 + i) / n;
-  for (uint32_t t = blockIdx.x * waves + wave; t < ntok; t += gridDim.x * waves) {
-    const typename Elem<kType>::T *row = logits + (uint64_t)t * stride;
-    float x[kPer], s[kPer], v[kPer];
-    if constexpr (kPer == 8) {
-      load8<kType>(row, e0, a.E, x);
-    } else {
+    for (int i = 0; i < kPer; i++) b[i] = kScores && bias && e0 + i < a.E ? bias[e0 + i] : 0.0f;
+    bool open = false, open_groups = false;
+    uint32_t my_key, my_id, floor, total;
+    float x[kPer], my_x, my_b = 0.0f, off_s = 0.0f;
+    for (; t < ntok; t += step) {
+      const typename Elem<kType>::T *row = logits + (uint64_t)t * stride;
+      float s[kPer], v[kPer];
+      if constexpr (kPer == 8) {
+        load8<kType>(row, e0, a.E, x);
+      } else {
 #pragma unroll
-      for (int i = 0; i < kPer; i++) x[i] = e0 + i < a.E ? (float)row[e0 + i] : 0.0f;
-    }
+        for (int i = 0; i < kPer; i++) x[i] = e0 + i < a.E ? (float)row[e0 + i] : 0.0f;
+      }
 #pragma unroll
-    for (int i = 0; i < kPer; i++) x[i] = e0 + i < a.E && x[i] > -INFINITY ? x[i] : -INFINITY;
-    float top = x[0], sum = 0.0f;
+      for (int i = 0; i < kPer; i++) x[i] = e0 + i < a.E && x[i] > -INFINITY ? x[i] : -INFINITY;  // (no NaN)
+      float top = x[0], sum = 0.0f;
 #pragma unroll
-    for (int i = 1; i < kPer; i++) top = fmaxf(top, x[i]);
-    top = key_float(wave_max_u32(float_key(top)));
-    if (!a.sigmoid && (kScores || !a.renorm)) {
+      for (int i = 1; i < kPer; i++) top = fmaxf(top, x[i]);
+      top = key_float(wave_max_u32(float_key(top)));
+      if (!a.sigmoid && (kScores || !a.renorm)) {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+          s[i] = x[i] == -INFINITY ? 0.0f : x[i] == top ? 1.0f : exp_f32(x[i] - top);
+          sum += s[i];
+        }
+        sum = wave_sum_f32(sum);
+      }
+      const float per_sum = a.sigmoid ? 1.0f : __builtin_amdgcn_rcpf(sum);
 #pragma unroll
       for (int i = 0; i < kPer; i++) {
-        s[i] = x[i] == -INFINITY ? 0.0f : x[i] == top ? 1.0f : exp_f32(x[i] - top);
-        sum += s[i];
+        if (kScores) {
+          const float p = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_f32(-x[i])) : s[i] * per_sum;
+          v[i] = x[i] > -INFINITY && b[i] > -INFINITY ? p + b[i] : -INFINITY;
+        } else {
+          v[i] = x[i];
+        }
       }
-      sum = wave_sum_f32(sum);
-    }
+      // A score's bound: a few units of its own for the exponential, the quotient and a softmax's sum, and |x - top| of
+      // them for the difference, of which e^(x - top) |x - top| <= 0.37 stays: within 2^-20 of the largest score.
+      off_s = per_sum * 0x1p-20f + 0x1p-120f;
+      if (a.groups > 1 && !decided) {
+        float b1 = -INFINITY, b2 = -INFINITY;
+        uint32_t at = lane;  // this lane's group; of a run of lanes a group, each has it
+        if (run) {
 #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-      if (kScores) {
-        const float b = bias && e0 + i < a.E ? bias[e0 + i] : 0.0f;
-        const float p = a.sigmoid ? 1.0f / (1.0f + exp_f32(-x[i])) : s[i] / sum;
-        v[i] = x[i] > -INFINITY && b > -INFINITY ? p + b : -INFINITY;
-      } else {
-        v[i] = x[i];
+          for (int i = 0; i < kPer; i++) b2 = fmaxf(b2, fminf(b1, v[i])), b1 = fmaxf(b1, v[i]);
+          const auto merge = [&](float o1, float o2) { b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2)), b1 = fmaxf(b1, o1); };
+          if (run > 1) merge(dpp_f32<kDppXor1>(b1), dpp_f32<kDppXor1>(b2));
+          if (run > 2) merge(dpp_f32<kDppXor2>(b1), dpp_f32<kDppXor2>(b2));
+          if (run > 4) merge(dpp_f32<kDppHalfMirror>(b1), dpp_f32<kDppHalfMirror>(b2));
+          if (run > 8) merge(dpp_f32<kDppMirror>(b1), dpp_f32<kDppMirror>(b2));
+          if (run > 16) merge(__shfl_xor(b1, 16, 64), __shfl_xor(b2, 16, 64));
+          if (run > 32) merge(__shfl_xor(b1, 32, 64), __shfl_xor(b2, 32, 64));
+          at = e0 / n;
+        } else {
+          // Lane g goes through group g's values, from a place of its own on, so that the lanes' banks differ.
+#pragma unroll
+          for (int i = 0; i < kPer; i++)
+            if (e0 + i < a.E) lds.v[e0 + i] = v[i];
+          lds_done();
+          if (lane < a.groups)
+            for (uint32_t j = 0, k = lane % n; j < n; j++, k = k + 1 == n ? 0 : k + 1) {
+              const float o = lds.v[lane * n + k];
+              b2 = fmaxf(b2, fminf(b1, o)), b1 = fmaxf(b1, o);
+            }
+          lds_done();
+        }
+        const float mine = a.best > 1 && b2 > -INFINITY ? b1 + b2 : b1;
+        uint32_t place = 0;
+        for (uint32_t g = 0; g < a.groups; g++) {
+          const float o = lane_f32(mine, run ? g * run : g);
+          place += o > mine || (o == mine && g < at);
+        }
+        const uint64_t keep = __ballot(at < a.groups && place < a.kept);
+        stays = keep;
+        if (run > 1) {
+          stays = 0;
+          for (uint32_t g = 0; g < a.groups; g++) stays |= (keep >> (g * run) & 1) << g;
+        }
+        if (kScores && a.kept < a.groups) {
+          const uint32_t in = (uint32_t)__ffsll(__ballot(at < a.groups && place == a.kept - 1)) - 1;
+          const uint32_t out = (uint32_t)__ffsll(__ballot(at < a.groups && place == a.kept)) - 1;
+          const float wi = lane_f32(mine, in), wo = lane_f32(mine, out);
+          // Four scores, and the roundings of their sums.
+          open_groups = wo > -INFINITY && !(wi - wo > 4.0f * off_s + 0x1p-20f * (fabsf(wi) + fabsf(wo)));
+          if (open_groups) break;
+        }
       }
-    }
-    bool open = false;  // the order is not certain
-    // A score's bound: a few units of its own for the exponential, the quotient and a softmax's sum, and |x - top| of
-    // them for the difference, of which e^(x - top) |x - top| <= 0.37 stays: within 2^-20 of the largest score.
-    const float off_s = (a.sigmoid ? 1.0f : 1.0f / sum) * 0x1p-20f + 0x1p-120f;
-    uint64_t stays = ~0ull;
-    if (a.groups > 1) {
-      // Lane g goes through group g's values, from a place of its own on, so that the lanes' banks differ.
+      uint32_t key[kPer];
 #pragma unroll
       for (int i = 0; i < kPer; i++)
-        if (e0 + i < a.E) lds.v[e0 + i] = v[i];
-      lds_done();
-      float b1 = -INFINITY, b2 = -INFINITY;
-      if (lane < a.groups)
-        for (uint32_t j = 0, at = lane % n; j < n; j++, at = at + 1 == n ? 0 : at + 1) {
-          const float o = lds.v[lane * n + at];
-          b2 = o > b1 ? b1 : fmaxf(b2, o), b1 = fmaxf(b1, o);
-        }
-      lds_done();
-      const float mine = a.best > 1 && b2 > -INFINITY ? b1 + b2 : b1;
-      uint32_t place = 0;
-      for (uint32_t g = 0; g < a.groups; g++) {
-        const float o = lane_f32(mine, g);
-        place += o > mine || (o == mine && g < lane);
-      }
-      stays = __ballot(lane < a.groups && place < a.kept);
-      if (kScores && a.kept < a.groups) {
-        const uint32_t in = (uint32_t)__ffsll(__ballot(lane < a.groups && place == a.kept - 1)) - 1;
-        const uint32_t out = (uint32_t)__ffsll(__ballot(lane < a.groups && place == a.kept)) - 1;
-        const float wi = lane_f32(mine, in), wo = lane_f32(mine, out);
-        // Four scores, and the roundings of their sums.
-        if (wo > -INFINITY) open = !(wi - wo > 4.0f * off_s + 0x1p-20f * (fabsf(wi) + fabsf(wo)));
-      }
-    }
-    uint32_t key[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; i++)
-      key[i] = v[i] > -INFINITY && (a.groups <= 1 || (stays >> group[i] & 1)) ? float_key(v[i]) : 0u;
-    uint32_t my_key, my_id;
-    select_ranks<kPer>(key, kScores ? a.K + 1 : a.K, lds, my_key, my_id);
-    const bool mine = my_key != 0 && lane <= a.K;
-    float my_x = mine ? (float)row[my_id] : 0.0f, my_s = 0.0f;
-    if (kScores) {
-      const float my_b = mine && bias ? bias[my_id] : 0.0f;
-      my_s = a.sigmoid ? 1.0f / (1.0f + exp_f32(-my_x)) : (my_x == top ? 1.0f : exp_f32(my_x - top)) / sum;
-      if (!mine) my_s = 0.0f;
-      // Rank r against rank r + 1 (any later one's value is no larger, and its bound is the same).
-      const float my_v = key_float(my_key);
-      const uint32_t next = (lane + 1) & 63;
-      const uint32_t nk = __shfl(my_key, next, 64);
-      const float nx = __shfl(my_x, next, 64), nb = __shfl(my_b, next, 64);
-      const float nv = key_float(nk);
-      const bool equal = nx == my_x && nb == my_b;
-      const float off = 2.0f * off_s + 0x1p-22f * (fabsf(my_v) + fabsf(nv));
-      open |= __any(lane < a.K && mine && nk != 0 && !equal && !(my_v - nv > off));
-    } else {
-      if (a.sigmoid)
-        my_s = 1.0f / (1.0f + exp_f32(-my_x));
+        key[i] = v[i] > -INFINITY && (a.groups <= 1 || (stays >> ((e0 + i) * per_group >> 20) & 1)) ? float_key(v[i]) : 0u;
+      // (A few ranks past the last, so that what an open order may move lies among them.)
+      total = select_ranks<kPer>(key, kScores ? a.K + 4 : a.K, lds, my_key, my_id, floor);
+      const bool mine = my_key != 0 && lane <= a.K;
+      my_x = my_key != 0 ? (float)row[my_id] : -INFINITY;
+      float my_s;
+      if (kScores || a.sigmoid || !a.renorm)
+        my_s = a.sigmoid ? 1.0f / (1.0f + exp_f32(-my_x)) : (my_x == top ? 1.0f : exp_f32(my_x - top)) / sum;
       else  // with renorm the common factor drops out: relative to the first chosen
-        my_s = a.renorm ? (my_x == lane_f32(my_x, 0) ? 1.0f : exp_f32(my_x - lane_f32(my_x, 0)))
-                        : (my_x == top ? 1.0f : exp_f32(my_x - top)) / sum;
+        my_s = my_x == lane_f32(my_x, 0) ? 1.0f : exp_f32(my_x - lane_f32(my_x, 0));
+      if (kScores) {
+        // Rank r against rank r + 1 (any later one's value is no larger, and its bound is the same).
+        my_b = my_key != 0 && bias ? bias[my_id] : 0.0f;
+        const float my_v = key_float(my_key);
+        const uint32_t next = (lane + 1) & 63;
+        const uint32_t nk = __shfl(my_key, next, 64);
+        const float nx = __shfl(my_x, next, 64), nb = __shfl(my_b, next, 64), nv = key_float(nk);
+        const float off = 2.0f * off_s + 0x1p-22f * (fabsf(my_v) + fabsf(nv));
+        open = __any(lane < a.K && mine && nk != 0 && !(nx == my_x && nb == my_b) && !(my_v - nv > off));
+        if (open) break;
+      }
+      finish(t, mine ? my_id : ~0u, my_s);
+      decided = false;
     }
-    if (kScores && open) {
-      const Ranked r = exact_token<kType, kPer>(a, row, bias);
-      my_id = r.id, my_s = r.s, my_key = r.id != ~0u;
+    if (!kScores || t >= ntok) break;
+    const Exact e(a, x);
+    if (open_groups) {
+      e.keys(a, x, b, lds.d);
+      stays = exact_groups(a, lds.d);
+      decided = true;
+      continue;
     }
-    if (!(my_key != 0 && lane < a.K)) my_s = 0.0f;
-    float total = 0.0f;
-    for (uint32_t k = 0; k < a.K; k++) total += lane_f32(my_s, k);
-    if (lane < a.K) {
-      const uint64_t at = (uint64_t)t * a.K + lane;
-      ids[at] = my_key ? (int32_t)my_id : -1;
-      w[at] = (a.renorm ? my_s / fmaxf(total, 1e-20f) : my_s) * a.scale;
-      if (load && my_key) atomicAdd(count + my_id, 1u);
+    // All that may belong to the first K are in the lanes if what is not there is below the K-th by more.
+    const float last = lane_f32(key_float(my_key), a.K - 1), rest = key_float(floor);
+    Ranked r;
+    if (!floor || readlane_u32(my_key, (int)a.K - 1) == 0 ||
+        last - rest > 2.0f * off_s + 0x1p-22f * (fabsf(last) + fabsf(rest))) {
+      r = exact_ranks(a, e, total, my_id, my_x, my_b);
+    } else {
+      e.keys(a, x, b, lds.d);
+      r = exact_all<kType, kPer>(a, e, logits + (uint64_t)t * stride, stays, lds.d);
     }
+    finish(t, r.id, r.s);
+    decided = false;
+    t += step;
   }
-  if (load) {
+  if (counts) {
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < a.E; e += blockDim.x) {
-      if (gridDim.x == 1)
-        load[e] = count[e];
-      else if (count[e])
-        atomicAdd(load + e, count[e]);
-    }
+    for (uint32_t e = threadIdx.x; e < a.E; e += blockDim.x) load[e] = count[e];
   }
+}
+
+// How often each expert is among the n ids, into load: stored by one work-group, added by several (load is cleared).
+// After the routing, so that the 512 counters see a few work-groups' sums and not each of hundreds (16384 tokens: +5 us
+// instead of +12).
+constexpr uint32_t kCountIds = 16384;  // a work-group's
+__global__ void __launch_bounds__(1024) route_count(const int32_t *ids, uint32_t n, uint32_t E, uint32_t *load) {
+  __shared__ uint32_t count[512];
+  if (threadIdx.x < 512) count[threadIdx.x] = 0;
+  __syncthreads();
+  const uint32_t end = min(n, (blockIdx.x + 1) * kCountIds);
+  for (uint32_t i = blockIdx.x * kCountIds + threadIdx.x; i < end; i += 1024) {
+    const int32_t id = ids[i];
+    if (id >= 0) atomicAdd(count + id, 1u);
+  }
+  __syncthreads();
+  if (threadIdx.x >= E) return;
+  if (gridDim.x == 1)
+    load[threadIdx.x] = count[threadIdx.x];
+  else if (count[threadIdx.x])
+    atomicAdd(load + threadIdx.x, count[threadIdx.x]);
 }
 
 __global__ void route_clear(uint32_t *load, uint32_t n) {
@@ -366,10 +460,11 @@ extern "C" MOE_API moe_status moe_route_async(const moe_route_config *cfg, const
                       c.scale == 0.0f ? 1.0f : c.scale};
     if (!ntok && !load) return;
     OnDevice on(c.device);
-    // Up to eight tokens are one work-group's, which stores load; more are dealt to at most four waves a SIMD.
+    // With load up to sixteen tokens are one work-group's, which counts (two tokens a wave cost less than another
+    // launch); more are dealt to at most eight waves a SIMD.
     const uint32_t waves = std::min(std::max(ntok, 1u), 8u);
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>((ntok + waves - 1) / waves, 512);
-    if (load && blocks != 1) op_launch(route_clear, 1, 512, stream, load, c.n_expert);
+    const uint32_t blocks = load && ntok <= 16 ? ntok != 0 : std::min((ntok + waves - 1) / waves, 1024u);
+    if (!ntok) return op_launch(route_clear, 1, 512, stream, load, c.n_expert);
     const bool scores = bias || (c.n_group > 1 && c.group_top > 1);
     const auto run = [&](auto kernel, auto *p) {
       op_launch_lds(kernel, blocks, 64 * waves, 2048 + waves * (uint32_t)sizeof(RouteScratch), stream, a, p, stride, bias, ntok,
@@ -385,5 +480,8 @@ extern "C" MOE_API moe_status moe_route_async(const moe_route_config *cfg, const
     if (c.type == QT_F32) typed(std::integral_constant<uint32_t, QT_F32>(), (const float *)logits);
     if (c.type == QT_F16) typed(std::integral_constant<uint32_t, QT_F16>(), (const _Float16 *)logits);
     if (c.type == QT_BF16) typed(std::integral_constant<uint32_t, QT_BF16>(), (const __bf16 *)logits);
+    const uint32_t n = ntok * c.n_used;
+    if (load && blocks > 1)
+      op_launch(route_count, (n + kCountIds - 1) / kCountIds, 1024, stream, (const int32_t *)ids, n, c.n_expert, load);
   });
 }
