@@ -1,7 +1,17 @@
 // The experts of routed tokens in MX4 (moe_mx4_experts_async).
+//
+// Many tokens: the assignments (token * n_used + rank) are sorted by expert and cut into MoeTiles of kRows positions;
+// gate and up of a tile are one product whose epilogue applies the SwiGLU and quantises h, 32 neighbours of a row being in
+// one wave's registers; down follows on the positions' rows, its sums go to the assignments' rows, and a last kernel adds
+// each token's in rank order. Bound by reading the experts' weights (once for all of a tile's tokens) until an expert has
+// some hundreds of tokens.
+#include "../../include/c0ven_moe_tile.h"
 #include "mx4.h"
 #include "mx4_api.h"
+#include "mx4_gemm.h"
 #include "ops.h"
+
+#include <algorithm>
 
 namespace c0ven {
 
@@ -11,7 +21,220 @@ __device__ __forceinline__ float mx_swiglu(float g, float u, float limit) {
     g = g > limit ? limit : g;
     u = u > limit ? limit : u < -limit ? -limit : u;
   }
-  return g / (1.0f + expf(-g)) * u;
+  return g / (1.0f + exp_f32(-g)) * u;
+}
+
+// ---- the assignments by expert
+
+constexpr uint32_t kSlice = 4096;  // ids a work-group sorts
+
+// How often each expert is in each slice.
+__global__ void __launch_bounds__(1024) mx4_count(const int32_t *ids, uint32_t A, uint32_t E, uint32_t *counts) {
+  __shared__ uint32_t n[512];
+  if (threadIdx.x < 512) n[threadIdx.x] = 0;
+  __syncthreads();
+  const uint32_t end = min(A, (blockIdx.x + 1) * kSlice);
+  for (uint32_t i = blockIdx.x * kSlice + threadIdx.x; i < end; i += 1024) {
+    const uint32_t e = (uint32_t)ids[i];
+    if (e < E) atomicAdd(n + e, 1u);
+  }
+  __syncthreads();
+  if (threadIdx.x < E) counts[blockIdx.x * E + threadIdx.x] = n[threadIdx.x];
+}
+
+// The inclusive sums of v over the work-group's 1024 threads in steps of 512 values: thread e's own (e < 512).
+__device__ __forceinline__ uint32_t scan512(uint32_t v, uint32_t *lds) {
+  const uint32_t e = threadIdx.x;
+  __syncthreads();
+  if (e < 512) lds[e] = v;
+  for (uint32_t d = 1; d < 512; d *= 2) {
+    __syncthreads();
+    const uint32_t add = e < 512 && e >= d ? lds[e - d] : 0;
+    __syncthreads();
+    if (e < 512) lds[e] += add;
+  }
+  __syncthreads();
+  return e < 512 ? lds[e] : 0;
+}
+
+// A slice's assignments to their places (order[place] = assignment; within an expert by slice), and, by the first
+// work-group, the tiles of at most `rows` places each. With one slice the counts are taken here.
+__global__ void __launch_bounds__(1024) mx4_place(const int32_t *ids, uint32_t A, uint32_t E, const uint32_t *counts,
+                                                  uint32_t rows, uint32_t *order, MoeTile *tiles, uint32_t *n_tiles) {
+  __shared__ uint32_t next[512];
+  __shared__ uint32_t lds[512];
+  const uint32_t e = threadIdx.x, first = blockIdx.x * kSlice, end = min(A, first + kSlice);
+  uint32_t all = 0, before = 0;  // expert e's assignments, those of the slices before this one
+  if (gridDim.x == 1) {
+    if (e < 512) next[e] = 0;
+    __syncthreads();
+    for (uint32_t i = e; i < end; i += 1024)
+      if ((uint32_t)ids[i] < E) atomicAdd(next + (uint32_t)ids[i], 1u);
+    __syncthreads();
+    all = e < E ? next[e] : 0;
+  } else if (e < E) {
+    for (uint32_t b = 0; b < gridDim.x; b++) {
+      const uint32_t n = counts[b * E + e];
+      all += n, before += b < blockIdx.x ? n : 0;
+    }
+  }
+  const uint32_t start = scan512(all, lds) - all;
+  if (blockIdx.x == 0) {
+    const uint32_t n = (all + rows - 1) / rows, last = scan512(n, lds);
+    if (e < E)
+      for (uint32_t j = 0; j < n; j++) tiles[last - n + j] = MoeTile{e, e, start + j * rows, min(rows, all - j * rows)};
+    if (e == 511) *n_tiles = last;
+  }
+  __syncthreads();
+  if (e < 512) next[e] = start + before;
+  __syncthreads();
+  for (uint32_t i = first + e; i < end; i += 1024) {
+    const uint32_t id = (uint32_t)ids[i];
+    if (id < E) order[atomicAdd(next + id, 1u)] = i;
+  }
+}
+
+// ---- the products
+
+struct MxExperts {
+  const uint8_t *gc, *gs, *uc, *us, *dc, *ds;
+  uint32_t E, K, H, F;
+  float limit;
+};
+
+// A launch's work-groups to its items so that neighbours in the list are on one XCD (work-groups go to the eight in turn):
+// an expert's tiles share its weights in that L2. ~0: none.
+__device__ __forceinline__ uint32_t item_of(uint32_t all) {
+  const uint32_t per = (all + 7) / 8, id = blockIdx.x % 8 * per + blockIdx.x / 8;
+  return blockIdx.x / 8 < per && id < all ? id : ~0u;
+}
+
+// An item: a tile and 128 columns of h (their rows of gate and of up). Writes the places' rows of h in MX4.
+template <int TM>
+__global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint8_t *xc, const uint8_t *xs, uint32_t ntok,
+                                                           const uint32_t *order, const MoeTile *tiles,
+                                                           const uint32_t *n_tiles, uint8_t *hc, uint8_t *hs) {
+  typedef MxTile<TM, 2, true> Tile;
+  __shared__ typename Tile::Stage s0;
+  __shared__ typename Tile::Stage s1;
+  const uint32_t steps = mx_steps(p.H), hsteps = mx_steps(p.F), item = item_of(*n_tiles * hsteps);
+  if (item == ~0u) return;
+  const MoeTile tile = tiles[item / hsteps];
+  const uint32_t f0 = item % hsteps * 128, stages = (steps + 1) / 2;
+  const uint64_t row = (uint64_t)tile.expert * p.F + f0, rest = (uint64_t)p.E * p.F - row;
+  const auto same = [](uint32_t r) { return r; };
+  const MxSource<Tile::BM> x(xc, xs, ntok, steps, [&](uint32_t r) { return order[tile.start + min(r, tile.count - 1)] / p.K; });
+  const MxSource<128> g(p.gc + row * steps * 64, p.gs + row * steps * 4, rest, steps, same);
+  const MxSource<128> u(p.uc + row * steps * 64, p.us + row * steps * 4, rest, steps, same);
+  const auto load = [&](typename Tile::Stage &s, uint32_t k) {
+    g.load(k, steps, s.w, s.sw);
+    u.load(k, steps, s.w + 128 * 128, s.sw + 256);
+    x.load(k, steps, s.x, s.sx);
+  };
+  Tile c;
+  c.clear();
+  load(s0, 0);
+  if (stages > 1) load(s1, 1);
+  dma_barrier();
+  c.start(s0);
+  for (uint32_t k = 0;; k += 2) {
+    c.template stage<0>(s0, s1, 2 * k + 1 >= steps, [&] {
+      if (k + 2 < stages) load(s0, k + 2);
+    });
+    if (k + 1 >= stages) break;
+    c.template stage<1>(s1, s0, 2 * k + 3 >= steps, [&] {
+      if (k + 3 < stages) load(s1, k + 3);
+    });
+    if (k + 2 >= stages) break;
+  }
+  // Lane l has 16 of its token's 32 columns of a wave (8 j + 4 (l / 32) + i), lane l ^ 32 the others.
+  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32, col = f0 + 32 * wave;
+#pragma unroll
+  for (int m = 0; m < TM; m++) {
+    float h[16];
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      h[i] = mx_swiglu(c.acc[0][m][i], c.acc[1][m][i], p.limit);
+      if (col + 8 * (i / 4) + 4 * q + i % 4 >= p.F) h[i] = 0.0f;
+      most = max(most, __float_as_uint(h[i]) & 0x7fffffffu);
+    }
+    most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+    const uint32_t s = mx_scale_of(most);
+    const uint32_t a = s == 255 ? 0u : mx_codes8(h, s), b = s == 255 ? 0u : mx_codes8(h + 8, s);
+    const uint32_t oa = (uint32_t)__shfl_xor((int)a, 32, 64), ob = (uint32_t)__shfl_xor((int)b, 32, 64);
+    const uint32_t r = 32 * m + lane % 32;
+    if (q == 0 && r < tile.count) {
+      const uint64_t at = (uint64_t)(tile.start + r) * hsteps * 4 + col / 32;
+      *(uint4 *)(hc + at * 16) = make_uint4((a & 0xffff) | oa << 16, (a >> 16) | (oa & 0xffff0000u), (b & 0xffff) | ob << 16,
+                                            (b >> 16) | (ob & 0xffff0000u));
+      hs[at] = (uint8_t)s;
+    }
+  }
+}
+
+// An item: a tile and `blocks` times 256 rows of down, one after the other on the same pipeline. Writes the sums to the
+// assignments' rows of o, `pitch` apart (a multiple of 256).
+template <int TM>
+__global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t *hc, const uint8_t *hs, uint32_t A,
+                                                        const uint32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
+                                                        uint32_t blocks, float *o, uint32_t pitch) {
+  typedef MxTile<TM, 2, true> Tile;
+  __shared__ typename Tile::Stage s0;
+  __shared__ typename Tile::Stage s1;
+  const uint32_t steps = mx_steps(p.F), parts = (pitch / 256 + blocks - 1) / blocks, item = item_of(*n_tiles * parts);
+  if (item == ~0u) return;
+  const MoeTile tile = tiles[item / parts];
+  const uint32_t b0 = item % parts * blocks, stages = (steps + 1) / 2, nb = min(blocks, pitch / 256 - b0), all = nb * stages;
+  const uint64_t row = (uint64_t)tile.expert * p.H + b0 * 256;
+  const auto same = [](uint32_t r) { return r; };
+  const MxSource<Tile::BM> x(hc, hs, A, steps, [&](uint32_t r) { return tile.start + min(r, tile.count - 1); });
+  const MxSource<256> w(p.dc + row * steps * 64, p.ds + row * steps * 4, (uint64_t)p.E * p.H - row, steps, same);
+  const auto load = [&](typename Tile::Stage &s, uint32_t i) {  // stage i of all
+    const uint32_t n = i / stages, k = i - n * stages;
+    w.load(k, steps, s.w, s.sw, n * 256);
+    x.load(k, steps, s.x, s.sx);
+  };
+  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32;
+  float *to[TM];
+#pragma unroll
+  for (int m = 0; m < TM; m++) {
+    const uint32_t r = 32 * m + lane % 32;
+    to[m] = r < tile.count ? o + (uint64_t)order[tile.start + r] * pitch + b0 * 256 + wave * 32 + 4 * q : nullptr;
+  }
+  Tile c;
+  c.clear();
+  uint32_t k = 0, n = 0;  // the stage's k and 256 rows
+  const auto done = [&] {
+    if (++k < stages) return;
+#pragma unroll
+    for (int m = 0; m < TM; m++)
+#pragma unroll
+      for (int v = 0; v < 2; v++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (to[m])
+            *(float4 *)(to[m] + n * 256 + v * 128 + 8 * j) = make_float4(c.acc[v][m][4 * j], c.acc[v][m][4 * j + 1],
+                                                                      c.acc[v][m][4 * j + 2], c.acc[v][m][4 * j + 3]);
+    c.clear();
+    k = 0, n++;
+  };
+  load(s0, 0);
+  if (all > 1) load(s1, 1);
+  dma_barrier();
+  c.start(s0);
+  for (uint32_t i = 0;; i += 2) {
+    c.template stage<0>(s0, s1, 2 * k + 1 >= steps, [&] {
+      if (i + 2 < all) load(s0, i + 2);
+    });
+    done();
+    if (i + 1 >= all) break;
+    c.template stage<1>(s1, s0, 2 * k + 1 >= steps, [&] {
+      if (i + 3 < all) load(s1, i + 3);
+    });
+    done();
+    if (i + 2 >= all) break;
+  }
 }
 
 // One wave 16 rows of an assignment's expert.
@@ -39,7 +262,7 @@ __global__ void __launch_bounds__(64) mx4_gate_up(const uint8_t *xc, const uint8
 
 __global__ void __launch_bounds__(64) mx4_down(const uint8_t *hc, const uint8_t *hs, const uint8_t *dc,
                                                const uint8_t *ds, const int32_t *ids, uint32_t E, uint32_t H, uint32_t F,
-                                               float *o) {
+                                               float *o, uint32_t pitch) {
   const uint32_t lane = threadIdx.x, q = lane / 16, nt = (H + 15) / 16, steps = mx_steps(F);
   const uint32_t a = blockIdx.x / nt, r0 = blockIdx.x % nt * 16;
   const uint32_t e = (uint32_t)ids[a];
@@ -52,19 +275,19 @@ __global__ void __launch_bounds__(64) mx4_down(const uint8_t *hc, const uint8_t 
   if (lane % 16 == 0)
 #pragma unroll
     for (uint32_t i = 0; i < 4; i++)
-      if (r0 + 4 * q + i < H) o[(uint64_t)a * H + r0 + 4 * q + i] = c[i];
+      if (r0 + 4 * q + i < H) o[(uint64_t)a * pitch + r0 + 4 * q + i] = c[i];
 }
 
 template <uint32_t kType>
 __global__ void mx4_combine(const float *o, const int32_t *ids, const float *w, uint32_t ntok, uint32_t E, uint32_t K,
-                            uint32_t H, typename Elem<kType>::T *y, uint64_t stride) {
+                            uint32_t H, uint32_t pitch, typename Elem<kType>::T *y, uint64_t stride) {
   const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const uint64_t t = i / H;
   const uint32_t c = (uint32_t)(i - t * H);
   if (t >= ntok) return;
   float s = 0.0f;
   for (uint32_t k = 0; k < K; k++)
-    if ((uint32_t)ids[t * K + k] < E) s += w[t * K + k] * o[(t * K + k) * H + c];
+    if ((uint32_t)ids[t * K + k] < E) s += w[t * K + k] * o[(t * K + k) * pitch + c];
   y[t * stride + c] = (typename Elem<kType>::T)s;
 }
 
@@ -88,21 +311,34 @@ void check_experts(const moe_mx4_experts *e, uint32_t ntok) {
   op_require(op_float(e->x_type) && op_float(e->y_type), "the element type must be QT_F32, QT_F16 or QT_BF16");
 }
 
-// The work buffer's parts: x's rows quantised, h and its rows quantised, the experts' outputs.
-struct Work {
-  uint64_t xc, xs, h, hc, hs, o, bytes;
-  Work(const moe_mx4_experts &e, uint64_t T) {
+// How a call runs: assignments at most kFew: without sorting them.
+constexpr uint32_t kFew = 256;
+
+struct Plan {
+  uint32_t A, rows, slices, pitch, max_tiles;
+  bool few;
+  uint64_t xc, xs, h, hc, hs, o, counts, order, tiles, n_tiles, bytes;  // the work buffer's parts
+
+  Plan(const moe_mx4_experts &e, uint32_t T) {
+    A = T * e.n_used, few = A <= kFew;
+    // Tiles of 32, 64 or 128 positions: the more an expert has on average, the fewer times its weights are read.
+    const uint32_t mean = A / e.n_expert;
+    rows = mean < 24 ? 32 : mean < 96 ? 64 : 128;
+    slices = (A + kSlice - 1) / kSlice;
+    pitch = (e.n_embd + 255) / 256 * 256;
+    max_tiles = std::min(A, e.n_expert + A / rows);
     uint64_t at = 0;
     const auto part = [&](uint64_t n) {
       const uint64_t was = at;
       at += (n + 255) / 256 * 256;
       return was;
     };
-    const uint64_t A = T * e.n_used;
-    xc = part(moe_mx4_code_bytes((uint32_t)T, e.n_embd)), xs = part(moe_mx4_scale_bytes((uint32_t)T, e.n_embd));
-    h = part(A * e.n_ff * 4);
-    hc = part(moe_mx4_code_bytes((uint32_t)A, e.n_ff)), hs = part(moe_mx4_scale_bytes((uint32_t)A, e.n_ff));
-    o = part(A * e.n_embd * 4);
+    xc = part(moe_mx4_code_bytes(T, e.n_embd)), xs = part(moe_mx4_scale_bytes(T, e.n_embd));
+    h = part(few ? (uint64_t)A * e.n_ff * 4 : 0);
+    hc = part(moe_mx4_code_bytes(A, e.n_ff)), hs = part(moe_mx4_scale_bytes(A, e.n_ff));
+    o = part((uint64_t)A * pitch * 4);
+    counts = part(few ? 0 : (uint64_t)slices * e.n_expert * 4), order = part(few ? 0 : (uint64_t)A * 4);
+    tiles = part(few ? 0 : (uint64_t)max_tiles * sizeof(MoeTile)), n_tiles = part(4);
     bytes = at;
   }
 };
@@ -115,7 +351,7 @@ MOE_API uint64_t moe_mx4_experts_work_bytes(const moe_mx4_experts *e, uint32_t n
   uint64_t n = 0;
   (void)op_guarded([&] {
     check_experts(e, ntok);
-    n = Work(*e, ntok).bytes;
+    n = Plan(*e, ntok).bytes;
   });
   return n;
 }
@@ -129,23 +365,42 @@ MOE_API moe_status moe_mx4_experts_async(const moe_mx4_experts *e, const void *x
     op_rows(x, x_stride, H, e->x_type);
     op_rows(y, y_stride, H, e->y_type);
     op_require(ids && w && op_aligned(ids, 4) && op_aligned(w, 4), "null or misaligned ids or w");
-    const Work at(*e, ntok);
+    const Plan at(*e, ntok);
     op_work(work, work_bytes, at.bytes);
     if (!ntok) return;
     OnDevice on(e->device);
     uint8_t *b = (uint8_t *)work;
     mx4_quantize_launch(e->x_type, x, x_stride, moe_mx4_matrix{b + at.xc, b + at.xs, ntok, H}, stream);
-    op_launch(mx4_gate_up, (uint64_t)A * ((F + 15) / 16), 64, stream, (const uint8_t *)(b + at.xc),
-              (const uint8_t *)(b + at.xs), (const uint8_t *)e->gate.codes, (const uint8_t *)e->gate.scales,
-              (const uint8_t *)e->up.codes, (const uint8_t *)e->up.scales, ids, E, K, H, F, e->swiglu_limit,
-              (float *)(b + at.h));
-    mx4_quantize_launch(QT_F32, b + at.h, F, moe_mx4_matrix{b + at.hc, b + at.hs, A, F}, stream);
-    op_launch(mx4_down, (uint64_t)A * ((H + 15) / 16), 64, stream, (const uint8_t *)(b + at.hc),
-              (const uint8_t *)(b + at.hs), (const uint8_t *)e->down.codes, (const uint8_t *)e->down.scales, ids, E, H, F,
-              (float *)(b + at.o));
+    const MxExperts p{e->gate.codes, e->gate.scales, e->up.codes, e->up.scales, e->down.codes, e->down.scales, E, K, H, F,
+                      e->swiglu_limit};
+    const uint8_t *xc = b + at.xc, *xs = b + at.xs;
+    uint8_t *hc = b + at.hc, *hs = b + at.hs;
+    float *o = (float *)(b + at.o);
+    if (at.few) {
+      op_launch(mx4_gate_up, (uint64_t)A * ((F + 15) / 16), 64, stream, xc, xs, p.gc, p.gs, p.uc, p.us, ids, E, K, H, F,
+                e->swiglu_limit, (float *)(b + at.h));
+      mx4_quantize_launch(QT_F32, b + at.h, F, moe_mx4_matrix{hc, hs, A, F}, stream);
+      op_launch(mx4_down, (uint64_t)A * ((H + 15) / 16), 64, stream, (const uint8_t *)hc, (const uint8_t *)hs, p.dc, p.ds,
+                ids, E, H, F, o, at.pitch);
+    } else {
+      uint32_t *counts = (uint32_t *)(b + at.counts), *order = (uint32_t *)(b + at.order), *nt = (uint32_t *)(b + at.n_tiles);
+      MoeTile *tiles = (MoeTile *)(b + at.tiles);
+      if (at.slices > 1) op_launch(mx4_count, at.slices, 1024, stream, ids, A, E, counts);
+      op_launch(mx4_place, at.slices, 1024, stream, ids, A, E, (const uint32_t *)counts, at.rows, order, tiles, nt);
+      const uint32_t blocks = 2, parts = (at.pitch / 256 + blocks - 1) / blocks;
+      const auto run = [&](auto gate_up, auto down) {
+        op_launch(gate_up, ((uint64_t)at.max_tiles * mx_steps(F) + 7) / 8 * 8, 256, stream, p, xc, xs, ntok,
+                  (const uint32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, hc, hs);
+        op_launch(down, ((uint64_t)at.max_tiles * parts + 7) / 8 * 8, 256, stream, p, (const uint8_t *)hc, (const uint8_t *)hs,
+                  A, (const uint32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, blocks, o, at.pitch);
+      };
+      if (at.rows == 32) run(mx4_gate_up_tiles<1>, mx4_down_tiles<1>);
+      if (at.rows == 64) run(mx4_gate_up_tiles<2>, mx4_down_tiles<2>);
+      if (at.rows == 128) run(mx4_gate_up_tiles<4>, mx4_down_tiles<4>);
+    }
     const uint64_t n = ((uint64_t)ntok * H + 255) / 256;
-    const auto run = [&](auto kernel, auto *p) {
-      op_launch(kernel, n, 256, stream, (const float *)(b + at.o), ids, w, ntok, E, K, H, p, y_stride);
+    const auto run = [&](auto kernel, auto *to) {
+      op_launch(kernel, n, 256, stream, (const float *)o, ids, w, ntok, E, K, H, at.pitch, to, y_stride);
     };
     if (e->y_type == QT_F32) run(mx4_combine<QT_F32>, (float *)y);
     if (e->y_type == QT_F16) run(mx4_combine<QT_F16>, (_Float16 *)y);

@@ -40,28 +40,29 @@ struct MxStage {
   alignas(16) uint32_t sw[BN * 2];
 };
 
-// kRows rows of a matrix from row r0 on, as the source of its stages: a wave loads every fourth kilobyte of a stage. Rows
-// past the last are out of the buffer (their results are not stored); what would lie past a row's end (a last stage of 128
-// values) is read from before it, and not used.
+// kRows rows as the source of stages: row r of them is row_of(r) of those at codes and scales (`rows` there are), `steps`
+// of 128 values each. A wave loads every fourth kilobyte of a stage. Rows past the last are out of the buffer (their results
+// are not stored); what would lie past a row's end (a last stage of 128 values) is read from before it, and not used.
 template <int kRows>
 struct MxSource {
   static constexpr int kCodes = kRows / 32, kScales = (kRows + 127) / 128;
   __amdgpu_buffer_rsrc_t codes, scales;
-  uint32_t at[kCodes], sat[kScales], steps;
+  uint32_t at[kCodes], sat[kScales];
 
-  __device__ __forceinline__ MxSource(const uint8_t *c, const uint8_t *s, uint32_t r0, uint32_t rows, uint32_t n)
-      : codes(mx_buffer(c + (uint64_t)r0 * n * 64, (uint64_t)(rows - r0) * n * 64)),
-        scales(mx_buffer(s + (uint64_t)r0 * n * 4, (uint64_t)(rows - r0) * n * 4)), steps(n) {
+  template <typename F>
+  __device__ __forceinline__ MxSource(const uint8_t *c, const uint8_t *s, uint64_t rows, uint32_t steps, F row_of)
+      : codes(mx_buffer(c, rows * steps * 64)), scales(mx_buffer(s, rows * steps * 4)) {
     const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
 #pragma unroll
-    for (int i = 0; i < kCodes; i++) at[i] = ((wave + 4 * i) * 8 + lane / 8) * n * 64;
+    for (int i = 0; i < kCodes; i++) at[i] = row_of((wave + 4 * i) * 8 + lane / 8) * steps * 64;
 #pragma unroll
-    for (int i = 0; i < kScales; i++) sat[i] = ((wave + 4 * i) * 32 + lane / 2) * n * 4;
+    for (int i = 0; i < kScales; i++) sat[i] = row_of(min((wave + 4 * i) * 32 + lane / 2, (uint32_t)kRows - 1)) * steps * 4;
   }
-  __device__ __forceinline__ void load(uint32_t k, uint8_t *c, uint32_t *s) const {
+  // Stage k, from `rows` rows on.
+  __device__ __forceinline__ void load(uint32_t k, uint32_t steps, uint8_t *c, uint32_t *s, uint32_t rows = 0) const {
     const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
-    const uint32_t col = min(k * 128 + ((lane % 8) ^ (lane / 8)) * 16, steps * 64 - 16);
-    const uint32_t scol = min(k * 8 + lane % 2 * 4, steps * 4 - 4);
+    const uint32_t col = min(k * 128 + ((lane % 8) ^ (lane / 8)) * 16, steps * 64 - 16) + rows * steps * 64;
+    const uint32_t scol = min(k * 8 + lane % 2 * 4, steps * 4 - 4) + rows * steps * 4;
 #pragma unroll
     for (int i = 0; i < kCodes; i++) lds_dma16(codes, at[i] + col, c + (wave + 4 * i) * 1024);
 #pragma unroll
@@ -70,11 +71,12 @@ struct MxSource {
   }
 };
 
-// A work-group of four waves, two by two, each TM x TN fragments of 32 x 32: operands one step of k = 64 ahead of the
-// matrix instructions, in registers, across the stages.
-template <int TM, int TN>
+// A work-group's four waves on a tile of BM rows of x and BN rows of w: two by two, each TM x TN fragments of 32 x 32
+// (kWide false), or all on the same 32 TM rows of x and each on TN runs of 32 rows of w, 128 apart (kWide). The operands
+// are one step of k = 64 ahead of the matrix instructions, in registers, across the stages.
+template <int TM, int TN, bool kWide = false>
 struct MxTile {
-  static constexpr int BM = 64 * TM, BN = 64 * TN;
+  static constexpr int BM = (kWide ? 32 : 64) * TM, BN = (kWide ? 128 : 64) * TN;
   typedef MxStage<BM, BN> Stage;
   mx_f16 acc[TN][TM];
   mx_i4 a[2][TN], b[2][TM];
@@ -88,28 +90,32 @@ struct MxTile {
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[n][m][i] = 0.0f;
   }
+  static __device__ __forceinline__ uint32_t x_row() { return kWide ? 0 : (mx_wave() & 1) * 32 * TM; }
+  static __device__ __forceinline__ uint32_t w_row() { return kWide ? mx_wave() * 32 : (mx_wave() >> 1) * 32 * TN; }
+  static constexpr uint32_t kStep = kWide ? 128 : 32;  // between the fragments of w
+
   template <int kParity>
   __device__ __forceinline__ void read_scales(const Stage &s) {
-    const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32, r = lane % 32;
+    const uint32_t lane = threadIdx.x & 63, q = lane / 32, r = lane % 32;
 #pragma unroll
     for (int m = 0; m < TM; m++) {
-      const uint2 v = *(const uint2 *)(s.sx + ((wave & 1) * 32 * TM + r + 32 * m) * 2);
+      const uint2 v = *(const uint2 *)(s.sx + (x_row() + r + 32 * m) * 2);
       sx[kParity][m][0] = v.x >> (8 * q), sx[kParity][m][1] = v.y >> (8 * q);
     }
 #pragma unroll
     for (int n = 0; n < TN; n++) {
-      const uint2 v = *(const uint2 *)(s.sw + ((wave >> 1) * 32 * TN + r + 32 * n) * 2);
+      const uint2 v = *(const uint2 *)(s.sw + (w_row() + r + kStep * n) * 2);
       sw[kParity][n][0] = v.x >> (8 * q), sw[kParity][n][1] = v.y >> (8 * q);
     }
   }
   template <int j>
   __device__ __forceinline__ void read(const Stage &s) {
-    const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32, r = lane % 32;
+    const uint32_t lane = threadIdx.x & 63, q = lane / 32, r = lane % 32;
     const uint32_t at = ((2 * j + q) ^ (r % 8)) * 16;
 #pragma unroll
-    for (int m = 0; m < TM; m++) b[j % 2][m] = *(const mx_i4 *)(s.x + ((wave & 1) * 32 * TM + r + 32 * m) * 128 + at);
+    for (int m = 0; m < TM; m++) b[j % 2][m] = *(const mx_i4 *)(s.x + (x_row() + r + 32 * m) * 128 + at);
 #pragma unroll
-    for (int n = 0; n < TN; n++) a[j % 2][n] = *(const mx_i4 *)(s.w + ((wave >> 1) * 32 * TN + r + 32 * n) * 128 + at);
+    for (int n = 0; n < TN; n++) a[j % 2][n] = *(const mx_i4 *)(s.w + (w_row() + r + kStep * n) * 128 + at);
   }
   template <int kParity, int j>
   __device__ __forceinline__ void multiply() {
@@ -121,23 +127,34 @@ struct MxTile {
         acc[n][m] = mx_mfma32<j % 2 * 2, j % 2 * 2>(a[j % 2][n], b[j % 2][m], acc[n][m], sw[kParity][n][j / 2], sx[kParity][m][j / 2]);
     __builtin_amdgcn_sched_barrier(0);
   }
-  // Stage `now`, of parity kParity; its step 0 is in registers. After the barrier `now` is free and `next` is whole (past
-  // the last stage its first step is read all the same, and not used). half: the row ends after two steps, the others add
-  // zeros.
+  // Stage `now`, of parity kParity; its step 0 is in registers. half: the row ends after its first two steps. After the
+  // barrier `now` is free (load() loads what comes after `next` into it) and `next` is whole; past the last stage its first
+  // step is read all the same, and not used. (The two halves are basic blocks of their own: 64 matrix instructions on all
+  // 256 accumulators in one are more than the compiler's register allocation holds without spills.)
   template <int kParity, typename Load>
   __device__ __forceinline__ void stage(const Stage &now, const Stage &next, bool half, Load load) {
     read<1>(now);
     multiply<kParity, 0>();
     read<2>(now);
     multiply<kParity, 1>();
-    if (half) return;  // (the last stage: the row ends here)
-    read<3>(now);
-    multiply<kParity, 2>();
-    dma_barrier();
-    load();
-    read<0>(next);
-    read_scales<kParity ^ 1>(next);
-    multiply<kParity, 3>();
+    if (!half) {
+      read<3>(now);
+      multiply<kParity, 2>();
+      dma_barrier();
+      load();
+      read<0>(next);
+      read_scales<kParity ^ 1>(next);
+      multiply<kParity, 3>();
+    } else {
+      dma_barrier();
+      load();
+      read<0>(next);
+      read_scales<kParity ^ 1>(next);
+    }
+  }
+  __device__ __forceinline__ void start(const Stage &first) {
+    read<0>(first);
+    read_scales<0>(first);
   }
 };
 

@@ -111,19 +111,19 @@ __global__ void __launch_bounds__(256, TM *TN > 8 ? 1 : 2)
   const uint32_t p = id / (tm * tn), t = id % (tm * tn), group = t / (8 * tn), rows = min(tm - group * 8, 8u);
   const uint32_t m0 = (group * 8 + t % (8 * tn) % rows) * BM, n0 = t % (8 * tn) / rows * BN;
   const uint32_t k0 = p * span, k1 = min(k0 + span, stages);
-  const MxSource<BM> sx(xc, xs, m0, M, steps);
-  const MxSource<BN> sw(wc, ws, n0, N, steps);
+  const auto same = [](uint32_t r) { return r; };
+  const MxSource<BM> sx(xc + (uint64_t)m0 * steps * 64, xs + (uint64_t)m0 * steps * 4, M - m0, steps, same);
+  const MxSource<BN> sw(wc + (uint64_t)n0 * steps * 64, ws + (uint64_t)n0 * steps * 4, N - n0, steps, same);
   const auto load = [&](typename Tile::Stage &s, uint32_t k) {
-    sx.load(k, s.x, s.sx);
-    sw.load(k, s.w, s.sw);
+    sx.load(k, steps, s.x, s.sx);
+    sw.load(k, steps, s.w, s.sw);
   };
   Tile c;
   c.clear();
   load(s0, k0);
   if (k0 + 1 < k1) load(s1, k0 + 1);
   dma_barrier();
-  c.template read<0>(s0);
-  c.template read_scales<0>(s0);
+  c.start(s0);
   for (uint32_t k = k0;; k += 2) {
     c.template stage<0>(s0, s1, 2 * k + 1 >= steps, [&] {
       if (k + 2 < k1) load(s0, k + 2);
