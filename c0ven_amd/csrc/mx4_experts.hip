@@ -109,26 +109,27 @@ __device__ __forceinline__ uint32_t item_of(uint32_t all) {
   return blockIdx.x / 8 < per && id < all ? id : ~0u;
 }
 
-// An item: a tile and 128 columns of h (their rows of gate and of up). Writes the places' rows of h in MX4.
-template <int TM>
+// An item: a tile and 32 WN columns of h (their rows of gate and of up). Writes the places' rows of h in MX4.
+template <int TM, int WM>
 __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint8_t *xc, const uint8_t *xs, uint32_t ntok,
-                                                           const uint32_t *order, const MoeTile *tiles,
-                                                           const uint32_t *n_tiles, uint8_t *hc, uint8_t *hs) {
-  typedef MxTile<TM, 2, true> Tile;
+                                                         const uint32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
+                                                         uint8_t *hc, uint8_t *hs) {
+  typedef MxTile<TM, 2, WM, true> Tile;
+  constexpr uint32_t kCols = Tile::BN / 2;
   __shared__ typename Tile::Stage s0;
   __shared__ typename Tile::Stage s1;
-  const uint32_t steps = mx_steps(p.H), hsteps = mx_steps(p.F), item = item_of(*n_tiles * hsteps);
+  const uint32_t steps = mx_steps(p.H), hsteps = mx_steps(p.F), parts = hsteps * 128 / kCols, item = item_of(*n_tiles * parts);
   if (item == ~0u) return;
-  const MoeTile tile = tiles[item / hsteps];
-  const uint32_t f0 = item % hsteps * 128, stages = (steps + 1) / 2;
-  const uint64_t row = (uint64_t)tile.expert * p.F + f0, rest = (uint64_t)p.E * p.F - row;
+  const MoeTile tile = tiles[item / parts];
+  const uint32_t f0 = item % parts * kCols, stages = (steps + 1) / 2;
+  const uint64_t row = (uint64_t)tile.expert * p.F + f0, rest = (uint64_t)p.E * p.F - min(row, (uint64_t)p.E * p.F);
   const auto same = [](uint32_t r) { return r; };
   const MxSource<Tile::BM> x(xc, xs, ntok, steps, [&](uint32_t r) { return order[tile.start + min(r, tile.count - 1)] / p.K; });
-  const MxSource<128> g(p.gc + row * steps * 64, p.gs + row * steps * 4, rest, steps, same);
-  const MxSource<128> u(p.uc + row * steps * 64, p.us + row * steps * 4, rest, steps, same);
+  const MxSource<kCols> g(p.gc + row * steps * 64, p.gs + row * steps * 4, rest, steps, same);
+  const MxSource<kCols> u(p.uc + row * steps * 64, p.us + row * steps * 4, rest, steps, same);
   const auto load = [&](typename Tile::Stage &s, uint32_t k) {
     g.load(k, steps, s.w, s.sw);
-    u.load(k, steps, s.w + 128 * 128, s.sw + 256);
+    u.load(k, steps, s.w + kCols * 128, s.sw + kCols * 2);
     x.load(k, steps, s.x, s.sx);
   };
   Tile c;
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint
     if (k + 2 >= stages) break;
   }
   // Lane l has 16 of its token's 32 columns of a wave (8 j + 4 (l / 32) + i), lane l ^ 32 the others.
-  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32, col = f0 + 32 * wave;
+  const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = f0 + Tile::w_row();
 #pragma unroll
   for (int m = 0; m < TM; m++) {
     float h[16];
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint
     const uint32_t s = mx_scale_of(most);
     const uint32_t a = s == 255 ? 0u : mx_codes8(h, s), b = s == 255 ? 0u : mx_codes8(h + 8, s);
     const uint32_t oa = (uint32_t)__shfl_xor((int)a, 32, 64), ob = (uint32_t)__shfl_xor((int)b, 32, 64);
-    const uint32_t r = 32 * m + lane % 32;
+    const uint32_t r = Tile::x_row() + 32 * m + lane % 32;
     if (q == 0 && r < tile.count) {
       const uint64_t at = (uint64_t)(tile.start + r) * hsteps * 4 + col / 32;
       *(uint4 *)(hc + at * 16) = make_uint4((a & 0xffff) | oa << 16, (a >> 16) | (oa & 0xffff0000u), (b & 0xffff) | ob << 16,
@@ -173,38 +174,39 @@ __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint
   }
 }
 
-// An item: a tile and `blocks` times 256 rows of down, one after the other on the same pipeline. Writes the sums to the
-// assignments' rows of o, `pitch` apart (a multiple of 256).
-template <int TM>
+// An item: a tile and up to `blocks` times BN of the `cols` rows of down from r0 on, one after the other on the same
+// pipeline. Writes the sums to the assignments' rows of o, `cols` apart (a multiple of 256).
+template <int TM, int WM>
 __global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t *hc, const uint8_t *hs, uint32_t A,
-                                                        const uint32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
-                                                        uint32_t blocks, float *o, uint32_t pitch) {
-  typedef MxTile<TM, 2, true> Tile;
+                                                      const uint32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
+                                                      uint32_t blocks, uint32_t r0, uint32_t cols, float *o) {
+  typedef MxTile<TM, 2, WM, true> Tile;
   __shared__ typename Tile::Stage s0;
   __shared__ typename Tile::Stage s1;
-  const uint32_t steps = mx_steps(p.F), parts = (pitch / 256 + blocks - 1) / blocks, item = item_of(*n_tiles * parts);
+  const uint32_t steps = mx_steps(p.F), total = cols / Tile::BN, parts = (total + blocks - 1) / blocks;
+  const uint32_t item = item_of(*n_tiles * parts);
   if (item == ~0u) return;
   const MoeTile tile = tiles[item / parts];
-  const uint32_t b0 = item % parts * blocks, stages = (steps + 1) / 2, nb = min(blocks, pitch / 256 - b0), all = nb * stages;
-  const uint64_t row = (uint64_t)tile.expert * p.H + b0 * 256;
+  const uint32_t b0 = item % parts * blocks, stages = (steps + 1) / 2, nb = min(blocks, total - b0), all = nb * stages;
+  const uint64_t row = (uint64_t)tile.expert * p.H + r0 + b0 * Tile::BN, rest = (uint64_t)p.E * p.H - min(row, (uint64_t)p.E * p.H);
   const auto same = [](uint32_t r) { return r; };
   const MxSource<Tile::BM> x(hc, hs, A, steps, [&](uint32_t r) { return tile.start + min(r, tile.count - 1); });
-  const MxSource<256> w(p.dc + row * steps * 64, p.ds + row * steps * 4, (uint64_t)p.E * p.H - row, steps, same);
+  const MxSource<Tile::BN> w(p.dc + row * steps * 64, p.ds + row * steps * 4, rest, steps, same);
   const auto load = [&](typename Tile::Stage &s, uint32_t i) {  // stage i of all
     const uint32_t n = i / stages, k = i - n * stages;
-    w.load(k, steps, s.w, s.sw, n * 256);
+    w.load(k, steps, s.w, s.sw, n * Tile::BN);
     x.load(k, steps, s.x, s.sx);
   };
-  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32;
+  const uint32_t lane = threadIdx.x & 63, q = lane / 32;
   float *to[TM];
 #pragma unroll
   for (int m = 0; m < TM; m++) {
-    const uint32_t r = 32 * m + lane % 32;
-    to[m] = r < tile.count ? o + (uint64_t)order[tile.start + r] * pitch + b0 * 256 + wave * 32 + 4 * q : nullptr;
+    const uint32_t r = Tile::x_row() + 32 * m + lane % 32;
+    to[m] = r < tile.count ? o + (uint64_t)order[tile.start + r] * cols + b0 * Tile::BN + Tile::w_row() + 4 * q : nullptr;
   }
   Tile c;
   c.clear();
-  uint32_t k = 0, n = 0;  // the stage's k and 256 rows
+  uint32_t k = 0, n = 0;  // the stage's k and BN rows
   const auto done = [&] {
     if (++k < stages) return;
 #pragma unroll
@@ -214,8 +216,8 @@ __global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t
 #pragma unroll
         for (int j = 0; j < 4; j++)
           if (to[m])
-            *(float4 *)(to[m] + n * 256 + v * 128 + 8 * j) = make_float4(c.acc[v][m][4 * j], c.acc[v][m][4 * j + 1],
-                                                                      c.acc[v][m][4 * j + 2], c.acc[v][m][4 * j + 3]);
+            *(float4 *)(to[m] + n * Tile::BN + v * Tile::kStep + 8 * j) =
+                make_float4(c.acc[v][m][4 * j], c.acc[v][m][4 * j + 1], c.acc[v][m][4 * j + 2], c.acc[v][m][4 * j + 3]);
     c.clear();
     k = 0, n++;
   };
@@ -278,17 +280,45 @@ __global__ void __launch_bounds__(64) mx4_down(const uint8_t *hc, const uint8_t 
       if (r0 + 4 * q + i < H) o[(uint64_t)a * pitch + r0 + 4 * q + i] = c[i];
 }
 
+// y's columns c0 .. c0 + cols (a multiple of 4 wide; H ends them) from the assignments' sums, `cols` apart, each token's in
+// rank order: four columns a thread, all ranks' sums loaded before the first is added.
 template <uint32_t kType>
-__global__ void mx4_combine(const float *o, const int32_t *ids, const float *w, uint32_t ntok, uint32_t E, uint32_t K,
-                            uint32_t H, uint32_t pitch, typename Elem<kType>::T *y, uint64_t stride) {
-  const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const uint64_t t = i / H;
-  const uint32_t c = (uint32_t)(i - t * H);
-  if (t >= ntok) return;
-  float s = 0.0f;
-  for (uint32_t k = 0; k < K; k++)
-    if ((uint32_t)ids[t * K + k] < E) s += w[t * K + k] * o[(t * K + k) * pitch + c];
-  y[t * stride + c] = (typename Elem<kType>::T)s;
+__global__ void __launch_bounds__(256) mx4_combine(const float *o, const int32_t *ids, const float *w, uint32_t ntok, uint32_t E,
+                                                   uint32_t K, uint32_t H, uint32_t c0, uint32_t cols,
+                                                   typename Elem<kType>::T *y, uint64_t stride) {
+  typedef typename Elem<kType>::T T;
+  const uint32_t per = cols / 4;  // threads a token
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint64_t t = i / per;
+  const uint32_t c = (uint32_t)(i - t * per) * 4;
+  if (t >= ntok || c0 + c >= H) return;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const float *from = o + t * K * cols + c;
+#pragma unroll
+  for (uint32_t k0 = 0; k0 < 16; k0 += 8) {
+    float4 v[8];
+    float f[8];
+#pragma unroll
+    for (uint32_t k = 0; k < 8; k++) {
+      const bool on = k0 + k < K && (uint32_t)ids[t * K + min(k0 + k, K - 1)] < E;
+      f[k] = on ? w[t * K + k0 + k] : 0.0f;
+      v[k] = on ? *(const float4 *)(from + (uint64_t)(k0 + k) * cols) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 8; k++)
+      s.x += f[k] * v[k].x, s.y += f[k] * v[k].y, s.z += f[k] * v[k].z, s.w += f[k] * v[k].w;
+    if (K <= 8) break;
+  }
+  T *to = y + t * stride + c0 + c;
+  const T e[4] = {(T)s.x, (T)s.y, (T)s.z, (T)s.w};
+  if (c0 + c + 4 <= H) {
+    struct __attribute__((packed)) Four {
+      T e[4];
+    };
+    *(Four *)to = Four{{e[0], e[1], e[2], e[3]}};
+  } else {
+    for (uint32_t j = 0; c0 + c + j < H; j++) to[j] = e[j];
+  }
 }
 
 }  // namespace c0ven
@@ -313,9 +343,10 @@ void check_experts(const moe_mx4_experts *e, uint32_t ntok) {
 
 // How a call runs: assignments at most kFew: without sorting them.
 constexpr uint32_t kFew = 256;
+constexpr uint64_t kChunkBytes = 96 << 20;
 
 struct Plan {
-  uint32_t A, rows, slices, pitch, max_tiles;
+  uint32_t A, rows, slices, pitch, chunk, max_tiles;
   bool few;
   uint64_t xc, xs, h, hc, hs, o, counts, order, tiles, n_tiles, bytes;  // the work buffer's parts
 
@@ -326,6 +357,9 @@ struct Plan {
     rows = mean < 24 ? 32 : mean < 96 ? 64 : 128;
     slices = (A + kSlice - 1) / kSlice;
     pitch = (e.n_embd + 255) / 256 * 256;
+    // The sums of all assignments at once, or of a part of the columns at a time that the last-level cache (256 MB) keeps
+    // until they are added.
+    chunk = few ? pitch : std::min<uint64_t>(pitch, std::max<uint64_t>(256, kChunkBytes / (4ull * A) / 256 * 256));
     max_tiles = std::min(A, e.n_expert + A / rows);
     uint64_t at = 0;
     const auto part = [&](uint64_t n) {
@@ -336,7 +370,7 @@ struct Plan {
     xc = part(moe_mx4_code_bytes(T, e.n_embd)), xs = part(moe_mx4_scale_bytes(T, e.n_embd));
     h = part(few ? (uint64_t)A * e.n_ff * 4 : 0);
     hc = part(moe_mx4_code_bytes(A, e.n_ff)), hs = part(moe_mx4_scale_bytes(A, e.n_ff));
-    o = part((uint64_t)A * pitch * 4);
+    o = part((uint64_t)A * chunk * 4);
     counts = part(few ? 0 : (uint64_t)slices * e.n_expert * 4), order = part(few ? 0 : (uint64_t)A * 4);
     tiles = part(few ? 0 : (uint64_t)max_tiles * sizeof(MoeTile)), n_tiles = part(4);
     bytes = at;
@@ -376,35 +410,40 @@ MOE_API moe_status moe_mx4_experts_async(const moe_mx4_experts *e, const void *x
     const uint8_t *xc = b + at.xc, *xs = b + at.xs;
     uint8_t *hc = b + at.hc, *hs = b + at.hs;
     float *o = (float *)(b + at.o);
+    const auto combine = [&](uint32_t c0, uint32_t cols) {
+      const uint64_t n = ((uint64_t)ntok * (cols / 4) + 255) / 256;
+      const auto run = [&](auto kernel, auto *to) {
+        op_launch(kernel, n, 256, stream, (const float *)o, ids, w, ntok, E, K, H, c0, cols, to, y_stride);
+      };
+      if (e->y_type == QT_F32) run(mx4_combine<QT_F32>, (float *)y);
+      if (e->y_type == QT_F16) run(mx4_combine<QT_F16>, (_Float16 *)y);
+      if (e->y_type == QT_BF16) run(mx4_combine<QT_BF16>, (__bf16 *)y);
+    };
     if (at.few) {
       op_launch(mx4_gate_up, (uint64_t)A * ((F + 15) / 16), 64, stream, xc, xs, p.gc, p.gs, p.uc, p.us, ids, E, K, H, F,
                 e->swiglu_limit, (float *)(b + at.h));
       mx4_quantize_launch(QT_F32, b + at.h, F, moe_mx4_matrix{hc, hs, A, F}, stream);
       op_launch(mx4_down, (uint64_t)A * ((H + 15) / 16), 64, stream, (const uint8_t *)hc, (const uint8_t *)hs, p.dc, p.ds,
                 ids, E, H, F, o, at.pitch);
-    } else {
-      uint32_t *counts = (uint32_t *)(b + at.counts), *order = (uint32_t *)(b + at.order), *nt = (uint32_t *)(b + at.n_tiles);
-      MoeTile *tiles = (MoeTile *)(b + at.tiles);
-      if (at.slices > 1) op_launch(mx4_count, at.slices, 1024, stream, ids, A, E, counts);
-      op_launch(mx4_place, at.slices, 1024, stream, ids, A, E, (const uint32_t *)counts, at.rows, order, tiles, nt);
-      const uint32_t blocks = 2, parts = (at.pitch / 256 + blocks - 1) / blocks;
-      const auto run = [&](auto gate_up, auto down) {
-        op_launch(gate_up, ((uint64_t)at.max_tiles * mx_steps(F) + 7) / 8 * 8, 256, stream, p, xc, xs, ntok,
-                  (const uint32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, hc, hs);
-        op_launch(down, ((uint64_t)at.max_tiles * parts + 7) / 8 * 8, 256, stream, p, (const uint8_t *)hc, (const uint8_t *)hs,
-                  A, (const uint32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, blocks, o, at.pitch);
-      };
-      if (at.rows == 32) run(mx4_gate_up_tiles<1>, mx4_down_tiles<1>);
-      if (at.rows == 64) run(mx4_gate_up_tiles<2>, mx4_down_tiles<2>);
-      if (at.rows == 128) run(mx4_gate_up_tiles<4>, mx4_down_tiles<4>);
+      return combine(0, at.pitch);
     }
-    const uint64_t n = ((uint64_t)ntok * H + 255) / 256;
-    const auto run = [&](auto kernel, auto *to) {
-      op_launch(kernel, n, 256, stream, (const float *)o, ids, w, ntok, E, K, H, at.pitch, to, y_stride);
+    uint32_t *counts = (uint32_t *)(b + at.counts), *order = (uint32_t *)(b + at.order), *nt = (uint32_t *)(b + at.n_tiles);
+    MoeTile *tiles = (MoeTile *)(b + at.tiles);
+    if (at.slices > 1) op_launch(mx4_count, at.slices, 1024, stream, ids, A, E, counts);
+    op_launch(mx4_place, at.slices, 1024, stream, ids, A, E, (const uint32_t *)counts, at.rows, order, tiles, nt);
+    const auto run = [&](auto gate_up, auto down, uint32_t bn) {
+      op_launch(gate_up, ((uint64_t)at.max_tiles * (mx_steps(F) * 128 / (bn / 2)) + 7) / 8 * 8, 256, stream, p, xc, xs, ntok,
+                (const uint32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, hc, hs);
+      for (uint32_t c = 0; c < at.pitch; c += at.chunk) {
+        const uint32_t cols = std::min(at.chunk, at.pitch - c), blocks = 1024 / bn, parts = (cols / bn + blocks - 1) / blocks;
+        op_launch(down, ((uint64_t)at.max_tiles * parts + 7) / 8 * 8, 256, stream, p, (const uint8_t *)hc, (const uint8_t *)hs,
+                  A, (const uint32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, blocks, c, cols, o);
+        combine(c, cols);
+      }
     };
-    if (e->y_type == QT_F32) run(mx4_combine<QT_F32>, (float *)y);
-    if (e->y_type == QT_F16) run(mx4_combine<QT_F16>, (_Float16 *)y);
-    if (e->y_type == QT_BF16) run(mx4_combine<QT_BF16>, (__bf16 *)y);
+    if (at.rows == 32) run(mx4_gate_up_tiles<1, 1>, mx4_down_tiles<1, 1>, 256);
+    if (at.rows == 64) run(mx4_gate_up_tiles<1, 2>, mx4_down_tiles<1, 2>, 128);
+    if (at.rows == 128) run(mx4_gate_up_tiles<2, 2>, mx4_down_tiles<2, 2>, 128);
   });
 }
 

@@ -71,12 +71,13 @@ struct MxSource {
   }
 };
 
-// A work-group's four waves on a tile of BM rows of x and BN rows of w: two by two, each TM x TN fragments of 32 x 32
-// (kWide false), or all on the same 32 TM rows of x and each on TN runs of 32 rows of w, 128 apart (kWide). The operands
-// are one step of k = 64 ahead of the matrix instructions, in registers, across the stages.
-template <int TM, int TN, bool kWide = false>
+// A work-group's four waves on a tile of BM rows of x and BN rows of w: WM of them along x's rows, 4 / WM along w's, each on
+// TM runs of 32 rows of x and TN runs of 32 rows of w. kApart: a wave's runs of w lie 32 times the waves apart (gate's rows
+// and up's), else they follow one another. The operands are one step of k = 64 ahead of the matrix instructions, in
+// registers, across the stages.
+template <int TM, int TN, int WM = 2, bool kApart = false>
 struct MxTile {
-  static constexpr int BM = (kWide ? 32 : 64) * TM, BN = (kWide ? 128 : 64) * TN;
+  static constexpr int WN = 4 / WM, BM = 32 * WM * TM, BN = 32 * WN * TN;
   typedef MxStage<BM, BN> Stage;
   mx_f16 acc[TN][TM];
   mx_i4 a[2][TN], b[2][TM];
@@ -90,9 +91,9 @@ struct MxTile {
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[n][m][i] = 0.0f;
   }
-  static __device__ __forceinline__ uint32_t x_row() { return kWide ? 0 : (mx_wave() & 1) * 32 * TM; }
-  static __device__ __forceinline__ uint32_t w_row() { return kWide ? mx_wave() * 32 : (mx_wave() >> 1) * 32 * TN; }
-  static constexpr uint32_t kStep = kWide ? 128 : 32;  // between the fragments of w
+  static __device__ __forceinline__ uint32_t x_row() { return mx_wave() % WM * 32 * TM; }
+  static __device__ __forceinline__ uint32_t w_row() { return mx_wave() / WM * 32 * (kApart ? 1 : TN); }
+  static constexpr uint32_t kStep = kApart ? 32 * WN : 32;  // between a wave's runs of w
 
   template <int kParity>
   __device__ __forceinline__ void read_scales(const Stage &s) {
