@@ -102,11 +102,19 @@ struct MxExperts {
   float limit;
 };
 
-// A launch's work-groups to its items so that neighbours in the list are on one XCD (work-groups go to the eight in turn):
-// an expert's tiles share its weights in that L2. ~0: none.
-__device__ __forceinline__ uint32_t item_of(uint32_t all) {
-  const uint32_t per = (all + 7) / 8, id = blockIdx.x % 8 * per + blockIdx.x / 8;
-  return blockIdx.x / 8 < per && id < all ? id : ~0u;
+// A launch's work-groups to its items (parts a tile) so that an XCD (work-groups go to the eight in turn) has runs of four
+// tiles: an expert's tiles share its weights in that L2, while the experts with one tile are dealt over all of them (whole
+// eighths of the list on an XCD left most of the distinct weights to a few: 4096 skewed tokens 132 us instead of the
+// figures below). ~0: none.
+constexpr uint32_t kTileRun = 4;
+__device__ __forceinline__ uint32_t item_of(uint32_t all, uint32_t parts) {
+  const uint32_t run = kTileRun * parts, j = blockIdx.x / 8, id = (j / run * 8 + blockIdx.x % 8) * run + j % run;
+  return id < all ? id : ~0u;
+}
+// The work-groups that cover `all` items.
+inline uint64_t item_blocks(uint64_t all, uint64_t parts) {
+  const uint64_t run = kTileRun * parts;
+  return (all + 8 * run - 1) / (8 * run) * (8 * run);
 }
 
 // An item: a tile and 32 WN columns of h (their rows of gate and of up). Writes the places' rows of h in MX4.
@@ -118,7 +126,7 @@ __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint
   constexpr uint32_t kCols = Tile::BN / 2;
   __shared__ typename Tile::Stage s0;
   __shared__ typename Tile::Stage s1;
-  const uint32_t steps = mx_steps(p.H), hsteps = mx_steps(p.F), parts = hsteps * 128 / kCols, item = item_of(*n_tiles * parts);
+  const uint32_t steps = mx_steps(p.H), hsteps = mx_steps(p.F), parts = hsteps * 128 / kCols, item = item_of(*n_tiles * parts, parts);
   if (item == ~0u) return;
   const MoeTile tile = tiles[item / parts];
   const uint32_t f0 = item % parts * kCols, stages = (steps + 1) / 2;
@@ -174,17 +182,21 @@ __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint
   }
 }
 
-// An item: a tile and up to `blocks` times BN of the `cols` rows of down from r0 on, one after the other on the same
-// pipeline. Writes the sums to the assignments' rows of o, `cols` apart (a multiple of 256).
+// An item: a tile and a few times BN of the `cols` rows of down from r0 on, one after the other on the same pipeline, so many
+// that the launch has about 2048 items. Writes the sums to the assignments' rows of o, `cols` apart (a multiple of 256): a
+// lane has a column of 16 rows, so that a store is of whole lines (two rows of 32 columns; with a row's four neighbours a
+// lane it was 32 rows of 32 bytes: 4096 tokens 172 us in all, now see below).
 template <int TM, int WM>
 __global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t *hc, const uint8_t *hs, uint32_t A,
                                                       const uint32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
-                                                      uint32_t blocks, uint32_t r0, uint32_t cols, float *o) {
-  typedef MxTile<TM, 2, WM, true> Tile;
+                                                      uint32_t r0, uint32_t cols, float *o) {
+  typedef MxTile<TM, 2, WM, true, true> Tile;
   __shared__ typename Tile::Stage s0;
   __shared__ typename Tile::Stage s1;
-  const uint32_t steps = mx_steps(p.F), total = cols / Tile::BN, parts = (total + blocks - 1) / blocks;
-  const uint32_t item = item_of(*n_tiles * parts);
+  __shared__ __align__(16) uint32_t place[Tile::BM];  // a row's assignment (~0: no row)
+  const uint32_t steps = mx_steps(p.F), total = cols / Tile::BN, nt = *n_tiles;
+  const uint32_t blocks = min(max(nt * total / 2048, 1u), total), parts = (total + blocks - 1) / blocks;
+  const uint32_t item = item_of(nt * parts, parts);
   if (item == ~0u) return;
   const MoeTile tile = tiles[item / parts];
   const uint32_t b0 = item % parts * blocks, stages = (steps + 1) / 2, nb = min(blocks, total - b0), all = nb * stages;
@@ -198,12 +210,8 @@ __global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t
     x.load(k, steps, s.x, s.sx);
   };
   const uint32_t lane = threadIdx.x & 63, q = lane / 32;
-  float *to[TM];
-#pragma unroll
-  for (int m = 0; m < TM; m++) {
-    const uint32_t r = Tile::x_row() + 32 * m + lane % 32;
-    to[m] = r < tile.count ? o + (uint64_t)order[tile.start + r] * cols + b0 * Tile::BN + Tile::w_row() + 4 * q : nullptr;
-  }
+  if (threadIdx.x < Tile::BM) place[threadIdx.x] = threadIdx.x < tile.count ? order[tile.start + threadIdx.x] : ~0u;
+  float *to = o + b0 * Tile::BN + Tile::w_row() + lane % 32;
   Tile c;
   c.clear();
   uint32_t k = 0, n = 0;  // the stage's k and BN rows
@@ -212,12 +220,15 @@ __global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t
 #pragma unroll
     for (int m = 0; m < TM; m++)
 #pragma unroll
-      for (int v = 0; v < 2; v++)
+      for (int j = 0; j < 4; j++) {
+        const uint4 v = *(const uint4 *)(place + Tile::x_row() + 32 * m + 8 * j + 4 * q);
+        const uint32_t at[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (to[m])
-            *(float4 *)(to[m] + n * Tile::BN + v * Tile::kStep + 8 * j) =
-                make_float4(c.acc[v][m][4 * j], c.acc[v][m][4 * j + 1], c.acc[v][m][4 * j + 2], c.acc[v][m][4 * j + 3]);
+        for (int i = 0; i < 4; i++)
+          if (at[i] != ~0u)
+#pragma unroll
+            for (int f = 0; f < 2; f++) to[(uint64_t)at[i] * cols + n * Tile::BN + f * Tile::kStep] = c.acc[f][m][4 * j + i];
+      }
     c.clear();
     k = 0, n++;
   };
@@ -432,12 +443,12 @@ MOE_API moe_status moe_mx4_experts_async(const moe_mx4_experts *e, const void *x
     if (at.slices > 1) op_launch(mx4_count, at.slices, 1024, stream, ids, A, E, counts);
     op_launch(mx4_place, at.slices, 1024, stream, ids, A, E, (const uint32_t *)counts, at.rows, order, tiles, nt);
     const auto run = [&](auto gate_up, auto down, uint32_t bn) {
-      op_launch(gate_up, ((uint64_t)at.max_tiles * (mx_steps(F) * 128 / (bn / 2)) + 7) / 8 * 8, 256, stream, p, xc, xs, ntok,
+      op_launch(gate_up, item_blocks((uint64_t)at.max_tiles * (mx_steps(F) * 256 / bn), mx_steps(F) * 256 / bn), 256, stream, p, xc, xs, ntok,
                 (const uint32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, hc, hs);
       for (uint32_t c = 0; c < at.pitch; c += at.chunk) {
-        const uint32_t cols = std::min(at.chunk, at.pitch - c), blocks = 1024 / bn, parts = (cols / bn + blocks - 1) / blocks;
-        op_launch(down, ((uint64_t)at.max_tiles * parts + 7) / 8 * 8, 256, stream, p, (const uint8_t *)hc, (const uint8_t *)hs,
-                  A, (const uint32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, blocks, c, cols, o);
+        const uint32_t cols = std::min(at.chunk, at.pitch - c);
+        op_launch(down, item_blocks((uint64_t)at.max_tiles * (cols / bn), cols / bn), 256, stream, p, (const uint8_t *)hc,
+                  (const uint8_t *)hs, A, (const uint32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, c, cols, o);
         combine(c, cols);
       }
     };

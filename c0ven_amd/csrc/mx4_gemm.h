@@ -73,9 +73,10 @@ struct MxSource {
 
 // A work-group's four waves on a tile of BM rows of x and BN rows of w: WM of them along x's rows, 4 / WM along w's, each on
 // TM runs of 32 rows of x and TN runs of 32 rows of w. kApart: a wave's runs of w lie 32 times the waves apart (gate's rows
-// and up's), else they follow one another. The operands are one step of k = 64 ahead of the matrix instructions, in
+// and up's), else they follow one another. kAcross: a lane's sums are one w row's with 16 of x's, instead of one x row's with 16
+// of w's. The operands are one step of k = 64 ahead of the matrix instructions, in
 // registers, across the stages.
-template <int TM, int TN, int WM = 2, bool kApart = false>
+template <int TM, int TN, int WM = 2, bool kApart = false, bool kAcross = false>
 struct MxTile {
   static constexpr int WN = 4 / WM, BM = 32 * WM * TM, BN = 32 * WN * TN;
   typedef MxStage<BM, BN> Stage;
@@ -125,7 +126,8 @@ struct MxTile {
     for (int n = 0; n < TN; n++)
 #pragma unroll
       for (int m = 0; m < TM; m++)
-        acc[n][m] = mx_mfma32<j % 2 * 2, j % 2 * 2>(a[j % 2][n], b[j % 2][m], acc[n][m], sw[kParity][n][j / 2], sx[kParity][m][j / 2]);
+        acc[n][m] = kAcross ? mx_mfma32<j % 2 * 2, j % 2 * 2>(b[j % 2][m], a[j % 2][n], acc[n][m], sx[kParity][m][j / 2], sw[kParity][n][j / 2])
+                            : mx_mfma32<j % 2 * 2, j % 2 * 2>(a[j % 2][n], b[j % 2][m], acc[n][m], sw[kParity][n][j / 2], sx[kParity][m][j / 2]);
     __builtin_amdgcn_sched_barrier(0);
   }
   // Stage `now`, of parity kParity; its step 0 is in registers. half: the row ends after its first two steps. After the
