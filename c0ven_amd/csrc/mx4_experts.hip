@@ -119,13 +119,14 @@ inline uint64_t item_blocks(uint64_t all, uint64_t parts) {
 
 // An item: a tile and 32 WN columns of h (their rows of gate and of up). Writes the places' rows of h in MX4.
 template <int TM, int WM>
-__global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint8_t *xc, const uint8_t *xs, uint32_t ntok,
+__global__ void __launch_bounds__(256, TM == 1 && WM == 2 ? 3 : 2) mx4_gate_up_tiles(MxExperts p, const uint8_t *xc, const uint8_t *xs, uint32_t ntok,
                                                          const uint32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
                                                          uint8_t *hc, uint8_t *hs) {
   typedef MxTile<TM, 2, WM, true> Tile;
   constexpr uint32_t kCols = Tile::BN / 2;
   __shared__ typename Tile::Stage s0;
   __shared__ typename Tile::Stage s1;
+  __shared__ typename Tile::Scales scales;
   const uint32_t steps = mx_steps(p.H), hsteps = mx_steps(p.F), parts = hsteps * 128 / kCols, item = item_of(*n_tiles * parts, parts);
   if (item == ~0u) return;
   const MoeTile tile = tiles[item / parts];
@@ -135,27 +136,15 @@ __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint
   const MxSource<Tile::BM> x(xc, xs, ntok, steps, [&](uint32_t r) { return order[tile.start + min(r, tile.count - 1)] / p.K; });
   const MxSource<kCols> g(p.gc + row * steps * 64, p.gs + row * steps * 4, rest, steps, same);
   const MxSource<kCols> u(p.uc + row * steps * 64, p.us + row * steps * 4, rest, steps, same);
-  const auto load = [&](typename Tile::Stage &s, uint32_t k) {
-    g.load(k, steps, s.w, s.sw);
-    u.load(k, steps, s.w + kCols * 128, s.sw + kCols * 2);
-    x.load(k, steps, s.x, s.sx);
-  };
   Tile c;
   c.clear();
-  load(s0, 0);
-  if (stages > 1) load(s1, 1);
-  dma_barrier();
-  c.start(s0);
-  for (uint32_t k = 0;; k += 2) {
-    c.template stage<0>(s0, s1, 2 * k + 1 >= steps, [&] {
-      if (k + 2 < stages) load(s0, k + 2);
-    });
-    if (k + 1 >= stages) break;
-    c.template stage<1>(s1, s0, 2 * k + 3 >= steps, [&] {
-      if (k + 3 < stages) load(s1, k + 3);
-    });
-    if (k + 2 >= stages) break;
-  }
+  c.run(
+      s0, s1, scales, stages,
+      [&](typename Tile::Stage &s, uint32_t k) { g.load(k, s.w), u.load(k, s.w + kCols * 128), x.load(k, s.x); },
+      [&](typename Tile::Scales &s, uint32_t k) {
+        g.load_scales(k, s.w), u.load_scales(k, s.w + kCols * mx_pitch(k, steps)), x.load_scales(k, s.x);
+      },
+      [&](uint32_t k) { return mx_pitch(k, steps); }, [&](uint32_t k) { return min(steps - 2 * k, 2u); }, [](uint32_t) {});
   // Lane l has 16 of its token's 32 columns of a wave (8 j + 4 (l / 32) + i), lane l ^ 32 the others.
   const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = f0 + Tile::w_row();
 #pragma unroll
@@ -187,36 +176,34 @@ __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint
 // lane has a column of 16 rows, so that a store is of whole lines (two rows of 32 columns; with a row's four neighbours a
 // lane it was 32 rows of 32 bytes: 4096 tokens 172 us in all, now see below).
 template <int TM, int WM>
-__global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t *hc, const uint8_t *hs, uint32_t A,
+__global__ void __launch_bounds__(256, TM == 1 && WM == 2 ? 3 : 2) mx4_down_tiles(MxExperts p, const uint8_t *hc, const uint8_t *hs, uint32_t A,
                                                       const uint32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
                                                       uint32_t r0, uint32_t cols, float *o) {
   typedef MxTile<TM, 2, WM, true, true> Tile;
   __shared__ typename Tile::Stage s0;
   __shared__ typename Tile::Stage s1;
-  __shared__ __align__(16) uint32_t place[Tile::BM];  // a row's assignment (~0: no row)
+  __shared__ typename Tile::Scales scales;
+  __shared__ __align__(16) uint32_t place[Tile::BM];  // where a row of the tile goes, in bytes
+  constexpr uint32_t kNowhere = 0xf0000000u;           // (out of the buffer: a store there is dropped)
   const uint32_t steps = mx_steps(p.F), total = cols / Tile::BN, nt = *n_tiles;
   const uint32_t blocks = min(max(nt * total / 2048, 1u), total), parts = (total + blocks - 1) / blocks;
   const uint32_t item = item_of(nt * parts, parts);
   if (item == ~0u) return;
   const MoeTile tile = tiles[item / parts];
-  const uint32_t b0 = item % parts * blocks, stages = (steps + 1) / 2, nb = min(blocks, total - b0), all = nb * stages;
+  const uint32_t b0 = item % parts * blocks, nb = min(blocks, total - b0);
+  const uint32_t stages = (steps + 3) / 4 * 2;  // of BN rows: whole pairs (the last one may be empty)
   const uint64_t row = (uint64_t)tile.expert * p.H + r0 + b0 * Tile::BN, rest = (uint64_t)p.E * p.H - min(row, (uint64_t)p.E * p.H);
   const auto same = [](uint32_t r) { return r; };
   const MxSource<Tile::BM> x(hc, hs, A, steps, [&](uint32_t r) { return tile.start + min(r, tile.count - 1); });
   const MxSource<Tile::BN> w(p.dc + row * steps * 64, p.ds + row * steps * 4, rest, steps, same);
-  const auto load = [&](typename Tile::Stage &s, uint32_t i) {  // stage i of all
-    const uint32_t n = i / stages, k = i - n * stages;
-    w.load(k, steps, s.w, s.sw, n * Tile::BN);
-    x.load(k, steps, s.x, s.sx);
-  };
   const uint32_t lane = threadIdx.x & 63, q = lane / 32;
-  if (threadIdx.x < Tile::BM) place[threadIdx.x] = threadIdx.x < tile.count ? order[tile.start + threadIdx.x] : ~0u;
-  float *to = o + b0 * Tile::BN + Tile::w_row() + lane % 32;
+  if (threadIdx.x < Tile::BM)
+    place[threadIdx.x] = threadIdx.x < tile.count ? order[tile.start + threadIdx.x] * cols * 4 : kNowhere;
+  const __amdgpu_buffer_rsrc_t to = mx_buffer((const uint8_t *)o, (uint64_t)A * cols * 4);
+  const uint32_t col = (b0 * Tile::BN + Tile::w_row() + lane % 32) * 4;
   Tile c;
   c.clear();
-  uint32_t k = 0, n = 0;  // the stage's k and BN rows
-  const auto done = [&] {
-    if (++k < stages) return;
+  const auto store = [&](uint32_t n) {  // the sums of the n-th BN rows
 #pragma unroll
     for (int m = 0; m < TM; m++)
 #pragma unroll
@@ -225,29 +212,28 @@ __global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t
         const uint32_t at[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; i++)
-          if (at[i] != ~0u)
 #pragma unroll
-            for (int f = 0; f < 2; f++) to[(uint64_t)at[i] * cols + n * Tile::BN + f * Tile::kStep] = c.acc[f][m][4 * j + i];
+          for (int f = 0; f < 2; f++)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(c.acc[f][m][4 * j + i]), to, at[i] + col,
+                                                  (n * Tile::BN + f * Tile::kStep) * 4, 0);
       }
     c.clear();
-    k = 0, n++;
   };
-  load(s0, 0);
-  if (all > 1) load(s1, 1);
-  dma_barrier();
-  c.start(s0);
-  for (uint32_t i = 0;; i += 2) {
-    c.template stage<0>(s0, s1, 2 * k + 1 >= steps, [&] {
-      if (i + 2 < all) load(s0, i + 2);
-    });
-    done();
-    if (i + 1 >= all) break;
-    c.template stage<1>(s1, s0, 2 * k + 1 >= steps, [&] {
-      if (i + 3 < all) load(s1, i + 3);
-    });
-    done();
-    if (i + 2 >= all) break;
-  }
+  c.run(
+      s0, s1, scales, nb * stages,
+      [&](typename Tile::Stage &s, uint32_t i) {
+        const uint32_t n = i / stages, k = i - n * stages;
+        if (2 * k < steps) w.load(k, s.w, n * Tile::BN), x.load(k, s.x);
+      },
+      [&](typename Tile::Scales &s, uint32_t i) {
+        const uint32_t n = i / stages, k = i - n * stages;
+        w.load_scales(k, s.w, n * Tile::BN), x.load_scales(k, s.x);
+      },
+      [&](uint32_t i) { return mx_pitch(i % stages, steps); },
+      [&](uint32_t i) { return min(steps - min(2 * (i % stages), steps), 2u); },
+      [&](uint32_t i) {
+        if (i % stages == stages - 1) store(i / stages);
+      });
 }
 
 // One wave 16 rows of an assignment's expert.

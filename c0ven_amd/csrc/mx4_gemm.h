@@ -31,13 +31,19 @@ __device__ __forceinline__ void dma_barrier() {
 }
 
 // One stage of k = 256: 128 bytes of codes a row, its eight 16-byte pieces exchanged by the row (piece p of row r at
-// p ^ r % 8) so that a fragment's reads fall on all banks; two words of scales a row.
+// p ^ r / 2 % 8) so that a fragment's reads (16 rows at a time) fall on all 64 banks: 142 us of a 4096 x 8192 x 8192 product
+// went to the reads alone with r % 8, 98 with r / 2 % 8.
 template <int BM, int BN>
 struct MxStage {
   alignas(16) uint8_t x[BM * 128];
   alignas(16) uint8_t w[BN * 128];
-  alignas(16) uint32_t sx[BM * 2];
-  alignas(16) uint32_t sw[BN * 2];
+};
+// The scales of two stages, 16 bytes a row. (A load whose neighbouring lanes do not share a line takes a clock a lane, so
+// eight bytes a row and stage cost as much as the codes: 53 us of the same product.)
+template <int BM, int BN>
+struct MxScales {
+  alignas(16) uint32_t x[BM * 4];
+  alignas(16) uint32_t w[BN * 4];
 };
 
 // kRows rows as the source of stages: row r of them is row_of(r) of those at codes and scales (`rows` there are), `steps`
@@ -45,31 +51,58 @@ struct MxStage {
 // are not stored); what would lie past a row's end (a last stage of 128 values) is read from before it, and not used.
 template <int kRows>
 struct MxSource {
-  static constexpr int kCodes = kRows / 32, kScales = (kRows + 127) / 128;
+  static constexpr int kCodes = kRows / 32, kScales = (kRows + 255) / 256;
   __amdgpu_buffer_rsrc_t codes, scales;
-  uint32_t at[kCodes], sat[kScales];
+  uint32_t at[kCodes], sat[kScales], steps;
 
   template <typename F>
-  __device__ __forceinline__ MxSource(const uint8_t *c, const uint8_t *s, uint64_t rows, uint32_t steps, F row_of)
-      : codes(mx_buffer(c, rows * steps * 64)), scales(mx_buffer(s, rows * steps * 4)) {
+  __device__ __forceinline__ MxSource(const uint8_t *c, const uint8_t *s, uint64_t rows, uint32_t n, F row_of)
+      : codes(mx_buffer(c, rows * n * 64)), scales(mx_buffer(s, rows * n * 4)), steps(n) {
     const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
 #pragma unroll
-    for (int i = 0; i < kCodes; i++) at[i] = row_of((wave + 4 * i) * 8 + lane / 8) * steps * 64;
+    for (int i = 0; i < kCodes; i++) at[i] = row_of((wave + 4 * i) * 8 + lane / 8) * n * 64;
 #pragma unroll
-    for (int i = 0; i < kScales; i++) sat[i] = row_of(min((wave + 4 * i) * 32 + lane / 2, (uint32_t)kRows - 1)) * steps * 4;
+    for (int i = 0; i < kScales; i++) sat[i] = row_of(min((wave + 4 * i) * 64 + lane, (uint32_t)kRows - 1)) * n * 4;
   }
   // Stage k, from `rows` rows on.
-  __device__ __forceinline__ void load(uint32_t k, uint32_t steps, uint8_t *c, uint32_t *s, uint32_t rows = 0) const {
+  __device__ __forceinline__ void load(uint32_t k, uint8_t *c, uint32_t rows = 0) const {
     const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
-    const uint32_t col = min(k * 128 + ((lane % 8) ^ (lane / 8)) * 16, steps * 64 - 16) + rows * steps * 64;
-    const uint32_t scol = min(k * 8 + lane % 2 * 4, steps * 4 - 4) + rows * steps * 4;
+    const uint32_t piece = (lane % 8) ^ (wave % 2 * 4 + lane / 16);
+    const uint32_t col = min(k * 128 + piece * 16, steps * 64 - 16) + rows * steps * 64;
 #pragma unroll
     for (int i = 0; i < kCodes; i++) lds_dma16(codes, at[i] + col, c + (wave + 4 * i) * 1024);
+  }
+  // The scales of stages k and k + 1 (k even): pitch(k, steps) words a row.
+  __device__ __forceinline__ void load_scales(uint32_t k, uint32_t *s, uint32_t rows = 0) const {
+    const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), from = rows * steps * 4 + k * 8, left = steps - 2 * k;
 #pragma unroll
-    for (int i = 0; i < kScales; i++)
-      if (kRows % 128 == 0 || (wave + 4 * i) * 32 < kRows) lds_dma4(scales, sat[i] + scol, s + (wave + 4 * i) * 64);
+    for (int i = 0; i < kScales; i++) {
+      if (kRows % 256 != 0 && (wave + 4 * i) * 64 >= kRows) continue;
+      uint32_t *to = s + (wave + 4 * i) * 256;
+      const auto word = [&](uint32_t row, uint32_t w, uint32_t *to) {  // (row's address is in that lane)
+        lds_dma4(scales, (uint32_t)__shfl((int)sat[i], (int)row, 64) + from + 4 * w, to);
+      };
+      if (left >= 4) {
+        if (kRows >= 64 || lane < kRows) lds_dma16(scales, sat[i] + from, to);
+      } else if (left == 3) {
+#pragma unroll
+        for (uint32_t j = 0; j < (kRows < 64 ? kRows : 64) / 16; j++) word(16 * j + lane / 4, min(lane % 4, 2u), to + j * 64);
+      } else if (left == 2) {
+        to = s + (wave + 4 * i) * 128;
+#pragma unroll
+        for (uint32_t j = 0; j < (kRows < 64 ? kRows : 64) / 32; j++) word(32 * j + lane / 2, lane % 2, to + j * 64);
+      } else {
+        to = s + (wave + 4 * i) * 64;
+        if (kRows >= 64 || lane < kRows) lds_dma4(scales, sat[i] + from, to);
+      }
+    }
   }
 };
+// The words a row of a pair of stages' scales: four, or as many as the row has left (three: four).
+__device__ __forceinline__ uint32_t mx_pitch(uint32_t k, uint32_t steps) {
+  const uint32_t left = steps - 2 * k;
+  return left < 3 ? left : 4;
+}
 
 // A work-group's four waves on a tile of BM rows of x and BN rows of w: WM of them along x's rows, 4 / WM along w's, each on
 // TM runs of 32 rows of x and TN runs of 32 rows of w. kApart: a wave's runs of w lie 32 times the waves apart (gate's rows
@@ -80,9 +113,11 @@ template <int TM, int TN, int WM = 2, bool kApart = false, bool kAcross = false>
 struct MxTile {
   static constexpr int WN = 4 / WM, BM = 32 * WM * TM, BN = 32 * WN * TN;
   typedef MxStage<BM, BN> Stage;
+  typedef MxScales<BM, BN> Scales;
   mx_f16 acc[TN][TM];
   mx_i4 a[2][TN], b[2][TM];
-  uint32_t sx[2][TM][2], sw[2][TN][2];
+  uint32_t sx[TM][4], sw[TN][4];        // the pair's scales, this lane's block of each 128 in the lowest byte
+  uint32_t next_sx[TM][4], next_sw[TN][4];  // the next pair's words
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -96,24 +131,36 @@ struct MxTile {
   static __device__ __forceinline__ uint32_t w_row() { return mx_wave() / WM * 32 * (kApart ? 1 : TN); }
   static constexpr uint32_t kStep = kApart ? 32 * WN : 32;  // between a wave's runs of w
 
-  template <int kParity>
-  __device__ __forceinline__ void read_scales(const Stage &s) {
-    const uint32_t lane = threadIdx.x & 63, q = lane / 32, r = lane % 32;
+  // The next pair's scales, their words `pitch` a row; then they are the pair's.
+  __device__ __forceinline__ void read_scales(const Scales &s, uint32_t pitch) {
+    const uint32_t r = threadIdx.x & 31;
+    const auto row = [&](const uint32_t *from, uint32_t row, uint32_t (&to)[4]) {
+      if (pitch == 4) {
+        const uint4 v = *(const uint4 *)(from + row * 4);
+        to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+      } else {  // (one or two)
+        to[0] = from[row * pitch], to[1] = from[row * pitch + 1];
+      }
+    };
 #pragma unroll
-    for (int m = 0; m < TM; m++) {
-      const uint2 v = *(const uint2 *)(s.sx + (x_row() + r + 32 * m) * 2);
-      sx[kParity][m][0] = v.x >> (8 * q), sx[kParity][m][1] = v.y >> (8 * q);
-    }
+    for (int m = 0; m < TM; m++) row(s.x, x_row() + r + 32 * m, next_sx[m]);
 #pragma unroll
-    for (int n = 0; n < TN; n++) {
-      const uint2 v = *(const uint2 *)(s.sw + (w_row() + r + kStep * n) * 2);
-      sw[kParity][n][0] = v.x >> (8 * q), sw[kParity][n][1] = v.y >> (8 * q);
+    for (int n = 0; n < TN; n++) row(s.w, w_row() + r + kStep * n, next_sw[n]);
+  }
+  __device__ __forceinline__ void adopt_scales() {
+    const uint32_t q = (threadIdx.x & 63) / 32;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+#pragma unroll
+      for (int m = 0; m < TM; m++) sx[m][i] = next_sx[m][i] >> (8 * q);
+#pragma unroll
+      for (int n = 0; n < TN; n++) sw[n][i] = next_sw[n][i] >> (8 * q);
     }
   }
   template <int j>
   __device__ __forceinline__ void read(const Stage &s) {
     const uint32_t lane = threadIdx.x & 63, q = lane / 32, r = lane % 32;
-    const uint32_t at = ((2 * j + q) ^ (r % 8)) * 16;
+    const uint32_t at = ((2 * j + q) ^ (r / 2 % 8)) * 16;
 #pragma unroll
     for (int m = 0; m < TM; m++) b[j % 2][m] = *(const mx_i4 *)(s.x + (x_row() + r + 32 * m) * 128 + at);
 #pragma unroll
@@ -121,43 +168,73 @@ struct MxTile {
   }
   template <int kParity, int j>
   __device__ __forceinline__ void multiply() {
+    constexpr int w = 2 * kParity + j / 2;
     __builtin_amdgcn_sched_barrier(0);  // (the reads of the next step are issued first)
 #pragma unroll
     for (int n = 0; n < TN; n++)
 #pragma unroll
       for (int m = 0; m < TM; m++)
-        acc[n][m] = kAcross ? mx_mfma32<j % 2 * 2, j % 2 * 2>(b[j % 2][m], a[j % 2][n], acc[n][m], sx[kParity][m][j / 2], sw[kParity][n][j / 2])
-                            : mx_mfma32<j % 2 * 2, j % 2 * 2>(a[j % 2][n], b[j % 2][m], acc[n][m], sw[kParity][n][j / 2], sx[kParity][m][j / 2]);
+        acc[n][m] = kAcross ? mx_mfma32<j % 2 * 2, j % 2 * 2>(b[j % 2][m], a[j % 2][n], acc[n][m], sx[m][w], sw[n][w])
+                            : mx_mfma32<j % 2 * 2, j % 2 * 2>(a[j % 2][n], b[j % 2][m], acc[n][m], sw[n][w], sx[m][w]);
     __builtin_amdgcn_sched_barrier(0);
   }
-  // Stage `now`, of parity kParity; its step 0 is in registers. half: the row ends after its first two steps. After the
-  // barrier `now` is free (load() loads what comes after `next` into it) and `next` is whole; past the last stage its first
-  // step is read all the same, and not used. (The two halves are basic blocks of their own: 64 matrix instructions on all
-  // 256 accumulators in one are more than the compiler's register allocation holds without spills.)
+  // Stage `now`, of parity kParity; its step 0 is in registers. steps: of 128 that it has (2, 1 or 0). After the barrier
+  // `now` is free (load() loads what comes after `next` into it) and `next` is whole, as are, after the second of a pair,
+  // the next pair's scales. Past the last stage its first step is read all the same, and not used. The reads of the scales
+  // come before load(): after it they would wait for it. (The two halves are basic blocks of their own: 64 matrix
+  // instructions on all 256 accumulators in one are more than the compiler's register allocation holds without spills.)
   template <int kParity, typename Load>
-  __device__ __forceinline__ void stage(const Stage &now, const Stage &next, bool half, Load load) {
-    read<1>(now);
-    multiply<kParity, 0>();
-    read<2>(now);
-    multiply<kParity, 1>();
-    if (!half) {
+  __device__ __forceinline__ void stage(const Stage &now, const Stage &next, const Scales &scales, uint32_t pitch, uint32_t steps,
+                                        Load load) {
+    if (steps != 0) {
+      read<1>(now);
+      multiply<kParity, 0>();
+      read<2>(now);
+      multiply<kParity, 1>();
+    }
+    if (steps == 2) {
       read<3>(now);
       multiply<kParity, 2>();
       dma_barrier();
+      if (kParity == 1) read_scales(scales, pitch);
       load();
       read<0>(next);
-      read_scales<kParity ^ 1>(next);
       multiply<kParity, 3>();
     } else {
       dma_barrier();
+      if (kParity == 1) read_scales(scales, pitch);
       load();
       read<0>(next);
-      read_scales<kParity ^ 1>(next);
     }
+    if (kParity == 1) adopt_scales();
   }
-  __device__ __forceinline__ void start(const Stage &first) {
-    read<0>(first);
-    read_scales<0>(first);
+  // All stages 0 .. n - 1 of a product: load(stage, k) loads stage k's codes, load_scales(scales, k) stages k's and k + 1's
+  // scales (k even), pitch(k) words a row; steps(k): how many steps of 128 stage k has; done(k) after each.
+  template <typename Load, typename LoadScales, typename Pitch, typename Steps, typename Done>
+  __device__ __forceinline__ void run(Stage &s0, Stage &s1, Scales &scales, uint32_t n, Load load, LoadScales load_scales,
+                                      Pitch pitch, Steps steps, Done done) {
+    load(s0, 0);
+    load_scales(scales, 0);
+    if (n > 1) load(s1, 1);
+    dma_barrier();
+    read_scales(scales, pitch(0));
+    adopt_scales();
+    read<0>(s0);
+    dma_barrier();  // (every wave has its scales)
+    if (n > 2) load_scales(scales, 2);
+    for (uint32_t k = 0;; k += 2) {
+      stage<0>(s0, s1, scales, 4, steps(k), [&] {
+        if (k + 2 < n) load(s0, k + 2);
+        if (k != 0 && k + 2 < n) load_scales(scales, k + 2);
+      });
+      done(k);
+      if (k + 1 >= n) break;
+      stage<1>(s1, s0, scales, k + 2 < n ? pitch(k + 2) : 4, steps(k + 1), [&] {
+        if (k + 3 < n) load(s1, k + 3);
+      });
+      done(k + 1);
+      if (k + 2 >= n) break;
+    }
   }
 };
 

@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(256, TM *TN > 8 ? 1 : 2)
   typedef typename Elem<kType>::T T;
   __shared__ typename Tile::Stage s0;
   __shared__ typename Tile::Stage s1;
+  __shared__ typename Tile::Scales scales;
   const uint32_t tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN, stages = (steps + 1) / 2;
   const uint32_t parts = (stages + span - 1) / span, all = tm * tn * parts;
   const uint32_t per = (all + 7) / 8, id = blockIdx.x % 8 * per + blockIdx.x / 8;
@@ -114,26 +115,14 @@ __global__ void __launch_bounds__(256, TM *TN > 8 ? 1 : 2)
   const auto same = [](uint32_t r) { return r; };
   const MxSource<BM> sx(xc + (uint64_t)m0 * steps * 64, xs + (uint64_t)m0 * steps * 4, M - m0, steps, same);
   const MxSource<BN> sw(wc + (uint64_t)n0 * steps * 64, ws + (uint64_t)n0 * steps * 4, N - n0, steps, same);
-  const auto load = [&](typename Tile::Stage &s, uint32_t k) {
-    sx.load(k, steps, s.x, s.sx);
-    sw.load(k, steps, s.w, s.sw);
-  };
   Tile c;
   c.clear();
-  load(s0, k0);
-  if (k0 + 1 < k1) load(s1, k0 + 1);
-  dma_barrier();
-  c.start(s0);
-  for (uint32_t k = k0;; k += 2) {
-    c.template stage<0>(s0, s1, 2 * k + 1 >= steps, [&] {
-      if (k + 2 < k1) load(s0, k + 2);
-    });
-    if (k + 1 >= k1) break;
-    c.template stage<1>(s1, s0, 2 * k + 3 >= steps, [&] {
-      if (k + 3 < k1) load(s1, k + 3);
-    });
-    if (k + 2 >= k1) break;
-  }
+  c.run(
+      s0, s1, scales, k1 - k0,
+      [&](typename Tile::Stage &s, uint32_t k) { sx.load(k0 + k, s.x), sw.load(k0 + k, s.w); },
+      [&](typename Tile::Scales &s, uint32_t k) { sx.load_scales(k0 + k, s.x), sw.load_scales(k0 + k, s.w); },
+      [&](uint32_t k) { return mx_pitch(k0 + k, steps); }, [&](uint32_t k) { return min(steps - 2 * (k0 + k), 2u); },
+      [](uint32_t) {});
   __builtin_amdgcn_s_barrier();  // (the stages' LDS is used again)
   // Each wave's 32 rows at a time through its part of LDS, so that a row's neighbours are stored together.
   const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32, r = lane % 32;
