@@ -4,6 +4,8 @@
 #include "mx4.h"
 #include "ops.h"
 
+#include <type_traits>
+
 namespace c0ven {
 
 inline void op_mx4(const moe_mx4_matrix *m) {
@@ -14,6 +16,14 @@ inline void op_mx4(const moe_mx4_matrix *m) {
 inline void op_work(const void *work, uint64_t bytes, uint64_t needed) {
   op_require(bytes >= needed && (work || !needed), "the work buffer is smaller than the call's work bytes");
   op_require(op_aligned(work, 16), "the work buffer must be 16-byte aligned");
+}
+
+// f with the element type as a constant.
+template <typename F>
+void op_by_type(uint32_t type, F f) {
+  if (type == QT_F32) f(std::integral_constant<uint32_t, QT_F32>());
+  if (type == QT_F16) f(std::integral_constant<uint32_t, QT_F16>());
+  if (type == QT_BF16) f(std::integral_constant<uint32_t, QT_BF16>());
 }
 
 // x (m.rows rows) into m, on the current device.

@@ -236,45 +236,253 @@ __global__ void __launch_bounds__(256, TM == 1 && WM == 2 ? 3 : 2) mx4_down_tile
       });
 }
 
-// One wave 16 rows of an assignment's expert.
-__global__ void __launch_bounds__(64) mx4_gate_up(const uint8_t *xc, const uint8_t *xs, const uint8_t *gc,
-                                                  const uint8_t *gs, const uint8_t *uc, const uint8_t *us,
-                                                  const int32_t *ids, uint32_t E, uint32_t K, uint32_t H, uint32_t F,
-                                                  float limit, float *h) {
-  const uint32_t lane = threadIdx.x, q = lane / 16, nt = (F + 15) / 16, steps = mx_steps(H);
-  const uint32_t a = blockIdx.x / nt, f0 = blockIdx.x % nt * 16;
-  const uint32_t e = (uint32_t)ids[a];
-  if (e >= E) return;
-  const uint64_t wr = ((uint64_t)e * F + min(f0 + lane % 16, F - 1)) * steps, xr = (uint64_t)(a / K) * steps;
-  mx_f4 g = {0, 0, 0, 0}, u = g;
-  for (uint32_t k = 0; k < steps; k++) {
-    const mx_i4 x = *(const mx_i4 *)(xc + (xr + k) * 64 + q * 16);
-    const uint32_t sx = xs[(xr + k) * 4 + q];
-    g = mx_mfma16<0, 0>(*(const mx_i4 *)(gc + (wr + k) * 64 + q * 16), x, g, gs[(wr + k) * 4 + q], sx);
-    u = mx_mfma16<0, 0>(*(const mx_i4 *)(uc + (wr + k) * 64 + q * 16), x, u, us[(wr + k) * 4 + q], sx);
-  }
-  if (lane % 16 == 0)
-#pragma unroll
-    for (uint32_t i = 0; i < 4; i++)
-      if (f0 + 4 * q + i < F) h[(uint64_t)a * F + f0 + 4 * q + i] = mx_swiglu(g[i], u[i], limit);
+// ---- few assignments (at most kFew): no sorting, two launches. Bound by latency and by reading the experts' weights, which
+// go to LDS as whole rows (a matrix instruction's operand straight from memory is 16 rows of 64 bytes, a clock a lane; whole
+// rows are 4 lanes a clock): all that a work-group needs is on its way at once.
+
+constexpr uint32_t kFew = 160;
+
+// What lane l of 64 holds (flag) as the number of lanes below it that do.
+__device__ __forceinline__ uint32_t lanes_below(uint64_t ballot) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(ballot >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0u));
 }
 
-__global__ void __launch_bounds__(64) mx4_down(const uint8_t *hc, const uint8_t *hs, const uint8_t *dc,
-                                               const uint8_t *ds, const int32_t *ids, uint32_t E, uint32_t H, uint32_t F,
-                                               float *o, uint32_t pitch) {
-  const uint32_t lane = threadIdx.x, q = lane / 16, nt = (H + 15) / 16, steps = mx_steps(F);
-  const uint32_t a = blockIdx.x / nt, r0 = blockIdx.x % nt * 16;
-  const uint32_t e = (uint32_t)ids[a];
-  if (e >= E) return;
-  const uint64_t wr = ((uint64_t)e * H + min(r0 + lane % 16, H - 1)) * steps, xr = (uint64_t)a * steps;
-  mx_f4 c = {0, 0, 0, 0};
-  for (uint32_t k = 0; k < steps; k++)
-    c = mx_mfma16<0, 0>(*(const mx_i4 *)(dc + (wr + k) * 64 + q * 16), *(const mx_i4 *)(hc + (xr + k) * 64 + q * 16), c,
-                        ds[(wr + k) * 4 + q], hs[(xr + k) * 4 + q]);
-  if (lane % 16 == 0)
+// A work-group: an expert and 32 columns of h, for the tokens that use the expert, eight at a time: the assignment that is
+// the first with its expert does the work, the others' work-groups leave. Quantises x itself (while the weights come) and
+// writes the assignments' rows of h in MX4. Four waves share the k axis, kSteps steps of 128 at a time (all of n_embd, where
+// it is not longer); the sums are joined in LDS.
+template <uint32_t kX, int kSteps>
+__global__ void __launch_bounds__(256) mx4_gate_up_few(MxExperts p, const typename Elem<kX>::T *x, uint64_t stride,
+                                                       const int32_t *ids, uint32_t A, uint8_t *hc, uint8_t *hs) {
+  constexpr uint32_t kTok = 8, kPitch = kSteps * 64, kXPitch = kSteps * 64 + 16;
+  __shared__ __align__(16) uint8_t wc[64 * kPitch];     // gate's 32 rows, up's; a row's 16-byte pieces exchanged by r % 16
+  __shared__ __align__(16) uint32_t wsc[64 * kSteps];   // their scales, a word a step
+  constexpr uint32_t kXBytes = kTok * kXPitch + kTok * kSteps * 4, kSumBytes = 4 * 64 * kTok * 4;
+  __shared__ __align__(16) uint8_t shared[kXBytes > kSumBytes ? kXBytes : kSumBytes];  // x's rows, then the waves' sums
+  __shared__ float h[kTok][33];
+  __shared__ uint16_t member[kFew];
+  __shared__ uint32_t counts[4];
+  uint8_t *xc = shared;
+  uint32_t *xsc = (uint32_t *)(shared + kTok * kXPitch);
+  float *sums = (float *)shared;  // [wave][row][token]
+  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 16, r = lane % 16;
+  const uint32_t steps = mx_steps(p.H), hsteps = mx_steps(p.F), blocks = hsteps * 4;
+  const uint32_t first = blockIdx.x / blocks, f0 = blockIdx.x % blocks * 32;
+  const uint32_t e = (uint32_t)ids[first];
+  if (e >= p.E) return;
+  const bool mine = threadIdx.x < A && (uint32_t)ids[threadIdx.x] == e;
+  const uint64_t row = (uint64_t)e * p.F + f0, rest = (uint64_t)p.E * p.F - min(row, (uint64_t)p.E * p.F);
+  const __amdgpu_buffer_rsrc_t g = mx_buffer(p.gc + row * steps * 64, rest * steps * 64);
+  const __amdgpu_buffer_rsrc_t u = mx_buffer(p.uc + row * steps * 64, rest * steps * 64);
+  const __amdgpu_buffer_rsrc_t gs = mx_buffer(p.gs + row * steps * 4, rest * steps * 4);
+  const __amdgpu_buffer_rsrc_t us = mx_buffer(p.us + row * steps * 4, rest * steps * 4);
+  // The members, in order; an earlier one: its work-group has this expert.
+  const uint64_t ballot = __ballot(mine);
+  if (lane == 0) counts[wave] = (uint32_t)__popcll(ballot);
+  if (__syncthreads_or(mine && threadIdx.x < first)) return;
+  uint32_t n = 0, at = lanes_below(ballot);
+  for (uint32_t v = 0; v < 4; v++) {
+    if (v < wave) at += counts[v];
+    n += counts[v];
+  }
+  if (mine) member[at] = (uint16_t)threadIdx.x;
+  for (uint32_t m0 = 0; m0 < n; m0 += kTok) {
+    const uint32_t nm = min(n - m0, kTok);
+    mx_f4 acc[4];
 #pragma unroll
-    for (uint32_t i = 0; i < 4; i++)
-      if (r0 + 4 * q + i < H) o[(uint64_t)a * pitch + r0 + 4 * q + i] = c[i];
+    for (int i = 0; i < 4; i++) acc[i] = mx_f4{0, 0, 0, 0};
+    for (uint32_t s0 = 0; s0 < steps; s0 += kSteps) {
+      const uint32_t ns = min(steps - s0, (uint32_t)kSteps);
+      __syncthreads();  // (member; the LDS of the round before)
+      if (m0 == 0 || steps > kSteps) {
+        // A row a load (or two): wave w has 16 rows, of gate or of up.
+#pragma unroll 4
+        for (uint32_t i = 0; i < 16; i++) {
+          const uint32_t lr = wave * 16 + i, from = (lr % 32 * steps + s0) * 64;
+#pragma unroll
+          for (uint32_t j = 0; j < (kPitch + 1023) / 1024; j++) {
+            const uint32_t piece = j * 64 + lane;
+            if (piece < kPitch / 16 && piece < (ns + 3) / 4 * 16)
+              lds_dma16(wave < 2 ? g : u, from + min((piece ^ (lr % 16)) * 16, ns * 64 - 16), wc + lr * kPitch + j * 1024);
+          }
+        }
+        for (uint32_t i = wave % 2 * 64; i < 32 * ns; i += 128) {  // two waves gate's words, two up's
+          const uint32_t lr = (i + lane) / ns, word = (i + lane) - lr * ns;
+          if (i + lane < 32 * ns) lds_dma4(wave < 2 ? gs : us, (lr * steps + s0 + word) * 4, wsc + (wave < 2 ? 0 : 32 * ns) + i);
+        }
+      }
+      for (uint32_t i = threadIdx.x; i < nm * ns * 16; i += 256) {
+        const uint32_t xr = i / (ns * 16), gr = i - xr * (ns * 16);
+        float v[8];
+        load8<kX>(x + member[m0 + xr] / p.K * stride, (s0 * 16 + gr) * 8, p.H, v);
+        uint32_t s;
+        *(uint32_t *)(xc + xr * kXPitch + gr * 4) = mx_quantize8(v, s);
+        if (gr % 4 == 0) ((uint8_t *)xsc)[xr * kSteps * 4 + gr / 4] = (uint8_t)s;
+      }
+      dma_barrier();
+      const uint32_t xr = min(r, nm - 1);
+      for (uint32_t k = wave; k < ns; k += 4) {
+        const mx_i4 b = *(const mx_i4 *)(xc + xr * kXPitch + k * 64 + q * 16);
+        const uint32_t sb = xsc[xr * kSteps + k] >> (8 * q);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+          const mx_i4 a = *(const mx_i4 *)(wc + (16 * i + r) * kPitch + ((4 * k + q) ^ r) * 16);
+          acc[i] = mx_mfma16<0, 0>(a, b, acc[i], wsc[(16 * i + r) * ns + k] >> (8 * q), sb);
+        }
+      }
+    }
+    __syncthreads();  // (x's rows are read)
+    if (r < kTok)
+#pragma unroll
+      for (uint32_t i = 0; i < 4; i++)
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) sums[(wave * 64 + 16 * i + 4 * q + j) * kTok + r] = acc[i][j];
+    __syncthreads();
+    const uint32_t col = threadIdx.x % 32, t = threadIdx.x / 32;
+    float gv = 0.0f, uv = 0.0f;
+#pragma unroll
+    for (uint32_t v = 0; v < 4; v++) gv += sums[(v * 64 + col) * kTok + t], uv += sums[(v * 64 + 32 + col) * kTok + t];
+    h[t][col] = f0 + col < p.F ? mx_swiglu(gv, uv, p.limit) : 0.0f;
+    __syncthreads();
+    if (threadIdx.x < 4 * nm) {
+      const uint32_t m = threadIdx.x / 4, part = threadIdx.x % 4;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = h[m][8 * part + j];
+      uint32_t s;
+      const uint32_t c = mx_quantize8(v, s);
+      const uint64_t to = (uint64_t)member[m0 + m] * hsteps * 4 + f0 / 32;
+      *(uint32_t *)(hc + to * 16 + part * 4) = c;
+      if (part == 0) hs[to] = (uint8_t)s;
+    }
+  }
+}
+
+// A work-group: 16 rows of down for all assignments, and y's 16 columns. A wave takes every eighth of the experts that are
+// used (its assignments 16 at a time), four steps of 128 a load, two loads of its own on their way.
+constexpr uint32_t kFewHq = 56 * 1024;  // the assignments' rows of h in LDS
+
+template <uint32_t kType>
+__global__ void __launch_bounds__(512) mx4_down_few(MxExperts p, const uint8_t *hc, const uint8_t *hs, const int32_t *ids,
+                                                    const float *w, uint32_t ntok, typename Elem<kType>::T *y, uint64_t stride) {
+  struct Slot {
+    alignas(16) uint8_t c[16 * 256];  // 16 rows, their 16-byte pieces exchanged by the row
+    uint32_t s[16 * 4];
+  };
+  __shared__ Slot slot0[8];
+  __shared__ Slot slot1[8];
+  __shared__ __align__(16) uint8_t hq[kFewHq];
+  __shared__ __align__(16) float o[kFew * 16];
+  __shared__ uint32_t first[512];
+  __shared__ uint16_t id[kFew], used[kFew], member[8][kFew];
+  __shared__ uint32_t counts[8];
+  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 16, r = lane % 16, A = ntok * p.K;
+  const uint32_t steps = mx_steps(p.F), r0 = blockIdx.x * 16, pitch = steps * 64 + 16;
+  uint32_t *hsc = (uint32_t *)(hq + A * pitch);  // [assignment][step]
+  first[threadIdx.x] = ~0u;
+  uint32_t e = p.E;
+  if (threadIdx.x < A) {
+    e = min((uint32_t)ids[threadIdx.x], p.E);
+    id[threadIdx.x] = (uint16_t)e;
+  }
+  __syncthreads();
+  if (e < p.E) atomicMin(first + e, threadIdx.x);
+  __syncthreads();
+  const bool owner = e < p.E && first[e] == threadIdx.x;
+  const uint64_t ballot = __ballot(owner);
+  if (lane == 0) counts[wave] = (uint32_t)__popcll(ballot);
+  __syncthreads();
+  uint32_t n = 0, at = lanes_below(ballot);
+  for (uint32_t v = 0; v < 8; v++) {
+    if (v < wave) at += counts[v];
+    n += counts[v];
+  }
+  if (owner) used[at] = (uint16_t)threadIdx.x;
+  __syncthreads();
+  const uint32_t chunks = (steps + 3) / 4, units = wave < n ? ((n - 1 - wave) / 8 + 1) * chunks : 0;
+  const uint32_t dr = lane / 16;  // (a load's rows: 4 j + dr)
+  const auto load = [&](Slot &s, uint32_t unit) {
+    const uint32_t ex = (uint32_t)__builtin_amdgcn_readfirstlane(id[used[wave + unit / chunks * 8]]), k = unit % chunks * 4;
+    const uint32_t ns = min(steps - k, 4u);
+    const uint64_t row = (uint64_t)ex * p.H + r0, rest = (uint64_t)p.E * p.H - row;
+    const __amdgpu_buffer_rsrc_t c = mx_buffer(p.dc + row * steps * 64, rest * steps * 64);
+    const __amdgpu_buffer_rsrc_t sc = mx_buffer(p.ds + row * steps * 4, rest * steps * 4);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+      const uint32_t lr = 4 * j + dr;
+      lds_dma16(c, (lr * steps + k) * 64 + min(((lane % 16) ^ lr) * 16, ns * 64 - 16), s.c + j * 1024);
+    }
+    lds_dma4(sc, (lane / 4 * steps + k + min(lane % 4, ns - 1)) * 4, s.s);
+  };
+  if (units > 0) load(slot0[wave], 0);
+  if (units > 1) load(slot1[wave], 1);
+  for (uint32_t i = threadIdx.x; i < A * steps * 4; i += 512) {
+    const uint32_t a = i / (steps * 4), piece = i - a * (steps * 4);
+    *(uint4 *)(hq + a * pitch + piece * 16) = ((const uint4 *)hc)[i];
+  }
+  for (uint32_t i = threadIdx.x; i < A * steps; i += 512) hsc[i] = ((const uint32_t *)hs)[i];
+  __syncthreads();
+  uint32_t nm = 0;
+  const auto use = [&](const Slot &s, uint32_t unit, bool more) {
+    // This unit's load has arrived; the next one's five may be outstanding.
+    asm volatile("" ::: "memory");
+    if (more)
+      __builtin_amdgcn_s_waitcnt(0x0f75);
+    else
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
+    const uint32_t k = unit % chunks * 4, ns = min(steps - k, 4u);
+    if (k == 0) {  // the expert's assignments
+      const uint32_t ex = id[used[wave + unit / chunks * 8]];
+      nm = 0;
+      for (uint32_t a0 = 0; a0 < A; a0 += 64) {
+        const bool is = a0 + lane < A && id[a0 + lane] == ex;
+        const uint64_t bal = __ballot(is);
+        if (is) member[wave][nm + lanes_below(bal)] = (uint16_t)(a0 + lane);
+        nm += (uint32_t)__popcll(bal);
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      __builtin_amdgcn_wave_barrier();
+    }
+    mx_i4 a[4];
+    uint32_t sa[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+      a[j] = *(const mx_i4 *)(s.c + r * 256 + ((4 * j + q) ^ r) * 16);
+      sa[j] = s.s[r * 4 + j] >> (8 * q);
+    }
+    for (uint32_t m0 = 0; m0 < nm; m0 += 16) {
+      const uint32_t as = member[wave][min(m0 + r, nm - 1)];
+      mx_f4 c = {0, 0, 0, 0};
+      float4 *to = (float4 *)(o + as * 16 + 4 * q);
+      if (k != 0) {
+        const float4 v = *to;
+        c = mx_f4{v.x, v.y, v.z, v.w};
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) {
+        if (j >= ns) break;
+        const mx_i4 b = *(const mx_i4 *)(hq + as * pitch + (k + j) * 64 + q * 16);
+        c = mx_mfma16<0, 0>(a[j], b, c, sa[j], hsc[as * steps + k + j] >> (8 * q));
+      }
+      if (m0 + r < nm) *to = make_float4(c[0], c[1], c[2], c[3]);
+    }
+  };
+  for (uint32_t i = 0; i < units; i += 2) {
+    use(slot0[wave], i, i + 1 < units);
+    if (i + 2 < units) load(slot0[wave], i + 2);
+    if (i + 1 >= units) break;
+    use(slot1[wave], i + 1, i + 2 < units);
+    if (i + 3 < units) load(slot1[wave], i + 3);
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < ntok * 16; i += 512) {
+    const uint32_t t = i / 16, c = i % 16;
+    float s = 0.0f;
+    for (uint32_t k = 0; k < p.K; k++)
+      if (id[t * p.K + k] < p.E) s += w[t * p.K + k] * o[(t * p.K + k) * 16 + c];
+    if (r0 + c < p.H) y[(uint64_t)t * stride + r0 + c] = (typename Elem<kType>::T)s;
+  }
 }
 
 // y's columns c0 .. c0 + cols (a multiple of 4 wide; H ends them) from the assignments' sums, `cols` apart, each token's in
@@ -338,17 +546,17 @@ void check_experts(const moe_mx4_experts *e, uint32_t ntok) {
   op_require(op_float(e->x_type) && op_float(e->y_type), "the element type must be QT_F32, QT_F16 or QT_BF16");
 }
 
-// How a call runs: assignments at most kFew: without sorting them.
-constexpr uint32_t kFew = 256;
+// How a call runs: at most kFew assignments whose rows of h fit LDS without sorting them.
 constexpr uint64_t kChunkBytes = 96 << 20;
 
 struct Plan {
   uint32_t A, rows, slices, pitch, chunk, max_tiles;
   bool few;
-  uint64_t xc, xs, h, hc, hs, o, counts, order, tiles, n_tiles, bytes;  // the work buffer's parts
+  uint64_t xc, xs, hc, hs, o, counts, order, tiles, n_tiles, bytes;  // the work buffer's parts
 
   Plan(const moe_mx4_experts &e, uint32_t T) {
-    A = T * e.n_used, few = A <= kFew;
+    A = T * e.n_used;
+    few = A <= kFew && A * (mx_steps(e.n_ff) * 68 + 16) <= kFewHq;
     // Tiles of 32, 64 or 128 positions: the more an expert has on average, the fewer times its weights are read.
     const uint32_t mean = A / e.n_expert;
     rows = mean < 24 ? 32 : mean < 96 ? 64 : 128;
@@ -356,7 +564,7 @@ struct Plan {
     pitch = (e.n_embd + 255) / 256 * 256;
     // The sums of all assignments at once, or of a part of the columns at a time that the last-level cache (256 MB) keeps
     // until they are added.
-    chunk = few ? pitch : std::min<uint64_t>(pitch, std::max<uint64_t>(256, kChunkBytes / (4ull * A) / 256 * 256));
+    chunk = std::min<uint64_t>(pitch, std::max<uint64_t>(256, kChunkBytes / (4ull * A) / 256 * 256));
     max_tiles = std::min(A, e.n_expert + A / rows);
     uint64_t at = 0;
     const auto part = [&](uint64_t n) {
@@ -364,12 +572,11 @@ struct Plan {
       at += (n + 255) / 256 * 256;
       return was;
     };
-    xc = part(moe_mx4_code_bytes(T, e.n_embd)), xs = part(moe_mx4_scale_bytes(T, e.n_embd));
-    h = part(few ? (uint64_t)A * e.n_ff * 4 : 0);
+    xc = part(few ? 0 : moe_mx4_code_bytes(T, e.n_embd)), xs = part(few ? 0 : moe_mx4_scale_bytes(T, e.n_embd));
     hc = part(moe_mx4_code_bytes(A, e.n_ff)), hs = part(moe_mx4_scale_bytes(A, e.n_ff));
-    o = part((uint64_t)A * chunk * 4);
+    o = part(few ? 0 : (uint64_t)A * chunk * 4);
     counts = part(few ? 0 : (uint64_t)slices * e.n_expert * 4), order = part(few ? 0 : (uint64_t)A * 4);
-    tiles = part(few ? 0 : (uint64_t)max_tiles * sizeof(MoeTile)), n_tiles = part(4);
+    tiles = part(few ? 0 : (uint64_t)max_tiles * sizeof(MoeTile)), n_tiles = part(few ? 0 : 4);
     bytes = at;
   }
 };
@@ -401,12 +608,29 @@ MOE_API moe_status moe_mx4_experts_async(const moe_mx4_experts *e, const void *x
     if (!ntok) return;
     OnDevice on(e->device);
     uint8_t *b = (uint8_t *)work;
-    mx4_quantize_launch(e->x_type, x, x_stride, moe_mx4_matrix{b + at.xc, b + at.xs, ntok, H}, stream);
     const MxExperts p{e->gate.codes, e->gate.scales, e->up.codes, e->up.scales, e->down.codes, e->down.scales, E, K, H, F,
                       e->swiglu_limit};
     const uint8_t *xc = b + at.xc, *xs = b + at.xs;
     uint8_t *hc = b + at.hc, *hs = b + at.hs;
     float *o = (float *)(b + at.o);
+    if (at.few) {
+      op_by_type(e->x_type, [&](auto t) {
+        constexpr uint32_t kX = decltype(t)::value;
+        const auto run = [&](auto kernel) {
+          op_launch(kernel, (uint64_t)A * mx_steps(F) * 4, 256, stream, p, (const typename Elem<kX>::T *)x, x_stride, ids, A, hc, hs);
+        };
+        if (mx_steps(H) <= 16)
+          run(mx4_gate_up_few<kX, 16>);
+        else
+          run(mx4_gate_up_few<kX, 24>);
+      });
+      op_by_type(e->y_type, [&](auto t) {
+        constexpr uint32_t kY = decltype(t)::value;
+        op_launch(mx4_down_few<kY>, (H + 15) / 16, 512, stream, p, (const uint8_t *)hc, (const uint8_t *)hs, ids, w, ntok,
+                  (typename Elem<kY>::T *)y, y_stride);
+      });
+      return;
+    }
     const auto combine = [&](uint32_t c0, uint32_t cols) {
       const uint64_t n = ((uint64_t)ntok * (cols / 4) + 255) / 256;
       const auto run = [&](auto kernel, auto *to) {
@@ -416,14 +640,7 @@ MOE_API moe_status moe_mx4_experts_async(const moe_mx4_experts *e, const void *x
       if (e->y_type == QT_F16) run(mx4_combine<QT_F16>, (_Float16 *)y);
       if (e->y_type == QT_BF16) run(mx4_combine<QT_BF16>, (__bf16 *)y);
     };
-    if (at.few) {
-      op_launch(mx4_gate_up, (uint64_t)A * ((F + 15) / 16), 64, stream, xc, xs, p.gc, p.gs, p.uc, p.us, ids, E, K, H, F,
-                e->swiglu_limit, (float *)(b + at.h));
-      mx4_quantize_launch(QT_F32, b + at.h, F, moe_mx4_matrix{hc, hs, A, F}, stream);
-      op_launch(mx4_down, (uint64_t)A * ((H + 15) / 16), 64, stream, (const uint8_t *)hc, (const uint8_t *)hs, p.dc, p.ds,
-                ids, E, H, F, o, at.pitch);
-      return combine(0, at.pitch);
-    }
+    mx4_quantize_launch(e->x_type, x, x_stride, moe_mx4_matrix{b + at.xc, b + at.xs, ntok, H}, stream);
     uint32_t *counts = (uint32_t *)(b + at.counts), *order = (uint32_t *)(b + at.order), *nt = (uint32_t *)(b + at.n_tiles);
     MoeTile *tiles = (MoeTile *)(b + at.tiles);
     if (at.slices > 1) op_launch(mx4_count, at.slices, 1024, stream, ids, A, E, counts);

@@ -196,18 +196,11 @@ struct Plan {
   uint64_t bytes(uint32_t M, uint32_t N) const { return parts > 1 ? (uint64_t)parts * M * N * 4 : 0; }
 };
 
-template <typename F>
-void by_type(uint32_t type, F f) {
-  if (type == QT_F32) f(std::integral_constant<uint32_t, QT_F32>());
-  if (type == QT_F16) f(std::integral_constant<uint32_t, QT_F16>());
-  if (type == QT_BF16) f(std::integral_constant<uint32_t, QT_BF16>());
-}
-
 template <uint32_t kX>
 void launch_few(const void *x, uint64_t x_stride, const uint8_t *xc, const uint8_t *xs, uint32_t M, const moe_mx4_matrix *w,
                 uint32_t y_type, void *y, uint64_t stride, void *stream) {
   const uint32_t N = w->rows, blocks = (N + 15) / 16;
-  by_type(y_type, [&](auto t) {
+  op_by_type(y_type, [&](auto t) {
     constexpr uint32_t kType = decltype(t)::value;
     const auto run = [&](auto kernel, uint32_t waves) {
       op_launch(kernel, blocks, 64 * waves, stream, x, x_stride, xc, xs, (const uint8_t *)w->codes,
@@ -237,9 +230,9 @@ void launch_matmul(const uint8_t *xc, const uint8_t *xs, uint32_t M, const moe_m
     if (p.tile == 2) run(mx4_gemm<kType, 2, 2>);
     if (p.tile == 1) run(mx4_gemm<kType, 1, 1>);
   };
-  if (p.parts == 1) return by_type(y_type, [&](auto t) { tiles(t, y, stride); });
+  if (p.parts == 1) return op_by_type(y_type, [&](auto t) { tiles(t, y, stride); });
   tiles(std::integral_constant<uint32_t, QT_F32>(), work, N);
-  by_type(y_type, [&](auto t) {
+  op_by_type(y_type, [&](auto t) {
     constexpr uint32_t kType = decltype(t)::value;
     op_launch(mx4_join<kType>, ((uint64_t)M * N + 255) / 256, 256, stream, (const float *)work, p.parts, M, N,
               (typename Elem<kType>::T *)y, stride);
@@ -296,7 +289,7 @@ MOE_API moe_status moe_mx4_linear_async(int32_t device, uint32_t x_type, const v
     if (!ntok || !w->rows) return;
     OnDevice on(device);
     if (quantises_itself(ntok, w->cols))
-      return by_type(x_type, [&](auto t) {
+      return op_by_type(x_type, [&](auto t) {
         launch_few<decltype(t)::value>(x, x_stride, nullptr, nullptr, ntok, w, y_type, y, y_stride, stream);
       });
     uint8_t *xc = (uint8_t *)work, *xs = xc + moe_mx4_code_bytes(ntok, w->cols);
