@@ -119,7 +119,7 @@ inline uint64_t item_blocks(uint64_t all, uint64_t parts) {
 
 // An item: a tile and 32 WN columns of h (their rows of gate and of up). Writes the places' rows of h in MX4.
 template <int TM, int WM>
-__global__ void __launch_bounds__(256, TM == 1 && WM == 2 ? 3 : 2) mx4_gate_up_tiles(MxExperts p, const uint8_t *xc, const uint8_t *xs, uint32_t ntok,
+__global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint8_t *xc, const uint8_t *xs, uint32_t ntok,
                                                          const uint32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
                                                          uint8_t *hc, uint8_t *hs) {
   typedef MxTile<TM, 2, WM, true> Tile;
@@ -137,14 +137,13 @@ __global__ void __launch_bounds__(256, TM == 1 && WM == 2 ? 3 : 2) mx4_gate_up_t
   const MxSource<kCols> g(p.gc + row * steps * 64, p.gs + row * steps * 4, rest, steps, same);
   const MxSource<kCols> u(p.uc + row * steps * 64, p.us + row * steps * 4, rest, steps, same);
   Tile c;
-  c.clear();
   c.run(
       s0, s1, scales, stages,
       [&](typename Tile::Stage &s, uint32_t k) { g.load(k, s.w), u.load(k, s.w + kCols * 128), x.load(k, s.x); },
       [&](typename Tile::Scales &s, uint32_t k) {
-        g.load_scales(k, s.w), u.load_scales(k, s.w + kCols * mx_pitch(k, steps)), x.load_scales(k, s.x);
+        g.load_scales(k, s.w), u.load_scales(k, s.w + kCols * 4), x.load_scales(k, s.x);
       },
-      [&](uint32_t k) { return mx_pitch(k, steps); }, [&](uint32_t k) { return min(steps - 2 * k, 2u); }, [](uint32_t) {});
+      [&](uint32_t k) { return min(steps - 2 * k, 2u); });
   // Lane l has 16 of its token's 32 columns of a wave (8 j + 4 (l / 32) + i), lane l ^ 32 the others.
   const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = f0 + Tile::w_row();
 #pragma unroll
@@ -176,15 +175,14 @@ __global__ void __launch_bounds__(256, TM == 1 && WM == 2 ? 3 : 2) mx4_gate_up_t
 // lane has a column of 16 rows, so that a store is of whole lines (two rows of 32 columns; with a row's four neighbours a
 // lane it was 32 rows of 32 bytes: 4096 tokens 172 us in all, now see below).
 template <int TM, int WM>
-__global__ void __launch_bounds__(256, TM == 1 && WM == 2 ? 3 : 2) mx4_down_tiles(MxExperts p, const uint8_t *hc, const uint8_t *hs, uint32_t A,
+__global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t *hc, const uint8_t *hs, uint32_t A,
                                                       const uint32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
                                                       uint32_t r0, uint32_t cols, float *o) {
   typedef MxTile<TM, 2, WM, true, true> Tile;
   __shared__ typename Tile::Stage s0;
   __shared__ typename Tile::Stage s1;
   __shared__ typename Tile::Scales scales;
-  __shared__ __align__(16) uint32_t place[Tile::BM];  // where a row of the tile goes, in bytes
-  constexpr uint32_t kNowhere = 0xf0000000u;           // (out of the buffer: a store there is dropped)
+  __shared__ __align__(16) uint32_t place[Tile::BM];  // where a row of the tile goes, in bytes (kNowhere: dropped)
   const uint32_t steps = mx_steps(p.F), total = cols / Tile::BN, nt = *n_tiles;
   const uint32_t blocks = min(max(nt * total / 2048, 1u), total), parts = (total + blocks - 1) / blocks;
   const uint32_t item = item_of(nt * parts, parts);
@@ -202,13 +200,14 @@ __global__ void __launch_bounds__(256, TM == 1 && WM == 2 ? 3 : 2) mx4_down_tile
   const __amdgpu_buffer_rsrc_t to = mx_buffer((const uint8_t *)o, (uint64_t)A * cols * 4);
   const uint32_t col = (b0 * Tile::BN + Tile::w_row() + lane % 32) * 4;
   Tile c;
-  c.clear();
   const auto store = [&](uint32_t n) {  // the sums of the n-th BN rows
+    uint32_t row = Tile::x_row() + 4 * q;
+    asm volatile("" : "+v"(row));  // (place is read here, for each n: kept in registers it is 16 of them)
 #pragma unroll
     for (int m = 0; m < TM; m++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const uint4 v = *(const uint4 *)(place + Tile::x_row() + 32 * m + 8 * j + 4 * q);
+        const uint4 v = *(const uint4 *)(place + row + 32 * m + 8 * j);
         const uint32_t at[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -217,23 +216,12 @@ __global__ void __launch_bounds__(256, TM == 1 && WM == 2 ? 3 : 2) mx4_down_tile
             __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(c.acc[f][m][4 * j + i]), to, at[i] + col,
                                                   (n * Tile::BN + f * Tile::kStep) * 4, 0);
       }
-    c.clear();
   };
-  c.run(
-      s0, s1, scales, nb * stages,
-      [&](typename Tile::Stage &s, uint32_t i) {
-        const uint32_t n = i / stages, k = i - n * stages;
-        if (2 * k < steps) w.load(k, s.w, n * Tile::BN), x.load(k, s.x);
-      },
-      [&](typename Tile::Scales &s, uint32_t i) {
-        const uint32_t n = i / stages, k = i - n * stages;
-        w.load_scales(k, s.w, n * Tile::BN), x.load_scales(k, s.x);
-      },
-      [&](uint32_t i) { return mx_pitch(i % stages, steps); },
-      [&](uint32_t i) { return min(steps - min(2 * (i % stages), steps), 2u); },
-      [&](uint32_t i) {
-        if (i % stages == stages - 1) store(i / stages);
-      });
+  c.run_blocks(
+      s0, s1, scales, nb, stages,
+      [&](typename Tile::Stage &s, uint32_t n, uint32_t k) { w.load(k, s.w, n * Tile::BN), x.load(k, s.x); },
+      [&](typename Tile::Scales &s, uint32_t n, uint32_t k) { w.load_scales(k, s.w, n * Tile::BN), x.load_scales(k, s.x); },
+      store);
 }
 
 // ---- few assignments (at most kFew): no sorting, two launches. Bound by latency and by reading the experts' weights, which

@@ -5,12 +5,13 @@
 
 namespace c0ven {
 
-// A buffer of n bytes from a wave-uniform address: reads past it give nothing and fault nowhere.
+// A buffer of n bytes from a wave-uniform address: reads past it (from kNowhere at the latest) give zeros and fault nowhere.
+constexpr uint32_t kNowhere = 0xf0000000u;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const uint8_t *p, uint64_t n) {
   const uint64_t b = (uint64_t)p;
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
-  const uint32_t size = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)min(n, (uint64_t)0xffffffffu));
+  const uint32_t size = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)min(n, (uint64_t)kNowhere));
   return __builtin_amdgcn_make_buffer_rsrc((void *)(((uint64_t)hi << 32) | lo), 0, size, 0x00020000u);
 }
 // 16 (or 4) bytes a lane from off into LDS at to + 16 (4) * lane (to wave-uniform).
@@ -46,63 +47,59 @@ struct MxScales {
   alignas(16) uint32_t w[BN * 4];
 };
 
-// kRows rows as the source of stages: row r of them is row_of(r) of those at codes and scales (`rows` there are), `steps`
-// of 128 values each. A wave loads every fourth kilobyte of a stage. Rows past the last are out of the buffer (their results
-// are not stored); what would lie past a row's end (a last stage of 128 values) is read from before it, and not used.
+// kRows rows as the source of stages: row r of them is row_of(r) of those at codes and scales (`rows` there are, of less than
+// kNowhere bytes as far as row_of reaches), `steps` of 128 values each. A wave loads every fourth kilobyte of a stage. Zeros
+// stand for rows past the last and for what is past a row's end (codes and scales of zero: products of zero).
 template <int kRows>
 struct MxSource {
   static constexpr int kCodes = kRows / 32, kScales = (kRows + 255) / 256;
-  __amdgpu_buffer_rsrc_t codes, scales;
+  const uint8_t *codes, *scales;
+  uint64_t rows;
   uint32_t at[kCodes], sat[kScales], steps;
 
   template <typename F>
   __device__ __forceinline__ MxSource(const uint8_t *c, const uint8_t *s, uint64_t rows, uint32_t n, F row_of)
-      : codes(mx_buffer(c, rows * n * 64)), scales(mx_buffer(s, rows * n * 4)), steps(n) {
+      : codes(c), scales(s), rows(rows), steps(n) {
     const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
 #pragma unroll
-    for (int i = 0; i < kCodes; i++) at[i] = row_of((wave + 4 * i) * 8 + lane / 8) * n * 64;
+    for (int i = 0; i < kCodes; i++)
+      at[i] = row_of((wave + 4 * i) * 8 + lane / 8) * n * 64 + ((lane % 8) ^ (wave % 2 * 4 + lane / 16)) * 16;
 #pragma unroll
     for (int i = 0; i < kScales; i++) sat[i] = row_of(min((wave + 4 * i) * 64 + lane, (uint32_t)kRows - 1)) * n * 4;
   }
-  // Stage k, from `rows` rows on.
-  __device__ __forceinline__ void load(uint32_t k, uint8_t *c, uint32_t rows = 0) const {
-    const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
-    const uint32_t piece = (lane % 8) ^ (wave % 2 * 4 + lane / 16);
-    const uint32_t col = min(k * 128 + piece * 16, steps * 64 - 16) + rows * steps * 64;
-#pragma unroll
-    for (int i = 0; i < kCodes; i++) lds_dma16(codes, at[i] + col, c + (wave + 4 * i) * 1024);
+  // The buffer from row r0's byte `from` on (in scalar registers, so that a lane's offsets are the same for every stage).
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t part(const uint8_t *p, uint64_t rows, uint32_t row, uint32_t r0,
+                                                                uint32_t from) {
+    const uint64_t off = (uint64_t)r0 * row + from, all = rows * row;
+    return mx_buffer(p + off, all > off ? all - off : 0);
   }
-  // The scales of stages k and k + 1 (k even): pitch(k, steps) words a row.
-  __device__ __forceinline__ void load_scales(uint32_t k, uint32_t *s, uint32_t rows = 0) const {
-    const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), from = rows * steps * 4 + k * 8, left = steps - 2 * k;
+  // Stage k, from row r0 on.
+  __device__ __forceinline__ void load(uint32_t k, uint8_t *c, uint32_t r0 = 0) const {
+    const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
+    const auto from = part(codes, rows, steps * 64, r0, k * 128);
+    const bool in = k * 128 + ((lane % 8) ^ (wave % 2 * 4 + lane / 16)) * 16 < steps * 64;
+#pragma unroll
+    for (int i = 0; i < kCodes; i++) lds_dma16(from, in ? at[i] : kNowhere, c + (wave + 4 * i) * 1024);
+  }
+  // The scales of stages k and k + 1 (k even).
+  __device__ __forceinline__ void load_scales(uint32_t k, uint32_t *s, uint32_t r0 = 0) const {
+    const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), left = steps - 2 * k;
+    const auto from = part(scales, rows, steps * 4, r0, k * 8);
 #pragma unroll
     for (int i = 0; i < kScales; i++) {
       if (kRows % 256 != 0 && (wave + 4 * i) * 64 >= kRows) continue;
       uint32_t *to = s + (wave + 4 * i) * 256;
-      const auto word = [&](uint32_t row, uint32_t w, uint32_t *to) {  // (row's address is in that lane)
-        lds_dma4(scales, (uint32_t)__shfl((int)sat[i], (int)row, 64) + from + 4 * w, to);
-      };
       if (left >= 4) {
-        if (kRows >= 64 || lane < kRows) lds_dma16(scales, sat[i] + from, to);
-      } else if (left == 3) {
-#pragma unroll
-        for (uint32_t j = 0; j < (kRows < 64 ? kRows : 64) / 16; j++) word(16 * j + lane / 4, min(lane % 4, 2u), to + j * 64);
-      } else if (left == 2) {
-        to = s + (wave + 4 * i) * 128;
-#pragma unroll
-        for (uint32_t j = 0; j < (kRows < 64 ? kRows : 64) / 32; j++) word(32 * j + lane / 2, lane % 2, to + j * 64);
-      } else {
-        to = s + (wave + 4 * i) * 64;
-        if (kRows >= 64 || lane < kRows) lds_dma4(scales, sat[i] + from, to);
+        if (kRows >= 64 || lane < kRows) lds_dma16(from, sat[i], to);
+      } else {  // word by word (a row's address is in its lane)
+        for (uint32_t j = 0; j < (kRows < 64 ? kRows : 64) / 16; j++) {
+          const uint32_t row = (uint32_t)__shfl((int)sat[i], (int)(16 * j + lane / 4), 64);
+          lds_dma4(from, lane % 4 < left ? row + lane % 4 * 4 : kNowhere, to + j * 64);
+        }
       }
     }
   }
 };
-// The words a row of a pair of stages' scales: four, or as many as the row has left (three: four).
-__device__ __forceinline__ uint32_t mx_pitch(uint32_t k, uint32_t steps) {
-  const uint32_t left = steps - 2 * k;
-  return left < 3 ? left : 4;
-}
 
 // A work-group's four waves on a tile of BM rows of x and BN rows of w: WM of them along x's rows, 4 / WM along w's, each on
 // TM runs of 32 rows of x and TN runs of 32 rows of w. kApart: a wave's runs of w lie 32 times the waves apart (gate's rows
@@ -112,6 +109,7 @@ __device__ __forceinline__ uint32_t mx_pitch(uint32_t k, uint32_t steps) {
 template <int TM, int TN, int WM = 2, bool kApart = false, bool kAcross = false>
 struct MxTile {
   static constexpr int WN = 4 / WM, BM = 32 * WM * TM, BN = 32 * WN * TN;
+  static constexpr bool kSkips = TM * TN >= 16;
   typedef MxStage<BM, BN> Stage;
   typedef MxScales<BM, BN> Scales;
   mx_f16 acc[TN][TM];
@@ -131,16 +129,12 @@ struct MxTile {
   static __device__ __forceinline__ uint32_t w_row() { return mx_wave() / WM * 32 * (kApart ? 1 : TN); }
   static constexpr uint32_t kStep = kApart ? 32 * WN : 32;  // between a wave's runs of w
 
-  // The next pair's scales, their words `pitch` a row; then they are the pair's.
-  __device__ __forceinline__ void read_scales(const Scales &s, uint32_t pitch) {
+  // The next pair's scales; adopted, they are the pair's.
+  __device__ __forceinline__ void read_scales(const Scales &s) {
     const uint32_t r = threadIdx.x & 31;
     const auto row = [&](const uint32_t *from, uint32_t row, uint32_t (&to)[4]) {
-      if (pitch == 4) {
-        const uint4 v = *(const uint4 *)(from + row * 4);
-        to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
-      } else {  // (one or two)
-        to[0] = from[row * pitch], to[1] = from[row * pitch + 1];
-      }
+      const uint4 v = *(const uint4 *)(from + row * 4);
+      to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
     };
 #pragma unroll
     for (int m = 0; m < TM; m++) row(s.x, x_row() + r + 32 * m, next_sx[m]);
@@ -178,62 +172,100 @@ struct MxTile {
                             : mx_mfma32<j % 2 * 2, j % 2 * 2>(a[j % 2][n], b[j % 2][m], acc[n][m], sw[n][w], sx[m][w]);
     __builtin_amdgcn_sched_barrier(0);
   }
-  // Stage `now`, of parity kParity; its step 0 is in registers. steps: of 128 that it has (2, 1 or 0). After the barrier
+  // The matrix instructions so far stay before what follows (the compiler moves them past the barrier and the loads' blocks
+  // to where their sums are used next, and keeps all their operands till then).
+  __device__ __forceinline__ void pin() {
+#pragma unroll
+    for (int n = 0; n < TN; n++)
+#pragma unroll
+      for (int m = 0; m < TM; m++) asm volatile("" : "+a"(acc[n][m]));
+  }
+  // Stage `now`, of parity kParity; its step 0 is in registers. steps: of 128 that it has (the rest zeros). After the barrier
   // `now` is free (load() loads what comes after `next` into it) and `next` is whole, as are, after the second of a pair,
   // the next pair's scales. Past the last stage its first step is read all the same, and not used. The reads of the scales
-  // come before load(): after it they would wait for it. (The two halves are basic blocks of their own: 64 matrix
-  // instructions on all 256 accumulators in one are more than the compiler's register allocation holds without spills.)
+  // come before load(): after it they would wait for it. (The largest tile's two halves are basic blocks of their own: 64
+  // matrix instructions on all 256 accumulators in one are more than the compiler's register allocation holds without
+  // spills; the others' in one: the branch made it copy their accumulators, 96 registers of 32.)
   template <int kParity, typename Load>
-  __device__ __forceinline__ void stage(const Stage &now, const Stage &next, const Scales &scales, uint32_t pitch, uint32_t steps,
-                                        Load load) {
-    if (steps != 0) {
+  __device__ __forceinline__ void stage(const Stage &now, const Stage &next, const Scales &scales, uint32_t steps, Load load) {
+    if (!kSkips || steps != 0) {
       read<1>(now);
       multiply<kParity, 0>();
       read<2>(now);
       multiply<kParity, 1>();
     }
-    if (steps == 2) {
+    if (!kSkips || steps == 2) {
       read<3>(now);
       multiply<kParity, 2>();
+      pin();
       dma_barrier();
-      if (kParity == 1) read_scales(scales, pitch);
+      if (kParity == 1) read_scales(scales);
       load();
       read<0>(next);
       multiply<kParity, 3>();
+      pin();
     } else {
       dma_barrier();
-      if (kParity == 1) read_scales(scales, pitch);
+      if (kParity == 1) read_scales(scales);
       load();
       read<0>(next);
     }
     if (kParity == 1) adopt_scales();
   }
-  // All stages 0 .. n - 1 of a product: load(stage, k) loads stage k's codes, load_scales(scales, k) stages k's and k + 1's
-  // scales (k even), pitch(k) words a row; steps(k): how many steps of 128 stage k has; done(k) after each.
-  template <typename Load, typename LoadScales, typename Pitch, typename Steps, typename Done>
-  __device__ __forceinline__ void run(Stage &s0, Stage &s1, Scales &scales, uint32_t n, Load load, LoadScales load_scales,
-                                      Pitch pitch, Steps steps, Done done) {
+  // The first stages of n into LDS, step 0 of the first and the first pair's scales into registers.
+  template <typename Load, typename LoadScales>
+  __device__ __forceinline__ void start(Stage &s0, Stage &s1, Scales &scales, uint32_t n, Load load, LoadScales load_scales) {
     load(s0, 0);
     load_scales(scales, 0);
     if (n > 1) load(s1, 1);
     dma_barrier();
-    read_scales(scales, pitch(0));
+    read_scales(scales);
     adopt_scales();
     read<0>(s0);
     dma_barrier();  // (every wave has its scales)
     if (n > 2) load_scales(scales, 2);
-    for (uint32_t k = 0;; k += 2) {
-      stage<0>(s0, s1, scales, 4, steps(k), [&] {
+  }
+  // All stages 0 .. n - 1 of a product: load(stage, k) loads stage k's codes, load_scales(scales, k) stages k's and k + 1's
+  // scales (k even); steps(k): how many steps of 128 stage k has.
+  template <typename Load, typename LoadScales, typename Steps>
+  __device__ __forceinline__ void run(Stage &s0, Stage &s1, Scales &scales, uint32_t n, Load load, LoadScales load_scales,
+                                      Steps steps) {
+    clear();
+    start(s0, s1, scales, n, load, load_scales);
+    uint32_t k = 0;
+    for (; k + (kSkips ? 0 : 1) < n; k += 2) {
+      stage<0>(s0, s1, scales, steps(k), [&] {
         if (k + 2 < n) load(s0, k + 2);
         if (k != 0 && k + 2 < n) load_scales(scales, k + 2);
       });
-      done(k);
-      if (k + 1 >= n) break;
-      stage<1>(s1, s0, scales, k + 2 < n ? pitch(k + 2) : 4, steps(k + 1), [&] {
+      stage<1>(s1, s0, scales, k + 1 < n ? steps(k + 1) : 0, [&] {
         if (k + 3 < n) load(s1, k + 3);
       });
-      done(k + 1);
-      if (k + 2 >= n) break;
+    }
+    if (!kSkips && k < n) stage<0>(s0, s1, scales, steps(k), [] {});
+  }
+  // The same for `blocks` products of n stages (an even number; the last one may be all zeros) one after the other, without
+  // a pause between them: load and load_scales go by block and stage, done(block) takes a block's sums.
+  template <typename Load, typename LoadScales, typename Done>
+  __device__ __forceinline__ void run_blocks(Stage &s0, Stage &s1, Scales &scales, uint32_t blocks, uint32_t n, Load load,
+                                             LoadScales load_scales, Done done) {
+    start(
+        s0, s1, scales, blocks * n, [&](Stage &s, uint32_t k) { load(s, 0, k); },
+        [&](Scales &s, uint32_t k) { n > 2 ? load_scales(s, 0, k) : load_scales(s, k / 2, 0); });
+    for (uint32_t block = 0; block < blocks; block++) {
+      clear();
+      for (uint32_t k = 0; k < n; k += 2) {
+        const bool last = k + 2 == n, more = !last || block + 1 < blocks;  // (the pair that comes next)
+        const uint32_t next = last ? block + 1 : block, nk = last ? 0 : k + 2;
+        stage<0>(s0, s1, scales, 2, [&] {
+          if (more) load(s0, next, nk);
+          if (more && (block != 0 || k != 0)) load_scales(scales, next, nk);
+        });
+        stage<1>(s1, s0, scales, 2, [&] {
+          if (more) load(s1, next, nk + 1);
+        });
+      }
+      done(block);
     }
   }
 };

@@ -116,13 +116,11 @@ __global__ void __launch_bounds__(256, TM *TN > 8 ? 1 : 2)
   const MxSource<BM> sx(xc + (uint64_t)m0 * steps * 64, xs + (uint64_t)m0 * steps * 4, M - m0, steps, same);
   const MxSource<BN> sw(wc + (uint64_t)n0 * steps * 64, ws + (uint64_t)n0 * steps * 4, N - n0, steps, same);
   Tile c;
-  c.clear();
   c.run(
       s0, s1, scales, k1 - k0,
       [&](typename Tile::Stage &s, uint32_t k) { sx.load(k0 + k, s.x), sw.load(k0 + k, s.w); },
       [&](typename Tile::Scales &s, uint32_t k) { sx.load_scales(k0 + k, s.x), sw.load_scales(k0 + k, s.w); },
-      [&](uint32_t k) { return mx_pitch(k0 + k, steps); }, [&](uint32_t k) { return min(steps - 2 * (k0 + k), 2u); },
-      [](uint32_t) {});
+      [&](uint32_t k) { return min(steps - 2 * (k0 + k), 2u); });
   __builtin_amdgcn_s_barrier();  // (the stages' LDS is used again)
   // Each wave's 32 rows at a time through its part of LDS, so that a row's neighbours are stored together.
   const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32, r = lane % 32;
