@@ -24,73 +24,74 @@ __device__ __forceinline__ float mx_swiglu(float g, float u, float limit) {
   return g / (1.0f + exp_f32(-g)) * u;
 }
 
-// ---- the assignments by expert
+// ---- the assignments by expert, and x in MX4
 
-constexpr uint32_t kSlice = 4096;  // ids a work-group sorts
+constexpr uint32_t kSlice = 4096;   // ids a work-group sorts
+constexpr uint32_t kGroups = 4096;  // groups of eight values a work-group quantises
 
-// How often each expert is in each slice.
-__global__ void __launch_bounds__(1024) mx4_count(const int32_t *ids, uint32_t A, uint32_t E, uint32_t *counts) {
-  __shared__ uint32_t n[512];
-  if (threadIdx.x < 512) n[threadIdx.x] = 0;
-  __syncthreads();
-  const uint32_t end = min(A, (blockIdx.x + 1) * kSlice);
-  for (uint32_t i = blockIdx.x * kSlice + threadIdx.x; i < end; i += 1024) {
-    const uint32_t e = (uint32_t)ids[i];
-    if (e < E) atomicAdd(n + e, 1u);
-  }
-  __syncthreads();
-  if (threadIdx.x < E) counts[blockIdx.x * E + threadIdx.x] = n[threadIdx.x];
-}
-
-// The inclusive sums of v over the work-group's 1024 threads in steps of 512 values: thread e's own (e < 512).
-__device__ __forceinline__ uint32_t scan512(uint32_t v, uint32_t *lds) {
+// The first `slices` work-groups: each takes every id (counting all of them costs a work-group less than a launch for the
+// counts does), then puts its slice's assignments to their places (order[place] = assignment; within an expert by slice);
+// the first one writes the tiles of at most `rows` places each. The others quantise x, of mx_steps(H) steps.
+template <uint32_t kX>
+__global__ void __launch_bounds__(1024) mx4_prepare(const int32_t *ids, uint32_t A, uint32_t E, uint32_t slices, uint32_t rows,
+                                                    uint32_t *order, MoeTile *tiles, uint32_t *n_tiles,
+                                                    const typename Elem<kX>::T *x, uint64_t stride, uint32_t ntok, uint32_t H,
+                                                    uint8_t *xc, uint8_t *xs) {
   const uint32_t e = threadIdx.x;
+  if (blockIdx.x >= slices) {
+    const uint32_t per = mx_steps(H) * 16, end = ntok * per, g0 = (blockIdx.x - slices) * kGroups + e;
+    float v[kGroups / 1024][8];
+#pragma unroll
+    for (uint32_t i = 0; i < kGroups / 1024; i++) {
+      const uint32_t g = min(g0 + i * 1024, end - 1);
+      load8<kX>(x + g / per * stride, g % per * 8, H, v[i]);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kGroups / 1024; i++) {
+      const uint32_t g = g0 + i * 1024;
+      uint32_t s;
+      const uint32_t c = mx_quantize8(v[i], s);
+      if (g >= end) break;
+      ((uint32_t *)xc)[g] = c;
+      if (g % 4 == 0) xs[g / 4] = (uint8_t)s;
+    }
+    return;
+  }
+  __shared__ uint32_t before[512], other[512];  // an expert's assignments: in the slices before this one, elsewhere
+  __shared__ uint32_t sums[2][8];
+  const uint32_t first = blockIdx.x * kSlice, end = min(A, first + kSlice);
+  if (e < 512) before[e] = other[e] = 0;
   __syncthreads();
-  if (e < 512) lds[e] = v;
-  for (uint32_t d = 1; d < 512; d *= 2) {
-    __syncthreads();
-    const uint32_t add = e < 512 && e >= d ? lds[e - d] : 0;
-    __syncthreads();
-    if (e < 512) lds[e] += add;
+  for (uint32_t i0 = e; i0 < A; i0 += 8 * 1024) {
+    uint32_t id[8];
+#pragma unroll
+    for (uint32_t j = 0; j < 8; j++) id[j] = i0 + j * 1024 < A ? (uint32_t)ids[i0 + j * 1024] : ~0u;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; j++)
+      if (id[j] < E) atomicAdd((i0 + j * 1024 < first ? before : other) + id[j], 1u);
   }
   __syncthreads();
-  return e < 512 ? lds[e] : 0;
-}
-
-// A slice's assignments to their places (order[place] = assignment; within an expert by slice), and, by the first
-// work-group, the tiles of at most `rows` places each. With one slice the counts are taken here.
-__global__ void __launch_bounds__(1024) mx4_place(const int32_t *ids, uint32_t A, uint32_t E, const uint32_t *counts,
-                                                  uint32_t rows, uint32_t *order, MoeTile *tiles, uint32_t *n_tiles) {
-  __shared__ uint32_t next[512];
-  __shared__ uint32_t lds[512];
-  const uint32_t e = threadIdx.x, first = blockIdx.x * kSlice, end = min(A, first + kSlice);
-  uint32_t all = 0, before = 0;  // expert e's assignments, those of the slices before this one
-  if (gridDim.x == 1) {
-    if (e < 512) next[e] = 0;
-    __syncthreads();
-    for (uint32_t i = e; i < end; i += 1024)
-      if ((uint32_t)ids[i] < E) atomicAdd(next + (uint32_t)ids[i], 1u);
-    __syncthreads();
-    all = e < E ? next[e] : 0;
-  } else if (e < E) {
-    for (uint32_t b = 0; b < gridDim.x; b++) {
-      const uint32_t n = counts[b * E + e];
-      all += n, before += b < blockIdx.x ? n : 0;
+  const uint32_t was = e < 512 ? before[e] : 0, all = e < 512 ? was + other[e] : 0, n = (all + rows - 1) / rows;
+  uint32_t place = all, tile = n;  // their sums up to this expert
+  for (uint32_t d = 1; d < 64; d *= 2) {
+    const uint32_t p = (uint32_t)__shfl_up((int)place, d, 64), t = (uint32_t)__shfl_up((int)tile, d, 64);
+    if (e % 64 >= d) place += p, tile += t;
+  }
+  if (e < 512 && e % 64 == 63) sums[0][e / 64] = place, sums[1][e / 64] = tile;
+  __syncthreads();
+  if (e < 512) {
+    for (uint32_t v = 0; v < e / 64; v++) place += sums[0][v], tile += sums[1][v];
+    before[e] = place - all + was;
+    if (blockIdx.x == 0) {
+      for (uint32_t j = 0; j < n; j++)
+        tiles[tile - n + j] = MoeTile{e, e, place - all + j * rows, min(rows, all - j * rows)};
+      if (e == 511) *n_tiles = tile;
     }
   }
-  const uint32_t start = scan512(all, lds) - all;
-  if (blockIdx.x == 0) {
-    const uint32_t n = (all + rows - 1) / rows, last = scan512(n, lds);
-    if (e < E)
-      for (uint32_t j = 0; j < n; j++) tiles[last - n + j] = MoeTile{e, e, start + j * rows, min(rows, all - j * rows)};
-    if (e == 511) *n_tiles = last;
-  }
-  __syncthreads();
-  if (e < 512) next[e] = start + before;
   __syncthreads();
   for (uint32_t i = first + e; i < end; i += 1024) {
     const uint32_t id = (uint32_t)ids[i];
-    if (id < E) order[atomicAdd(next + id, 1u)] = i;
+    if (id < E) order[atomicAdd(before + id, 1u)] = i;
   }
 }
 
@@ -538,9 +539,9 @@ void check_experts(const moe_mx4_experts *e, uint32_t ntok) {
 constexpr uint64_t kChunkBytes = 96 << 20;
 
 struct Plan {
-  uint32_t A, rows, slices, pitch, chunk, max_tiles;
+  uint32_t A, rows, pitch, chunk, max_tiles;
   bool few;
-  uint64_t xc, xs, hc, hs, o, counts, order, tiles, n_tiles, bytes;  // the work buffer's parts
+  uint64_t xc, xs, hc, hs, o, order, tiles, n_tiles, bytes;  // the work buffer's parts
 
   Plan(const moe_mx4_experts &e, uint32_t T) {
     A = T * e.n_used;
@@ -548,7 +549,6 @@ struct Plan {
     // Tiles of 32, 64 or 128 positions: the more an expert has on average, the fewer times its weights are read.
     const uint32_t mean = A / e.n_expert;
     rows = mean < 24 ? 32 : mean < 96 ? 64 : 128;
-    slices = (A + kSlice - 1) / kSlice;
     pitch = (e.n_embd + 255) / 256 * 256;
     // The sums of all assignments at once, or of a part of the columns at a time that the last-level cache (256 MB) keeps
     // until they are added.
@@ -563,7 +563,7 @@ struct Plan {
     xc = part(few ? 0 : moe_mx4_code_bytes(T, e.n_embd)), xs = part(few ? 0 : moe_mx4_scale_bytes(T, e.n_embd));
     hc = part(moe_mx4_code_bytes(A, e.n_ff)), hs = part(moe_mx4_scale_bytes(A, e.n_ff));
     o = part(few ? 0 : (uint64_t)A * chunk * 4);
-    counts = part(few ? 0 : (uint64_t)slices * e.n_expert * 4), order = part(few ? 0 : (uint64_t)A * 4);
+    order = part(few ? 0 : (uint64_t)A * 4);
     tiles = part(few ? 0 : (uint64_t)max_tiles * sizeof(MoeTile)), n_tiles = part(few ? 0 : 4);
     bytes = at;
   }
@@ -628,11 +628,14 @@ MOE_API moe_status moe_mx4_experts_async(const moe_mx4_experts *e, const void *x
       if (e->y_type == QT_F16) run(mx4_combine<QT_F16>, (_Float16 *)y);
       if (e->y_type == QT_BF16) run(mx4_combine<QT_BF16>, (__bf16 *)y);
     };
-    mx4_quantize_launch(e->x_type, x, x_stride, moe_mx4_matrix{b + at.xc, b + at.xs, ntok, H}, stream);
-    uint32_t *counts = (uint32_t *)(b + at.counts), *order = (uint32_t *)(b + at.order), *nt = (uint32_t *)(b + at.n_tiles);
+    uint32_t *order = (uint32_t *)(b + at.order), *nt = (uint32_t *)(b + at.n_tiles);
     MoeTile *tiles = (MoeTile *)(b + at.tiles);
-    if (at.slices > 1) op_launch(mx4_count, at.slices, 1024, stream, ids, A, E, counts);
-    op_launch(mx4_place, at.slices, 1024, stream, ids, A, E, (const uint32_t *)counts, at.rows, order, tiles, nt);
+    op_by_type(e->x_type, [&](auto t) {
+      constexpr uint32_t kX = decltype(t)::value;
+      const uint32_t slices = (A + kSlice - 1) / kSlice, groups = ntok * mx_steps(H) * 16;
+      op_launch(mx4_prepare<kX>, slices + (groups + kGroups - 1) / kGroups, 1024, stream, ids, A, E, slices, at.rows, order,
+                tiles, nt, (const typename Elem<kX>::T *)x, x_stride, ntok, H, b + at.xc, b + at.xs);
+    });
     const auto run = [&](auto gate_up, auto down, uint32_t bn) {
       op_launch(gate_up, item_blocks((uint64_t)at.max_tiles * (mx_steps(F) * 256 / bn), mx_steps(F) * 256 / bn), 256, stream, p, xc, xs, ntok,
                 (const uint32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, hc, hs);
