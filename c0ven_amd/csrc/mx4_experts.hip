@@ -143,8 +143,7 @@ __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint
       [&](typename Tile::Stage &s, uint32_t k) { g.load(k, s.w), u.load(k, s.w + kCols * 128), x.load(k, s.x); },
       [&](typename Tile::Scales &s, uint32_t k) {
         g.load_scales(k, s.w), u.load_scales(k, s.w + kCols * 4), x.load_scales(k, s.x);
-      },
-      [&](uint32_t k) { return min(steps - 2 * k, 2u); });
+      });
   // Lane l has 16 of its token's 32 columns of a wave (8 j + 4 (l / 32) + i), lane l ^ 32 the others.
   const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = f0 + Tile::w_row();
 #pragma unroll

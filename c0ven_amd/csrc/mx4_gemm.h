@@ -48,11 +48,11 @@ struct MxScales {
 };
 
 // kRows rows as the source of stages: row r of them is row_of(r) of those at codes and scales (`rows` there are, of less than
-// kNowhere bytes as far as row_of reaches), `steps` of 128 values each. A wave loads every fourth kilobyte of a stage. Zeros
+// kNowhere bytes as far as row_of reaches), `steps` of 128 values each. The waves load a kilobyte of a stage each in turn. Zeros
 // stand for rows past the last and for what is past a row's end (codes and scales of zero: products of zero).
-template <int kRows>
+template <int kRows, int kWaves = 4>
 struct MxSource {
-  static constexpr int kCodes = kRows / 32, kScales = (kRows + 255) / 256;
+  static constexpr int kCodes = kRows / 8 / kWaves, kScales = (kRows + 64 * kWaves - 1) / (64 * kWaves);
   const uint8_t *codes, *scales;
   uint64_t rows;
   uint32_t at[kCodes], sat[kScales], steps;
@@ -63,9 +63,9 @@ struct MxSource {
     const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
 #pragma unroll
     for (int i = 0; i < kCodes; i++)
-      at[i] = row_of((wave + 4 * i) * 8 + lane / 8) * n * 64 + ((lane % 8) ^ (wave % 2 * 4 + lane / 16)) * 16;
+      at[i] = row_of((wave + kWaves * i) * 8 + lane / 8) * n * 64 + ((lane % 8) ^ (wave % 2 * 4 + lane / 16)) * 16;
 #pragma unroll
-    for (int i = 0; i < kScales; i++) sat[i] = row_of(min((wave + 4 * i) * 64 + lane, (uint32_t)kRows - 1)) * n * 4;
+    for (int i = 0; i < kScales; i++) sat[i] = row_of(min((wave + kWaves * i) * 64 + lane, (uint32_t)kRows - 1)) * n * 4;
   }
   // The buffer from row r0's byte `from` on (in scalar registers, so that a lane's offsets are the same for every stage).
   static __device__ __forceinline__ __amdgpu_buffer_rsrc_t part(const uint8_t *p, uint64_t rows, uint32_t row, uint32_t r0,
@@ -79,7 +79,7 @@ struct MxSource {
     const auto from = part(codes, rows, steps * 64, r0, k * 128);
     const bool in = k * 128 + ((lane % 8) ^ (wave % 2 * 4 + lane / 16)) * 16 < steps * 64;
 #pragma unroll
-    for (int i = 0; i < kCodes; i++) lds_dma16(from, in ? at[i] : kNowhere, c + (wave + 4 * i) * 1024);
+    for (int i = 0; i < kCodes; i++) lds_dma16(from, in ? at[i] : kNowhere, c + (wave + kWaves * i) * 1024);
   }
   // The scales of stages k and k + 1 (k even).
   __device__ __forceinline__ void load_scales(uint32_t k, uint32_t *s, uint32_t r0 = 0) const {
@@ -87,8 +87,8 @@ struct MxSource {
     const auto from = part(scales, rows, steps * 4, r0, k * 8);
 #pragma unroll
     for (int i = 0; i < kScales; i++) {
-      if (kRows % 256 != 0 && (wave + 4 * i) * 64 >= kRows) continue;
-      uint32_t *to = s + (wave + 4 * i) * 256;
+      if (kRows % (64 * kWaves) != 0 && (wave + kWaves * i) * 64 >= kRows) continue;
+      uint32_t *to = s + (wave + kWaves * i) * 256;
       if (left >= 4) {
         if (kRows >= 64 || lane < kRows) lds_dma16(from, sat[i], to);
       } else {  // word by word (a row's address is in its lane)
@@ -101,15 +101,14 @@ struct MxSource {
   }
 };
 
-// A work-group's four waves on a tile of BM rows of x and BN rows of w: WM of them along x's rows, 4 / WM along w's, each on
+// A work-group's kWaves waves on a tile of BM rows of x and BN rows of w: WM of them along x's rows, WN along w's, each on
 // TM runs of 32 rows of x and TN runs of 32 rows of w. kApart: a wave's runs of w lie 32 times the waves apart (gate's rows
 // and up's), else they follow one another. kAcross: a lane's sums are one w row's with 16 of x's, instead of one x row's with 16
 // of w's. The operands are one step of k = 64 ahead of the matrix instructions, in
 // registers, across the stages.
-template <int TM, int TN, int WM = 2, bool kApart = false, bool kAcross = false>
+template <int TM, int TN, int WM = 2, bool kApart = false, bool kAcross = false, int kWaves = 4>
 struct MxTile {
-  static constexpr int WN = 4 / WM, BM = 32 * WM * TM, BN = 32 * WN * TN;
-  static constexpr bool kSkips = TM * TN >= 16;
+  static constexpr int WN = kWaves / WM, BM = 32 * WM * TM, BN = 32 * WN * TN;
   typedef MxStage<BM, BN> Stage;
   typedef MxScales<BM, BN> Scales;
   mx_f16 acc[TN][TM];
@@ -180,36 +179,25 @@ struct MxTile {
 #pragma unroll
       for (int m = 0; m < TM; m++) asm volatile("" : "+a"(acc[n][m]));
   }
-  // Stage `now`, of parity kParity; its step 0 is in registers. steps: of 128 that it has (the rest zeros). After the barrier
-  // `now` is free (load() loads what comes after `next` into it) and `next` is whole, as are, after the second of a pair,
-  // the next pair's scales. Past the last stage its first step is read all the same, and not used. The reads of the scales
-  // come before load(): after it they would wait for it. (The largest tile's two halves are basic blocks of their own: 64
-  // matrix instructions on all 256 accumulators in one are more than the compiler's register allocation holds without
-  // spills; the others' in one: the branch made it copy their accumulators, 96 registers of 32.)
+  // Stage `now`, of parity kParity; its step 0 is in registers. After the barrier `now` is free (load() loads what comes after
+  // `next` into it) and `next` is whole, as are, after the second of a pair, the next pair's scales. Past the last stage its
+  // first step is read all the same, and not used. The reads of the scales come before load(): after it they would wait for
+  // it.
   template <int kParity, typename Load>
-  __device__ __forceinline__ void stage(const Stage &now, const Stage &next, const Scales &scales, uint32_t steps, Load load) {
-    if (!kSkips || steps != 0) {
-      read<1>(now);
-      multiply<kParity, 0>();
-      read<2>(now);
-      multiply<kParity, 1>();
-    }
-    if (!kSkips || steps == 2) {
-      read<3>(now);
-      multiply<kParity, 2>();
-      pin();
-      dma_barrier();
-      if (kParity == 1) read_scales(scales);
-      load();
-      read<0>(next);
-      multiply<kParity, 3>();
-      pin();
-    } else {
-      dma_barrier();
-      if (kParity == 1) read_scales(scales);
-      load();
-      read<0>(next);
-    }
+  __device__ __forceinline__ void stage(const Stage &now, const Stage &next, const Scales &scales, Load load) {
+    read<1>(now);
+    multiply<kParity, 0>();
+    read<2>(now);
+    multiply<kParity, 1>();
+    read<3>(now);
+    multiply<kParity, 2>();
+    pin();
+    dma_barrier();
+    if (kParity == 1) read_scales(scales);
+    load();
+    read<0>(next);
+    multiply<kParity, 3>();
+    pin();
     if (kParity == 1) adopt_scales();
   }
   // The first stages of n into LDS, step 0 of the first and the first pair's scales into registers.
@@ -226,23 +214,22 @@ struct MxTile {
     if (n > 2) load_scales(scales, 2);
   }
   // All stages 0 .. n - 1 of a product: load(stage, k) loads stage k's codes, load_scales(scales, k) stages k's and k + 1's
-  // scales (k even); steps(k): how many steps of 128 stage k has.
-  template <typename Load, typename LoadScales, typename Steps>
-  __device__ __forceinline__ void run(Stage &s0, Stage &s1, Scales &scales, uint32_t n, Load load, LoadScales load_scales,
-                                      Steps steps) {
+  // scales (k even).
+  template <typename Load, typename LoadScales>
+  __device__ __forceinline__ void run(Stage &s0, Stage &s1, Scales &scales, uint32_t n, Load load, LoadScales load_scales) {
     clear();
     start(s0, s1, scales, n, load, load_scales);
     uint32_t k = 0;
-    for (; k + (kSkips ? 0 : 1) < n; k += 2) {
-      stage<0>(s0, s1, scales, steps(k), [&] {
+    for (; k + 1 < n; k += 2) {
+      stage<0>(s0, s1, scales, [&] {
         if (k + 2 < n) load(s0, k + 2);
         if (k != 0 && k + 2 < n) load_scales(scales, k + 2);
       });
-      stage<1>(s1, s0, scales, k + 1 < n ? steps(k + 1) : 0, [&] {
+      stage<1>(s1, s0, scales, [&] {
         if (k + 3 < n) load(s1, k + 3);
       });
     }
-    if (!kSkips && k < n) stage<0>(s0, s1, scales, steps(k), [] {});
+    if (k < n) stage<0>(s0, s1, scales, [] {});
   }
   // The same for `blocks` products of n stages (an even number; the last one may be all zeros) one after the other, without
   // a pause between them: load and load_scales go by block and stage, done(block) takes a block's sums.
@@ -257,11 +244,11 @@ struct MxTile {
       for (uint32_t k = 0; k < n; k += 2) {
         const bool last = k + 2 == n, more = !last || block + 1 < blocks;  // (the pair that comes next)
         const uint32_t next = last ? block + 1 : block, nk = last ? 0 : k + 2;
-        stage<0>(s0, s1, scales, 2, [&] {
+        stage<0>(s0, s1, scales, [&] {
           if (more) load(s0, next, nk);
           if (more && (block != 0 || k != 0)) load_scales(scales, next, nk);
         });
-        stage<1>(s1, s0, scales, 2, [&] {
+        stage<1>(s1, s0, scales, [&] {
           if (more) load(s1, next, nk + 1);
         });
       }

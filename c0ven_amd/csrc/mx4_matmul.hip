@@ -95,11 +95,11 @@ __global__ void __launch_bounds__(256) mx4_join(const float *sums, uint32_t part
 }
 
 // A tile of y a work-group, k split into parts of `span` stages (256 each); part p's sums go to y + p * part.
-template <uint32_t kType, int TM, int TN>
-__global__ void __launch_bounds__(256, TM *TN > 8 ? 1 : 2)
+template <uint32_t kType, int TM, int TN, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves, 2)
     mx4_gemm(const uint8_t *xc, const uint8_t *xs, const uint8_t *wc, const uint8_t *ws, uint32_t M, uint32_t N,
              uint32_t steps, uint32_t span, typename Elem<kType>::T *y, uint64_t stride, uint64_t part) {
-  typedef MxTile<TM, TN> Tile;
+  typedef MxTile<TM, TN, 2, false, false, kWaves> Tile;
   constexpr int BM = Tile::BM, BN = Tile::BN;
   typedef typename Elem<kType>::T T;
   __shared__ typename Tile::Stage s0;
@@ -113,21 +113,21 @@ __global__ void __launch_bounds__(256, TM *TN > 8 ? 1 : 2)
   const uint32_t m0 = (group * 8 + t % (8 * tn) % rows) * BM, n0 = t % (8 * tn) / rows * BN;
   const uint32_t k0 = p * span, k1 = min(k0 + span, stages);
   const auto same = [](uint32_t r) { return r; };
-  const MxSource<BM> sx(xc + (uint64_t)m0 * steps * 64, xs + (uint64_t)m0 * steps * 4, M - m0, steps, same);
-  const MxSource<BN> sw(wc + (uint64_t)n0 * steps * 64, ws + (uint64_t)n0 * steps * 4, N - n0, steps, same);
+  const MxSource<BM, kWaves> sx(xc + (uint64_t)m0 * steps * 64, xs + (uint64_t)m0 * steps * 4, M - m0, steps, same);
+  const MxSource<BN, kWaves> sw(wc + (uint64_t)n0 * steps * 64, ws + (uint64_t)n0 * steps * 4, N - n0, steps, same);
   Tile c;
   c.run(
       s0, s1, scales, k1 - k0,
       [&](typename Tile::Stage &s, uint32_t k) { sx.load(k0 + k, s.x), sw.load(k0 + k, s.w); },
-      [&](typename Tile::Scales &s, uint32_t k) { sx.load_scales(k0 + k, s.x), sw.load_scales(k0 + k, s.w); },
-      [&](uint32_t k) { return min(steps - 2 * (k0 + k), 2u); });
+      [&](typename Tile::Scales &s, uint32_t k) { sx.load_scales(k0 + k, s.x), sw.load_scales(k0 + k, s.w); });
   __builtin_amdgcn_s_barrier();  // (the stages' LDS is used again)
   // Each wave's 32 rows at a time through its part of LDS, so that a row's neighbours are stored together.
   const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32, r = lane % 32;
   constexpr uint32_t kWide = 32 * TN, kPitch = kWide + 4;
-  float *mine = (float *)(wave < 2 ? (uint8_t *)&s0 : (uint8_t *)&s1) + (wave & 1) * 32 * kPitch;
-  static_assert(2 * 32 * kPitch * 4 <= sizeof(s0), "two waves' rows in a stage");
-  const uint32_t wm = m0 + (wave & 1) * 32 * TM, wn = n0 + (wave >> 1) * kWide;
+  constexpr uint32_t kHalf = kWaves / 2;
+  float *mine = (float *)(wave < kHalf ? (uint8_t *)&s0 : (uint8_t *)&s1) + wave % kHalf * 32 * kPitch;
+  static_assert(kHalf * 32 * kPitch * 4 <= sizeof(s0), "half the waves' rows in a stage");
+  const uint32_t wm = m0 + Tile::x_row(), wn = n0 + Tile::w_row();
   y += p * part;
   const bool whole = wn + kWide <= N && stride % 4 == 0 && ((uintptr_t)y & (4 * sizeof(T) - 1)) == 0;
 #pragma unroll
@@ -219,14 +219,14 @@ void launch_matmul(const uint8_t *xc, const uint8_t *xs, uint32_t M, const moe_m
   const Plan p(M, N, steps);
   const auto tiles = [&](auto t, void *to, uint64_t to_stride) {
     constexpr uint32_t kType = decltype(t)::value;
-    const auto run = [&](auto kernel) {
-      op_launch(kernel, (p.tiles * p.parts + 7) / 8 * 8, 256, stream, xc, xs, (const uint8_t *)w->codes,
+    const auto run = [&](auto kernel, uint32_t waves) {
+      op_launch(kernel, (p.tiles * p.parts + 7) / 8 * 8, 64 * waves, stream, xc, xs, (const uint8_t *)w->codes,
                 (const uint8_t *)w->scales, M, N, steps, p.span, (typename Elem<kType>::T *)to, to_stride,
                 (uint64_t)M * N);
     };
-    if (p.tile == 4) run(mx4_gemm<kType, 4, 4>);
-    if (p.tile == 2) run(mx4_gemm<kType, 2, 2>);
-    if (p.tile == 1) run(mx4_gemm<kType, 1, 1>);
+    if (p.tile == 4) run(mx4_gemm<kType, 4, 2, 8>, 8);
+    if (p.tile == 2) run(mx4_gemm<kType, 2, 2, 4>, 4);
+    if (p.tile == 1) run(mx4_gemm<kType, 1, 1, 4>, 4);
   };
   if (p.parts == 1) return op_by_type(y_type, [&](auto t) { tiles(t, y, stride); });
   tiles(std::integral_constant<uint32_t, QT_F32>(), work, N);
