@@ -68,7 +68,7 @@ class OnDevice {
 // A launch that reports its own error and no earlier one's.
 template <typename... P, typename... A>
 void op_launch_lds(void (*kernel)(P...), uint64_t blocks, uint32_t threads, uint32_t lds, void *stream, A... args) {
-  op_require(blocks <= 0x7fffffffull, "too many rows");
+  op_require(blocks <= 0xffffffffull / threads, "too many rows");  // (a launch has less than 2^32 threads)
   if (!blocks) return;
   static_assert(sizeof...(P) == sizeof...(A), "a kernel's arguments");
   [&](P... a) {

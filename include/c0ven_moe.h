@@ -347,7 +347,7 @@ MOE_API moe_status moe_route_async(const moe_route_config *cfg, const void *logi
  * padded to C = cols rounded up to 128 values: C / 2 bytes of codes (value 2 i in the low half of byte i: a sign bit and
  * the index into 0, 0.5, 1, 1.5, 2, 3, 4, 6) and C / 32 bytes of scales, one per 32 values (2^(s - 127); 255 makes the
  * block's values NaN). Codes past cols are 0. Rows follow one another; both pointers are 16-byte aligned. At most
- * 2^30 rows of 1 to 2^20 cols. */
+ * 2^27 rows of 1 to 2^20 cols. */
 typedef struct {
   uint8_t *codes;
   uint8_t *scales;
@@ -365,9 +365,9 @@ MOE_API moe_status moe_mx4_quantize_async(int32_t device, uint32_t type, const v
 MOE_API moe_status moe_mx4_dequantize_async(int32_t device, const moe_mx4_matrix *m, uint32_t type, void *out,
                                             uint64_t stride, void *stream);
 
-/* y = x w^T (y x->rows x w->rows of y_type, rows y_stride apart): the MX4 values' products summed in fp32 on the matrix
- * cores and rounded once. x->cols == w->cols. work: at least moe_mx4_matmul_work_bytes(w, x->rows) bytes, 16-byte
- * aligned (may be null where that is 0). */
+/* y = x w^T (y x->rows x w->rows of y_type, at most 2^38 elements, rows y_stride apart): the MX4 values' products summed in
+ * fp32 on the matrix cores and rounded once. x->cols == w->cols. work: at least moe_mx4_matmul_work_bytes(w, x->rows)
+ * bytes, 16-byte aligned (may be null where that is 0). */
 MOE_API uint64_t moe_mx4_matmul_work_bytes(const moe_mx4_matrix *w, uint32_t ntok);
 MOE_API moe_status moe_mx4_matmul_async(int32_t device, const moe_mx4_matrix *x, const moe_mx4_matrix *w,
                                         uint32_t y_type, void *y, uint64_t y_stride, void *work, uint64_t work_bytes,

@@ -119,7 +119,8 @@ def close(got, x, w, type):
 
 
 SHAPES = [(1, 1, 1), (1, 16, 128), (2, 65, 640), (5, 300, 2048), (1, 2049, 1000), (16, 129, 4000), (17, 33, 129),
-          (33, 512, 256), (64, 100, 1000), (65, 257, 384), (130, 70, 4096), (256, 256, 512), (301, 515, 1000), (513, 300, 640)]
+          (33, 512, 256), (64, 100, 1000), (65, 257, 384), (130, 70, 4096), (256, 256, 512), (301, 515, 1000), (513, 300, 640),
+          (17, 40, 8192), (48, 70, 16000), (20, 33, 5000), (1, 8200, 1920), (15, 100, 1024), (1800, 2000, 300), (1750, 2001, 640)]
 
 
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
@@ -136,6 +137,29 @@ def test_matmul(M, N, K, out):
     got = decode(y.get(), out)
     close(got[:M, :N], xv, wv, out)
     assert (got[M:] == 7.0).all() and (got[:, N:] == 7.0).all() and (work.get()[n:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(3700, 3601, 130), (3601, 3700, 700), (4000, 3600, 900)])
+def test_matmul_of_the_largest_tiles(M, N, K):
+    """Some rows and columns of y against sums in 64 bits, the others by their checksums along both axes: x times w's columns'
+    sum, and x's rows' sum times w."""
+    say("large tiles", M, N, K)
+    x, xb, xv, _, _ = random_mx4(M, K, M + K, 1)
+    w, wb, wv, _, _ = random_mx4(N, K, N + K + 1, 1)
+    y = hip.full((M + 1, N), 7)
+    n = moe.mx4_matmul_work_bytes(w, M)
+    work = room(n + 64)
+    moe.mx4_matmul_async(x, w, moe.QT_F32, y.ptr, work.ptr, n)
+    got = y.get().astype(np.float64)
+    assert (got[M:] == 7.0).all()
+    got = got[:M]
+    rows = np.r_[0:3, 200:320:7, M - 70:M]
+    close(got[rows], xv[rows], wv, "f32")
+    close(got[:, N - 70:], xv, wv[N - 70:], "f32")
+    # A sum of n results is off by their bounds' sum: the same bound, on the absolute values' sum.
+    for v, want, S in ((got.sum(0), xv.sum(0) @ wv.T, np.abs(xv).sum(0) @ np.abs(wv).T),
+                       (got.sum(1), xv @ wv.sum(0), np.abs(xv) @ np.abs(wv).sum(0))):
+        assert np.all(np.abs(v - want) <= (2 * (K / 32 + 24) + 2) * 2.0 ** -24 * S)
 
 
 @pytest.mark.parametrize("type,out", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32"), ("f32", "f16")])

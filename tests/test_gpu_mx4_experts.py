@@ -1,5 +1,7 @@
 """The experts of routed tokens in microscaled 4-bit floats, against the plain form in 64 bits within the bound that
 tests/ops_ref.py derives (and one rounding to the result's type), alone and behind the routing."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -61,12 +63,59 @@ def tokens(T, H, E, K, seed, dropped=0.0, repeat=False):
 @pytest.mark.parametrize("T,H,F,E,K", [(1, 128, 32, 4, 2), (1, 1000, 200, 8, 3), (1, 512, 256, 16, 10), (2, 33, 7, 3, 1),
                                        (5, 640, 96, 32, 6), (8, 256, 160, 64, 8), (16, 512, 128, 8, 4), (17, 256, 96, 16, 4),
                                        (33, 1, 1, 2, 2), (40, 384, 128, 4, 4), (70, 320, 260, 5, 2), (150, 256, 64, 3, 2),
-                                       (9, 2560, 640, 6, 4), (300, 130, 129, 40, 5)])
+                                       (9, 2560, 640, 6, 4), (300, 130, 129, 40, 5),
+                                       (16, 256, 600, 12, 10), (23, 256, 64, 12, 7), (16, 200, 700, 12, 10),
+                                       (3, 2100, 64, 4, 2), (20, 3200, 96, 2, 2), (200, 640, 640, 64, 2), (90, 384, 300, 4, 2)])
 def test_experts(T, H, F, E, K):
     say("experts", T, H, F, E, K)
     model = Model(E, H, F, T + H)
     check(model, *tokens(T, H, E, K, T))
     check(model, *tokens(T, H, E, K, T + 1, 0.3, True), limit=0.05, extra=3)
+
+
+def check_some(model, x, ids, w, rows):
+    """All tokens' call; those of `rows` against the plain form."""
+    got, values = run(model, x, ids, w)
+    y, off = ref.experts(values[rows], ids[rows], w[rows].astype(np.float32).astype(np.float64), *model.v)
+    off = off + ref.EPS["f32"] * (np.abs(y) + off) + 2.0 ** -126
+    assert np.all(np.abs(got[rows] - y) <= off)
+
+
+@pytest.mark.parametrize("T,H,F,E,K,skew", [(1100, 64, 40, 100, 4, 0.0), (1100, 64, 40, 100, 4, 0.9), (1050, 5700, 40, 8, 4, 0.0),
+                                            (600, 2300, 8, 512, 4, 0.0), (600, 2300, 8, 300, 8, 0.0)])
+def test_many(T, H, F, E, K, skew):
+    """More ids than a work-group sorts, more columns than down takes at a time, several blocks of them an item, most tokens
+    on one expert."""
+    say("many", T, H, F, E, K, skew)
+    x, ids, w = tokens(T, H, E, K, 7, 0.05)
+    ids[np.random.default_rng(1).random(T) < skew, 0] = E - 1
+    check_some(Model(E, H, F, 5), x, ids, w, np.r_[0:20, T // 2:T // 2 + 20, T - 20:T])
+
+
+def test_threads_and_streams():
+    """Calls from four threads at once, each on a stream and buffers of its own, few and many tokens."""
+    say("threads")
+    model = Model(12, 256, 96, 4)
+    jobs = []
+    for i, T in enumerate((1, 30, 200, 9)):
+        x, ids, w = tokens(T, 256, 12, 4, i, 0.1)
+        want = run(model, x, ids, w)[0]
+        op, s = model.op(4), hip.stream()
+        bufs = [hip.put(x), hip.put(ids.astype(np.int32)), hip.put(w.astype(np.float32)), hip.full((T, 256), 7.0),
+                room(op.work_bytes(T))]
+        jobs.append((op, T, s, bufs, want))
+
+    def call(op, T, s, b):
+        for _ in range(20):
+            op.forward_async(b[0].ptr, T, b[1].ptr, b[2].ptr, b[3].ptr, b[4].ptr, b[4].nbytes, stream=s)
+
+    threads = [threading.Thread(target=call, args=j[:4]) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for op, T, s, b, want in jobs:
+        assert np.array_equal(b[3].get(), want)
 
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
@@ -179,8 +228,9 @@ def test_far_experts():
             parts.append(b)
         far.hold += parts
         far.m.append(moe.Mx4Matrix(parts[0].ptr, parts[1].ptr, rows, cols))
-    for T in (1, 20):
+    for T in (1, 20, 200):
         x, _, w = tokens(T, H, 2, 1, 3)
         got, values = run(far, x, np.full((T, 1), E - 1), w)
-        y, off = ref.experts(values, np.zeros((T, 1), int), w.astype(np.float32).astype(np.float64), *model.v)
-        assert np.all(np.abs(got - y) <= off + 2.0 ** -24 * (np.abs(y) + off))
+        rows = np.arange(T)[-20:]
+        y, off = ref.experts(values[rows], np.zeros((len(rows), 1), int), w[rows].astype(np.float32).astype(np.float64), *model.v)
+        assert np.all(np.abs(got[rows] - y) <= off + 2.0 ** -24 * (np.abs(y) + off))

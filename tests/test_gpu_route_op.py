@@ -133,7 +133,17 @@ def test_masked(groups, sigmoid):
 def test_large():
     print("large", flush=True)
     check(logits(5000, 512, 11), 10)
+    check(logits(4097, 24, 14), 4)
+    check(logits(70000, 8, 15), 1, "bf16")
     check(logits(5000, 256, 12), 8, "bf16", True, logits(1, 256, 13, 0.1)[0], 8, 4, 2, True, 2.5)
+
+
+@pytest.mark.parametrize("T", [2, 9, 15, 16, 17, 33])
+def test_few(T):
+    """Around the number of tokens whose load one work-group counts."""
+    x = logits(T, 96, T)
+    check(x, 6)
+    check(x, 16, "f16", True, logits(1, 96, 3, 0.1)[0], 8, 4, 2)
 
 
 def test_no_load_and_no_tokens():

@@ -63,7 +63,7 @@ def mat(rows=64, cols=256, codes=P, scales=P):
 
 
 @pytest.mark.parametrize("m", [mat(cols=0), mat(codes=None), mat(scales=None), mat(codes=P + 8), mat(scales=P + 4),
-                               mat(cols=(1 << 24) + 1), mat(rows=(1 << 30) + 1)])
+                               mat(cols=(1 << 20) + 1), mat(rows=(1 << 27) + 1)])
 def test_mx4_refuses_matrices(m):
     big = 1 << 40
     refused(lambda: moe.mx4_quantize_async(moe.QT_F32, P, m, stride=big))
@@ -82,6 +82,8 @@ def test_mx4_refuses_buffers():
         refused(lambda: moe.mx4_matmul_async(m, mat(256), t, p, P, big, y_stride=stride))
         refused(lambda: moe.mx4_linear_async(moe.QT_F32, P, 4, mat(256), t, p, P, big, y_stride=stride))
         refused(lambda: moe.mx4_linear_async(t, p, 4, m, moe.QT_F32, P, P, big, x_stride=stride))
+    refused(lambda: moe.mx4_linear_async(moe.QT_F32, P, (1 << 27) + 1, m, moe.QT_F32, P, P, big), "tokens")
+    refused(lambda: moe.mx4_matmul_async(mat(1 << 27), mat((1 << 11) + 1), moe.QT_F32, P, P, big), "2^38")
     refused(lambda: moe.mx4_matmul_async(m, mat(cols=257), moe.QT_F32, P, P, big), "same cols")
     need = moe.mx4_linear_work_bytes(m, 40)
     assert need > 0
