@@ -9,10 +9,12 @@
 
 namespace c0ven {
 
-// Few rows of x (at most 16): y = x w^T is bound by reading w. A work-group has 16 rows of w, its kWaves waves each a run
-// of their k, four steps of 128 in flight a wave; the waves' sums are added in their order. kX kQuantised: x is quantised
-// already (xc, xs); else x are floats of that type (QT_F32 is 0), which the work-group quantises into LDS while its first loads of w are on
-// their way.
+// Few rows of x (at most 16): y = x w^T is bound by reading w, and by its loads: 16 rows' 64 bytes are a clock a lane. So a
+// row's scales come for four steps of 128 at a time (one by one: as long as the codes; 16 x 8192 x 8192 22.7 us, now 18.9).
+// A work-group has 16 rows of w, its kWaves waves each a run of their k, four steps in use and four more on their way; the
+// waves' sums are added in their order. kX kQuantised: x is quantised already (xc, xs); else x are floats of that type
+// (QT_F32 is 0), which the work-group quantises into LDS while its first loads of w are on their way (1 x 8192 x 2048 4.7 us,
+// 7.6 with a launch for it). 1 x 16384 x 8192: 20 us, 3.5 TB/s.
 constexpr uint32_t kQuantised = ~0u;
 constexpr uint32_t kFewRows = 16, kFewLds = 16384;  // the most values of x that a work-group quantises for itself
 
@@ -31,20 +33,35 @@ __global__ void __launch_bounds__(64 * kWaves)
   const uint64_t row = (uint64_t)min(n0 + r, N - 1) * steps;
   const uint32_t m = min(r, M - 1);
   constexpr int kAhead = 4;
-  mx_i4 a[kAhead], b[kAhead];
-  uint32_t sa[kAhead], sb[kAhead];
-  const auto load = [&](uint32_t k) {
+  struct Ahead {
+    mx_i4 a[kAhead], b[kAhead];
+    uint32_t sa[kAhead], sb[kAhead];
+  } one, two;
+  const auto words = [&](uint32_t (&to)[kAhead], const uint8_t *from, uint32_t k) {  // a row's scales from step k on
+    if (k + kAhead <= steps) {
+      struct __attribute__((packed, aligned(4))) Words {
+        uint32_t w[kAhead];
+      };
+      const Words v = *(const Words *)(from + k * 4);
 #pragma unroll
-    for (int j = 0; j < kAhead; j++) {
-      const uint64_t at = row + min(k + j, steps - 1);
-      a[j] = *(const mx_i4 *)(wc + at * 64 + q * 16), sa[j] = *(const uint32_t *)(ws + at * 4);
-      if constexpr (!kFloats) {
-        const uint64_t ax = (uint64_t)m * steps + min(k + j, steps - 1);
-        b[j] = *(const mx_i4 *)(xc + ax * 64 + q * 16), sb[j] = *(const uint32_t *)(xs + ax * 4);
-      }
+      for (int j = 0; j < kAhead; j++) to[j] = v.w[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kAhead; j++)
+        if (k + j < k1) to[j] = *(const uint32_t *)(from + (k + j) * 4);
     }
   };
-  load(k0);
+  const auto load = [&](Ahead &to, uint32_t k) {
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      if (k + j >= k1) break;
+      to.a[j] = *(const mx_i4 *)(wc + (row + k + j) * 64 + q * 16);
+      if constexpr (!kFloats) to.b[j] = *(const mx_i4 *)(xc + ((uint64_t)m * steps + k + j) * 64 + q * 16);
+    }
+    words(to.sa, ws + row * 4, k);
+    if constexpr (!kFloats) words(to.sb, xs + (uint64_t)m * steps * 4, k);
+  };
+  load(one, k0);
   const uint32_t pitch = steps * 64 + 16;
   if constexpr (kFloats) {
     typedef typename Elem<kX>::T X;
@@ -60,17 +77,22 @@ __global__ void __launch_bounds__(64 * kWaves)
     __syncthreads();
   }
   mx_f4 c = {0, 0, 0, 0};
-  for (uint32_t k = k0; k < k1; k += kAhead) {
-    if (k != k0) load(k);
+  const auto use = [&](Ahead &v, uint32_t k) {
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
       if (k + j >= k1) break;
       if constexpr (kFloats) {
-        b[j] = *(const mx_i4 *)(lc + m * pitch + (k + j) * 64 + q * 16);
-        sb[j] = *(const uint32_t *)(ls + (m * steps + k + j) * 4);
+        v.b[j] = *(const mx_i4 *)(lc + m * pitch + (k + j) * 64 + q * 16);
+        v.sb[j] = *(const uint32_t *)(ls + (m * steps + k + j) * 4);
       }
-      c = mx_mfma16<0, 0>(a[j], b[j], c, sa[j] >> (8 * q), sb[j] >> (8 * q));
+      c = mx_mfma16<0, 0>(v.a[j], v.b[j], c, v.sa[j] >> (8 * q), v.sb[j] >> (8 * q));
     }
+  };
+  for (uint32_t k = k0; k < k1; k += 2 * kAhead) {
+    if (k + kAhead < k1) load(two, k + kAhead);
+    use(one, k);
+    if (k + 2 * kAhead < k1) load(one, k + 2 * kAhead);
+    use(two, k + kAhead);
   }
 #pragma unroll
   for (int i = 0; i < 4; i++) sums[wave][r][4 * q + i] = c[i];
@@ -204,11 +226,14 @@ void launch_few(const void *x, uint64_t x_stride, const uint8_t *xc, const uint8
       op_launch(kernel, blocks, 64 * waves, stream, x, x_stride, xc, xs, (const uint8_t *)w->codes,
                 (const uint8_t *)w->scales, M, N, w->cols, (typename Elem<kType>::T *)y, stride);
     };
-    // Sixteen waves a work-group where there are too few work-groups of four to fill the CUs.
-    if (blocks >= 512 || mx_steps(w->cols) <= 8)
-      run(mx4_few<kX, kType, 4>, 4);
-    else
+    // Sixteen waves a work-group where there are few of them, for a long k (16 x 2048 x 8192 10.1 us, with four 11.1; x 2048
+    // 7.0 and 6.6) and for many values to quantise (4 x 512 x 1024 3.2 us, with four 3.6; 16 x 2048 x 1024 3.9 and 5.6; 1 x
+    // 2048 x 1024 3.2 and 2.9). With more work-groups four hide each other's latency (4 x 16384 x 2048 8.4 us, 16: 10.0).
+    const bool many = kX == kQuantised ? mx_steps(w->cols) >= 64 : M * mx_steps(w->cols) * kMxRow >= 4096;
+    if (blocks <= 512 && many)
       run(mx4_few<kX, kType, 16>, 16);
+    else
+      run(mx4_few<kX, kType, 4>, 4);
   });
 }
 
