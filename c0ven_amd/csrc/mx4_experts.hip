@@ -104,9 +104,8 @@ struct MxExperts {
 };
 
 // A launch's work-groups to its items (parts a tile) so that an XCD (work-groups go to the eight in turn) has runs of four
-// tiles: an expert's tiles share its weights in that L2, while the experts with one tile are dealt over all of them (whole
-// eighths of the list on an XCD left most of the distinct weights to a few: 4096 skewed tokens 132 us instead of the
-// figures below). ~0: none.
+// tiles: an expert's tiles share its weights in that L2, while the experts with one tile are dealt over all of them (4096
+// tokens of 10 of 512 experts 392 us, with the items in order 430; of 4 of 16 experts 114 and 119). ~0: none.
 constexpr uint32_t kTileRun = 4;
 __device__ __forceinline__ uint32_t item_of(uint32_t all, uint32_t parts) {
   const uint32_t run = kTileRun * parts, j = blockIdx.x / 8, id = (j / run * 8 + blockIdx.x % 8) * run + j % run;
@@ -170,10 +169,9 @@ __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint
   }
 }
 
-// An item: a tile and a few times BN of the `cols` rows of down from r0 on, one after the other on the same pipeline, so many
-// that the launch has about 2048 items. Writes the sums to the assignments' rows of o, `cols` apart (a multiple of 256): a
-// lane has a column of 16 rows, so that a store is of whole lines (two rows of 32 columns; with a row's four neighbours a
-// lane it was 32 rows of 32 bytes: 4096 tokens 172 us in all, now see below).
+// An item: a tile and BN of the `cols` rows of down from r0 on. Writes the sums to the assignments' rows of o, `cols` apart (a
+// multiple of 256): a lane has a column of 16 rows, so that a store is of whole lines (two rows of 32 columns; with a row's
+// four neighbours a lane it was 32 rows of 32 bytes: 4096 tokens 172 us in all, now 128).
 template <int TM, int WM>
 __global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t *hc, const uint8_t *hs, uint32_t A,
                                                       const uint32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
@@ -183,45 +181,36 @@ __global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t
   __shared__ typename Tile::Stage s1;
   __shared__ typename Tile::Scales scales;
   __shared__ __align__(16) uint32_t place[Tile::BM];  // where a row of the tile goes, in bytes (kNowhere: dropped)
-  const uint32_t steps = mx_steps(p.F), total = cols / Tile::BN, nt = *n_tiles;
-  const uint32_t blocks = min(max(nt * total / 2048, 1u), total), parts = (total + blocks - 1) / blocks;
-  const uint32_t item = item_of(nt * parts, parts);
+  const uint32_t steps = mx_steps(p.F), parts = cols / Tile::BN, item = item_of(*n_tiles * parts, parts);
   if (item == ~0u) return;
   const MoeTile tile = tiles[item / parts];
-  const uint32_t b0 = item % parts * blocks, nb = min(blocks, total - b0);
-  const uint32_t stages = (steps + 3) / 4 * 2;  // of BN rows: whole pairs (the last one may be empty)
-  const uint64_t row = (uint64_t)tile.expert * p.H + r0 + b0 * Tile::BN, rest = (uint64_t)p.E * p.H - min(row, (uint64_t)p.E * p.H);
+  const uint32_t c0 = item % parts * Tile::BN;
+  const uint64_t row = (uint64_t)tile.expert * p.H + r0 + c0, rest = (uint64_t)p.E * p.H - min(row, (uint64_t)p.E * p.H);
   const auto same = [](uint32_t r) { return r; };
   const MxSource<Tile::BM> x(hc, hs, A, steps, [&](uint32_t r) { return tile.start + min(r, tile.count - 1); });
   const MxSource<Tile::BN> w(p.dc + row * steps * 64, p.ds + row * steps * 4, rest, steps, same);
   const uint32_t lane = threadIdx.x & 63, q = lane / 32;
   if (threadIdx.x < Tile::BM)
     place[threadIdx.x] = threadIdx.x < tile.count ? order[tile.start + threadIdx.x] * cols * 4 : kNowhere;
-  const __amdgpu_buffer_rsrc_t to = mx_buffer((const uint8_t *)o, (uint64_t)A * cols * 4);
-  const uint32_t col = (b0 * Tile::BN + Tile::w_row() + lane % 32) * 4;
   Tile c;
-  const auto store = [&](uint32_t n) {  // the sums of the n-th BN rows
-    uint32_t row = Tile::x_row() + 4 * q;
-    asm volatile("" : "+v"(row));  // (place is read here, for each n: kept in registers it is 16 of them)
+  c.run(
+      s0, s1, scales, (steps + 1) / 2,
+      [&](typename Tile::Stage &s, uint32_t k) { w.load(k, s.w), x.load(k, s.x); },
+      [&](typename Tile::Scales &s, uint32_t k) { w.load_scales(k, s.w), x.load_scales(k, s.x); });
+  const __amdgpu_buffer_rsrc_t to = mx_buffer((const uint8_t *)o, (uint64_t)A * cols * 4);
+  const uint32_t col = (c0 + Tile::w_row() + lane % 32) * 4;
 #pragma unroll
-    for (int m = 0; m < TM; m++)
+  for (int m = 0; m < TM; m++)
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const uint4 v = *(const uint4 *)(place + row + 32 * m + 8 * j);
-        const uint32_t at[4] = {v.x, v.y, v.z, v.w};
+    for (int j = 0; j < 4; j++) {
+      const uint4 v = *(const uint4 *)(place + Tile::x_row() + 32 * m + 8 * j + 4 * q);
+      const uint32_t at[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+      for (int i = 0; i < 4; i++)
 #pragma unroll
-          for (int f = 0; f < 2; f++)
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(c.acc[f][m][4 * j + i]), to, at[i] + col,
-                                                  (n * Tile::BN + f * Tile::kStep) * 4, 0);
-      }
-  };
-  c.run_blocks(
-      s0, s1, scales, nb, stages,
-      [&](typename Tile::Stage &s, uint32_t n, uint32_t k) { w.load(k, s.w, n * Tile::BN), x.load(k, s.x); },
-      [&](typename Tile::Scales &s, uint32_t n, uint32_t k) { w.load_scales(k, s.w, n * Tile::BN), x.load_scales(k, s.x); },
-      store);
+        for (int f = 0; f < 2; f++)
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(c.acc[f][m][4 * j + i]), to, at[i] + col, f * Tile::kStep * 4, 0);
+    }
 }
 
 // ---- few assignments (at most kFew): no sorting, two launches. Bound by latency and by reading the experts' weights, which
@@ -534,8 +523,10 @@ void check_experts(const moe_mx4_experts *e, uint32_t ntok) {
   op_require(op_float(e->x_type) && op_float(e->y_type), "the element type must be QT_F32, QT_F16 or QT_BF16");
 }
 
-// How a call runs: at most kFew assignments whose rows of h fit LDS without sorting them.
-constexpr uint64_t kChunkBytes = 96 << 20;
+// How a call runs. Few assignments, whose rows of h fit LDS, without sorting them: up to 96 (8 tokens of 10 of 512 experts 41
+// us, sorted 45; 12 of 64 experts' 10: 35 us, sorted 32), or to kFew where they are of few experts (32 tokens of 4 of 16
+// experts 21 us, sorted 25). n_embd 2048, n_ff 512 here and below.
+constexpr uint64_t kChunkBytes = 256 << 20;
 
 struct Plan {
   uint32_t A, rows, pitch, chunk, max_tiles;
@@ -544,13 +535,15 @@ struct Plan {
 
   Plan(const moe_mx4_experts &e, uint32_t T) {
     A = T * e.n_used;
-    few = A <= kFew && A * (mx_steps(e.n_ff) * 68 + 16) <= kFewHq;
-    // Tiles of 32, 64 or 128 positions: the more an expert has on average, the fewer times its weights are read.
+    few = A <= (e.n_expert <= 32 ? kFew : 96) && A * (mx_steps(e.n_ff) * 68 + 16) <= kFewHq;
+    // Tiles of 32, 64 or 128 positions: the more an expert has on average, the fewer times its weights are read. 301 tokens
+    // of 10 of 512 experts (6 each) 181, 191 and 243 us; 2048 (40) 290, 261 and 302; 4096 (80) 430, 397 and 374, with skewed
+    // experts 463, 416 and 436; 1024 of 8 of 128 (64) 97, 88 and 92; 4096 of 4 of 16 (1024) 131, 112 and 113.
     const uint32_t mean = A / e.n_expert;
     rows = mean < 24 ? 32 : mean < 96 ? 64 : 128;
     pitch = (e.n_embd + 255) / 256 * 256;
-    // The sums of all assignments at once, or of a part of the columns at a time that the last-level cache (256 MB) keeps
-    // until they are added.
+    // The sums of all assignments at once, or of as many columns at a time as 256 MB hold, about the last-level cache (4096
+    // tokens of 10 experts: 335 MB of sums, 304 us; 96 MB at a time 312, all at once 303, but up to 17 GB of work).
     chunk = std::min<uint64_t>(pitch, std::max<uint64_t>(256, kChunkBytes / (4ull * A) / 256 * 256));
     max_tiles = std::min(A, e.n_expert + A / rows);
     uint64_t at = 0;

@@ -67,24 +67,21 @@ struct MxSource {
 #pragma unroll
     for (int i = 0; i < kScales; i++) sat[i] = row_of(min((wave + kWaves * i) * 64 + lane, (uint32_t)kRows - 1)) * n * 4;
   }
-  // The buffer from row r0's byte `from` on (in scalar registers, so that a lane's offsets are the same for every stage).
-  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t part(const uint8_t *p, uint64_t rows, uint32_t row, uint32_t r0,
-                                                                uint32_t from) {
-    const uint64_t off = (uint64_t)r0 * row + from, all = rows * row;
-    return mx_buffer(p + off, all > off ? all - off : 0);
+  // The buffer of n bytes from byte `from` on (in scalar registers, so that a lane's offsets are the same for every stage).
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t part(const uint8_t *p, uint64_t n, uint32_t from) {
+    return mx_buffer(p + from, n > from ? n - from : 0);
   }
-  // Stage k, from row r0 on.
-  __device__ __forceinline__ void load(uint32_t k, uint8_t *c, uint32_t r0 = 0) const {
+  __device__ __forceinline__ void load(uint32_t k, uint8_t *c) const {
     const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
-    const auto from = part(codes, rows, steps * 64, r0, k * 128);
+    const auto from = part(codes, rows * steps * 64, k * 128);
     const bool in = k * 128 + ((lane % 8) ^ (wave % 2 * 4 + lane / 16)) * 16 < steps * 64;
 #pragma unroll
     for (int i = 0; i < kCodes; i++) lds_dma16(from, in ? at[i] : kNowhere, c + (wave + kWaves * i) * 1024);
   }
   // The scales of stages k and k + 1 (k even).
-  __device__ __forceinline__ void load_scales(uint32_t k, uint32_t *s, uint32_t r0 = 0) const {
+  __device__ __forceinline__ void load_scales(uint32_t k, uint32_t *s) const {
     const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), left = steps - 2 * k;
-    const auto from = part(scales, rows, steps * 4, r0, k * 8);
+    const auto from = part(scales, rows * steps * 4, k * 8);
 #pragma unroll
     for (int i = 0; i < kScales; i++) {
       if (kRows % (64 * kWaves) != 0 && (wave + kWaves * i) * 64 >= kRows) continue;
@@ -230,30 +227,6 @@ struct MxTile {
       });
     }
     if (k < n) stage<0>(s0, s1, scales, [] {});
-  }
-  // The same for `blocks` products of n stages (an even number; the last one may be all zeros) one after the other, without
-  // a pause between them: load and load_scales go by block and stage, done(block) takes a block's sums.
-  template <typename Load, typename LoadScales, typename Done>
-  __device__ __forceinline__ void run_blocks(Stage &s0, Stage &s1, Scales &scales, uint32_t blocks, uint32_t n, Load load,
-                                             LoadScales load_scales, Done done) {
-    start(
-        s0, s1, scales, blocks * n, [&](Stage &s, uint32_t k) { load(s, 0, k); },
-        [&](Scales &s, uint32_t k) { n > 2 ? load_scales(s, 0, k) : load_scales(s, k / 2, 0); });
-    for (uint32_t block = 0; block < blocks; block++) {
-      clear();
-      for (uint32_t k = 0; k < n; k += 2) {
-        const bool last = k + 2 == n, more = !last || block + 1 < blocks;  // (the pair that comes next)
-        const uint32_t next = last ? block + 1 : block, nk = last ? 0 : k + 2;
-        stage<0>(s0, s1, scales, [&] {
-          if (more) load(s0, next, nk);
-          if (more && (block != 0 || k != 0)) load_scales(scales, next, nk);
-        });
-        stage<1>(s1, s0, scales, [&] {
-          if (more) load(s1, next, nk + 1);
-        });
-      }
-      done(block);
-    }
   }
 };
 
