@@ -5,28 +5,27 @@
 
 namespace c0ven {
 
-// Both kernels take eight values a thread and kMxAhead such groups, all loaded before the first is used: bound by memory,
-// they need the bytes in flight. A work-group has 256 / 2^shift rows of 2^shift threads (whole rows where they are short),
-// each 2^shift kMxAhead groups wide.
-constexpr int kMxAhead = 4;
-
+// Both kernels take eight values a thread and kAhead such groups, all loaded before the first is used. A work-group has 256 /
+// 2^shift rows of 2^shift threads (whole rows where they are short), each 2^shift kAhead groups wide. Bound by memory: 16384 x
+// 8192 bf16 are quantised in 74 us (4.6 TB/s; with two groups a thread 77, four 83, eight 87), and back in 59 (5.8 TB/s) with
+// four (two 69, eight 71).
 struct MxRows {
   uint32_t rows, cols, shift, wide;  // wide: work-groups a row takes
 };
 
-template <uint32_t kType>
+template <uint32_t kType, int kAhead>
 __global__ void __launch_bounds__(256) mx4_quantize(const typename Elem<kType>::T *x, uint64_t stride, MxRows a,
                                                     uint8_t *codes, uint8_t *scales) {
   const uint32_t ng = mx_steps(a.cols) * 16;
   const uint32_t r = (blockIdx.x / a.wide << (8 - a.shift)) + (threadIdx.x >> a.shift);
-  const uint32_t g0 = (blockIdx.x % a.wide * kMxAhead << a.shift) + (threadIdx.x & ((1u << a.shift) - 1));
+  const uint32_t g0 = (blockIdx.x % a.wide * kAhead << a.shift) + (threadIdx.x & ((1u << a.shift) - 1));
   if (r >= a.rows) return;  // (four neighbours of a block are in one row)
   const typename Elem<kType>::T *row = x + r * stride;
-  float v[kMxAhead][8];
+  float v[kAhead][8];
 #pragma unroll
-  for (int i = 0; i < kMxAhead; i++) load8<kType>(row, (g0 + (i << a.shift)) * 8, a.cols, v[i]);
+  for (int i = 0; i < kAhead; i++) load8<kType>(row, (g0 + (i << a.shift)) * 8, a.cols, v[i]);
 #pragma unroll
-  for (int i = 0; i < kMxAhead; i++) {
+  for (int i = 0; i < kAhead; i++) {
     const uint32_t g = g0 + (i << a.shift);
     uint32_t s;
     const uint32_t c = mx_quantize8(v[i], s);
@@ -36,21 +35,21 @@ __global__ void __launch_bounds__(256) mx4_quantize(const typename Elem<kType>::
   }
 }
 
-template <uint32_t kType>
+template <uint32_t kType, int kAhead>
 __global__ void __launch_bounds__(256) mx4_dequantize(const uint8_t *codes, const uint8_t *scales, MxRows a,
                                                       typename Elem<kType>::T *out, uint64_t stride) {
   const uint32_t ng = mx_steps(a.cols) * 16;
   const uint32_t r = (blockIdx.x / a.wide << (8 - a.shift)) + (threadIdx.x >> a.shift);
-  const uint32_t g0 = (blockIdx.x % a.wide * kMxAhead << a.shift) + (threadIdx.x & ((1u << a.shift) - 1));
+  const uint32_t g0 = (blockIdx.x % a.wide * kAhead << a.shift) + (threadIdx.x & ((1u << a.shift) - 1));
   if (r >= a.rows) return;
-  uint32_t c[kMxAhead], s[kMxAhead];
+  uint32_t c[kAhead], s[kAhead];
 #pragma unroll
-  for (int i = 0; i < kMxAhead; i++) {
+  for (int i = 0; i < kAhead; i++) {
     const uint64_t at = (uint64_t)r * ng + min(g0 + (i << a.shift), ng - 1);
     c[i] = ((const uint32_t *)codes)[at], s[i] = scales[at / 4];
   }
 #pragma unroll
-  for (int i = 0; i < kMxAhead; i++) {
+  for (int i = 0; i < kAhead; i++) {
     float v[8];
     mx_values8(c[i], mx_pow2(s[i]), v);
     store8<kType>(out + r * stride, (g0 + (i << a.shift)) * 8, a.cols, v);
@@ -63,11 +62,11 @@ using namespace c0ven;
 
 namespace {
 
-MxRows rows_of(uint32_t rows, uint32_t cols, uint64_t &blocks) {
+MxRows rows_of(uint32_t rows, uint32_t cols, uint32_t ahead, uint64_t &blocks) {
   const uint32_t ng = mx_steps(cols) * 16;
   uint32_t shift = 4;
-  while (shift < 8 && (uint32_t)kMxAhead << shift < ng) shift++;
-  const uint32_t wide = (ng + (kMxAhead << shift) - 1) / (kMxAhead << shift);
+  while (shift < 8 && ahead << shift < ng) shift++;
+  const uint32_t wide = (ng + (ahead << shift) - 1) / (ahead << shift);
   blocks = (((uint64_t)rows + (256 >> shift) - 1) / (256 >> shift)) * wide;
   return MxRows{rows, cols, shift, wide};
 }
@@ -76,11 +75,11 @@ MxRows rows_of(uint32_t rows, uint32_t cols, uint64_t &blocks) {
 
 void c0ven::mx4_quantize_launch(uint32_t type, const void *x, uint64_t stride, const moe_mx4_matrix &m, void *stream) {
   uint64_t n;
-  const MxRows a = rows_of(m.rows, m.cols, n);
+  const MxRows a = rows_of(m.rows, m.cols, 1, n);
   const auto run = [&](auto kernel, auto *p) { op_launch(kernel, n, 256, stream, p, stride, a, m.codes, m.scales); };
-  if (type == QT_F32) run(mx4_quantize<QT_F32>, (const float *)x);
-  if (type == QT_F16) run(mx4_quantize<QT_F16>, (const _Float16 *)x);
-  if (type == QT_BF16) run(mx4_quantize<QT_BF16>, (const __bf16 *)x);
+  if (type == QT_F32) run(mx4_quantize<QT_F32, 1>, (const float *)x);
+  if (type == QT_F16) run(mx4_quantize<QT_F16, 1>, (const _Float16 *)x);
+  if (type == QT_BF16) run(mx4_quantize<QT_BF16, 1>, (const __bf16 *)x);
 }
 
 extern "C" {
@@ -104,14 +103,22 @@ MOE_API moe_status moe_mx4_dequantize_async(int32_t device, const moe_mx4_matrix
     op_mx4(m);
     op_rows(out, stride, m->cols, type);
     OnDevice on(device);
-    uint64_t n;
-    const MxRows a = rows_of(m->rows, m->cols, n);
-    const auto run = [&](auto kernel, auto *p) {
-      op_launch(kernel, n, 256, stream, (const uint8_t *)m->codes, (const uint8_t *)m->scales, a, p, stride);
+    const auto go = [&](auto ahead) {
+      constexpr int kAhead = decltype(ahead)::value;
+      uint64_t n;
+      const MxRows a = rows_of(m->rows, m->cols, kAhead, n);
+      const auto run = [&](auto kernel, auto *p) {
+        op_launch(kernel, n, 256, stream, (const uint8_t *)m->codes, (const uint8_t *)m->scales, a, p, stride);
+      };
+      if (type == QT_F32) run(mx4_dequantize<QT_F32, kAhead>, (float *)out);
+      if (type == QT_F16) run(mx4_dequantize<QT_F16, kAhead>, (_Float16 *)out);
+      if (type == QT_BF16) run(mx4_dequantize<QT_BF16, kAhead>, (__bf16 *)out);
     };
-    if (type == QT_F32) run(mx4_dequantize<QT_F32>, (float *)out);
-    if (type == QT_F16) run(mx4_dequantize<QT_F16>, (_Float16 *)out);
-    if (type == QT_BF16) run(mx4_dequantize<QT_BF16>, (__bf16 *)out);
+    // (Rows too short for four groups a thread in sixteen threads leave threads without work: 25915 x 100 9.5 us, 4.7 with one.)
+    if (mx_steps(m->cols) >= 4)
+      go(std::integral_constant<int, 4>());
+    else
+      go(std::integral_constant<int, 1>());
   });
 }
 

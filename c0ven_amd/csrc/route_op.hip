@@ -415,11 +415,15 @@ __global__ void __launch_bounds__(1024) route_count(const int32_t *ids, uint32_t
   __shared__ uint32_t count[512];
   if (threadIdx.x < 512) count[threadIdx.x] = 0;
   __syncthreads();
-  const uint32_t end = min(n, (blockIdx.x + 1) * kCountIds);
-  for (uint32_t i = blockIdx.x * kCountIds + threadIdx.x; i < end; i += 1024) {
-    const int32_t id = ids[i];
-    if (id >= 0) atomicAdd(count + id, 1u);
+  int32_t id[kCountIds / 1024];
+#pragma unroll
+  for (uint32_t j = 0; j < kCountIds / 1024; j++) {
+    const uint32_t i = blockIdx.x * kCountIds + j * 1024 + threadIdx.x;
+    id[j] = i < n ? ids[i] : -1;
   }
+#pragma unroll
+  for (uint32_t j = 0; j < kCountIds / 1024; j++)
+    if (id[j] >= 0) atomicAdd(count + id[j], 1u);
   __syncthreads();
   if (threadIdx.x >= E) return;
   if (gridDim.x == 1)
