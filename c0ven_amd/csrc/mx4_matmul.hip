@@ -16,7 +16,8 @@ namespace c0ven {
 // (QT_F32 is 0), which the work-group quantises into LDS while its first loads of w are on their way (1 x 8192 x 2048 4.7 us,
 // 7.6 with a launch for it). 1 x 16384 x 8192: 20 us, 3.5 TB/s.
 constexpr uint32_t kQuantised = ~0u;
-constexpr uint32_t kFewRows = 16, kFewLds = 16384;  // the most values of x that a work-group quantises for itself
+constexpr uint32_t kFewRows = 16;    // (16 x 4096 x 4096 7.5 us, 17 rows by tiles 11.9; 8192 x 8192 18.0 and 18.3)
+constexpr uint32_t kFewLds = 16384;  // the most values of x that a work-group quantises for itself
 
 template <uint32_t kX, uint32_t kType, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves)
@@ -116,7 +117,11 @@ __global__ void __launch_bounds__(256) mx4_join(const float *sums, uint32_t part
   y[i / N * stride + i % N] = (typename Elem<kType>::T)s;
 }
 
-// A tile of y a work-group, k split into parts of `span` stages (256 each); part p's sums go to y + p * part.
+// A tile of y a work-group, k split into parts of `span` stages (256 each); part p's sums go to y + p * part. Work-groups to
+// tiles so that an XCD has neighbours: eight tiles down, then across. The 256 tile takes eight waves, two a SIMD (four with
+// 256 sums a lane: 177 us at 4096 x 8192 x 8448). That product takes 166 us, 3.4 PFLOP/s; with the loop's loads left out 132:
+// the matrix instructions on random codes are at 4.3 to 5.6 PFLOP/s, below the 8.2 of constant ones, and what the loads add
+// is the wait for a stage that 64 KB a CU cannot hide, since two stages fill LDS.
 template <uint32_t kType, int TM, int TN, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves, 2)
     mx4_gemm(const uint8_t *xc, const uint8_t *xs, const uint8_t *wc, const uint8_t *ws, uint32_t M, uint32_t N,
@@ -192,8 +197,10 @@ using namespace c0ven;
 namespace {
 
 // How a product of M rows with N rows runs: tiles of 64 t by 64 t, k in parts of span stages of 256. The largest tile that
-// still gives every CU one (a 256 tile moves a quarter of the bytes of a 64 tile through LDS per product, but a product
-// bound by latency wants work-groups); if even the smallest leaves CUs without one, the k axis is split.
+// still gives most CUs one (a 256 tile moves a quarter of the bytes of a 64 tile through LDS per product): 2048 x 8192 x 4096
+// with 256 tiles (256 of them) 51 us, 128 58, 64 82; 1024 x 8192 x 8192 with 256 tiles (128) 72, 128 (512) 56, 64 80; 512 x
+// 8192 x 8192 with 128 (256) 40, 64 44. If even the smallest leaves CUs without one, the k axis is split: 64 x 4096 x 8192
+// 17.6 us (in one 23.5), 17 x 1024 x 8192 13 (22).
 struct Plan {
   uint32_t tile = 1, span, parts = 1;
   uint64_t tiles;
