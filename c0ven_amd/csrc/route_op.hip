@@ -230,7 +230,7 @@ __device__ __forceinline__ uint32_t select_ranks(const uint32_t (&key)[kPer], ui
 // kScores: the order is that of s + bias. Tokens go round the grid's waves. load (or null): one work-group counts it; of
 // several the first clears it for route_count.
 template <uint32_t kType, bool kScores, int kPer>
-__global__ void __launch_bounds__(512) moe_route(RouteArgs a, const typename Elem<kType>::T *logits, uint64_t stride,
+__global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(RouteArgs a, const typename Elem<kType>::T *logits, uint64_t stride,
                                                  const float *bias, uint32_t ntok, int32_t *ids, float *w, uint32_t *load) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   uint32_t *count = (uint32_t *)dynamic;  // 512
@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(512) moe_route(RouteArgs a, const typename Ele
             if (e0 + i < a.E) lds.v[e0 + i] = v[i];
           lds_done();
           if (lane < a.groups)
+#pragma unroll 8
             for (uint32_t j = 0, k = lane % n; j < n; j++, k = k + 1 == n ? 0 : k + 1) {
               const float o = lds.v[lane * n + k];
               b2 = fmaxf(b2, fminf(b1, o)), b1 = fmaxf(b1, o);
@@ -461,16 +462,17 @@ extern "C" MOE_API moe_status moe_route_async(const moe_route_config *cfg, const
     op_rows(logits, stride, c.n_expert, c.type);
     op_require(ids && w && op_aligned(ids, 4) && op_aligned(w, 4) && op_aligned(bias, 4) && op_aligned(load, 4),
                "null or misaligned ids, w, bias or load");
-    const RouteArgs a{c.n_expert, c.n_used, c.n_group, c.top_group, c.group_top, c.renorm, c.score == MOE_SCORE_SIGMOID,
+    const uint32_t groups = c.top_group < c.n_group ? c.n_group : 1;  // (all of them kept: as none)
+    const RouteArgs a{c.n_expert, c.n_used, groups, c.top_group, c.group_top, c.renorm, c.score == MOE_SCORE_SIGMOID,
                       c.scale == 0.0f ? 1.0f : c.scale};
     if (!ntok && !load) return;
     OnDevice on(c.device);
-    // With load up to sixteen tokens are one work-group's, which counts (two tokens a wave cost less than another
-    // launch); more are dealt to at most eight waves a SIMD.
-    const uint32_t waves = std::min(std::max(ntok, 1u), 8u);
-    const uint32_t blocks = load && ntok <= 16 ? ntok != 0 : std::min((ntok + waves - 1) / waves, 1024u);
     if (!ntok) return op_launch(route_clear, 1, 512, stream, load, c.n_expert);
-    const bool scores = bias || (c.n_group > 1 && c.group_top > 1);
+    const bool scores = bias || (groups > 1 && c.group_top > 1);
+    // With load as many tokens as a work-group has waves are one work-group's, which counts (13 tokens of 160 experts with
+    // groups 10.6 us, two tokens a wave 17.0; another launch is 2 to 3); more are dealt to at most eight waves a SIMD.
+    const bool one = load && ntok <= (scores && c.n_expert > 256 ? 8u : 16u);
+    const uint32_t waves = std::min(ntok, one ? 16u : 8u), blocks = one ? 1 : std::min((ntok + waves - 1) / waves, 1024u);
     const auto run = [&](auto kernel, auto *p) {
       op_launch_lds(kernel, blocks, 64 * waves, 2048 + waves * (uint32_t)sizeof(RouteScratch), stream, a, p, stride, bias, ntok,
                     ids, w, load);
