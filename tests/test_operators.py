@@ -1,6 +1,8 @@
 """The operators on device buffers without a GPU: their sizes, and the calls that they refuse before they touch a device
 (the pointers here are never followed)."""
 import ctypes as C
+import os
+import re
 
 import numpy as np
 import pytest
@@ -133,3 +135,20 @@ def test_reference_quantisation():
     assert np.array_equal(got[:16], x[0, :16])
     assert np.array_equal(got[16:23], [0, 1, 1, 2, 2, 4, 4])
     assert np.array_equal(ref.mx4(np.array([[7.9, 5.1, 0.2]])), [[6, 6, 0]])
+
+
+def test_kernels_do_not_spill():
+    """Every kernel of the operators holds what it needs in registers; the experts' tiles of 64 run three waves a SIMD."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "c0ven_amd", "_build", "kernel_resources.txt")
+    if not os.path.exists(path):
+        pytest.skip("no build in this tree (run __graft_entry__.build())")
+    rows = {}
+    for line in open(path):
+        name, *kv = line.split()
+        if re.match(r"_ZN5c0ven\d+(mx4_|moe_route|route_)", name):
+            rows[name] = {k: int(v) if v.isdigit() else v for k, v in (x.split("=") for x in kv)}
+    assert len(rows) >= 60
+    for n, r in rows.items():
+        assert r["scratch"] == 0, (n, r)
+        if re.search(r"mx4_(gate_up|down)_tilesILi1ELi2E", n):
+            assert r["occupancy"] >= 3, (n, r)
