@@ -31,6 +31,7 @@ struct RouteArgs {
 struct RouteScratch {
   union {
     float v[512];       // the selection values, for the groups
+    float2 best[64];    // a lane's largest two
     double d[512];      // the same in fp64
     uint2 cand[64];     // the candidates
   };
@@ -319,6 +320,20 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
           if (run > 16) merge(__shfl_xor(b1, 16, 64), __shfl_xor(b2, 16, 64));
           if (run > 32) merge(__shfl_xor(b1, 32, 64), __shfl_xor(b2, 32, 64));
           at = e0 / n;
+        } else if (n % kPer == 0) {
+          // Lane g joins its group's lanes' largest two.
+#pragma unroll
+          for (int i = 0; i < kPer; i++) b2 = fmaxf(b2, fminf(b1, v[i])), b1 = fmaxf(b1, v[i]);
+          lds.best[lane] = make_float2(b1, b2);
+          lds_done();
+          b1 = b2 = -INFINITY;
+          const uint32_t lanes = n / kPer;
+          if (lane < a.groups)
+            for (uint32_t j = 0; j < lanes; j++) {
+              const float2 o = lds.best[lane * lanes + j];
+              b2 = fmaxf(fminf(b1, o.x), fmaxf(b2, o.y)), b1 = fmaxf(b1, o.x);
+            }
+          lds_done();
         } else {
           // Lane g goes through group g's values, from a place of its own on, so that the lanes' banks differ.
 #pragma unroll
