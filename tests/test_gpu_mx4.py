@@ -271,6 +271,19 @@ def test_far_offsets():
     close(y.get()[:, -40:].astype(np.float64), vv, ref.mx4_values(want_c, want_s, cols), "f32")
 
 
+def test_no_such_device():
+    """A device that is not there is an error of that call alone."""
+    x = np.random.default_rng(2).normal(size=(3, 200)).astype(np.float32)
+    b = hip.put(x)
+    m, codes, scales = matrix(3, 200)
+    for device in (99, -1):
+        with pytest.raises(moe.MoeError):
+            moe.mx4_quantize_async(moe.QT_F32, b.ptr, m, device=device)
+    assert (codes.get() == 0xA5).all()
+    moe.mx4_quantize_async(moe.QT_F32, b.ptr, m)
+    assert np.array_equal(codes.get()[:3], ref.mx4_quantize(x.astype(np.float64))[0])
+
+
 def test_nothing_to_do():
     m, codes, scales = matrix(0, 64)
     moe.mx4_quantize_async(moe.QT_F32, codes.ptr, m)

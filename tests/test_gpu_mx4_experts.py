@@ -160,6 +160,19 @@ def test_nans_stay_with_their_token(T):
     assert not np.isnan(got).any()
 
 
+@pytest.mark.parametrize("T", [3, 12, 100, 900])
+def test_padded_batch(T):
+    """Tokens that stand for nothing (no expert, rows and weights of NaNs) get zeros and change nobody else's result."""
+    say("padded", T)
+    model = Model(6, 256, 96, 8)
+    x, ids, w = tokens(T, 256, 6, 2, 5)
+    clean, _ = run(model, x, ids, w)
+    pad = np.arange(T) % 3 == 1
+    x[pad], ids[pad], w[pad] = np.nan, -1, np.nan
+    got, _ = run(model, x, ids, w)
+    assert not got[pad].any() and np.array_equal(got[~pad], clean[~pad])
+
+
 @pytest.mark.parametrize("T", [1, 12, 100])
 def test_twice_the_same(T):
     """The sums' order is fixed: equal calls give equal bits, whatever the work buffer held, and a token's result does not
