@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(256) mx4_gate_up_few(MxExperts p, const typena
     for (int i = 0; i < 4; i++) acc[i] = mx_f4{0, 0, 0, 0};
     for (uint32_t s0 = 0; s0 < steps; s0 += kSteps) {
       const uint32_t ns = min(steps - s0, (uint32_t)kSteps);
-      __syncthreads();  // (member; the LDS of the round before)
+      __syncthreads();  // (member; the LDS of the pass before)
       if (m0 == 0 || steps > kSteps) {
         // A row a load (or two): wave w has 16 rows, of gate or of up.
 #pragma unroll 4

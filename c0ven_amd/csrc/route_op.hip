@@ -27,6 +27,13 @@ struct RouteArgs {
   float scale;
 };
 
+// The same values as ones of their own to the compiler: what is computed from them where few tokens come is not computed
+// before the loop that all pass (16 x 256 with groups 7.9 us, 7.5 with this).
+__device__ __forceinline__ RouteArgs apart(RouteArgs a) {
+  asm volatile("" : "+s"(a.E), "+s"(a.K), "+s"(a.groups), "+s"(a.kept), "+s"(a.best), "+s"(a.sigmoid));
+  return a;
+}
+
 // A token's scratch in LDS, a wave's own.
 struct RouteScratch {
   union {
@@ -397,22 +404,23 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
       decided = false;
     }
     if (!kScores || t >= ntok) break;
-    const Exact e(a, x);
+    const RouteArgs c = apart(a);
+    const Exact e(c, x);
     if (open_groups) {
-      e.keys(a, x, b, lds.d);
-      stays = exact_groups(a, lds.d);
+      e.keys(c, x, b, lds.d);
+      stays = exact_groups(c, lds.d);
       decided = true;
       continue;
     }
     // All that may belong to the first K are in the lanes if what is not there is below the K-th by more.
-    const float last = lane_f32(key_float(my_key), a.K - 1), rest = key_float(floor);
+    const float last = lane_f32(key_float(my_key), c.K - 1), rest = key_float(floor);
     Ranked r;
-    if (!floor || readlane_u32(my_key, (int)a.K - 1) == 0 ||
+    if (!floor || readlane_u32(my_key, (int)c.K - 1) == 0 ||
         last - rest > 2.0f * off_s + 0x1p-22f * (fabsf(last) + fabsf(rest))) {
-      r = exact_ranks(a, e, total, my_id, my_x, my_b);
+      r = exact_ranks(c, e, total, my_id, my_x, my_b);
     } else {
-      e.keys(a, x, b, lds.d);
-      r = exact_all<kType, kPer>(a, e, logits + (uint64_t)t * stride, stays, lds.d);
+      e.keys(c, x, b, lds.d);
+      r = exact_all<kType, kPer>(c, e, logits + (uint64_t)t * stride, stays, lds.d);
     }
     finish(t, r.id, r.s);
     decided = false;
