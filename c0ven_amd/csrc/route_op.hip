@@ -169,9 +169,10 @@ __device__ __forceinline__ Ranked exact_all(const RouteArgs &a, const Exact &e, 
   return mine;
 }
 
-// The n largest keys of the wave (0: no key), the lower id first among equals: lane r receives the r-th one's key and id
-// (key 0 where there are fewer), for r below the number returned, at least n where there are so many; every other expert's
-// key is at most floor (0: there is no other).
+// The n largest keys of the wave (up to kNoKey: none), the lower id first among equals: lane r receives the r-th one's key and
+// id (key 0 where there are fewer), for r below the number returned, at least n where there are so many; every other
+// expert's key is at most floor.
+constexpr uint32_t kNoKey = 0x007fffffu;  // minus infinity's
 template <int kPer>
 __device__ __forceinline__ uint32_t select_ranks(const uint32_t (&key)[kPer], uint32_t n, RouteScratch &lds, uint32_t &my_key,
                                                  uint32_t &my_id, uint32_t &floor) {
@@ -187,27 +188,27 @@ __device__ __forceinline__ uint32_t select_ranks(const uint32_t (&key)[kPer], ui
     if (reach == n) break;  // (no lower bit changes who reaches it)
   }
   floor = tau;
-  tau = max(tau, 1u);
-  uint32_t cnt = 0, pos = 0, total = 0;  // this lane's candidates, those of the lanes below, all
+  tau = max(tau, kNoKey + 1);
+  uint32_t total = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; i++) cnt += key[i] >= tau ? 1u : 0u;
-#pragma unroll
-  for (int b = 0; b < 4; b++) {
-    const uint64_t bal = __ballot((cnt >> b) & 1u);
-    pos += __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0u)) << b;
-    total += (uint32_t)__popcll(bal) << b;
-  }
+  for (int i = 0; i < kPer; i++) total += (uint32_t)__popcll(__ballot(key[i] >= tau));
   if (total <= 64) {
+    uint32_t base = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; i++)
-      if (key[i] >= tau) lds.cand[pos++] = make_uint2(key[i], e0 + i);
+    for (int i = 0; i < kPer; i++) {
+      const uint64_t bal = __ballot(key[i] >= tau);
+      const uint32_t pos = __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bal, base));
+      if (key[i] >= tau) lds.cand[pos] = make_uint2(key[i], e0 + i);
+      base += (uint32_t)__popcll(bal);
+    }
     lds_done();
     const uint2 me = lane < total ? lds.cand[lane] : make_uint2(0u, 0u);
     lds_done();
     uint32_t rank = 0;
+    const uint64_t mine = (uint64_t)me.x << 32 | ~me.y;
     for (uint32_t i = 0; i < total; i++) {
       const uint32_t ok = readlane_u32(me.x, (int)i), oi = readlane_u32(me.y, (int)i);
-      rank += (ok > me.x) | ((ok == me.x) & (oi < me.y));
+      rank += ((uint64_t)ok << 32 | ~oi) > mine ? 1u : 0u;
     }
     const int to = 4 * (int)(lane < total ? rank : lane);  // a permutation of the lanes
     my_key = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)me.x);
@@ -226,7 +227,7 @@ __device__ __forceinline__ uint32_t select_ranks(const uint32_t (&key)[kPer], ui
       if (!(gone >> i & 1) && key[i] >= b) b = key[i], at = i;
     const uint32_t top = wave_max_u32(b);
     floor = top;
-    if (!top) break;
+    if (top <= kNoKey) break;
     const uint32_t who = (uint32_t)__ffsll(__ballot(b == top)) - 1;
     if (lane == who) gone |= 1u << at;
     const uint32_t id = who * kPer + readlane_u32(at, (int)who);
@@ -255,8 +256,11 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
   const uint32_t step = gridDim.x * waves, n = a.groups > 1 ? a.E / a.groups : a.E;
   const auto finish = [&](uint32_t t, uint32_t id, float score) {  // lane r < K: rank r's expert (~0: none)
     if (id == ~0u || lane >= a.K) score = 0.0f;
-    float all_s = 0.0f;
-    for (uint32_t k = 0; k < a.K; k++) all_s += lane_f32(score, k);
+    float all_s = score;  // the sum of the first sixteen lanes
+    all_s += dpp_f32<kDppXor1>(all_s);
+    all_s += dpp_f32<kDppXor2>(all_s);
+    all_s += dpp_f32<kDppHalfMirror>(all_s);
+    all_s += dpp_f32<kDppMirror>(all_s);
     if (lane >= a.K) return;
     const uint64_t at = (uint64_t)t * a.K + lane;
     ids[at] = (int32_t)id;
@@ -287,7 +291,11 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
         for (int i = 0; i < kPer; i++) x[i] = e0 + i < a.E ? (float)row[e0 + i] : 0.0f;
       }
 #pragma unroll
-      for (int i = 0; i < kPer; i++) x[i] = e0 + i < a.E && x[i] > -INFINITY ? x[i] : -INFINITY;  // (no NaN)
+      for (int i = 0; i < kPer; i++) x[i] = x[i] > -INFINITY ? x[i] : -INFINITY;  // (no NaN)
+      if (a.E < 64 * kPer) {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) x[i] = e0 + i < a.E ? x[i] : -INFINITY;
+      }
       float top = x[0], sum = 0.0f;
 #pragma unroll
       for (int i = 1; i < kPer; i++) top = fmaxf(top, x[i]);
@@ -378,8 +386,11 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
       }
       uint32_t key[kPer];
 #pragma unroll
-      for (int i = 0; i < kPer; i++)
-        key[i] = v[i] > -INFINITY && (a.groups <= 1 || (stays >> ((e0 + i) * per_group >> 20) & 1)) ? float_key(v[i]) : 0u;
+      for (int i = 0; i < kPer; i++) key[i] = float_key(v[i]);
+      if (a.groups > 1) {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) key[i] = stays >> ((e0 + i) * per_group >> 20) & 1 ? key[i] : 0u;
+      }
       // (A few ranks past the last, so that what an open order may move lies among them.)
       total = select_ranks<kPer>(key, kScores ? a.K + 4 : a.K, lds, my_key, my_id, floor);
       const bool mine = my_key != 0 && lane <= a.K;
@@ -415,7 +426,7 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
     // All that may belong to the first K are in the lanes if what is not there is below the K-th by more.
     const float last = lane_f32(key_float(my_key), c.K - 1), rest = key_float(floor);
     Ranked r;
-    if (!floor || readlane_u32(my_key, (int)c.K - 1) == 0 ||
+    if (floor <= kNoKey || readlane_u32(my_key, (int)c.K - 1) == 0 ||
         last - rest > 2.0f * off_s + 0x1p-22f * (fabsf(last) + fabsf(rest))) {
       r = exact_ranks(c, e, total, my_id, my_x, my_b);
     } else {
