@@ -303,20 +303,22 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
       if (!a.sigmoid && (kScores || !a.renorm)) {
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-          s[i] = x[i] == -INFINITY ? 0.0f : x[i] == top ? 1.0f : exp_f32(x[i] - top);
+          const float p = exp_f32(x[i] - top);
+          s[i] = x[i] == top ? 1.0f : p;
+          s[i] = x[i] > -INFINITY ? s[i] : 0.0f;
           sum += s[i];
         }
         sum = wave_sum_f32(sum);
       }
       const float per_sum = a.sigmoid ? 1.0f : __builtin_amdgcn_rcpf(sum);
+      if (kScores && a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) s[i] = __builtin_amdgcn_rcpf(1.0f + exp_f32(-x[i]));
+      }
 #pragma unroll
       for (int i = 0; i < kPer; i++) {
-        if (kScores) {
-          const float p = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_f32(-x[i])) : s[i] * per_sum;
-          v[i] = x[i] > -INFINITY && b[i] > -INFINITY ? p + b[i] : -INFINITY;
-        } else {
-          v[i] = x[i];
-        }
+        v[i] = kScores ? s[i] * per_sum + b[i] : x[i];
+        if (kScores) v[i] = (x[i] > -INFINITY) & (b[i] > -INFINITY) ? v[i] : -INFINITY;
       }
       // A score's bound: a few units of its own for the exponential, the quotient and a softmax's sum, and |x - top| of
       // them for the difference, of which e^(x - top) |x - top| <= 0.37 stays: within 2^-20 of the largest score.
@@ -504,9 +506,11 @@ extern "C" MOE_API moe_status moe_route_async(const moe_route_config *cfg, const
     if (!ntok) return op_launch(route_clear, 1, 512, stream, load, c.n_expert);
     const bool scores = bias || (groups > 1 && c.group_top > 1);
     // With load as many tokens as a work-group has waves are one work-group's, which counts (13 tokens of 160 experts with
-    // groups 10.6 us, two tokens a wave 17.0; another launch is 2 to 3); more are dealt to at most eight waves a SIMD.
+    // groups 10.6 us, two tokens a wave 17.0; another launch is 2 to 3); more are dealt to as many work-groups as the CUs
+    // hold at once, three a CU or, of the scores' larger ones, two (16384 x 512 without a bias with 768 of them 13.3 us, with
+    // 512 15.7, with 1024 14.8; with one 41.5, 39.8, 43.6).
     const bool one = load && ntok <= (scores && c.n_expert > 256 ? 8u : 16u);
-    const uint32_t waves = std::min(ntok, one ? 16u : 8u), blocks = one ? 1 : std::min((ntok + waves - 1) / waves, 1024u);
+    const uint32_t waves = std::min(ntok, one ? 16u : 8u), blocks = one ? 1 : std::min((ntok + waves - 1) / waves, scores ? 512u : 768u);
     const auto run = [&](auto kernel, auto *p) {
       op_launch_lds(kernel, blocks, 64 * waves, 2048 + waves * (uint32_t)sizeof(RouteScratch), stream, a, p, stride, bias, ntok,
                     ids, w, load);
