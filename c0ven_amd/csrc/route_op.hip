@@ -236,6 +236,26 @@ __device__ __forceinline__ uint32_t select_ranks(const uint32_t (&key)[kPer], ui
   return k;
 }
 
+// A row's kPer values from column c on (0 past cols), in one load where all are there.
+template <uint32_t kType, int kPer>
+__device__ __forceinline__ void load_run(const typename Elem<kType>::T *row, uint32_t c, uint32_t cols, float (&v)[kPer]) {
+  typedef typename Elem<kType>::T T;
+  struct __attribute__((packed)) Pack {
+    T e[kPer];
+  };
+#pragma unroll
+  for (int j = 0; j < kPer; j++) v[j] = 0.0f;
+  if (c + kPer <= cols) {
+    const Pack p = *(const Pack *)(row + c);
+#pragma unroll
+    for (int j = 0; j < kPer; j++) v[j] = (float)p.e[j];
+  } else if (c < cols) {
+#pragma unroll
+    for (uint32_t j = 0; j < kPer - 1; j++)
+      if (c + j < cols) v[j] = (float)row[c + j];
+  }
+}
+
 // kScores: the order is that of s + bias. Tokens go round the grid's waves. load (or null): one work-group counts it; of
 // several the first clears it for route_count.
 template <uint32_t kType, bool kScores, int kPer>
@@ -275,21 +295,15 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
   uint64_t stays = ~0ull;
   bool decided = false;  // stays, for token t, in fp64
   for (uint32_t t = blockIdx.x * waves + wave; t < ntok;) {
-    float b[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; i++) b[i] = kScores && bias && e0 + i < a.E ? bias[e0 + i] : 0.0f;
+    float b[kPer] = {};
+    if (kScores && bias) load_run<QT_F32, kPer>(bias, e0, a.E, b);
     bool open = false, open_groups = false;
     uint32_t my_key, my_id, floor, total;
     float x[kPer], my_x, my_b = 0.0f, off_s = 0.0f;
     for (; t < ntok; t += step) {
       const typename Elem<kType>::T *row = logits + (uint64_t)t * stride;
       float s[kPer], v[kPer];
-      if constexpr (kPer == 8) {
-        load8<kType>(row, e0, a.E, x);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPer; i++) x[i] = e0 + i < a.E ? (float)row[e0 + i] : 0.0f;
-      }
+      load_run<kType, kPer>(row, e0, a.E, x);
 #pragma unroll
       for (int i = 0; i < kPer; i++) x[i] = x[i] > -INFINITY ? x[i] : -INFINITY;  // (no NaN)
       if (a.E < 64 * kPer) {
