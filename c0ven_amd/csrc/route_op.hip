@@ -10,9 +10,10 @@
 // bounds, the wave decides that in fp64: among the candidates, or among all where too many are near. Equal logits under equal biases need no bound: their order
 // is by id either way.
 //
-// Bound by the launch where tokens are few (one of 512 experts, top 10: 4.6 us), else by the instructions of a token, some 600
-// a wave: 16384 x 512 fp32, top 10, 17.5 us (1.9 TB/s; the logits alone are 6.8 us at 5.1) and 4.3 for the load. 999 x 256 bf16
-// with biases and groups 11.5 and 3 us: one token a wave, its latency, and some tokens' fp64.
+// Bound by the launch where tokens are few (one of 512 experts, top 10: 4.2 us), else by the instructions of a token, some 330
+// vector ones a wave: 16384 x 512 fp32, top 10, 13.0 us (2.6 TB/s; the logits alone are 6.8 us at 5.1) and 3.5 for the load;
+// with biases 32 us. 999 x 256 bf16 with biases and groups 7.1 and 2.5 us: one token a wave, its latency, and some tokens'
+// fp64.
 #include "device_math.h"
 #include "mx4.h"
 #include "ops.h"
@@ -27,8 +28,9 @@ struct RouteArgs {
   float scale;
 };
 
-// The same values as ones of their own to the compiler: what is computed from them where few tokens come is not computed
-// before the loop that all pass (16 x 256 with groups 7.9 us, 7.5 with this).
+// The same values as ones of their own to the compiler, so that what is computed from them stays where it is used: it moved
+// some 30 conditions before the tokens' loop and kept them, two scalars each, in lanes of a register (999 x 256 with groups
+// 9.6 us, 7.1 with this).
 __device__ __forceinline__ RouteArgs apart(RouteArgs a) {
   asm volatile("" : "+s"(a.E), "+s"(a.K), "+s"(a.groups), "+s"(a.kept), "+s"(a.best), "+s"(a.sigmoid));
   return a;
@@ -301,20 +303,23 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
     uint32_t my_key, my_id, floor, total;
     float x[kPer], my_x, my_b = 0.0f, off_s = 0.0f;
     for (; t < ntok; t += step) {
+      const RouteArgs h = apart(a);  // (the arguments, here)
+      uint32_t lanes_of = run;
+      asm volatile("" : "+s"(lanes_of));
       const typename Elem<kType>::T *row = logits + (uint64_t)t * stride;
       float s[kPer], v[kPer];
-      load_run<kType, kPer>(row, e0, a.E, x);
+      load_run<kType, kPer>(row, e0, h.E, x);
 #pragma unroll
       for (int i = 0; i < kPer; i++) x[i] = x[i] > -INFINITY ? x[i] : -INFINITY;  // (no NaN)
-      if (a.E < 64 * kPer) {
+      if (h.E < 64 * kPer) {
 #pragma unroll
-        for (int i = 0; i < kPer; i++) x[i] = e0 + i < a.E ? x[i] : -INFINITY;
+        for (int i = 0; i < kPer; i++) x[i] = e0 + i < h.E ? x[i] : -INFINITY;
       }
       float top = x[0], sum = 0.0f;
 #pragma unroll
       for (int i = 1; i < kPer; i++) top = fmaxf(top, x[i]);
       top = key_float(wave_max_u32(float_key(top)));
-      if (!a.sigmoid && (kScores || !a.renorm)) {
+      if (!h.sigmoid && (kScores || !h.renorm)) {
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
           const float p = exp_f32(x[i] - top);
@@ -324,8 +329,8 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
         }
         sum = wave_sum_f32(sum);
       }
-      const float per_sum = a.sigmoid ? 1.0f : __builtin_amdgcn_rcpf(sum);
-      if (kScores && a.sigmoid) {
+      const float per_sum = h.sigmoid ? 1.0f : __builtin_amdgcn_rcpf(sum);
+      if (kScores && h.sigmoid) {
 #pragma unroll
         for (int i = 0; i < kPer; i++) s[i] = __builtin_amdgcn_rcpf(1.0f + exp_f32(-x[i]));
       }
@@ -337,19 +342,19 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
       // A score's bound: a few units of its own for the exponential, the quotient and a softmax's sum, and |x - top| of
       // them for the difference, of which e^(x - top) |x - top| <= 0.37 stays: within 2^-20 of the largest score.
       off_s = per_sum * 0x1p-20f + 0x1p-120f;
-      if (a.groups > 1 && !decided) {
+      if (h.groups > 1 && !decided) {
         float b1 = -INFINITY, b2 = -INFINITY;
-        uint32_t at = lane;  // this lane's group; of a run of lanes a group, each has it
-        if (run) {
+        uint32_t at = lane;  // this lane's group; of a lanes_of of lanes a group, each has it
+        if (lanes_of) {
 #pragma unroll
           for (int i = 0; i < kPer; i++) b2 = fmaxf(b2, fminf(b1, v[i])), b1 = fmaxf(b1, v[i]);
           const auto merge = [&](float o1, float o2) { b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2)), b1 = fmaxf(b1, o1); };
-          if (run > 1) merge(dpp_f32<kDppXor1>(b1), dpp_f32<kDppXor1>(b2));
-          if (run > 2) merge(dpp_f32<kDppXor2>(b1), dpp_f32<kDppXor2>(b2));
-          if (run > 4) merge(dpp_f32<kDppHalfMirror>(b1), dpp_f32<kDppHalfMirror>(b2));
-          if (run > 8) merge(dpp_f32<kDppMirror>(b1), dpp_f32<kDppMirror>(b2));
-          if (run > 16) merge(__shfl_xor(b1, 16, 64), __shfl_xor(b2, 16, 64));
-          if (run > 32) merge(__shfl_xor(b1, 32, 64), __shfl_xor(b2, 32, 64));
+          if (lanes_of > 1) merge(dpp_f32<kDppXor1>(b1), dpp_f32<kDppXor1>(b2));
+          if (lanes_of > 2) merge(dpp_f32<kDppXor2>(b1), dpp_f32<kDppXor2>(b2));
+          if (lanes_of > 4) merge(dpp_f32<kDppHalfMirror>(b1), dpp_f32<kDppHalfMirror>(b2));
+          if (lanes_of > 8) merge(dpp_f32<kDppMirror>(b1), dpp_f32<kDppMirror>(b2));
+          if (lanes_of > 16) merge(__shfl_xor(b1, 16, 64), __shfl_xor(b2, 16, 64));
+          if (lanes_of > 32) merge(__shfl_xor(b1, 32, 64), __shfl_xor(b2, 32, 64));
           at = e0 / n;
         } else if (n % kPer == 0) {
           // Lane g joins its group's lanes' largest two.
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
           lds_done();
           b1 = b2 = -INFINITY;
           const uint32_t lanes = n / kPer;
-          if (lane < a.groups)
+          if (lane < h.groups)
             for (uint32_t j = 0; j < lanes; j++) {
               const float2 o = lds.best[lane * lanes + j];
               b2 = fmaxf(fminf(b1, o.x), fmaxf(b2, o.y)), b1 = fmaxf(b1, o.x);
@@ -369,9 +374,9 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
           // Lane g goes through group g's values, from a place of its own on, so that the lanes' banks differ.
 #pragma unroll
           for (int i = 0; i < kPer; i++)
-            if (e0 + i < a.E) lds.v[e0 + i] = v[i];
+            if (e0 + i < h.E) lds.v[e0 + i] = v[i];
           lds_done();
-          if (lane < a.groups)
+          if (lane < h.groups)
 #pragma unroll 8
             for (uint32_t j = 0, k = lane % n; j < n; j++, k = k + 1 == n ? 0 : k + 1) {
               const float o = lds.v[lane * n + k];
@@ -379,21 +384,21 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
             }
           lds_done();
         }
-        const float mine = a.best > 1 && b2 > -INFINITY ? b1 + b2 : b1;
+        const float mine = h.best > 1 && b2 > -INFINITY ? b1 + b2 : b1;
         uint32_t place = 0;
-        for (uint32_t g = 0; g < a.groups; g++) {
-          const float o = lane_f32(mine, run ? g * run : g);
+        for (uint32_t g = 0; g < h.groups; g++) {
+          const float o = lane_f32(mine, lanes_of ? g * lanes_of : g);
           place += o > mine || (o == mine && g < at);
         }
-        const uint64_t keep = __ballot(at < a.groups && place < a.kept);
+        const uint64_t keep = __ballot(at < h.groups && place < h.kept);
         stays = keep;
-        if (run > 1) {
+        if (lanes_of > 1) {
           stays = 0;
-          for (uint32_t g = 0; g < a.groups; g++) stays |= (keep >> (g * run) & 1) << g;
+          for (uint32_t g = 0; g < h.groups; g++) stays |= (keep >> (g * lanes_of) & 1) << g;
         }
-        if (kScores && a.kept < a.groups) {
-          const uint32_t in = (uint32_t)__ffsll(__ballot(at < a.groups && place == a.kept - 1)) - 1;
-          const uint32_t out = (uint32_t)__ffsll(__ballot(at < a.groups && place == a.kept)) - 1;
+        if (kScores && h.kept < h.groups) {
+          const uint32_t in = (uint32_t)__ffsll(__ballot(at < h.groups && place == h.kept - 1)) - 1;
+          const uint32_t out = (uint32_t)__ffsll(__ballot(at < h.groups && place == h.kept)) - 1;
           const float wi = lane_f32(mine, in), wo = lane_f32(mine, out);
           // Four scores, and the roundings of their sums.
           open_groups = wo > -INFINITY && !(wi - wo > 4.0f * off_s + 0x1p-20f * (fabsf(wi) + fabsf(wo)));
@@ -403,17 +408,17 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
       uint32_t key[kPer];
 #pragma unroll
       for (int i = 0; i < kPer; i++) key[i] = float_key(v[i]);
-      if (a.groups > 1) {
+      if (h.groups > 1) {
 #pragma unroll
         for (int i = 0; i < kPer; i++) key[i] = stays >> ((e0 + i) * per_group >> 20) & 1 ? key[i] : 0u;
       }
       // (A few ranks past the last, so that what an open order may move lies among them.)
-      total = select_ranks<kPer>(key, kScores ? a.K + 4 : a.K, lds, my_key, my_id, floor);
-      const bool mine = my_key != 0 && lane <= a.K;
+      total = select_ranks<kPer>(key, kScores ? h.K + 4 : h.K, lds, my_key, my_id, floor);
+      const bool mine = my_key != 0 && lane <= h.K;
       my_x = my_key != 0 ? (float)row[my_id] : -INFINITY;
       float my_s;
-      if (kScores || a.sigmoid || !a.renorm)
-        my_s = a.sigmoid ? 1.0f / (1.0f + exp_f32(-my_x)) : (my_x == top ? 1.0f : exp_f32(my_x - top)) / sum;
+      if (kScores || h.sigmoid || !h.renorm)
+        my_s = h.sigmoid ? 1.0f / (1.0f + exp_f32(-my_x)) : (my_x == top ? 1.0f : exp_f32(my_x - top)) / sum;
       else  // with renorm the common factor drops out: relative to the first chosen
         my_s = my_x == lane_f32(my_x, 0) ? 1.0f : exp_f32(my_x - lane_f32(my_x, 0));
       if (kScores) {
@@ -424,7 +429,7 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
         const uint32_t nk = __shfl(my_key, next, 64);
         const float nx = __shfl(my_x, next, 64), nb = __shfl(my_b, next, 64), nv = key_float(nk);
         const float off = 2.0f * off_s + 0x1p-22f * (fabsf(my_v) + fabsf(nv));
-        open = __any(lane < a.K && mine && nk != 0 && !(nx == my_x && nb == my_b) && !(my_v - nv > off));
+        open = __any(lane < h.K && mine && nk != 0 && !(nx == my_x && nb == my_b) && !(my_v - nv > off));
         if (open) break;
       }
       finish(t, mine ? my_id : ~0u, my_s);
