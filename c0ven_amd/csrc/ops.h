@@ -24,7 +24,9 @@ inline void op_require(bool ok, const char *why) {
   if (!ok) throw OpError(MOE_BAD_ARGUMENT, why);
 }
 inline void op_check(hipError_t e, const char *what) {
-  if (e != hipSuccess) throw OpError(MOE_ERROR, std::string(what) + ": " + hipGetErrorString(e));
+  if (e == hipSuccess) return;
+  (void)hipGetLastError();  // (this call's error is not the next one's)
+  throw OpError(MOE_ERROR, std::string(what) + ": " + hipGetErrorString(e));
 }
 
 // An operator's call: f checks and launches; what it throws becomes the status and the message.

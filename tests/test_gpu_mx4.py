@@ -279,6 +279,7 @@ def test_no_such_device():
     for device in (99, -1):
         with pytest.raises(moe.MoeError):
             moe.mx4_quantize_async(moe.QT_F32, b.ptr, m, device=device)
+        assert hip.rt.hipGetLastError() == 0  # nothing is left for whoever asks next
     assert (codes.get() == 0xA5).all()
     moe.mx4_quantize_async(moe.QT_F32, b.ptr, m)
     assert np.array_equal(codes.get()[:3], ref.mx4_quantize(x.astype(np.float64))[0])
