@@ -100,9 +100,8 @@ struct MxSource {
 
 // A work-group's kWaves waves on a tile of BM rows of x and BN rows of w: WM of them along x's rows, WN along w's, each on
 // TM runs of 32 rows of x and TN runs of 32 rows of w. kApart: a wave's runs of w lie 32 times the waves apart (gate's rows
-// and up's), else they follow one another. kAcross: a lane's sums are one w row's with 16 of x's, instead of one x row's with 16
-// of w's. The operands are one step of k = 64 ahead of the matrix instructions, in
-// registers, across the stages.
+// and up's), else they follow one another. kAcross: a lane's sums are one w row's with 16 of x's, instead of one x row's with
+// 16 of w's. The operands are one step of k = 64 ahead of the matrix instructions, in registers, across the stages.
 template <int TM, int TN, int WM = 2, bool kApart = false, bool kAcross = false, int kWaves = 4>
 struct MxTile {
   static constexpr int WN = kWaves / WM, BM = 32 * WM * TM, BN = 32 * WN * TN;

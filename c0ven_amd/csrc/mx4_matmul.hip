@@ -269,7 +269,7 @@ void launch_matmul(const uint8_t *xc, const uint8_t *xs, uint32_t M, const moe_m
   });
 }
 
-void op_size(uint64_t M, uint64_t N) { op_require(M * N <= 1ull << 38, "y of more than 2^38 elements"); }
+void op_results(uint64_t M, uint64_t N) { op_require(M * N <= 1ull << 38, "y of more than 2^38 elements"); }
 
 // x's rows quantised, in a work buffer.
 uint64_t quantised_bytes(uint32_t rows, uint32_t cols) {
@@ -296,7 +296,7 @@ MOE_API moe_status moe_mx4_matmul_async(int32_t device, const moe_mx4_matrix *x,
     op_mx4(x);
     op_mx4(w);
     op_require(x->cols == w->cols, "x and w must have the same cols");
-    op_size(x->rows, w->rows);
+    op_results(x->rows, w->rows);
     op_rows(y, y_stride, w->rows, y_type);
     op_work(work, work_bytes, moe_mx4_matmul_work_bytes(w, x->rows));
     if (!x->rows || !w->rows) return;
@@ -318,7 +318,7 @@ MOE_API moe_status moe_mx4_linear_async(int32_t device, uint32_t x_type, const v
     op_rows(x, x_stride, w->cols, x_type);
     op_rows(y, y_stride, w->rows, y_type);
     op_require(ntok <= 1u << 27, "at most 2^27 tokens");
-    op_size(ntok, w->rows);
+    op_results(ntok, w->rows);
     op_work(work, work_bytes, moe_mx4_linear_work_bytes(w, ntok));
     if (!ntok || !w->rows) return;
     OnDevice on(device);
