@@ -549,7 +549,8 @@ struct Plan {
     pitch = (e.n_embd + 255) / 256 * 256;
     // The sums of all assignments at once, or of as many columns at a time as 256 MB hold, about the last-level cache (4096
     // tokens of 10 experts: 335 MB of sums, 304 us; 96 MB at a time 312, all at once 303, but up to 17 GB of work).
-    chunk = std::min<uint64_t>(pitch, std::max<uint64_t>(256, kChunkBytes / (4ull * A) / 256 * 256));
+    // (few: there are no such sums, and A may be 0.)
+    chunk = few ? pitch : std::min<uint64_t>(pitch, std::max<uint64_t>(256, kChunkBytes / (4ull * A) / 256 * 256));
     max_tiles = std::min(A, e.n_expert + A / rows);
     uint64_t at = 0;
     const auto part = [&](uint64_t n) {

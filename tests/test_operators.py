@@ -121,6 +121,15 @@ def test_experts_refuses_buffers():
         refused(lambda: e.forward_async(**{**good, **bad}))
 
 
+@pytest.mark.parametrize("E", [8, 512])
+def test_experts_of_no_tokens(E):
+    """No work, nothing to do, no device touched."""
+    e = experts(E=E)
+    assert e.work_bytes(0) == 0
+    e.forward_async(P, 0, P, P, P, None, 0)
+    refused(lambda: e.forward_async(P, 0, P, P, P, None, 0, x_stride=255))
+
+
 def test_null_descriptions():
     assert _lib.lib.moe_route_async(None, P, 8, None, 1, P, P, None, None) == _lib.MOE_BAD_ARGUMENT
     assert _lib.lib.moe_mx4_experts_async(None, P, 8, 1, P, P, P, 8, P, 8, None) == _lib.MOE_BAD_ARGUMENT
