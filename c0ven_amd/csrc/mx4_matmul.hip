@@ -285,7 +285,7 @@ bool quantises_itself(uint32_t M, uint32_t cols) {
 extern "C" {
 
 MOE_API uint64_t moe_mx4_matmul_work_bytes(const moe_mx4_matrix *w, uint32_t ntok) {
-  if (!w || !w->cols || ntok <= kFewRows || !w->rows) return 0;
+  if (!w || !mx4_sizes(*w) || ntok <= kFewRows || ntok > kMxMostRows || !w->rows) return 0;
   return Plan(ntok, w->rows, mx_steps(w->cols)).bytes(ntok, w->rows);
 }
 
@@ -306,7 +306,7 @@ MOE_API moe_status moe_mx4_matmul_async(int32_t device, const moe_mx4_matrix *x,
 }
 
 MOE_API uint64_t moe_mx4_linear_work_bytes(const moe_mx4_matrix *w, uint32_t ntok) {
-  if (!w || !w->cols || quantises_itself(ntok, w->cols)) return 0;
+  if (!w || !mx4_sizes(*w) || ntok > kMxMostRows || quantises_itself(ntok, w->cols)) return 0;
   return quantised_bytes(ntok, w->cols) + moe_mx4_matmul_work_bytes(w, ntok);
 }
 
@@ -317,7 +317,7 @@ MOE_API moe_status moe_mx4_linear_async(int32_t device, uint32_t x_type, const v
     op_mx4(w);
     op_rows(x, x_stride, w->cols, x_type);
     op_rows(y, y_stride, w->rows, y_type);
-    op_require(ntok <= 1u << 27, "at most 2^27 tokens");
+    op_require(ntok <= kMxMostRows, "at most 2^27 tokens");
     op_results(ntok, w->rows);
     op_work(work, work_bytes, moe_mx4_linear_work_bytes(w, ntok));
     if (!ntok || !w->rows) return;

@@ -367,7 +367,8 @@ MOE_API moe_status moe_mx4_dequantize_async(int32_t device, const moe_mx4_matrix
 
 /* y = x w^T (y x->rows x w->rows of y_type, at most 2^38 elements, rows y_stride apart): the MX4 values' products summed in
  * fp32 on the matrix cores and rounded once. x->cols == w->cols. work: at least moe_mx4_matmul_work_bytes(w, x->rows)
- * bytes, 16-byte aligned (may be null where that is 0). */
+ * bytes, 16-byte aligned (may be null where that is 0). The sizes of work look at a description's rows and cols alone and
+ * are 0 where the call refuses them. */
 MOE_API uint64_t moe_mx4_matmul_work_bytes(const moe_mx4_matrix *w, uint32_t ntok);
 MOE_API moe_status moe_mx4_matmul_async(int32_t device, const moe_mx4_matrix *x, const moe_mx4_matrix *w,
                                         uint32_t y_type, void *y, uint64_t y_stride, void *work, uint64_t work_bytes,

@@ -95,6 +95,22 @@ def test_mx4_refuses_buffers():
         _lib._op(_lib.lib.moe_mx4_quantize_async(0, moe.QT_F32, P, 256, None, None))
 
 
+@pytest.mark.parametrize("cols", [0, (1 << 20) + 1, 0xFFFFFF00, 0xFFFFFF81, 0xFFFFFFFF])
+@pytest.mark.parametrize("rows,ntok", [(64, 40), (64, 4000), ((1 << 27) + 1, 40), (64, 1)])
+def test_work_of_refused_sizes(rows, ntok, cols):
+    """Sizes that the calls refuse ask for no work, where 32 bits hold no row's length rounded up among them."""
+    m = mat(rows, cols)
+    assert moe.mx4_matmul_work_bytes(m, ntok) == 0 and moe.mx4_linear_work_bytes(m, ntok) == 0
+
+
+def test_work_of_sizes():
+    m = mat(64, 1 << 20, None, None)
+    assert moe.mx4_matmul_work_bytes(m, 40) > 0 and moe.mx4_linear_work_bytes(m, 40) > 0
+    for rows, ntok in (((1 << 27) + 1, 40), (64, (1 << 27) + 1)):
+        m = mat(rows, 256)
+        assert moe.mx4_matmul_work_bytes(m, ntok) == 0 and moe.mx4_linear_work_bytes(m, ntok) == 0
+
+
 def experts(E=8, H=256, F=96, K=2, gate=None, up=None, down=None, **kw):
     return moe.Mx4Experts(H, F, E, K, gate or mat(F, H), up or mat(F, H), down or mat(H, F), **kw)
 
