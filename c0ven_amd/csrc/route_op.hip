@@ -422,15 +422,30 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
       else  // with renorm the common factor drops out: relative to the first chosen
         my_s = my_x == lane_f32(my_x, 0) ? 1.0f : exp_f32(my_x - lane_f32(my_x, 0));
       if (kScores) {
-        // Rank r against rank r + 1 (any later one's value is no larger, and its bound is the same).
+        // Rank r against rank r + 1 (any later one's value is no larger, and its bound is the same). Where the last rank's
+        // equal is next, with it every expert that is no larger: what is not its equal may be larger in fp64 than both.
         my_b = my_key != 0 && bias ? bias[my_id] : 0.0f;
         const float my_v = key_float(my_key);
         const uint32_t next = (lane + 1) & 63;
         const uint32_t nk = __shfl(my_key, next, 64);
         const float nx = __shfl(my_x, next, 64), nb = __shfl(my_b, next, 64), nv = key_float(nk);
         const float off = 2.0f * off_s + 0x1p-22f * (fabsf(my_v) + fabsf(nv));
-        open = __any(lane < h.K && mine && nk != 0 && !(nx == my_x && nb == my_b) && !(my_v - nv > off));
+        const bool equal = nx == my_x && nb == my_b;
+        open = __any(lane < h.K && mine && nk != 0 && !equal && !(my_v - nv > off));
         if (open) break;
+        if (__any(lane == h.K - 1 && mine && nk != 0 && equal)) {
+          const uint32_t last = readlane_u32(my_key, (int)h.K - 1);
+          const float lv = key_float(last), lx = lane_f32(my_x, h.K - 1), lb = lane_f32(my_b, h.K - 1);
+          bool near = false;
+#pragma unroll
+          for (int i = 0; i < kPer; i++) {
+            const float o = key_float(key[i]);
+            near |= key[i] > kNoKey && key[i] <= last && !(x[i] == lx && b[i] == lb) &&
+                    !(lv - o > 2.0f * off_s + 0x1p-22f * (fabsf(lv) + fabsf(o)));
+          }
+          open = __any(near);
+          if (open) break;
+        }
       }
       finish(t, mine ? my_id : ~0u, my_s);
       decided = false;

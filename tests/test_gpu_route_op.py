@@ -176,3 +176,29 @@ def test_graph():
             assert np.array_equal(a.get(), b.get())
         assert np.array_equal(out[0][0].get(), ref.route(x.get(), K, True)[0])
         assert int(out[0][2].get().sum()) == T * K
+
+
+@pytest.mark.parametrize("E", [64, 100, 256, 512])
+@pytest.mark.parametrize("grouped", [False, True])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_equal_at_the_last_rank(sigmoid, grouped, E):
+    """Equal experts at the last rank and behind it, and, further behind in 32 bits, one that is larger in 64: from one such
+    expert more than the ranks to all of them, more than a wave's candidates."""
+    print("equal at the last rank", sigmoid, grouped, E, flush=True)
+    K, n = 4, (3, 4, 5, 7, 9, 40, E - 3)
+    x = np.full((4 * len(n), E), -6.0)
+    for i, m in enumerate(n):
+        for j, at in enumerate((E - 1, E // 2, 0, E - 2)):
+            x[4 * i + j, :m] = 20.0
+            x[4 * i + j, at] = 25.0 if j < 3 else 19.5
+    bias = np.zeros(E)
+    if not sigmoid:  # scores far below the bias that all have: e^(20 - 60)
+        x[:, E - 3] = 60.0
+        bias += 1.0
+        bias[E - 3] = -2.0
+    groups = dict(groups=4, kept=3, best=2) if grouped else {}
+    check(x, K, "f32", sigmoid, bias, **groups)
+    check(x, K, "bf16", sigmoid, bias, renorm=False, **groups)
+    if sigmoid and grouped:
+        check(x, K, "f32", sigmoid, None, **groups)
+    check(np.full((3, E), 20.0), K, "f32", sigmoid, np.zeros(E), **groups)
