@@ -434,15 +434,14 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
         open = __any(lane < h.K && mine && nk != 0 && !equal && !(my_v - nv > off));
         if (open) break;
         if (__any(lane == h.K - 1 && mine && nk != 0 && equal)) {
+          // (o is near v if v - o <= 2 off_s + 2^-22 (|v| + |o|), so v - o is at most this:)
           const uint32_t last = readlane_u32(my_key, (int)h.K - 1);
           const float lv = key_float(last), lx = lane_f32(my_x, h.K - 1), lb = lane_f32(my_b, h.K - 1);
+          const float gap = 2.01f * off_s + 0x1.2p-21f * fabsf(lv);
+          const uint32_t low = max(float_key(lv < INFINITY ? lv - gap : lv), kNoKey + 1);
           bool near = false;
 #pragma unroll
-          for (int i = 0; i < kPer; i++) {
-            const float o = key_float(key[i]);
-            near |= key[i] > kNoKey && key[i] <= last && !(x[i] == lx && b[i] == lb) &&
-                    !(lv - o > 2.0f * off_s + 0x1p-22f * (fabsf(lv) + fabsf(o)));
-          }
+          for (int i = 0; i < kPer; i++) near |= (key[i] >= low) & (key[i] <= last) & ((x[i] != lx) | (b[i] != lb));
           open = __any(near);
           if (open) break;
         }
