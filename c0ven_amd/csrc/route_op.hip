@@ -400,8 +400,12 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
           const uint32_t in = (uint32_t)__ffsll(__ballot(at < h.groups && place == h.kept - 1)) - 1;
           const uint32_t out = (uint32_t)__ffsll(__ballot(at < h.groups && place == h.kept)) - 1;
           const float wi = lane_f32(mine, in), wo = lane_f32(mine, out);
-          // Four scores, and the roundings of their sums.
-          open_groups = wo > -INFINITY && !(wi - wo > 4.0f * off_s + 0x1p-20f * (fabsf(wi) + fabsf(wo)));
+          // Every group against halfway between the last kept and the next: two scores, and their sums' roundings, which are
+          // those of the larger value where the two cancel.
+          const float half = 0.5f * wi + 0.5f * wo;
+          const float off = 2.0f * off_s + 0x1p-20f * (h.best > 1 && b2 > -INFINITY ? fabsf(b1) + fabsf(b2) : fabsf(b1));
+          const bool far = place < h.kept ? mine - off > half : mine + off < half;
+          open_groups = wo > -INFINITY && __any(at < h.groups && mine > -INFINITY && !far);
           if (open_groups) break;
         }
       }

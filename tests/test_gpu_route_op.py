@@ -202,3 +202,21 @@ def test_equal_at_the_last_rank(sigmoid, grouped, E):
     if sigmoid and grouped:
         check(x, K, "f32", sigmoid, None, **groups)
     check(np.full((3, E), 20.0), K, "f32", sigmoid, np.zeros(E), **groups)
+
+
+@pytest.mark.parametrize("E,groups", [(32, 8), (60, 4), (128, 16), (256, 8), (512, 64), (500, 5)])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_groups_whose_biases_cancel(sigmoid, E, groups):
+    """A group's worth of one large and one as small value: its roundings are those of the values, not of their sum."""
+    print("cancelling biases", sigmoid, E, groups, flush=True)
+    x = logits(40, E, E)
+    n = E // groups
+    bias = np.zeros(E)
+    for g in range(0, groups, 2):
+        bias[g * n:(g + 1) * n] = -2.0 ** 26
+        bias[g * n], bias[g * n + 1] = 2.0 ** 24, -2.0 ** 24
+    for kept in (1, groups // 2, groups - 1):
+        check(x, 4, "f32", sigmoid, bias, groups, kept, 2)
+    bias[:] = 0.0
+    bias[:n], bias[n], bias[-1] = -1e9, 1e30, -3e38  # masked by a large number; one that is always chosen
+    check(x, 4, "f32", sigmoid, bias, groups, groups // 2, 2)
