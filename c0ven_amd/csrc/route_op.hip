@@ -541,7 +541,8 @@ extern "C" MOE_API moe_status moe_route_async(const moe_route_config *cfg, const
     if (!ntok && !load) return;
     OnDevice on(c.device);
     if (!ntok) return op_launch(route_clear, 1, 512, stream, load, c.n_expert);
-    const bool scores = bias || (groups > 1 && c.group_top > 1);
+    // The order is the scores', also where all groups are kept: logits that are apart may have equal ones in 64 bits.
+    const bool scores = bias || (c.n_group > 1 && c.group_top > 1);
     // With load as many tokens as a work-group has waves are one work-group's, which counts (13 tokens of 160 experts with
     // groups 10.6 us, two tokens a wave 17.0; another launch is 2 to 3); more are dealt to as many work-groups as the CUs
     // hold at once, three a CU or, of the scores' larger ones, two (16384 x 512 without a bias with 768 of them 13.3 us, with

@@ -220,3 +220,16 @@ def test_groups_whose_biases_cancel(sigmoid, E, groups):
     bias[:] = 0.0
     bias[:n], bias[n], bias[-1] = -1e9, 1e30, -3e38  # masked by a large number; one that is always chosen
     check(x, 4, "f32", sigmoid, bias, groups, groups // 2, 2)
+
+
+@pytest.mark.parametrize("E,groups", [(8, 2), (64, 8), (96, 3), (256, 8), (512, 4)])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_all_groups_kept(sigmoid, E, groups):
+    """A group's worth of two values: the order is the scores' in 64 bits, also where no group is left out."""
+    print("all groups kept", sigmoid, E, groups, flush=True)
+    x = logits(60, E, E + groups)
+    x[::3] += 40.0  # sigmoids that are all 1 in 64 bits
+    x[1::3] *= 1e-18  # exponentials and sigmoids that are all equal
+    check(x, 4, "f32", sigmoid, None, groups, groups, 2)
+    check(x, 4, "bf16", sigmoid, None, groups, groups, 2, renorm=False)
+    check(x, 4, "f32", sigmoid, None, groups, groups, 1)  # the logits' own order
