@@ -77,6 +77,30 @@ __device__ __forceinline__ void lds_done() {  // this wave's LDS accesses
   __builtin_amdgcn_wave_barrier();
 }
 
+// Chosen scores are held 2^70 times as large where they may be tiny: over the renormaliser's floor of 1e-20 the weights are
+// numbers of fp32 down to scores of 2^-192. A token whose order is the scores' is left to fp64 where a chosen one is below
+// kTiny (scores lifted in fp32 there too: 999 x 256 with groups 9.6 us, 9.4).
+constexpr float kLift = 0x1p70f;
+constexpr float kTiny = 0x1p-60f;
+// exp(z) as exp_f32, or where far (z < -80) kLift times it.
+__device__ __forceinline__ float exp_lifted(float z, bool far) {
+  z = z < -200.0f ? -200.0f : z > 89.0f ? 89.0f : z;
+  const float hi = z * 1.4426950216e+0f;
+  const float lo = __builtin_fmaf(z, 1.9259629911e-8f, __builtin_fmaf(z, 1.4426950216e+0f, -hi));
+  return __builtin_amdgcn_exp2f(far ? hi + 70.0f : hi) * __builtin_fmaf(lo, 0.69314718f, 1.0f);
+}
+// kLift times a sigmoid, and times a softmax's score of the largest logit top and the sum of e^(x - top).
+__device__ __forceinline__ float lifted_sigmoid(float x) {
+  const bool far = x < -80.0f;  // (1 + e^x is 1)
+  const float e = exp_lifted(far ? x : -x, far);
+  return far ? e : kLift / (1.0f + e);
+}
+__device__ __forceinline__ float lifted_softmax(float x, float top, float sum) {
+  const bool far = x - top < -80.0f;
+  const float e = exp_lifted(x - top, far);
+  return (x == top ? kLift : far ? e : kLift * e) / sum;
+}
+
 // The scores in fp64 of the lanes' logits (minus infinity: no score): a softmax's largest logit and sum (1 for a sigmoid).
 struct Exact {
   double top = -INFINITY, sum = 1.0;
@@ -130,7 +154,7 @@ __device__ __forceinline__ uint64_t exact_groups(const RouteArgs &a, const doubl
 
 struct Ranked {
   uint32_t id;  // ~0: none
-  float s;
+  float s;      // kLift times its score
 };
 // The ranks in fp64 among the candidates that lanes 0 .. total - 1 hold (id, logit, bias): lane r receives rank r.
 __device__ __forceinline__ Ranked exact_ranks(const RouteArgs &a, const Exact &e, uint32_t total, uint32_t id, float x, float b) {
@@ -143,7 +167,7 @@ __device__ __forceinline__ Ranked exact_ranks(const RouteArgs &a, const Exact &e
   }
   const int to = 4 * (int)(lane < total ? rank : lane);
   const uint32_t ri = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)id);
-  const float rs = __uint_as_float((uint32_t)__builtin_amdgcn_ds_permute(to, (int)__float_as_uint((float)s)));
+  const float rs = __uint_as_float((uint32_t)__builtin_amdgcn_ds_permute(to, (int)__float_as_uint((float)(s * (double)kLift))));
   return lane < total ? Ranked{ri, rs} : Ranked{~0u, 0.0f};
 }
 // The ranks of the values in d (changed) among the experts of the groups that stay, one after the other.
@@ -167,7 +191,7 @@ __device__ __forceinline__ Ranked exact_all(const RouteArgs &a, const Exact &e, 
     if (lane == k) mine.id = id;
   }
   lds_done();
-  if (mine.id != ~0u) mine.s = (float)e.score(a, (float)row[mine.id]);
+  if (mine.id != ~0u) mine.s = (float)(e.score(a, (float)row[mine.id]) * (double)kLift);
   return mine;
 }
 
@@ -276,7 +300,8 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
     for (uint32_t e = threadIdx.x; e < a.E; e += blockDim.x) load[e] = 0;
   }
   const uint32_t step = gridDim.x * waves, n = a.groups > 1 ? a.E / a.groups : a.E;
-  const auto finish = [&](uint32_t t, uint32_t id, float score) {  // lane r < K: rank r's expert (~0: none)
+  // lane r < K: rank r's expert (~0: none) and its score, or kLift times it
+  const auto finish = [&](uint32_t t, uint32_t id, float score, bool lifted) {
     if (id == ~0u || lane >= a.K) score = 0.0f;
     float all_s = score;  // the sum of the first sixteen lanes
     all_s += dpp_f32<kDppXor1>(all_s);
@@ -286,7 +311,7 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
     if (lane >= a.K) return;
     const uint64_t at = (uint64_t)t * a.K + lane;
     ids[at] = (int32_t)id;
-    w[at] = (a.renorm ? score / fmaxf(all_s, 1e-20f) : score) * a.scale;
+    w[at] = (a.renorm ? score / fmaxf(all_s, lifted ? 1e-20f * kLift : 1e-20f) : lifted ? score * (1.0f / kLift) : score) * a.scale;
     if (counts && id != ~0u) atomicAdd(count + id, 1u);
   };
   // The tokens whose order fp32 decides, one after the other; at one that it leaves open the loop is left and entered
@@ -421,10 +446,14 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
       const bool mine = my_key != 0 && lane <= h.K;
       my_x = my_key != 0 ? (float)row[my_id] : -INFINITY;
       float my_s;
-      if (kScores || h.sigmoid || !h.renorm)
+      if (kScores)
         my_s = h.sigmoid ? 1.0f / (1.0f + exp_f32(-my_x)) : (my_x == top ? 1.0f : exp_f32(my_x - top)) / sum;
+      else if (h.sigmoid)
+        my_s = lifted_sigmoid(my_x);
+      else if (!h.renorm)
+        my_s = lifted_softmax(my_x, top, sum);
       else  // with renorm the common factor drops out: relative to the first chosen
-        my_s = my_x == lane_f32(my_x, 0) ? 1.0f : exp_f32(my_x - lane_f32(my_x, 0));
+        my_s = kLift * (my_x == lane_f32(my_x, 0) ? 1.0f : exp_f32(my_x - lane_f32(my_x, 0)));
       if (kScores) {
         // Rank r against rank r + 1 (any later one's value is no larger, and its bound is the same). Where the last rank's
         // equal is next, with it every expert that is no larger: what is not its equal may be larger in fp64 than both.
@@ -435,7 +464,7 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
         const float nx = __shfl(my_x, next, 64), nb = __shfl(my_b, next, 64), nv = key_float(nk);
         const float off = 2.0f * off_s + 0x1p-22f * (fabsf(my_v) + fabsf(nv));
         const bool equal = nx == my_x && nb == my_b;
-        open = __any(lane < h.K && mine && nk != 0 && !equal && !(my_v - nv > off));
+        open = __any(lane < h.K && mine && ((nk != 0 && !equal && !(my_v - nv > off)) || my_s < kTiny));
         if (open) break;
         if (__any(lane == h.K - 1 && mine && nk != 0 && equal)) {
           // (o is near v if v - o <= 2 off_s + 2^-22 (|v| + |o|), so v - o is at most this:)
@@ -450,7 +479,7 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
           if (open) break;
         }
       }
-      finish(t, mine ? my_id : ~0u, my_s);
+      finish(t, mine ? my_id : ~0u, my_s, !kScores);
       decided = false;
     }
     if (!kScores || t >= ntok) break;
@@ -472,7 +501,7 @@ __global__ void __launch_bounds__(kScores && kPer == 8 ? 512 : 1024) moe_route(R
       e.keys(c, x, b, lds.d);
       r = exact_all<kType, kPer>(c, e, logits + (uint64_t)t * stride, stays, lds.d);
     }
-    finish(t, r.id, r.s);
+    finish(t, r.id, r.s, true);
     decided = false;
     t += step;
   }

@@ -233,3 +233,23 @@ def test_all_groups_kept(sigmoid, E, groups):
     check(x, 4, "f32", sigmoid, None, groups, groups, 2)
     check(x, 4, "bf16", sigmoid, None, groups, groups, 2, renorm=False)
     check(x, 4, "f32", sigmoid, None, groups, groups, 1)  # the logits' own order
+
+
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_tiny_scores(sigmoid, biased, renorm):
+    """Tokens whose chosen scores are all far below what fp32 holds: over the renormaliser's floor of 1e-20 their weights are
+    ordinary numbers, down to scores of 1e-57; beside a larger one they are as small as they are."""
+    print("tiny scores", sigmoid, biased, renorm, flush=True)
+    T, E, K = 64, 128, 6
+    r = np.random.default_rng(8)
+    x = -2.2 * np.arange(T)[:, None] - 10.0 * r.random((T, E))  # down to e^-150
+    x[::4, 7] = -45.0
+    bias = np.zeros(E) if biased else None
+    if not sigmoid:
+        x[:, 90] = 0.0  # the softmax's largest logit
+        if biased:
+            bias[90] = -2.0  # never chosen
+    check(x, K, "f32", sigmoid, bias, renorm=renorm)
+    check(x, K, "f32", sigmoid, bias, 8, 5, 2, renorm=renorm)
