@@ -3,6 +3,8 @@
 
 #include "mx4_api.h"
 
+#include <algorithm>
+
 namespace c0ven {
 
 // Both kernels take eight values a thread and kAhead such groups, all loaded before the first is used. A work-group has 256 /
@@ -62,24 +64,33 @@ using namespace c0ven;
 
 namespace {
 
-MxRows rows_of(uint32_t rows, uint32_t cols, uint32_t ahead, uint64_t &blocks) {
+// launch(r0, rows' shape, work-groups) for the rows r0 and on, as many as a launch has threads for (less than 2^32; 2^27 rows of
+// 129 values are two launches).
+template <typename F>
+void by_rows(uint32_t rows, uint32_t cols, uint32_t ahead, F launch) {
   const uint32_t ng = mx_steps(cols) * 16;
   uint32_t shift = 4;
   while (shift < 8 && ahead << shift < ng) shift++;
-  const uint32_t wide = (ng + (ahead << shift) - 1) / (ahead << shift);
-  blocks = (((uint64_t)rows + (256 >> shift) - 1) / (256 >> shift)) * wide;
-  return MxRows{rows, cols, shift, wide};
+  const uint32_t wide = (ng + (ahead << shift) - 1) / (ahead << shift), per = 256 >> shift;
+  const uint32_t most = ((1u << 24) - 1) / wide * per;
+  for (uint32_t r0 = 0; r0 < rows; r0 += most) {
+    const uint32_t n = std::min(rows - r0, most);
+    launch(r0, MxRows{n, cols, shift, wide}, (uint64_t)(n + per - 1) / per * wide);
+  }
 }
 
 }  // namespace
 
 void c0ven::mx4_quantize_launch(uint32_t type, const void *x, uint64_t stride, const moe_mx4_matrix &m, void *stream) {
-  uint64_t n;
-  const MxRows a = rows_of(m.rows, m.cols, 1, n);
-  const auto run = [&](auto kernel, auto *p) { op_launch(kernel, n, 256, stream, p, stride, a, m.codes, m.scales); };
-  if (type == QT_F32) run(mx4_quantize<QT_F32, 1>, (const float *)x);
-  if (type == QT_F16) run(mx4_quantize<QT_F16, 1>, (const _Float16 *)x);
-  if (type == QT_BF16) run(mx4_quantize<QT_BF16, 1>, (const __bf16 *)x);
+  by_rows(m.rows, m.cols, 1, [&](uint32_t r0, const MxRows &a, uint64_t n) {
+    const auto run = [&](auto kernel, auto *p) {
+      op_launch(kernel, n, 256, stream, p + r0 * stride, stride, a, m.codes + moe_mx4_code_bytes(r0, m.cols),
+                m.scales + moe_mx4_scale_bytes(r0, m.cols));
+    };
+    if (type == QT_F32) run(mx4_quantize<QT_F32, 1>, (const float *)x);
+    if (type == QT_F16) run(mx4_quantize<QT_F16, 1>, (const _Float16 *)x);
+    if (type == QT_BF16) run(mx4_quantize<QT_BF16, 1>, (const __bf16 *)x);
+  });
 }
 
 extern "C" {
@@ -105,14 +116,15 @@ MOE_API moe_status moe_mx4_dequantize_async(int32_t device, const moe_mx4_matrix
     OnDevice on(device);
     const auto go = [&](auto ahead) {
       constexpr int kAhead = decltype(ahead)::value;
-      uint64_t n;
-      const MxRows a = rows_of(m->rows, m->cols, kAhead, n);
-      const auto run = [&](auto kernel, auto *p) {
-        op_launch(kernel, n, 256, stream, (const uint8_t *)m->codes, (const uint8_t *)m->scales, a, p, stride);
-      };
-      if (type == QT_F32) run(mx4_dequantize<QT_F32, kAhead>, (float *)out);
-      if (type == QT_F16) run(mx4_dequantize<QT_F16, kAhead>, (_Float16 *)out);
-      if (type == QT_BF16) run(mx4_dequantize<QT_BF16, kAhead>, (__bf16 *)out);
+      by_rows(m->rows, m->cols, kAhead, [&](uint32_t r0, const MxRows &a, uint64_t n) {
+        const auto run = [&](auto kernel, auto *p) {
+          op_launch(kernel, n, 256, stream, (const uint8_t *)m->codes + moe_mx4_code_bytes(r0, m->cols),
+                    (const uint8_t *)m->scales + moe_mx4_scale_bytes(r0, m->cols), a, p + r0 * stride, stride);
+        };
+        if (type == QT_F32) run(mx4_dequantize<QT_F32, kAhead>, (float *)out);
+        if (type == QT_F16) run(mx4_dequantize<QT_F16, kAhead>, (_Float16 *)out);
+        if (type == QT_BF16) run(mx4_dequantize<QT_BF16, kAhead>, (__bf16 *)out);
+      });
     };
     // (Rows too short for four groups a thread in sixteen threads leave threads without work: 25915 x 100 9.5 us, 4.7 with one.)
     if (mx_steps(m->cols) >= 4)

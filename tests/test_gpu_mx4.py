@@ -294,3 +294,27 @@ def test_nothing_to_do():
     moe.mx4_matmul_async(m, w, moe.QT_F32, y.ptr)
     moe.mx4_linear_async(moe.QT_F32, codes.ptr, 0, w, moe.QT_F32, y.ptr, None, 0)
     assert (y.get() == 7.0).all() and (codes.get() == 0xA5).all()
+
+
+def test_most_rows():
+    """As many rows as a matrix may have, of two steps each: more values than a launch has threads for, there and back."""
+    say("most rows")
+    rows, cols = 1 << 27, 129  # 35 GB of fp16, 17 GB of codes
+    x = Raw(hip, rows * cols * 2)
+    r = np.random.default_rng(3)
+    at = (0, rows // 2 - 50, rows - 100)
+    parts = [encode(r.normal(size=(100, cols)), "f16") for _ in at]
+    for a, part in zip(at, parts):
+        x.put(part.view(np.uint8), a * cols * 2)
+    codes, scales = Raw(hip, rows * 128, 0xFF), Raw(hip, rows * 8, 0xFF)
+    m = moe.Mx4Matrix(codes.ptr, scales.ptr, rows, cols)
+    moe.mx4_quantize_async(moe.QT_F16, x.ptr, m)
+    want = [ref.mx4_quantize(decode(p, "f16")) for p in parts]
+    for a, (c, s) in zip(at, want):
+        assert np.array_equal(codes.get(a * 128, (100, 128)), c) and np.array_equal(scales.get(a * 8, (100, 8)), s)
+    assert not codes.get(100 * 128, (1 << 20,)).any() and not codes.get((rows - (1 << 13)) * 128 - 100 * 128, (1 << 20,)).any()
+    x.fill(0x11)
+    moe.mx4_dequantize_async(m, moe.QT_F16, x.ptr)
+    for a, (c, s) in zip(at, want):
+        assert np.array_equal(decode(x.get(a * cols * 2, (100, cols * 2)).view(np.float16), "f16"), ref.mx4_values(c, s, cols))
+    assert not x.get(100 * cols * 2, (1 << 20,)).any()
