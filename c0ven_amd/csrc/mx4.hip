@@ -102,7 +102,8 @@ MOE_API moe_status moe_mx4_quantize_async(int32_t device, uint32_t type, const v
                                           const moe_mx4_matrix *m, void *stream) {
   return op_guarded([&] {
     op_mx4(m);
-    op_rows(x, stride, m->cols, type);
+    op_rows(x, stride, m->rows, m->cols, type);
+    if (!m->rows) return;
     OnDevice on(device);
     mx4_quantize_launch(type, x, stride, *m, stream);
   });
@@ -112,7 +113,8 @@ MOE_API moe_status moe_mx4_dequantize_async(int32_t device, const moe_mx4_matrix
                                             uint64_t stride, void *stream) {
   return op_guarded([&] {
     op_mx4(m);
-    op_rows(out, stride, m->cols, type);
+    op_rows(out, stride, m->rows, m->cols, type);
+    if (!m->rows) return;
     OnDevice on(device);
     const auto go = [&](auto ahead) {
       constexpr int kAhead = decltype(ahead)::value;

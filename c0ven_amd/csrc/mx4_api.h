@@ -11,7 +11,7 @@ namespace c0ven {
 constexpr uint32_t kMxMostRows = 1u << 27, kMxMostCols = 1u << 20;
 inline bool mx4_sizes(const moe_mx4_matrix &m) { return m.cols >= 1 && m.cols <= kMxMostCols && m.rows <= kMxMostRows; }
 inline void op_mx4(const moe_mx4_matrix *m) {
-  op_require(m && m->codes && m->scales, "null argument");
+  op_require(m && ((m->codes && m->scales) || !m->rows), "null argument");
   op_require(op_aligned(m->codes, 16) && op_aligned(m->scales, 16), "an MX4 matrix must be 16-byte aligned");
   op_require(mx4_sizes(*m), "an MX4 matrix has 1..2^20 cols and at most 2^27 rows");
 }

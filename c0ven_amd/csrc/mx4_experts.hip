@@ -586,9 +586,9 @@ MOE_API moe_status moe_mx4_experts_async(const moe_mx4_experts *e, const void *x
   return op_guarded([&] {
     check_experts(e, ntok);
     const uint32_t H = e->n_embd, F = e->n_ff, E = e->n_expert, K = e->n_used, A = ntok * K;
-    op_rows(x, x_stride, H, e->x_type);
-    op_rows(y, y_stride, H, e->y_type);
-    op_require(ids && w && op_aligned(ids, 4) && op_aligned(w, 4), "null or misaligned ids or w");
+    op_rows(x, x_stride, ntok, H, e->x_type);
+    op_rows(y, y_stride, ntok, H, e->y_type);
+    op_require(((ids && w) || !ntok) && op_aligned(ids, 4) && op_aligned(w, 4), "null or misaligned ids or w");
     const Plan at(*e, ntok);
     op_work(work, work_bytes, at.bytes);
     if (!ntok) return;

@@ -297,7 +297,7 @@ MOE_API moe_status moe_mx4_matmul_async(int32_t device, const moe_mx4_matrix *x,
     op_mx4(w);
     op_require(x->cols == w->cols, "x and w must have the same cols");
     op_results(x->rows, w->rows);
-    op_rows(y, y_stride, w->rows, y_type);
+    op_rows(y, y_stride, w->rows ? x->rows : 0, w->rows, y_type);
     op_work(work, work_bytes, moe_mx4_matmul_work_bytes(w, x->rows));
     if (!x->rows || !w->rows) return;
     OnDevice on(device);
@@ -315,8 +315,8 @@ MOE_API moe_status moe_mx4_linear_async(int32_t device, uint32_t x_type, const v
                                         uint64_t y_stride, void *work, uint64_t work_bytes, void *stream) {
   return op_guarded([&] {
     op_mx4(w);
-    op_rows(x, x_stride, w->cols, x_type);
-    op_rows(y, y_stride, w->rows, y_type);
+    op_rows(x, x_stride, ntok, w->cols, x_type);
+    op_rows(y, y_stride, w->rows ? ntok : 0, w->rows, y_type);
     op_require(ntok <= kMxMostRows, "at most 2^27 tokens");
     op_results(ntok, w->rows);
     op_work(work, work_bytes, moe_mx4_linear_work_bytes(w, ntok));

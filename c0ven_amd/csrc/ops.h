@@ -89,10 +89,10 @@ inline bool op_float(uint32_t t) { return t == QT_F32 || t == QT_F16 || t == QT_
 inline uint32_t op_size(uint32_t t) { return t == QT_F32 ? 4 : 2; }
 inline bool op_aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
-// A dense buffer's rows: a pointer to whole elements and a stride that holds a row.
-inline void op_rows(const void *p, uint64_t stride, uint32_t cols, uint32_t type) {
+// A dense buffer's rows: a pointer to whole elements (of no rows: null too) and a stride that holds a row.
+inline void op_rows(const void *p, uint64_t stride, uint32_t rows, uint32_t cols, uint32_t type) {
   op_require(op_float(type), "the element type must be QT_F32, QT_F16 or QT_BF16");
-  op_require(p != nullptr, "null argument");
+  op_require(p || !rows, "null argument");
   op_require(op_aligned(p, op_size(type)), "a buffer must be aligned to its elements");
   op_require(stride >= cols && stride <= (1ull << 40), "a stride must hold a row");
 }

@@ -561,8 +561,8 @@ extern "C" MOE_API moe_status moe_route_async(const moe_route_config *cfg, const
       op_require(c.group_top == 1 || c.group_top == 2, "group_top must be 1 or 2");
       op_require(c.n_used <= c.n_expert / c.n_group * c.top_group, "n_used exceeds the kept groups' experts");
     }
-    op_rows(logits, stride, c.n_expert, c.type);
-    op_require(ids && w && op_aligned(ids, 4) && op_aligned(w, 4) && op_aligned(bias, 4) && op_aligned(load, 4),
+    op_rows(logits, stride, ntok, c.n_expert, c.type);
+    op_require(((ids && w) || !ntok) && op_aligned(ids, 4) && op_aligned(w, 4) && op_aligned(bias, 4) && op_aligned(load, 4),
                "null or misaligned ids, w, bias or load");
     const uint32_t groups = c.top_group < c.n_group ? c.n_group : 1;  // (all of them kept: as none)
     const RouteArgs a{c.n_expert, c.n_used, groups, c.top_group, c.group_top, c.renorm, c.score == MOE_SCORE_SIGMOID,

@@ -315,8 +315,8 @@ MOE_API uint64_t moe_row_bytes(uint32_t type, uint32_t cols);
  * buffer share its contents: order them (one stream, or event waits), graphs that were captured with it among them. A
  * refused call enqueues nothing; its message is moe_last_error(null) on the calling thread. Any number of host threads
  * may call. Element types are QT_F32, QT_F16 or QT_BF16; strides count elements from row to row and are at least a row's
- * values. ntok 0 is accepted and writes nothing (moe_route_async: load, if given, is cleared). Inputs and outputs do not
- * overlap. */
+ * values. ntok 0 is accepted and writes nothing (moe_route_async: load, if given, is cleared); buffers
+ * without an element may be null. Inputs and outputs do not overlap. */
 
 /* The routing of logits, per token: the scores s_e (over the experts whose logit is neither -inf nor NaN), selection
  * values v_e = s_e + bias_e, the experts of the best groups, of those the n_used largest v_e (the lower id first among

@@ -146,6 +146,22 @@ def test_experts_of_no_tokens(E):
     refused(lambda: e.forward_async(P, 0, P, P, P, None, 0, x_stride=255))
 
 
+def test_empty_batches():
+    """Buffers of no tokens may be null, as an empty tensor's are; those that do hold something may not."""
+    w, none = mat(), moe.Mx4Matrix(None, None, 0, 256)
+    moe.Router(**GOOD).route_async(None, 0, None, None)
+    moe.mx4_quantize_async(moe.QT_F16, None, none)
+    moe.mx4_dequantize_async(none, moe.QT_F16, None)
+    moe.mx4_matmul_async(none, w, moe.QT_F32, None)
+    moe.mx4_linear_async(moe.QT_F32, None, 0, w, moe.QT_F32, None, None, 0)
+    moe.mx4_linear_async(moe.QT_F32, P, 4, none, moe.QT_F32, None, None, 0)
+    experts().forward_async(None, 0, None, None, None, None, 0)
+    refused(lambda: moe.mx4_matmul_async(none, mat(codes=None), moe.QT_F32, None))
+    refused(lambda: moe.mx4_linear_async(moe.QT_F32, None, 4, none, moe.QT_F32, None, None, 0))
+    refused(lambda: experts(gate=mat(96, 256, None)).forward_async(None, 0, None, None, None, None, 0))
+    refused(lambda: moe.Router(**GOOD).route_async(None, 0, P + 1, None))
+
+
 def test_null_descriptions():
     assert _lib.lib.moe_route_async(None, P, 8, None, 1, P, P, None, None) == _lib.MOE_BAD_ARGUMENT
     assert _lib.lib.moe_mx4_experts_async(None, P, 8, 1, P, P, P, 8, P, 8, None) == _lib.MOE_BAD_ARGUMENT
