@@ -318,3 +318,19 @@ def test_most_rows():
     for a, (c, s) in zip(at, want):
         assert np.array_equal(decode(x.get(a * cols * 2, (100, cols * 2)).view(np.float16), "f16"), ref.mx4_values(c, s, cols))
     assert not x.get(100 * cols * 2, (1 << 20,)).any()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 64, 640), (40, 100, 8192), (300, 200, 700)])
+def test_whatever_the_work_buffer_held(M, N, K):
+    say("work buffer", M, N, K)
+    x, _ = hip.rows(np.random.default_rng(M).normal(size=(M, K)), "f32")
+    w, wb, _, _, _ = random_mx4(N, K, 9, 1)
+    y = hip.full((M, N), 0)
+    n = moe.mx4_linear_work_bytes(w, M)
+    work = room(n)
+    got = []
+    for value in (0x00, 0xFF, 0x7F):
+        work.put(np.full(n, value, np.uint8))
+        moe.mx4_linear_async(moe.QT_F32, x.ptr, M, w, moe.QT_F32, y.ptr, work.ptr, n)
+        got.append(y.get())
+    assert np.isfinite(got[0]).all() and all(np.array_equal(got[0], g) for g in got[1:])

@@ -247,3 +247,60 @@ def test_far_experts():
         rows = np.arange(T)[-20:]
         y, off = ref.experts(values[rows], np.zeros((len(rows), 1), int), w[rows].astype(np.float32).astype(np.float64), *model.v)
         assert np.all(np.abs(got[rows] - y) <= off + 2.0 ** -24 * (np.abs(y) + off))
+
+
+@pytest.mark.parametrize("T,H,F,E,K", [(4096, 2300, 40, 20, 16), (4200, 2300, 8, 400, 8)])
+def test_columns_in_parts(T, H, F, E, K):
+    """More sums than down takes at a time: parts of 1024, 1024 and 256 columns (256 MB hold 1024 of 65536 assignments), and of
+    1792 and 512; n_embd ends inside the last."""
+    say("columns in parts", T, H, F, E, K)
+    check_some(Model(E, H, F, 6), *tokens(T, H, E, K, 9, 0.05), np.r_[0:16, T // 2:T // 2 + 16, T - 16:T])
+
+
+def test_no_tokens():
+    say("no tokens")
+    model = Model(4, 128, 32, 1)
+    y = hip.full((2, 128), 7)
+    model.op(2).forward_async(y.ptr, 0, y.ptr, y.ptr, y.ptr, None, 0)
+    assert (y.get() == 7.0).all()
+
+
+@pytest.mark.parametrize("T", [1, 12, 100, 900])
+def test_whatever_the_work_buffer_held(T):
+    """Zeros, bytes whose floats, scales and counts are NaNs and -1, and what another batch left: the same bits. Ranks without
+    an expert leave rows of the work unwritten."""
+    say("work buffer", T)
+    model, K = Model(12, 512, 128, 4), 4
+    op = model.op(K)
+    n = op.work_bytes(T)
+    work = room(n)
+    batches = []
+    for seed in (6, 7):
+        x, ids, w = tokens(T, 512, 12, K, seed, 0.3)
+        batches.append((hip.put(x), hip.put(ids.astype(np.int32)), hip.put(w.astype(np.float32)), hip.full((T, 512), 7.0)))
+
+    def call(b):
+        x, ids, w, y = batches[b]
+        op.forward_async(x.ptr, T, ids.ptr, w.ptr, y.ptr, work.ptr, n)
+        return y.get()
+
+    got = []
+    for value in (0x00, 0xFF, 0x7F):
+        work.put(np.full(n, value, np.uint8))
+        got.append(call(0))
+    call(1)
+    got.append(call(0))
+    assert np.isfinite(got[0]).all()
+    assert all(np.array_equal(got[0], g) for g in got[1:])
+
+
+@pytest.mark.parametrize("T", [2, 12, 100, 900])
+def test_a_token_whatever_the_others(T):
+    """Batches of one size that share some tokens: these have the same bits, whoever uses their experts beside them."""
+    say("a token's own", T)
+    model = Model(12, 512, 128, 4)
+    (x, ids, w), (x2, ids2, w2) = (tokens(T, 512, 12, 4, s, 0.2) for s in (6, 7))
+    ids2[:] = np.where(np.arange(T)[:, None] % 2, ids2, 3)  # half of them on one expert
+    same = np.r_[T // 2, T - 1]
+    x2[same], ids2[same], w2[same] = x[same], ids[same], w[same]
+    assert np.array_equal(run(model, x, ids, w)[0][same], run(model, x2, ids2, w2)[0][same])
