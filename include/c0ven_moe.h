@@ -346,8 +346,8 @@ MOE_API moe_status moe_route_async(const moe_route_config *cfg, const void *logi
 /* A matrix in microscaled 4-bit floats (the OCP MX format MXFP4: E2M1 values, E8M0 scales), in device memory. A row is
  * padded to C = cols rounded up to 128 values: C / 2 bytes of codes (value 2 i in the low half of byte i: a sign bit and
  * the index into 0, 0.5, 1, 1.5, 2, 3, 4, 6) and C / 32 bytes of scales, one per 32 values (2^(s - 127); 255 makes the
- * block's values NaN). Codes past cols are 0. Rows follow one another; both pointers are 16-byte aligned. At most
- * 2^27 rows of 1 to 2^20 cols. */
+ * block's values NaN). Codes past cols are 0, scales of blocks past cols anything but 255 (quantisation writes 0). Rows
+ * follow one another; both pointers are 16-byte aligned. At most 2^27 rows of 1 to 2^20 cols. */
 typedef struct {
   uint8_t *codes;
   uint8_t *scales;
@@ -368,7 +368,8 @@ MOE_API moe_status moe_mx4_dequantize_async(int32_t device, const moe_mx4_matrix
 /* y = x w^T (y x->rows x w->rows of y_type, at most 2^38 elements, rows y_stride apart): the MX4 values' products summed in
  * fp32 on the matrix cores and rounded once. x->cols == w->cols. work: at least moe_mx4_matmul_work_bytes(w, x->rows)
  * bytes, 16-byte aligned (may be null where that is 0). The sizes of work look at a description's rows and cols alone and
- * are 0 where the call refuses them. */
+ * are 0 where the call refuses them. They do not grow with ntok throughout: a buffer for several ntok has the largest of
+ * their sizes. */
 MOE_API uint64_t moe_mx4_matmul_work_bytes(const moe_mx4_matrix *w, uint32_t ntok);
 MOE_API moe_status moe_mx4_matmul_async(int32_t device, const moe_mx4_matrix *x, const moe_mx4_matrix *w,
                                         uint32_t y_type, void *y, uint64_t y_stride, void *work, uint64_t work_bytes,
@@ -395,7 +396,8 @@ typedef struct {
   float swiglu_limit;   /* as moe_config's: > 0: gate at most L, up within -L .. L before the SiLU; 0: off */
   int32_t device;
 } moe_mx4_experts;
-/* Bytes of work a call of ntok tokens takes (0 for a description that the call refuses). */
+/* Bytes of work a call of ntok tokens takes (0 for a description that the call refuses); as above, for several ntok the
+ * largest of their sizes. */
 MOE_API uint64_t moe_mx4_experts_work_bytes(const moe_mx4_experts *e, uint32_t ntok);
 /* x ntok x n_embd of x_type, ids and w ntok x n_used, y ntok x n_embd of y_type; ntok at most 16384; work 16-byte
  * aligned. */
