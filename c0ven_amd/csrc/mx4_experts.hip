@@ -5,9 +5,9 @@
 // whose epilogue applies the SwiGLU and quantises h, 32 neighbours of a row being in one wave's registers; down follows on the
 // positions' rows, its fp32 sums go to the assignments' rows, and a last kernel adds each token's in rank order. 301 tokens of
 // 10 of 512 skewed experts, 2560 x 640, fp16: gate/up 50 us, down 34, combine 7, prepare 5; bound by the experts' weights (274
-// MB, 53 us at 5.2 TB/s). 4096 tokens, 2048 x 512: gate/up 118 us (a stage's latency at three work-groups a CU; its
+// MB, 53 us at 5.2 TB/s). 4096 tokens, 2048 x 512: gate/up 126 us (a stage's latency at three work-groups a CU; its
 // instructions and LDS are at a third), down 87 + 33 and combine 45 + 14 in two parts (335 MB of sums written and read back at 5.6 TB/s),
-// prepare 13.
+// prepare 15.
 #include "../../include/c0ven_moe_tile.h"
 #include "mx4.h"
 #include "mx4_api.h"

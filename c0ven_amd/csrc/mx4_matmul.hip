@@ -119,9 +119,9 @@ __global__ void __launch_bounds__(256) mx4_join(const float *sums, uint32_t part
 
 // A tile of y a work-group, k split into parts of `span` stages (256 each); part p's sums go to y + p * part. Work-groups to
 // tiles so that an XCD has neighbours: eight tiles down, then across. The 256 tile takes eight waves, two a SIMD (four with
-// 256 sums a lane: 177 us at 4096 x 8192 x 8448). That product takes 166 us, 3.4 PFLOP/s; with the loop's loads left out 132:
-// the matrix instructions on random codes are at 4.3 to 5.6 PFLOP/s, below the 8.2 of constant ones, and what the loads add
-// is the wait for a stage that 64 KB a CU cannot hide, since two stages fill LDS.
+// 256 sums a lane: 177 us at 4096 x 8192 x 8448, 166 with eight). 4096 x 8192 x 8192, after x's quantisation: 166 us on
+// average, 3.3 PFLOP/s (145 at least); called back to back 181, x 8448 (rows that are not a power of two apart) 170. Of these
+// 137 and 132 remained in a copy without the loop's loads: what the loads add is the wait for a stage that 64 KB a CU cannot hide, since two stages fill LDS.
 template <uint32_t kType, int TM, int TN, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves, 2)
     mx4_gemm(const uint8_t *xc, const uint8_t *xs, const uint8_t *wc, const uint8_t *ws, uint32_t M, uint32_t N,

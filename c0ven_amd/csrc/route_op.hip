@@ -6,14 +6,14 @@
 //
 // Where the order is that of the logits (no bias, a group's worth from one value) it is exact in fp32 and only the chosen
 // need an exponential. Otherwise the order is that of s + bias in fp64: it is formed in fp32 within a bound, and where two
-// neighbours of the order (the k-th and the next among them), or the last group kept and the next, are nearer than their
-// bounds, the wave decides that in fp64: among the candidates, or among all where too many are near. Equal logits under equal biases need no bound: their order
-// is by id either way.
+// neighbours of the order (the k-th and the next among them), or a group and the border between those kept and the others, are
+// nearer than their bounds, the wave decides that in fp64: among the candidates, or among all where too many are near. Equal
+// logits under equal biases need no bound: their order is by id either way.
 //
-// Bound by the launch where tokens are few (one of 512 experts, top 10: 4.2 us), else by the instructions of a token, some 330
-// vector ones a wave: 16384 x 512 fp32, top 10, 13.0 us (2.6 TB/s; the logits alone are 6.8 us at 5.1) and 3.5 for the load;
-// with biases 32 us. 999 x 256 bf16 with biases and groups 7.1 and 2.5 us: one token a wave, its latency, and some tokens'
-// fp64.
+// Bound by the launch where tokens are few (one of 512 experts, top 10: 4.4 us), else by the instructions of a token: 16384 x
+// 512 fp32, top 10, 293 vector and 219 scalar ones, 13.6 us (2.5 TB/s; the logits alone are 6.8 us at 5.1) and 3.8 for the load;
+// with biases 576 and 294 on half the waves (fp64's registers), 36 us and 4.5. 999 x 256 bf16 with biases and groups 10.4 and
+// 2.9 us (in a graph of such calls 7.0 and 2.4): one token a wave, its latency, and some tokens' fp64.
 #include "device_math.h"
 #include "mx4.h"
 #include "ops.h"
