@@ -9,3 +9,5 @@ from ._lib import (BLOCK, CODEBOOK_TYPES, EXPORTS, MOE_BAD_ARGUMENT, MOE_FLAG_EX
 from ._lib import (MOE_SCORE_SIGMOID, MOE_SCORE_SOFTMAX, QT_BF16, QT_F16, QT_F32, Mx4Experts, Mx4Matrix, Router,  # noqa: F401
                    mx4_code_bytes, mx4_dequantize_async, mx4_linear_async, mx4_linear_work_bytes, mx4_matmul_async,
                    mx4_matmul_work_bytes, mx4_quantize_async, mx4_scale_bytes)
+from ._lib import (Dispatch, I8Experts, I8Matrix, i8_code_bytes, i8_dequantize_async, i8_linear_async,  # noqa: F401
+                   i8_linear_work_bytes, i8_matmul_async, i8_matmul_work_bytes, i8_quantize_async)

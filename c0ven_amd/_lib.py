@@ -90,6 +90,22 @@ class MoeMx4Experts(C.Structure):
                 ("y_type", C.c_uint32), ("swiglu_limit", C.c_float), ("device", C.c_int32)]
 
 
+class MoeDispatchConfig(C.Structure):
+    _fields_ = [("n_expert", C.c_uint32), ("n_used", C.c_uint32), ("n_embd", C.c_uint32), ("type", C.c_uint32),
+                ("device", C.c_int32)]
+
+
+class I8Matrix(C.Structure):
+    """A matrix in 8-bit integers: I8Matrix(codes, scales, rows, cols), the first two device pointers."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_uint32), ("cols", C.c_uint32)]
+
+
+class MoeI8Experts(C.Structure):
+    _fields_ = [("n_embd", C.c_uint32), ("n_ff", C.c_uint32), ("n_expert", C.c_uint32), ("n_used", C.c_uint32),
+                ("gate", I8Matrix), ("up", I8Matrix), ("down", I8Matrix), ("x_type", C.c_uint32),
+                ("y_type", C.c_uint32), ("swiglu_limit", C.c_float), ("device", C.c_int32)]
+
+
 class GgufTensorInfo(C.Structure):
     _fields_ = [("name", C.c_char_p), ("type", C.c_uint32), ("n_dims", C.c_uint32), ("shape", C.c_uint64 * 4),
                 ("shard", C.c_uint32), ("offset", C.c_uint64), ("bytes", C.c_uint64), ("data", C.c_void_p)]
@@ -146,6 +162,20 @@ _SIGS = {
     "moe_mx4_linear_async": (_i32, [_i32, _u32, _P, _u64, _u32, C.POINTER(Mx4Matrix), _u32, _P, _u64, _P, _u64, _P]),
     "moe_mx4_experts_work_bytes": (_u64, [C.POINTER(MoeMx4Experts), _u32]),
     "moe_mx4_experts_async": (_i32, [C.POINTER(MoeMx4Experts), _P, _u64, _u32, _P, _P, _P, _u64, _P, _u64, _P]),
+    "moe_dispatch_work_bytes": (_u64, [C.POINTER(MoeDispatchConfig), _u32]),
+    "moe_dispatch_async": (_i32, [C.POINTER(MoeDispatchConfig), _P, _u64, _u32, _P, _P, _u64, _P, _P, _P, _P, _u64, _P]),
+    "moe_combine_async": (_i32, [C.POINTER(MoeDispatchConfig), _P, _u64, _u32, _P, _P, _P, _u64, _P]),
+    "moe_dispatch_backward_async": (_i32, [C.POINTER(MoeDispatchConfig), _P, _u64, _u32, _P, _P, _u64, _P]),
+    "moe_combine_backward_async": (_i32, [C.POINTER(MoeDispatchConfig), _P, _u64, _u32, _P, _P, _u64, _P, _P, _u64, _P, _P]),
+    "moe_i8_code_bytes": (_u64, [_u32, _u32]),
+    "moe_i8_quantize_async": (_i32, [_i32, _u32, _P, _u64, C.POINTER(I8Matrix), _P]),
+    "moe_i8_dequantize_async": (_i32, [_i32, C.POINTER(I8Matrix), _u32, _P, _u64, _P]),
+    "moe_i8_matmul_work_bytes": (_u64, [C.POINTER(I8Matrix), _u32]),
+    "moe_i8_matmul_async": (_i32, [_i32, C.POINTER(I8Matrix), C.POINTER(I8Matrix), _u32, _P, _u64, _P, _u64, _P]),
+    "moe_i8_linear_work_bytes": (_u64, [C.POINTER(I8Matrix), _u32]),
+    "moe_i8_linear_async": (_i32, [_i32, _u32, _P, _u64, _u32, C.POINTER(I8Matrix), _u32, _P, _u64, _P, _u64, _P]),
+    "moe_i8_experts_work_bytes": (_u64, [C.POINTER(MoeI8Experts), _u32]),
+    "moe_i8_experts_async": (_i32, [C.POINTER(MoeI8Experts), _P, _u64, _u32, _P, _P, _P, _u64, _P, _u64, _P]),
     "moe_abi_layout": (_u32, [C.POINTER(MoeAbiRow), _u32]),
     "moe_load_layer_gguf": (_i32, [_P, _u32, _P, _u32]),
     "moe_load_hc": (_i32, [_P, _u32, _P, _P, _P, _P]),
@@ -609,3 +639,84 @@ class Mx4Experts:
         H = self.cfg.n_embd
         _op(lib.moe_mx4_experts_async(self._cfg, x, H if x_stride is None else x_stride, ntok, ids, w, y,
                                       H if y_stride is None else y_stride, work, work_bytes, stream))
+
+
+class Dispatch:
+    """Tokens sorted by expert and back (moe_dispatch_async, moe_combine_async), and the gradients of both."""
+
+    def __init__(self, n_expert, n_used, n_embd, type=QT_BF16, device=0):
+        self.cfg = MoeDispatchConfig(n_expert, n_used, n_embd, type, device)
+        self._cfg = C.byref(self.cfg)
+
+    def _stride(self, stride):
+        return self.cfg.n_embd if stride is None else stride
+
+    def work_bytes(self, ntok):
+        return int(lib.moe_dispatch_work_bytes(self._cfg, ntok))
+
+    def dispatch_async(self, x, ntok, ids, xs, order, places, offsets, work=None, work_bytes=0, x_stride=None, xs_stride=None,
+                       stream=None):
+        _op(lib.moe_dispatch_async(self._cfg, x, self._stride(x_stride), ntok, ids, xs, self._stride(xs_stride), order, places,
+                                   offsets, work, work_bytes, stream))
+
+    def combine_async(self, o, ntok, places, y, w=None, o_stride=None, y_stride=None, stream=None):
+        _op(lib.moe_combine_async(self._cfg, o, self._stride(o_stride), ntok, places, w, y, self._stride(y_stride), stream))
+
+    def dispatch_backward_async(self, dxs, ntok, places, dx, dxs_stride=None, dx_stride=None, stream=None):
+        _op(lib.moe_dispatch_backward_async(self._cfg, dxs, self._stride(dxs_stride), ntok, places, dx, self._stride(dx_stride),
+                                            stream))
+
+    def combine_backward_async(self, dy, ntok, places, o=None, dout=None, dw=None, w=None, dy_stride=None, o_stride=None,
+                               dout_stride=None, stream=None):
+        _op(lib.moe_combine_backward_async(self._cfg, dy, self._stride(dy_stride), ntok, places, o, self._stride(o_stride), w, dout,
+                                           self._stride(dout_stride), dw, stream))
+
+
+def i8_code_bytes(rows, cols):
+    return int(lib.moe_i8_code_bytes(rows, cols))
+
+
+def i8_quantize_async(type, x, m, stride=None, device=0, stream=None):
+    """x (m.rows x m.cols of type) into the I8Matrix m."""
+    _op(lib.moe_i8_quantize_async(device, type, x, m.cols if stride is None else stride, m, stream))
+
+
+def i8_dequantize_async(m, type, out, stride=None, device=0, stream=None):
+    _op(lib.moe_i8_dequantize_async(device, m, type, out, m.cols if stride is None else stride, stream))
+
+
+def i8_matmul_work_bytes(w, ntok):
+    return int(lib.moe_i8_matmul_work_bytes(w, ntok))
+
+
+def i8_matmul_async(x, w, y_type, y, work=None, work_bytes=0, y_stride=None, device=0, stream=None):
+    """y = x w^T of two I8Matrix."""
+    _op(lib.moe_i8_matmul_async(device, x, w, y_type, y, w.rows if y_stride is None else y_stride, work, work_bytes, stream))
+
+
+def i8_linear_work_bytes(w, ntok):
+    return int(lib.moe_i8_linear_work_bytes(w, ntok))
+
+
+def i8_linear_async(x_type, x, ntok, w, y_type, y, work, work_bytes, x_stride=None, y_stride=None, device=0, stream=None):
+    """y = i8(x) w^T of ntok rows of floats."""
+    _op(lib.moe_i8_linear_async(device, x_type, x, w.cols if x_stride is None else x_stride, ntok, w, y_type, y,
+                                w.rows if y_stride is None else y_stride, work, work_bytes, stream))
+
+
+class I8Experts:
+    """The experts of routed tokens in I8 (moe_i8_experts_async): gate, up and down describe one expert's matrix and point to
+    n_expert of them."""
+
+    def __init__(self, n_embd, n_ff, n_expert, n_used, gate, up, down, x_type=QT_BF16, y_type=QT_BF16, swiglu_limit=0.0,
+                 device=0):
+        self.cfg = MoeI8Experts(n_embd, n_ff, n_expert, n_used, gate, up, down, x_type, y_type, swiglu_limit, device)
+        self._cfg = C.byref(self.cfg)
+
+    def work_bytes(self, ntok):
+        return int(lib.moe_i8_experts_work_bytes(self._cfg, ntok))
+
+    def forward_async(self, x, ntok, ids, w, y, work, work_bytes, x_stride=None, y_stride=None, stream=None):
+        H = self.cfg.n_embd
+        _op(lib.moe_i8_experts_async(self._cfg, x, H if x_stride is None else x_stride, ntok, ids, w, y,
+                                     H if y_stride is None else y_stride, work, work_bytes, stream))

@@ -1,0 +1,62 @@
+// 8-bit integers with a scale a row (I8) on the device: the conversions and the matrix-core products.
+#pragma once
+
+#include "mx4.h"
+
+namespace c0ven {
+
+constexpr uint32_t kI8Row = 128;  // a row's padding in bytes: four 32x32x32 or two 16x16x64 matrix instructions' k
+__host__ __device__ constexpr uint32_t i8_steps(uint32_t cols) { return (cols + kI8Row - 1) / kI8Row; }
+__host__ __device__ constexpr uint32_t i8_pitch(uint32_t cols) { return i8_steps(cols) * kI8Row; }
+
+typedef int i8_i16 __attribute__((ext_vector_type(16)));
+
+// A row's scale from the bits of its largest |x| (a float without its sign): that over 127, correctly rounded, at least 2^-100
+// (below, the exact test of a code's border would leave fp32's range); NaN for an infinity or a NaN, whose bits are the largest.
+__device__ __forceinline__ float i8_scale_of(uint32_t most) {
+  const float s = __uint_as_float(most) / 127.0f;
+  return most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : s < 0x1p-100f ? 0x1p-100f : s;
+}
+// The integer nearest to x / s (halves to even) exactly: floor of the product with 1 / s is off by at most one next to a whole
+// number, where the test against the half between does not depend on it; the fused x - (k + 1/2) s has the sign of the exact one,
+// since x is a multiple of 2^-149 and s of 2^-123.
+__device__ __forceinline__ uint32_t i8_code(float x, float s, float inv) {
+  const float k = __builtin_floorf(x * inv);
+  const float d = __builtin_fmaf(-(k + 0.5f), s, x);
+  const int i = (int)k;
+  return (uint32_t)(i + (d > 0.0f ? 1 : d == 0.0f ? i & 1 : 0)) & 0xffu;
+}
+// Eight values as two words of codes.
+__device__ __forceinline__ uint2 i8_codes8(const float v[8], float s) {
+  if (s != s) return make_uint2(0, 0);
+  const float inv = __builtin_amdgcn_rcpf(s);
+  uint32_t c[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) c[j] = i8_code(v[j], s, inv);
+  return make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+}
+__device__ __forceinline__ uint32_t most_of8(const float v[8]) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+  return most;
+}
+
+// c += a b^T on 16 rows each over k = 64: lane l gives row l % 16, bytes 16 (l / 16) and on; it receives c of a's rows
+// 4 (l / 16) + i, b's row l % 16.
+__device__ __forceinline__ mx_i4 i8_mfma16(mx_i4 a, mx_i4 b, mx_i4 c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+// The same on 32 rows each over k = 32: lane l gives row l % 32, bytes 16 (l / 32) and on; it receives c of a's rows
+// 8 (i / 4) + 4 (l / 32) + i % 4, b's row l % 32.
+__device__ __forceinline__ i8_i16 i8_mfma32(mx_i4 a, mx_i4 b, i8_i16 c) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+}
+
+// A sum of codes' products as a value: the smaller scale first, so that what is between leaves fp32's range only where the value
+// does (a scale is at least 2^-100, a sum at most 2^30). A scale that is NaN stays.
+__device__ __forceinline__ float i8_value(int sum, float sx, float sw) {
+  return sx < sw ? (float)sum * sx * sw : (float)sum * sw * sx;
+}
+
+}  // namespace c0ven

@@ -1671,6 +1671,14 @@ MOE_API uint32_t moe_abi_layout(moe_abi_row *table, uint32_t cap) {
       ROW(moe_mx4_experts, up),      ROW(moe_mx4_experts, down),    ROW(moe_mx4_experts, x_type),
       ROW(moe_mx4_experts, y_type),  ROW(moe_mx4_experts, swiglu_limit), ROW(moe_mx4_experts, device),
       STRUCT(moe_mx4_experts),
+      ROW(moe_dispatch_config, n_expert), ROW(moe_dispatch_config, n_used), ROW(moe_dispatch_config, n_embd),
+      ROW(moe_dispatch_config, type), ROW(moe_dispatch_config, device), STRUCT(moe_dispatch_config),
+      ROW(moe_i8_matrix, codes),     ROW(moe_i8_matrix, scales),    ROW(moe_i8_matrix, rows),
+      ROW(moe_i8_matrix, cols),      STRUCT(moe_i8_matrix),         ROW(moe_i8_experts, n_embd),
+      ROW(moe_i8_experts, n_ff),     ROW(moe_i8_experts, n_expert), ROW(moe_i8_experts, n_used),
+      ROW(moe_i8_experts, gate),     ROW(moe_i8_experts, up),       ROW(moe_i8_experts, down),
+      ROW(moe_i8_experts, x_type),   ROW(moe_i8_experts, y_type),   ROW(moe_i8_experts, swiglu_limit),
+      ROW(moe_i8_experts, device),   STRUCT(moe_i8_experts),
   };
   const uint32_t n = sizeof rows / sizeof rows[0];
   if (table)

@@ -9,6 +9,7 @@
 // instructions and LDS are at a third), down 87 + 33 and combine 45 + 14 in two parts (335 MB of sums written and read back at 5.6 TB/s),
 // prepare 15.
 #include "../../include/c0ven_moe_tile.h"
+#include "experts.h"
 #include "mx4.h"
 #include "mx4_api.h"
 #include "mx4_gemm.h"
@@ -17,15 +18,6 @@
 #include <algorithm>
 
 namespace c0ven {
-
-// silu(g) u with the limit of moe_config.swiglu_limit; NaNs stay.
-__device__ __forceinline__ float mx_swiglu(float g, float u, float limit) {
-  if (limit > 0.0f) {
-    g = g > limit ? limit : g;
-    u = u > limit ? limit : u < -limit ? -limit : u;
-  }
-  return g / (1.0f + exp_f32(-g)) * u;
-}
 
 // ---- the assignments by expert, and x in MX4
 
@@ -106,20 +98,6 @@ struct MxExperts {
   float limit;
 };
 
-// A launch's work-groups to its items (parts a tile) so that an XCD (work-groups go to the eight in turn) has runs of four
-// tiles: an expert's tiles share its weights in that L2, while the experts with one tile are dealt over all of them (4096
-// tokens of 10 of 512 experts 392 us, with the items in order 430; of 4 of 16 experts 114 and 119). ~0: none.
-constexpr uint32_t kTileRun = 4;
-__device__ __forceinline__ uint32_t item_of(uint32_t all, uint32_t parts) {
-  const uint32_t run = kTileRun * parts, j = blockIdx.x / 8, id = (j / run * 8 + blockIdx.x % 8) * run + j % run;
-  return id < all ? id : ~0u;
-}
-// The work-groups that cover `all` items.
-inline uint64_t item_blocks(uint64_t all, uint64_t parts) {
-  const uint64_t run = kTileRun * parts;
-  return (all + 8 * run - 1) / (8 * run) * (8 * run);
-}
-
 // An item: a tile and 32 WN columns of h (their rows of gate and of up). Writes the places' rows of h in MX4.
 template <int TM, int WM>
 __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint8_t *xc, const uint8_t *xs, uint32_t ntok,
@@ -154,7 +132,7 @@ __global__ void __launch_bounds__(256) mx4_gate_up_tiles(MxExperts p, const uint
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-      h[i] = mx_swiglu(c.acc[0][m][i], c.acc[1][m][i], p.limit);
+      h[i] = expert_swiglu(c.acc[0][m][i], c.acc[1][m][i], p.limit);
       if (col + 8 * (i / 4) + 4 * q + i % 4 >= p.F) h[i] = 0.0f;
       most = max(most, __float_as_uint(h[i]) & 0x7fffffffu);
     }
@@ -221,11 +199,6 @@ __global__ void __launch_bounds__(256) mx4_down_tiles(MxExperts p, const uint8_t
 // rows are 4 lanes a clock): all that a work-group needs is on its way at once.
 
 constexpr uint32_t kFew = 160;
-
-// What lane l of 64 holds (flag) as the number of lanes below it that do.
-__device__ __forceinline__ uint32_t lanes_below(uint64_t ballot) {
-  return __builtin_amdgcn_mbcnt_hi((uint32_t)(ballot >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0u));
-}
 
 // A work-group: an expert and 32 columns of h, for the tokens that use the expert, eight at a time: the assignment that is
 // the first with its expert does the work, the others' work-groups leave. Quantises x itself (while the weights come) and
@@ -324,7 +297,7 @@ __global__ void __launch_bounds__(256) mx4_gate_up_few(MxExperts p, const typena
     float gv = 0.0f, uv = 0.0f;
 #pragma unroll
     for (uint32_t v = 0; v < 4; v++) gv += sums[(v * 64 + col) * kTok + t], uv += sums[(v * 64 + 32 + col) * kTok + t];
-    h[t][col] = f0 + col < p.F ? mx_swiglu(gv, uv, p.limit) : 0.0f;
+    h[t][col] = f0 + col < p.F ? expert_swiglu(gv, uv, p.limit) : 0.0f;
     __syncthreads();
     if (threadIdx.x < 4 * nm) {
       const uint32_t m = threadIdx.x / 4, part = threadIdx.x % 4;

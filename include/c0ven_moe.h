@@ -306,8 +306,9 @@ MOE_API void moe_zipf_bias(uint64_t seed, uint32_t n_expert, float s, float *out
 MOE_API uint64_t moe_row_bytes(uint32_t type, uint32_t cols);
 
 /* ---------------------------------------------------------------------------------------------------------------------
- * Operators on device buffers: routing to experts, microscaled 4-bit floats (MX4) and the experts' products in them. No
- * counterpart in the reference, whose router is the block's and whose weights are integer grids.
+ * Operators on device buffers: routing to experts, the tokens sorted by expert and back, microscaled 4-bit floats (MX4), 8-bit
+ * integers with a scale a row (I8) and the experts' products in both. No counterpart in the reference, whose router is the
+ * block's and whose weights are integer grids.
  *
  * They take no context: every buffer is the caller's (device memory of the description's device), nothing is allocated,
  * copied to the host or waited for, and a call may be captured into a graph. Each is enqueued on stream (a hipStream_t of
@@ -315,7 +316,8 @@ MOE_API uint64_t moe_row_bytes(uint32_t type, uint32_t cols);
  * buffer share its contents: order them (one stream, or event waits), graphs that were captured with it among them. A
  * refused call enqueues nothing; its message is moe_last_error(null) on the calling thread. Any number of host threads
  * may call. Element types are QT_F32, QT_F16 or QT_BF16; strides count elements from row to row and are at least a row's
- * values. ntok 0 is accepted and writes nothing (moe_route_async: load, if given, is cleared); buffers
+ * values. ntok 0 is accepted and writes nothing (moe_route_async: load, if given, is cleared;
+ * moe_dispatch_async: offsets are); buffers
  * without an element may be null. Inputs and outputs do not overlap. */
 
 /* The routing of logits, per token: the scores s_e (over the experts whose logit is neither -inf nor NaN), selection
@@ -342,6 +344,42 @@ typedef struct {
  * null) receives the number of tokens that use each expert. */
 MOE_API moe_status moe_route_async(const moe_route_config *cfg, const void *logits, uint64_t stride, const float *bias,
                                    uint32_t ntok, int32_t *ids, float *w, uint32_t *load, void *stream);
+
+/* The routed tokens in their experts' order, and back, for experts of the caller's own. An assignment a = token * n_used + rank
+ * counts if its id is within 0 .. n_expert - 1 (moe_route_async's -1 is not); those that count are sorted by expert and within
+ * an expert by a. */
+typedef struct {
+  uint32_t n_expert; /* at most 512 */
+  uint32_t n_used;   /* at most 16 */
+  uint32_t n_embd;   /* values a row, at most 2^20 */
+  uint32_t type;     /* of the rows */
+  int32_t device;
+} moe_dispatch_config;
+/* Bytes of work a dispatch of ntok tokens takes (0 for what the call refuses); as below, for several ntok the largest of their
+ * sizes. */
+MOE_API uint64_t moe_dispatch_work_bytes(const moe_dispatch_config *cfg, uint32_t ntok);
+/* order (ntok x n_used) receives the assignment at each position (-1 past the last), places (ntok x n_used) each assignment's
+ * position (-1 for one that does not count), offsets (n_expert + 1) each expert's first position and, last, how many positions
+ * there are. xs (null: only the order) receives x's row of each position; its rows past the last position are left as they
+ * were: it has room for ntok n_used. ntok at most 2^20; work 16-byte aligned (may be null where its size is 0). */
+MOE_API moe_status moe_dispatch_async(const moe_dispatch_config *cfg, const void *x, uint64_t x_stride, uint32_t ntok,
+                                      const int32_t *ids, void *xs, uint64_t xs_stride, int32_t *order, int32_t *places,
+                                      uint32_t *offsets, void *work, uint64_t work_bytes, void *stream);
+/* y[t] = sum over t's ranks of w o[place], in rank order in fp32 (a rank's product fused into the sum), rounded once. o: a row a
+ * position; places as moe_dispatch_async wrote them: one outside 0 .. ntok n_used - 1 adds nothing and its weight is not used; w
+ * (ntok x n_used) null: ones. */
+MOE_API moe_status moe_combine_async(const moe_dispatch_config *cfg, const void *o, uint64_t o_stride, uint32_t ntok,
+                                     const int32_t *places, const float *w, void *y, uint64_t y_stride, void *stream);
+/* The gradient of moe_dispatch_async's xs with regard to x, from that of a loss with regard to xs: dx[t] = sum over t's ranks of
+ * dxs[place], as moe_combine_async with weights of one. */
+MOE_API moe_status moe_dispatch_backward_async(const moe_dispatch_config *cfg, const void *dxs, uint64_t dxs_stride, uint32_t ntok,
+                                               const int32_t *places, void *dx, uint64_t dx_stride, void *stream);
+/* The gradients of moe_combine_async with regard to o and w, from dy, that with regard to y: dout[place] = w dy[t], rounded once
+ * (rows without an assignment are left as they were); dw = <dy[t], o[place]> in fp32, in an order that goes by n_embd and type
+ * alone (0 for an assignment without a place). dout or dw may be null (not formed; without dw, o too); w null: ones. */
+MOE_API moe_status moe_combine_backward_async(const moe_dispatch_config *cfg, const void *dy, uint64_t dy_stride, uint32_t ntok,
+                                              const int32_t *places, const void *o, uint64_t o_stride, const float *w, void *dout,
+                                              uint64_t dout_stride, float *dw, void *stream);
 
 /* A matrix in microscaled 4-bit floats (the OCP MX format MXFP4: E2M1 values, E8M0 scales), in device memory. A row is
  * padded to C = cols rounded up to 128 values: C / 2 bytes of codes (value 2 i in the low half of byte i: a sign bit and
@@ -404,6 +442,58 @@ MOE_API uint64_t moe_mx4_experts_work_bytes(const moe_mx4_experts *e, uint32_t n
 MOE_API moe_status moe_mx4_experts_async(const moe_mx4_experts *e, const void *x, uint64_t x_stride, uint32_t ntok,
                                          const int32_t *ids, const float *w, void *y, uint64_t y_stride, void *work,
                                          uint64_t work_bytes, void *stream);
+
+/* A matrix in 8-bit integers with a scale a row (a token's, or an output channel's of weights), in device memory: value = code *
+ * scale. A row of codes is padded to a multiple of 128 bytes, zeros past cols; rows follow one another, codes 16-byte aligned. At
+ * most 2^27 rows of 1 to 65536 cols. Quantisation writes codes of -127 .. 127; a matrix from elsewhere may hold -128. */
+typedef struct {
+  int8_t *codes;
+  float *scales; /* rows of them */
+  uint32_t rows;
+  uint32_t cols;
+} moe_i8_matrix;
+MOE_API uint64_t moe_i8_code_bytes(uint32_t rows, uint32_t cols);
+/* x (m->rows x m->cols of type, rows stride apart) into m: a row's scale is its largest |x| / 127 rounded to fp32, at least
+ * 2^-100, its codes the integers nearest to x / scale (of the exact quotient; halves to even). A row with an infinity or a NaN
+ * gets the scale NaN and codes 0. */
+MOE_API moe_status moe_i8_quantize_async(int32_t device, uint32_t type, const void *x, uint64_t stride, const moe_i8_matrix *m,
+                                         void *stream);
+/* m's values, rounded to type, into out (rows stride apart). */
+MOE_API moe_status moe_i8_dequantize_async(int32_t device, const moe_i8_matrix *m, uint32_t type, void *out, uint64_t stride,
+                                           void *stream);
+
+/* y = x w^T (y x->rows x w->rows of y_type, at most 2^38 elements, rows y_stride apart): the codes' products summed exactly, the
+ * sum rounded to fp32, times the smaller of x's row's scale and w's, times the larger (each rounded), and rounded to y_type.
+ * x->cols == w->cols. work as moe_mx4_matmul_async's, of moe_i8_matmul_work_bytes(w, x->rows) bytes. */
+MOE_API uint64_t moe_i8_matmul_work_bytes(const moe_i8_matrix *w, uint32_t ntok);
+MOE_API moe_status moe_i8_matmul_async(int32_t device, const moe_i8_matrix *x, const moe_i8_matrix *w, uint32_t y_type, void *y,
+                                       uint64_t y_stride, void *work, uint64_t work_bytes, void *stream);
+/* The same for x of floats (ntok x w->cols of x_type, rows x_stride apart), quantised as by moe_i8_quantize_async. */
+MOE_API uint64_t moe_i8_linear_work_bytes(const moe_i8_matrix *w, uint32_t ntok);
+MOE_API moe_status moe_i8_linear_async(int32_t device, uint32_t x_type, const void *x, uint64_t x_stride, uint32_t ntok,
+                                       const moe_i8_matrix *w, uint32_t y_type, void *y, uint64_t y_stride, void *work,
+                                       uint64_t work_bytes, void *stream);
+
+/* The experts of routed tokens in I8: as moe_mx4_experts_async, with o = down(i8(h)), h = silu(gate(i8(x))) * up(i8(x)), i8() the
+ * quantisation above (of fp32 h, a row an assignment), each product's values in fp32. */
+typedef struct {
+  uint32_t n_embd;      /* at most 16384 */
+  uint32_t n_ff;        /* at most 16384 */
+  uint32_t n_expert;    /* at most 512 */
+  uint32_t n_used;      /* at most 16 */
+  moe_i8_matrix gate, up, down; /* one expert's rows and cols; n_expert such matrices, and their scales, one after the other */
+  uint32_t x_type;
+  uint32_t y_type;
+  float swiglu_limit;   /* as moe_mx4_experts's */
+  int32_t device;
+} moe_i8_experts;
+/* Bytes of work a call of ntok tokens takes (0 for a description that the call refuses); for several ntok the largest of their
+ * sizes. */
+MOE_API uint64_t moe_i8_experts_work_bytes(const moe_i8_experts *e, uint32_t ntok);
+/* x ntok x n_embd of x_type, ids and w ntok x n_used, y ntok x n_embd of y_type; ntok at most 16384; work 16-byte aligned. */
+MOE_API moe_status moe_i8_experts_async(const moe_i8_experts *e, const void *x, uint64_t x_stride, uint32_t ntok,
+                                        const int32_t *ids, const float *w, void *y, uint64_t y_stride, void *work,
+                                        uint64_t work_bytes, void *stream);
 
 /* For the ABI test: one row per field of every struct above, "struct.field" with its offset and size, then one row
  * per struct, "struct", offset 0 and its size. Returns the number of rows; table may be null. */
