@@ -125,81 +125,108 @@ __global__ void __launch_bounds__(64 * kSortWaves) sort_place(const int32_t *ids
   for (uint32_t i = max(first, total) + tid; i < end; i += 64 * kSortWaves) out.order[i] = -1;
 }
 
-// ---- rows out
+// ---- rows
 
-// 16 bytes of a row at whatever address (or what is left of it), two at a time at the end (rows are of whole elements).
-struct __attribute__((packed, aligned(2))) Piece {
-  uint16_t v[8];
-};
-__device__ __forceinline__ Piece piece_of(const uint8_t *row, uint64_t at, uint64_t n) {
-  if (at + 16 <= n) return *(const Piece *)(row + at);
-  Piece p = {};
-#pragma unroll
-  for (uint32_t j = 0; j < 8; j++)
-    if (at + 2 * j < n) p.v[j] = *(const uint16_t *)(row + at + 2 * j);
-  return p;
-}
-__device__ __forceinline__ void put_piece(uint8_t *row, uint64_t at, uint64_t n, const Piece &p) {
-  if (at + 16 <= n) {
-    *(Piece *)(row + at) = p;
-    return;
+// kN neighbouring elements: 16 bytes at whatever address, or one element (rows shorter than 16 bytes). Rows pass through once and
+// are far more than a cache holds, so they are loaded and stored past it (16384 x 10 rows of 4 KB: dispatched in 128 us, 150
+// without; combined in 126, 144).
+typedef uint32_t Quad __attribute__((ext_vector_type(4), aligned(2)));
+template <uint32_t kType, uint32_t kN>
+struct Few {
+  typedef typename Elem<kType>::T T;
+  struct Pack {
+    T e[kN];
+  };
+  typedef typename std::conditional<kN == 1, T, Quad>::type V;
+  V v;
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (kN == 1)
+      v = *p;
+    else
+      v = __builtin_nontemporal_load((const Quad *)p);
   }
-#pragma unroll
-  for (uint32_t j = 0; j < 8; j++)
-    if (at + 2 * j < n) *(uint16_t *)(row + at + 2 * j) = p.v[j];
-}
-
-// Which token and which piece (of `per` a row) a lane has: kWide: a wave's 64 pieces are one token's, so that what goes by the
-// token is scalar (rows of at least 32 pieces); else the lanes follow one another through the rows.
-constexpr uint32_t kWidePieces = 32;
-template <bool kWide>
-struct Items {
-  uint64_t n;     // waves (kWide) or lanes
-  uint32_t per;
-  __host__ __device__ Items(uint64_t rows, uint32_t pieces) : n(rows * (kWide ? (pieces + 63) / 64 : pieces)), per(pieces) {}
-  __host__ __device__ uint64_t blocks() const { return (n + (kWide ? 3 : 255)) / (kWide ? 4 : 256); }
-  // f(row, piece) of block b's lanes.
-  template <typename F>
-  __device__ __forceinline__ void each(uint64_t b, F f) const {
-    if (kWide) {
-      const uint32_t runs = (per + 63) / 64;
-      const uint64_t item = b * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-      if (item >= n) return;
-      const uint32_t row = (uint32_t)(item / runs), piece = (uint32_t)(item - (uint64_t)row * runs) * 64 + threadIdx.x % 64;
-      if (piece < per) f(row, piece);
+  __device__ __forceinline__ void store(T *p) const {
+    if constexpr (kN == 1)
+      *p = v;
+    else
+      __builtin_nontemporal_store(v, (Quad *)p);
+  }
+  __device__ __forceinline__ float operator[](uint32_t j) const {
+    if constexpr (kN == 1) {
+      return (float)v;
     } else {
-      const uint64_t i = b * 256 + threadIdx.x;
-      if (i >= n) return;
-      const uint32_t row = (uint32_t)(i / per);
-      f(row, (uint32_t)(i - (uint64_t)row * per));
+      return (float)__builtin_bit_cast(Pack, v).e[j];
     }
   }
+  static __device__ __forceinline__ Few of(const float f[kN]) {
+    Few r;
+    Pack p;
+#pragma unroll
+    for (uint32_t j = 0; j < kN; j++) p.e[j] = (T)f[j];
+    if constexpr (kN == 1)
+      r.v = p.e[0];
+    else
+      r.v = __builtin_bit_cast(V, p);
+    return r;
+  }
 };
-// Work-groups of a launch: as many as there are items, or what goes through them in turn.
-constexpr uint64_t kMostBlocks = 1 << 20;
+template <uint32_t kType>
+constexpr uint32_t kWhole = 16 / sizeof(typename Elem<kType>::T);  // elements of a whole piece
+
+// Which row (of n) and which of its pieces of kN elements a lane has: kWide: a wave's 64 pieces are one row's, so that what goes by
+// the row is scalar; else the lanes follow one another through the rows. The last piece of a row ends with it, and so shares some
+// elements with the one before (both write the same).
+template <bool kWide, uint32_t kN, typename F>
+__device__ __forceinline__ void each_piece(uint32_t n, uint32_t cols, F f) {
+  const uint32_t pieces = (cols + kN - 1) / kN;
+  if (kWide) {
+    const uint32_t runs = (pieces + 63) / 64, wave = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t row = wave / runs, piece = (wave - row * runs) * 64 + threadIdx.x % 64;
+    if (row < n && piece < pieces) f(row, min(piece * kN, cols - kN));
+  } else {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / pieces;
+    if (row < n) f(row, min((i - row * pieces) * kN, cols - kN));
+  }
+}
+
+// A value that is loaded here, whatever branch uses it (the compiler moves scalar loads into the branches, one wait each: a
+// dispatch's ten stores waited for ten of them).
+template <bool kWide, typename T>
+__device__ __forceinline__ void loaded(T &v) {
+  if (kWide)
+    asm volatile("" : "+s"(v));
+  else
+    asm volatile("" : "+v"(v));
+}
 
 // Each token's row to its ranks' places.
-template <bool kWide>
-__global__ void __launch_bounds__(256) dispatch_rows(const uint8_t *x, uint64_t x_stride, uint32_t ntok, uint32_t K, uint64_t bytes,
-                                                     const int32_t *places, uint8_t *xs, uint64_t xs_stride) {
-  const Items<kWide> items(ntok, (uint32_t)((bytes + 15) / 16));
-  for (uint64_t b = blockIdx.x; b < items.blocks(); b += gridDim.x)
-    items.each(b, [&](uint32_t t, uint32_t piece) {
-      const Piece p = piece_of(x + t * x_stride, (uint64_t)piece * 16, bytes);
-      int32_t to[16];
+template <bool kWide, uint32_t kType, uint32_t kN>
+__global__ void __launch_bounds__(256) dispatch_rows(const typename Elem<kType>::T *__restrict__ x, uint64_t x_stride, uint32_t ntok,
+                                                     uint32_t K, uint32_t cols, const int32_t *__restrict__ places,
+                                                     typename Elem<kType>::T *__restrict__ xs, uint64_t xs_stride) {
+  each_piece<kWide, kN>(ntok, cols, [&](uint32_t t, uint32_t c) {
+    Few<kType, kN> v;
+    v.load(x + t * x_stride + c);
+    int32_t to[16];
 #pragma unroll
-      for (uint32_t k = 0; k < 16; k++) to[k] = k < K ? places[(uint64_t)t * K + k] : -1;
+    for (uint32_t k = 0; k < 16; k++) to[k] = places[t * K + min(k, K - 1)];
 #pragma unroll
-      for (uint32_t k = 0; k < 16; k++)
-        if (to[k] >= 0) put_piece(xs + (uint64_t)(uint32_t)to[k] * xs_stride, (uint64_t)piece * 16, bytes, p);
-    });
+    for (uint32_t k = 0; k < 16; k++) loaded<kWide>(to[k]);
+#pragma unroll
+    for (uint32_t k = 0; k < 16; k++) {
+      if (k >= K) break;
+      if (to[k] >= 0) v.store(xs + (uint64_t)(uint32_t)to[k] * xs_stride + c);
+    }
+  });
 }
 
 // At most kFewIds ids: the sort and the rows in one launch, each wave counting its token's places itself (those of lower ids and
-// of equal ones before), the last work-group the offsets. bytes 0: no rows.
+// of equal ones before), the last work-group the offsets. cols 0: no rows.
 constexpr uint32_t kFewIds = 1024;
-__global__ void __launch_bounds__(256) dispatch_few(const int32_t *ids, uint32_t ntok, uint32_t K, uint32_t E, const uint8_t *x,
-                                                    uint64_t x_stride, uint64_t bytes, uint8_t *xs, uint64_t xs_stride, SortOut out) {
+template <uint32_t kType, uint32_t kN>
+__global__ void __launch_bounds__(256) dispatch_few(const int32_t *ids, uint32_t ntok, uint32_t K, uint32_t E,
+                                                    const typename Elem<kType>::T *x, uint64_t x_stride, uint32_t cols,
+                                                    typename Elem<kType>::T *xs, uint64_t xs_stride, SortOut out) {
   const uint32_t A = ntok * K, lane = threadIdx.x & 63;
   if (blockIdx.x == gridDim.x - 1) {
     __shared__ uint32_t n[kMostExperts];
@@ -231,11 +258,14 @@ __global__ void __launch_bounds__(256) dispatch_few(const int32_t *ids, uint32_t
   uint32_t id[kFewIds / 64];
 #pragma unroll
   for (uint32_t j = 0; j < kFewIds / 64; j++) id[j] = j * 64 + lane < A ? min((uint32_t)ids[j * 64 + lane], E) : E;
-  const uint32_t pieces = (uint32_t)((bytes + 15) / 16), runs = max((pieces + 63) / 64, 1u);
-  const uint64_t item = (uint64_t)blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  if (item >= (uint64_t)ntok * runs) return;
-  const uint32_t t = (uint32_t)(item / runs), run = (uint32_t)(item - (uint64_t)t * runs), piece = run * 64 + lane;
-  const Piece p = piece < pieces ? piece_of(x + t * x_stride, (uint64_t)piece * 16, bytes) : Piece{};
+  const uint32_t pieces = (cols + kN - 1) / kN, runs = max((pieces + 63) / 64, 1u);
+  const uint32_t wave = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t t = wave / runs, run = wave - t * runs, piece = run * 64 + lane;
+  if (t >= ntok) return;
+  const bool there = piece < pieces;
+  const uint32_t c = there ? min(piece * kN, cols - kN) : 0;
+  Few<kType, kN> v;
+  if (there) v.load(x + t * x_stride + c);
   for (uint32_t k = 0; k < K; k++) {
     const uint32_t a = t * K + k, e = min((uint32_t)ids[a], E);
     uint32_t place = 0;
@@ -248,134 +278,110 @@ __global__ void __launch_bounds__(256) dispatch_few(const int32_t *ids, uint32_t
       out.places[a] = e < E ? (int32_t)place : -1;
       if (e < E) out.order[place] = (int32_t)a;
     }
-    if (e < E && piece < pieces) put_piece(xs + (uint64_t)place * xs_stride, (uint64_t)piece * 16, bytes, p);
+    if (e < E && there) v.store(xs + (uint64_t)place * xs_stride + c);
   }
 }
 
-// ---- rows back
-
-// 16 bytes of elements, as they lie in memory.
-template <uint32_t kType>
-struct Few {
-  static constexpr uint32_t kN = 16 / sizeof(typename Elem<kType>::T);
-  typedef typename Elem<kType>::T T;
-  struct __attribute__((packed)) Pack {
-    T e[kN];
-  } p;
-  // Those from column c on (zeros past a row's end).
-  __device__ __forceinline__ void load(const T *row, uint32_t c, uint32_t cols) {
-    if (c + kN <= cols) {
-      p = *(const Pack *)(row + c);
-    } else {
+// A token's rows, eight ranks' loads on their way at a time; each rank's product is fused into the sum, in rank order. A: rows of o.
+template <bool kWide, uint32_t kIn, uint32_t kOut, uint32_t kN>
+__global__ void __launch_bounds__(256) combine_rows(const typename Elem<kIn>::T *__restrict__ o, uint64_t o_stride, uint32_t A,
+                                                    uint32_t ntok, uint32_t K, uint32_t cols, const int32_t *__restrict__ places,
+                                                    const float *__restrict__ w, typename Elem<kOut>::T *__restrict__ y,
+                                                    uint64_t y_stride) {
+  each_piece<kWide, kN>(ntok, cols, [&](uint32_t t, uint32_t c) {
+    float s[kN];
 #pragma unroll
-      for (uint32_t j = 0; j < kN; j++) p.e[j] = c + j < cols ? row[c + j] : (T)0.0f;
-    }
-  }
-  __device__ __forceinline__ float operator[](uint32_t j) const { return (float)p.e[j]; }
-};
-template <uint32_t kType, uint32_t kN>
-__device__ __forceinline__ void store_few(typename Elem<kType>::T *row, uint32_t c, uint32_t cols, const float v[kN]) {
-  typedef typename Elem<kType>::T T;
-  struct __attribute__((packed)) Pack {
-    T e[kN];
-  };
-  if (c + kN <= cols) {
-    Pack p;
+    for (uint32_t j = 0; j < kN; j++) s[j] = 0.0f;
 #pragma unroll
-    for (uint32_t j = 0; j < kN; j++) p.e[j] = (T)v[j];
-    *(Pack *)(row + c) = p;
-  } else {
+    for (uint32_t k0 = 0; k0 < 16; k0 += 8) {
+      if (k0 >= K) break;
+      Few<kIn, kN> v[8];
+      float f[8];
+      uint32_t p[8];
 #pragma unroll
-    for (uint32_t j = 0; j < kN; j++)
-      if (c + j < cols) row[c + j] = (T)v[j];
-  }
-}
-
-// A token's rows, eight ranks' loads on their way at a time; each rank's product is fused into the sum, in rank order.
-template <bool kWide, uint32_t kIn, uint32_t kOut>
-__global__ void __launch_bounds__(256) combine_rows(const typename Elem<kIn>::T *o, uint64_t o_stride, uint32_t ntok, uint32_t K,
-                                                    uint32_t cols, const int32_t *places, const float *w,
-                                                    typename Elem<kOut>::T *y, uint64_t y_stride) {
-  constexpr uint32_t kN = Few<kIn>::kN;
-  const uint32_t A = ntok * K;
-  const Items<kWide> items(ntok, (cols + kN - 1) / kN);
-  for (uint64_t b = blockIdx.x; b < items.blocks(); b += gridDim.x)
-    items.each(b, [&](uint32_t t, uint32_t piece) {
-      float s[kN];
-#pragma unroll
-      for (uint32_t j = 0; j < kN; j++) s[j] = 0.0f;
-#pragma unroll
-      for (uint32_t k0 = 0; k0 < 16; k0 += 8) {
-        if (k0 >= K) break;
-        Few<kIn> v[8];
-        float f[8];
-        bool on[8];
-#pragma unroll
-        for (uint32_t k = 0; k < 8; k++) {
-          const uint32_t a = t * K + min(k0 + k, K - 1), p = (uint32_t)places[a];
-          on[k] = k0 + k < K && p < A;
-          f[k] = w ? w[a] : 1.0f;
-          if (on[k]) v[k].load(o + p * o_stride, piece * kN, cols);
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < 8; k++)
-          if (on[k])
-#pragma unroll
-            for (uint32_t j = 0; j < kN; j++) s[j] = __builtin_fmaf(f[k], v[k][j], s[j]);
+      for (uint32_t k = 0; k < 8; k++) {
+        const uint32_t a = t * K + min(k0 + k, K - 1);
+        p[k] = (uint32_t)places[a];
+        f[k] = w ? w[a] : 1.0f;
       }
-      store_few<kOut, kN>(y + t * y_stride, piece * kN, cols, s);
-    });
+#pragma unroll
+      for (uint32_t k = 0; k < 8; k++) {
+        loaded<kWide>(p[k]), loaded<kWide>(f[k]);
+        if (k0 + k >= K) p[k] = ~0u;
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < 8; k++)
+        if (p[k] < A) v[k].load(o + p[k] * o_stride + c);
+#pragma unroll
+      for (uint32_t k = 0; k < 8; k++)
+        if (p[k] < A)
+#pragma unroll
+          for (uint32_t j = 0; j < kN; j++) s[j] = __builtin_fmaf(f[k], v[k][j], s[j]);
+    }
+    typedef typename Elem<kOut>::T T;
+    if constexpr (kN == 1) {
+      y[t * y_stride + c] = (T)s[0];
+    } else {
+      struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+        T e[kN];
+      } r;
+#pragma unroll
+      for (uint32_t j = 0; j < kN; j++) r.e[j] = (T)s[j];
+      *(Pack *)(y + t * y_stride + c) = r;
+    }
+  });
 }
 
 // A wave an assignment: do = w dy (rounded once) and dw = <dy, o>, four pieces of both rows on their way at a time; a lane's
 // products are added in column order, the lanes' sums by halves. dw or dout may be null.
-template <uint32_t kType>
-__global__ void __launch_bounds__(256) combine_gradient(const typename Elem<kType>::T *dy, uint64_t dy_stride, uint32_t A, uint32_t K,
-                                                        uint32_t cols, const int32_t *places, const typename Elem<kType>::T *o,
-                                                        uint64_t o_stride, const float *w, typename Elem<kType>::T *dout,
-                                                        uint64_t do_stride, float *dw) {
-  constexpr uint32_t kN = Few<kType>::kN, kRun = 64 * kN;
-  const uint32_t lane = threadIdx.x & 63;
-  for (uint64_t i = (uint64_t)blockIdx.x * 4; i < A; i += (uint64_t)gridDim.x * 4) {
-    const uint32_t a = (uint32_t)i + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    if (a >= A) continue;
-    const uint32_t p = (uint32_t)places[a];
-    if (p >= A) {
-      if (dw && lane == 0) dw[a] = 0.0f;
-      continue;
-    }
-    const float f = w ? w[a] : 1.0f;
-    const auto *from = dy + (uint64_t)(a / K) * dy_stride;
-    float s = 0.0f;
-    for (uint32_t c0 = lane * kN; c0 < cols; c0 += 4 * kRun) {
-      Few<kType> d[4], v[4];
+template <uint32_t kType, uint32_t kN>
+__global__ void __launch_bounds__(256) combine_gradient(const typename Elem<kType>::T *__restrict__ dy, uint64_t dy_stride, uint32_t A,
+                                                        uint32_t K, uint32_t cols, const int32_t *__restrict__ places,
+                                                        const typename Elem<kType>::T *__restrict__ o, uint64_t o_stride,
+                                                        const float *__restrict__ w, typename Elem<kType>::T *__restrict__ dout,
+                                                        uint64_t do_stride, float *__restrict__ dw) {
+  constexpr uint32_t kRun = 64 * kN;
+  const uint32_t lane = threadIdx.x & 63, a = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  if (a >= A) return;
+  const uint32_t p = (uint32_t)places[a];
+  if (p >= A) {
+    if (dw && lane == 0) dw[a] = 0.0f;
+    return;
+  }
+  const float f = w ? w[a] : 1.0f;
+  dy += a / K * dy_stride;
+  if (dw) o += p * o_stride;
+  if (dout) dout += p * do_stride;
+  float s = 0.0f;
+  for (uint32_t c0 = lane * kN; c0 < cols; c0 += 4 * kRun) {
+    Few<kType, kN> d[4], v[4];
 #pragma unroll
-      for (uint32_t j = 0; j < 4; j++) {
-        const uint32_t c = c0 + j * kRun;
-        if (c >= cols) break;
-        d[j].load(from, c, cols);
-        if (dw) v[j].load(o + p * o_stride, c, cols);
+    for (uint32_t j = 0; j < 4; j++) {
+      const uint32_t c = c0 + j * kRun;
+      if (c >= cols) break;
+      d[j].v = *(const typename Few<kType, kN>::V *)(dy + min(c, cols - kN));  // (read again by the token's other ranks)
+      if (dw) v[j].load(o + min(c, cols - kN));
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+      const uint32_t c = c0 + j * kRun, at = min(c, cols - kN);
+      if (c >= cols) break;
+      if (dw)
+#pragma unroll
+        for (uint32_t n = 0; n < kN; n++)
+          if (at + n >= c) s = __builtin_fmaf(d[j][n], v[j][n], s);  // (the others are the piece before's)
+      if (dout) {
+        float e[kN];
+#pragma unroll
+        for (uint32_t n = 0; n < kN; n++) e[n] = f * d[j][n];
+        Few<kType, kN>::of(e).store(dout + at);
       }
-#pragma unroll
-      for (uint32_t j = 0; j < 4; j++) {
-        const uint32_t c = c0 + j * kRun;
-        if (c >= cols) break;
-        if (dw)
-#pragma unroll
-          for (uint32_t n = 0; n < kN; n++) s = __builtin_fmaf(d[j][n], v[j][n], s);
-        if (dout) {
-          float e[kN];
-#pragma unroll
-          for (uint32_t n = 0; n < kN; n++) e[n] = f * d[j][n];
-          store_few<kType, kN>(dout + p * do_stride, c, cols, e);
-        }
-      }
     }
-    if (dw) {
+  }
+  if (dw) {
 #pragma unroll
-      for (uint32_t m = 32; m >= 1; m /= 2) s += __shfl_xor(s, (int)m, 64);
-      if (lane == 0) dw[a] = s;
-    }
+    for (uint32_t m = 32; m >= 1; m /= 2) s += __shfl_xor(s, (int)m, 64);
+    if (lane == 0) dw[a] = s;
   }
 }
 
@@ -389,13 +395,23 @@ uint32_t slice_of(uint32_t A) {
 }
 uint32_t slices_of(uint32_t A) { return A ? (A + slice_of(A) - 1) / slice_of(A) : 0; }
 
-// f with whether the rows' pieces are wide, as a constant.
+// f(whether the rows' pieces are wide, the elements of a piece) as constants, for rows of kType: waves of one row's pieces where
+// that leaves no more than half of the lanes without one.
+template <uint32_t kType, typename F>
+void op_by_pieces(uint32_t cols, F f) {
+  constexpr uint32_t kN = kWhole<kType>;
+  if (cols >= 32 * kN) return f(std::true_type(), std::integral_constant<uint32_t, kN>());
+  if (cols >= kN) return f(std::false_type(), std::integral_constant<uint32_t, kN>());
+  f(std::false_type(), std::integral_constant<uint32_t, 1>());
+}
+// launch(t0, tokens, work-groups) for as many tokens at a time as a launch has threads for.
 template <typename F>
-void op_by_width(uint64_t pieces, F f) {
-  if (pieces >= kWidePieces)
-    f(std::true_type());
-  else
-    f(std::false_type());
+void by_tokens(uint32_t ntok, bool wide, uint32_t pieces, F launch) {
+  const uint32_t runs = (pieces + 63) / 64, most = wide ? (1u << 25) / runs : ntok;
+  for (uint32_t t0 = 0; t0 < ntok; t0 += most) {
+    const uint32_t n = std::min(ntok - t0, most);
+    launch(t0, n, wide ? ((uint64_t)n * runs + 3) / 4 : ((uint64_t)n * pieces + 255) / 256);
+  }
 }
 
 }  // namespace
@@ -415,12 +431,14 @@ void combine_launch(uint32_t type, const void *o, uint64_t o_stride, uint32_t nt
     op_by_type(y_type, [&](auto out) {
       constexpr uint32_t kIn = decltype(in)::value, kOut = decltype(out)::value;
       if constexpr (kIn == QT_F32 || kIn == kOut) {
-        const uint32_t pieces = (cols + Few<kIn>::kN - 1) / Few<kIn>::kN;
-        op_by_width(pieces, [&](auto wide) {
+        op_by_pieces<kIn>(cols, [&](auto wide, auto piece) {
           constexpr bool kWide = decltype(wide)::value;
-          const uint64_t n = std::min(Items<kWide>(ntok, pieces).blocks(), kMostBlocks);
-          op_launch(combine_rows<kWide, kIn, kOut>, n, 256, stream, (const typename Elem<kIn>::T *)o, o_stride, ntok, K, cols, places,
-                    w, (typename Elem<kOut>::T *)y, y_stride);
+          constexpr uint32_t kN = decltype(piece)::value;
+          by_tokens(ntok, kWide, (cols + kN - 1) / kN, [&](uint32_t t0, uint32_t n, uint64_t blocks) {
+            op_launch(combine_rows<kWide, kIn, kOut, kN>, blocks, 256, stream, (const typename Elem<kIn>::T *)o, o_stride, ntok * K, n,
+                      K, cols, places + (uint64_t)t0 * K, w ? w + (uint64_t)t0 * K : nullptr,
+                      (typename Elem<kOut>::T *)y + t0 * y_stride, y_stride);
+          });
         });
       }
     });
@@ -475,21 +493,32 @@ MOE_API moe_status moe_dispatch_async(const moe_dispatch_config *cfg, const void
     op_work(work, work_bytes, sort_bytes(A, E));
     OnDevice on(cfg->device);
     const SortOut out{order, places, offsets, nullptr, nullptr, 1};
-    const uint8_t *from = (const uint8_t *)x;
-    uint8_t *to = (uint8_t *)xs;
-    const uint64_t bytes = xs ? (uint64_t)H * size : 0, pieces = (bytes + 15) / 16;
-    if (A <= kFewIds) {
-      const uint64_t waves = ntok * std::max<uint64_t>((pieces + 63) / 64, 1);
-      return op_launch(dispatch_few, (waves + 3) / 4 + 1, 256, stream, ids, ntok, K, E, from, x_stride * size, bytes, to,
-                       xs_stride * size, out);
-    }
-    sort_launch(ids, A, E, out, work, stream);
-    if (xs)
-      op_by_width(pieces, [&](auto wide) {
+    if (A > kFewIds) sort_launch(ids, A, E, out, work, stream);
+    // (Copies: the element type matters by its size alone.)
+    const auto rows = [&](auto t) {
+      constexpr uint32_t kType = decltype(t)::value;
+      const auto *from = (const typename Elem<kType>::T *)x;
+      auto *to = (typename Elem<kType>::T *)xs;
+      op_by_pieces<kType>(H, [&](auto wide, auto piece) {
         constexpr bool kWide = decltype(wide)::value;
-        op_launch(dispatch_rows<kWide>, std::min(Items<kWide>(ntok, (uint32_t)pieces).blocks(), kMostBlocks), 256, stream, from,
-                  x_stride * size, ntok, K, bytes, (const int32_t *)places, to, xs_stride * size);
+        constexpr uint32_t kN = decltype(piece)::value;
+        if (A <= kFewIds) {
+          const uint32_t cols = xs ? H : 0;
+          const uint64_t waves = (uint64_t)ntok * std::max(((cols + kN - 1) / kN + 63) / 64, 1u);
+          return op_launch(dispatch_few<kType, kN>, (waves + 3) / 4 + 1, 256, stream, ids, ntok, K, E, from, x_stride, cols, to,
+                           xs_stride, out);
+        }
+        if (!xs) return;
+        by_tokens(ntok, kWide, (H + kN - 1) / kN, [&](uint32_t t0, uint32_t n, uint64_t blocks) {
+          op_launch(dispatch_rows<kWide, kType, kN>, blocks, 256, stream, from + t0 * x_stride, x_stride, n, K, H,
+                    (const int32_t *)places + (uint64_t)t0 * K, to, xs_stride);
+        });
       });
+    };
+    if (size == 4)
+      rows(std::integral_constant<uint32_t, QT_F32>());
+    else
+      rows(std::integral_constant<uint32_t, QT_F16>());
   });
 }
 
@@ -526,9 +555,12 @@ MOE_API moe_status moe_combine_backward_async(const moe_dispatch_config *cfg, co
     if (!ntok || (!dw && !dout)) return;
     OnDevice on(cfg->device);
     op_by_type(cfg->type, [&](auto t) {
-      typedef typename Elem<decltype(t)::value>::T T;
-      op_launch(combine_gradient<decltype(t)::value>, std::min<uint64_t>(((uint64_t)A + 3) / 4, kMostBlocks), 256, stream,
-                (const T *)dy, dy_stride, A, K, H, places, (const T *)o, o_stride, w, (T *)dout, dout_stride, dw);
+      constexpr uint32_t kType = decltype(t)::value;
+      typedef typename Elem<kType>::T T;
+      op_by_pieces<kType>(H, [&](auto, auto piece) {
+        op_launch(combine_gradient<kType, decltype(piece)::value>, ((uint64_t)A + 3) / 4, 256, stream, (const T *)dy, dy_stride, A, K, H,
+                  places, (const T *)o, o_stride, w, (T *)dout, dout_stride, dw);
+      });
     });
   });
 }
