@@ -26,14 +26,29 @@ __device__ __forceinline__ uint32_t i8_code(float x, float s, float inv) {
   const int i = (int)k;
   return (uint32_t)(i + (d > 0.0f ? 1 : d == 0.0f ? i & 1 : 0)) & 0xffu;
 }
-// Eight values as two words of codes.
+// Eight values as two words of codes. x / s to 2^-14 lies in the low bits of x (1 / s) + 1.5 2^23, rounded once to a whole number;
+// where some lane's is that near a half (one group in 16), its eight by i8_code.
 __device__ __forceinline__ uint2 i8_codes8(const float v[8], float s) {
   if (s != s) return make_uint2(0, 0);
+  constexpr float kWhole = 12582912.0f;  // 1.5 2^23
   const float inv = __builtin_amdgcn_rcpf(s);
   uint32_t c[8];
+  float off = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 8; j++) c[j] = i8_code(v[j], s, inv);
-  return make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+  for (int j = 0; j < 8; j++) {
+    const float t = __builtin_fmaf(v[j], inv, kWhole);
+    c[j] = __float_as_uint(t);
+    off = __builtin_fmaxf(off, __builtin_fabsf(__builtin_fmaf(v[j], inv, kWhole - t)));
+  }
+  if (off > 0.5f - 0x1p-14f) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) c[j] = i8_code(v[j], s, inv);
+  }
+  const auto four = [&](int j) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[j + 3], c[j + 2], 0x0c0c0400u), __builtin_amdgcn_perm(c[j + 1], c[j], 0x0c0c0400u),
+                                 0x05040100u);
+  };
+  return make_uint2(four(0), four(4));
 }
 __device__ __forceinline__ uint32_t most_of8(const float v[8]) {
   uint32_t most = 0;

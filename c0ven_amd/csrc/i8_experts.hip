@@ -29,8 +29,10 @@ __global__ void __launch_bounds__(256) i8_gate_up_tiles(I8Experts p, const int8_
                                                         float *h, uint32_t pitch) {
   typedef I8Tile<TM, 2, WM, true, true> Tile;
   constexpr uint32_t kCols = Tile::BN / 2;
-  __shared__ typename Tile::Stage s0;
-  __shared__ typename Tile::Stage s1;
+  __shared__ typename Tile::X x0;
+  __shared__ typename Tile::X x1;
+  __shared__ typename Tile::W w0;
+  __shared__ typename Tile::W w1;
   __shared__ __align__(16) float sx[Tile::BM];
   const uint32_t steps = i8_steps(p.H), parts = (p.F + kCols - 1) / kCols, item = item_of(*n_tiles * parts, parts);
   if (item == ~0u) return;
@@ -44,7 +46,9 @@ __global__ void __launch_bounds__(256) i8_gate_up_tiles(I8Experts p, const int8_
   const I8Source<kCols> u(p.uc + row * steps * kI8Row, rest, steps, same);
   if (threadIdx.x < Tile::BM) sx[threadIdx.x] = threadIdx.x < tile.count ? xs[token(threadIdx.x)] : 0.0f;
   Tile c;
-  c.run(s0, s1, steps, [&](typename Tile::Stage &s, uint32_t k) { g.load(k, s.w), u.load(k, s.w + kCols * kI8Row), x.load(k, s.x); });
+  c.run2(
+      x0, x1, w0, w1, steps, [&](typename Tile::X &s, uint32_t k) { x.load(k, s.b); },
+      [&](typename Tile::W &s, uint32_t k) { g.load(k, s.b), u.load(k, s.b + kCols * kI8Row); });
   const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = Tile::w_row() + lane % 32;
   const bool in = f0 + col < p.F;
   const float sg = in ? p.gs[row + col] : 0.0f, su = in ? p.us[row + col] : 0.0f;
@@ -71,8 +75,10 @@ template <int TM, int WM>
 __global__ void __launch_bounds__(256) i8_down_tiles(I8Experts p, const int8_t *hc, const float *hs, const MoeTile *tiles,
                                                      const uint32_t *n_tiles, uint32_t r0, uint32_t cols, float *o) {
   typedef I8Tile<TM, 2, WM, true, true> Tile;
-  __shared__ typename Tile::Stage s0;
-  __shared__ typename Tile::Stage s1;
+  __shared__ typename Tile::X x0;
+  __shared__ typename Tile::X x1;
+  __shared__ typename Tile::W w0;
+  __shared__ typename Tile::W w1;
   __shared__ __align__(16) float sh[Tile::BM];
   const uint32_t steps = i8_steps(p.F), parts = cols / Tile::BN, item = item_of(*n_tiles * parts, parts);
   if (item == ~0u) return;
@@ -84,7 +90,9 @@ __global__ void __launch_bounds__(256) i8_down_tiles(I8Experts p, const int8_t *
   const I8Source<Tile::BN> w(p.dc + row * steps * kI8Row, all - row, steps, same);
   if (threadIdx.x < Tile::BM) sh[threadIdx.x] = threadIdx.x < tile.count ? hs[tile.start + threadIdx.x] : 0.0f;
   Tile c;
-  c.run(s0, s1, steps, [&](typename Tile::Stage &s, uint32_t k) { w.load(k, s.w), x.load(k, s.x); });
+  c.run2(
+      x0, x1, w0, w1, steps, [&](typename Tile::X &s, uint32_t k) { x.load(k, s.b); },
+      [&](typename Tile::W &s, uint32_t k) { w.load(k, s.b); });
   const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = Tile::w_row() + lane % 32;
   float sd[2];
 #pragma unroll

@@ -7,10 +7,9 @@
 namespace c0ven {
 
 // A stage of k = 128, its eight 16-byte pieces of a row exchanged as in MxStage.
-template <int BM, int BN>
-struct I8Stage {
-  alignas(16) uint8_t x[BM * kI8Row];
-  alignas(16) uint8_t w[BN * kI8Row];
+template <int kRows>
+struct I8Rows {
+  alignas(16) uint8_t b[kRows * kI8Row];
 };
 
 // kRows rows as the source of stages: row r of them is row_of(r) of the `rows` at codes (less than kNowhere bytes as far as row_of
@@ -45,7 +44,8 @@ struct I8Source {
 template <int TM, int TN, int WM = 2, bool kApart = false, bool kAcross = false, int kWaves = 4>
 struct I8Tile {
   static constexpr int WN = kWaves / WM, BM = 32 * WM * TM, BN = 32 * WN * TN;
-  typedef I8Stage<BM, BN> Stage;
+  typedef I8Rows<BM> X;
+  typedef I8Rows<BN> W;
   i8_i16 acc[TN][TM];
   mx_i4 a[2][TN], b[2][TM];
 
@@ -54,13 +54,13 @@ struct I8Tile {
   static constexpr uint32_t kStep = kApart ? 32 * WN : 32;  // between a wave's runs of w
 
   template <int j>
-  __device__ __forceinline__ void read(const Stage &s) {
+  __device__ __forceinline__ void read(const X &x, const W &w) {
     const uint32_t lane = threadIdx.x & 63, q = lane / 32, r = lane % 32;
     const uint32_t at = ((2 * j + q) ^ (r / 2 % 8)) * 16;
 #pragma unroll
-    for (int m = 0; m < TM; m++) b[j % 2][m] = *(const mx_i4 *)(s.x + (x_row() + r + 32 * m) * kI8Row + at);
+    for (int m = 0; m < TM; m++) b[j % 2][m] = *(const mx_i4 *)(x.b + (x_row() + r + 32 * m) * kI8Row + at);
 #pragma unroll
-    for (int n = 0; n < TN; n++) a[j % 2][n] = *(const mx_i4 *)(s.w + (w_row() + r + kStep * n) * kI8Row + at);
+    for (int n = 0; n < TN; n++) a[j % 2][n] = *(const mx_i4 *)(w.b + (w_row() + r + kStep * n) * kI8Row + at);
   }
   template <int j>
   __device__ __forceinline__ void multiply() {
@@ -79,46 +79,93 @@ struct I8Tile {
 #pragma unroll
       for (int m = 0; m < TM; m++) asm volatile("" : "+a"(acc[n][m]));
   }
-  // Stage `now`; its step 0 is in registers. After the barrier `now` is free (load() loads what comes after `next` into it) and
-  // `next` is whole. Past the last stage its first step is read all the same, and not used.
-  template <typename Load>
-  __device__ __forceinline__ void stage(const Stage &now, const Stage &next, Load load) {
-    read<1>(now);
-    multiply<0>();
-    read<2>(now);
-    multiply<1>();
-    read<3>(now);
-    multiply<2>();
-    pin();
-    dma_barrier();
-    load();
-    read<0>(next);
-    multiply<3>();
-    pin();
-  }
-  // All stages 0 .. n - 1 of a product (n > 0): load(stage, k) loads stage k's codes.
-  template <typename Load>
-  __device__ __forceinline__ void run(Stage &s0, Stage &s1, uint32_t n, Load load) {
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < TN; i++)
+    for (int n = 0; n < TN; n++)
 #pragma unroll
       for (int m = 0; m < TM; m++)
 #pragma unroll
-        for (int j = 0; j < 16; j++) acc[i][m][j] = 0;
-    load(s0, 0);
+        for (int j = 0; j < 16; j++) acc[n][m][j] = 0;
+  }
+  // Stage x, w; its step 0 is in registers. barrier() waits for the next stage's loads and for every wave; then x and w are free
+  // (load() loads what comes later into them). Past the last stage its first step is read all the same, and not used.
+  template <typename Barrier, typename Load>
+  __device__ __forceinline__ void stage(const X &x, const W &w, const X &next_x, const W &next_w, Barrier barrier, Load load) {
+    read<1>(x, w);
+    multiply<0>();
+    read<2>(x, w);
+    multiply<1>();
+    read<3>(x, w);
+    multiply<2>();
+    pin();
+    barrier();
+    load();
+    read<0>(next_x, next_w);
+    multiply<3>();
+    pin();
+  }
+  // All stages 0 .. n - 1 of a product (n > 0), two buffers each: load_x(buffer, k) and load_w load stage k's codes.
+  template <typename LoadX, typename LoadW>
+  __device__ __forceinline__ void run2(X &x0, X &x1, W &w0, W &w1, uint32_t n, LoadX load_x, LoadW load_w) {
+    clear();
+    load_w(w0, 0), load_x(x0, 0);
     dma_barrier();
-    if (n > 1) load(s1, 1);
-    read<0>(s0);
+    if (n > 1) load_w(w1, 1), load_x(x1, 1);
+    read<0>(x0, w0);
     uint32_t k = 0;
     for (; k + 1 < n; k += 2) {
-      stage(s0, s1, [&] {
-        if (k + 2 < n) load(s0, k + 2);
+      stage(x0, w0, x1, w1, dma_barrier, [&] {
+        if (k + 2 < n) load_w(w0, k + 2), load_x(x0, k + 2);
       });
-      stage(s1, s0, [&] {
-        if (k + 3 < n) load(s1, k + 3);
+      stage(x1, w1, x0, w0, dma_barrier, [&] {
+        if (k + 3 < n) load_w(w1, k + 3), load_x(x1, k + 3);
       });
     }
-    if (k < n) stage(s0, s1, [] {});
+    if (k < n) stage(x0, w0, x1, w1, dma_barrier, [] {});
+  }
+  // The same with three buffers of x and two of w (all of LDS with tiles of 256): x is loaded two stages ahead, so that half of a
+  // stage's bytes have two stages' time, and a barrier waits for w's (and the older x's) alone: all but the last kXLoads loads of
+  // a wave, which are one buffer of x's.
+  template <int kXLoads, typename LoadX, typename LoadW>
+  __device__ __forceinline__ void run5(X &x0, X &x1, X &x2, W &w0, W &w1, uint32_t n, LoadX load_x, LoadW load_w) {
+    clear();
+    load_w(w0, 0), load_x(x0, 0);
+    dma_barrier();
+    if (n > 1) load_x(x1, 1), load_w(w1, 1);
+    if (n > 2) load_x(x2, 2);
+    read<0>(x0, w0);
+    uint32_t k = 0;
+    const auto six = [&](auto each) {
+      each(x0, w0, x1, w1, k);
+      each(x1, w1, x2, w0, k + 1);
+      each(x2, w0, x0, w1, k + 2);
+      each(x0, w1, x1, w0, k + 3);
+      each(x1, w0, x2, w1, k + 4);
+      each(x2, w1, x0, w0, k + 5);
+    };
+    // (Without conditions, so that the compiler knows which loads are outstanding where.)
+    for (; k + 8 < n; k += 6)
+      six([&](X &x, W &w, const X &next_x, const W &next_w, uint32_t i) {
+        stage(
+            x, w, next_x, next_w,
+            [] {  // (no fence: it would wait for all loads)
+              asm volatile("" ::: "memory");
+              __builtin_amdgcn_s_waitcnt(0x0070 | kXLoads);  // vmcnt(kXLoads) lgkmcnt(0)
+              __builtin_amdgcn_s_barrier();
+              asm volatile("" ::: "memory");
+            },
+            [&] { load_w(w, i + 2), load_x(x, i + 3); });
+      });
+    const auto last = [&](X &x, W &w, const X &next_x, const W &next_w, uint32_t i) {
+      if (i < n)
+        stage(x, w, next_x, next_w, dma_barrier, [&] {
+          if (i + 2 < n) load_w(w, i + 2);
+          if (i + 3 < n) load_x(x, i + 3);
+        });
+    };
+    six(last);
+    last(x0, w0, x1, w1, k + 6);
+    last(x1, w1, x2, w0, k + 7);
   }
 };
 

@@ -89,17 +89,23 @@ __global__ void __launch_bounds__(256) i8_join(const int *sums, uint32_t parts, 
 }
 
 // A tile of y a work-group, k split into parts of `span` stages; kSums: the sums themselves, part p's to y + p M N, else y's
-// values. Work-groups to tiles so that an XCD has neighbours: eight tiles down, then across.
+// values. Work-groups to tiles so that an XCD has neighbours: eight tiles down, then across. The 256 tile has eight waves and
+// five buffers. 4096 x 8192 x 8192 on a layer's codes: 247 us, 2.2 POPS, and 254 to 300 with two buffers of each; the clock gives
+// way under such codes (on zeros 183 us, 3.0 POPS, and 202 with two buffers), and the matrix instructions alone, on operands
+// that stay in registers, take 185 on random ones. Four waves of 128 x 128 each read a third less of LDS but leave a SIMD one wave: 265.
 template <uint32_t kType, bool kSums, int TM, int TN, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves, 2)
     i8_gemm(const int8_t *xc, const float *xs, const int8_t *wc, const float *ws, uint32_t M, uint32_t N, uint32_t steps,
             uint32_t span, typename Elem<kType>::T *y, uint64_t stride) {
   typedef I8Tile<TM, TN, 2, false, false, kWaves> Tile;
   constexpr int BM = Tile::BM, BN = Tile::BN;
+  constexpr bool kFive = BM == 256;
   typedef typename Elem<kType>::T T;
   static_assert(!kSums || sizeof(T) == 4, "sums are 32 bits");
-  __shared__ typename Tile::Stage s0;
-  __shared__ typename Tile::Stage s1;
+  __shared__ typename Tile::X x0;
+  __shared__ typename Tile::X x1;
+  __shared__ typename Tile::W w0;
+  __shared__ typename Tile::W w1;
   const uint32_t tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
   const uint32_t parts = (steps + span - 1) / span, all = tm * tn * parts;
   const uint32_t per = (all + 7) / 8, id = blockIdx.x % 8 * per + blockIdx.x / 8;
@@ -110,16 +116,24 @@ __global__ void __launch_bounds__(64 * kWaves, 2)
   const auto same = [](uint32_t r) { return r; };
   const I8Source<BM, kWaves> sx(xc + (uint64_t)m0 * steps * kI8Row, M - m0, steps, same);
   const I8Source<BN, kWaves> sw(wc + (uint64_t)n0 * steps * kI8Row, N - n0, steps, same);
+  const auto load_x = [&](typename Tile::X &s, uint32_t k) { sx.load(k0 + k, s.b); };
+  const auto load_w = [&](typename Tile::W &s, uint32_t k) { sw.load(k0 + k, s.b); };
   Tile c;
-  c.run(s0, s1, k1 - k0, [&](typename Tile::Stage &s, uint32_t k) { sx.load(k0 + k, s.x), sw.load(k0 + k, s.w); });
+  if constexpr (kFive) {
+    __shared__ typename Tile::X x2;
+    c.template run5<I8Source<BM, kWaves>::kLoads>(x0, x1, x2, w0, w1, k1 - k0, load_x, load_w);
+  } else {
+    c.run2(x0, x1, w0, w1, k1 - k0, load_x, load_w);
+  }
   __builtin_amdgcn_s_barrier();  // (the stages' LDS is used again)
   // Each wave's 32 rows at a time through its part of LDS, so that a row's neighbours are stored together: a lane has four
   // columns, the same of every row.
   const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32, r = lane % 32;
-  constexpr uint32_t kWide = 32 * TN, kPitch = kWide + 4, kHalf = kWaves / 2;
+  constexpr uint32_t kWide = 32 * TN, kPitch = kWide + 4, kFour = kWaves / 4;
   static_assert(64 % (kWide / 4) == 0, "a lane's columns");
-  int *mine = (int *)(wave < kHalf ? (uint8_t *)&s0 : (uint8_t *)&s1) + wave % kHalf * 32 * kPitch;
-  static_assert(kHalf * 32 * kPitch * 4 <= sizeof(s0), "half the waves' rows in a stage");
+  static_assert(kWaves % 4 == 0 && kFour * 32 * kPitch * 4 <= sizeof(x0) && BM == BN, "a quarter of the waves' rows in a buffer");
+  const uint32_t b = wave / kFour;
+  int *mine = (int *)(b == 0 ? x0.b : b == 1 ? x1.b : b == 2 ? w0.b : w1.b) + wave % kFour * 32 * kPitch;
   const uint32_t wm = m0 + Tile::x_row(), gn = n0 + Tile::w_row() + lane % (kWide / 4) * 4;
   if (kSums) y += (uint64_t)p * M * N;
   const bool whole = gn + 4 <= N && stride % 4 == 0 && ((uintptr_t)y & (4 * sizeof(T) - 1)) == 0;
