@@ -57,6 +57,80 @@ __device__ __forceinline__ uint32_t most_of8(const float v[8]) {
   return most;
 }
 
+// Eight neighbours of a row from column c on, as they lie in memory: one (two for fp32) 16-byte load at whatever address and no
+// branch, so that several are on their way at once; past the row's end the load is of its last eight (cols >= 8), and values()
+// moves them down and fills up with zeros.
+template <uint32_t kType>
+struct Eight {
+  typedef typename Elem<kType>::T T;
+  typedef uint32_t Quad __attribute__((ext_vector_type(4), aligned(2)));
+  static constexpr int kQuads = sizeof(T) / 2;
+  uint32_t d[4 * kQuads];
+  __device__ __forceinline__ void load(const T *row, uint32_t c, uint32_t cols) {
+    const Quad *from = (const Quad *)(row + min(c, cols - 8));
+#pragma unroll
+    for (int i = 0; i < kQuads; i++) {
+      const Quad v = from[i];
+#pragma unroll
+      for (int j = 0; j < 4; j++) d[4 * i + j] = v[j];
+    }
+  }
+  __device__ __forceinline__ void values(uint32_t c, uint32_t cols, float v[8]) {
+    const uint32_t past = c + 8 > cols ? c + 8 - cols : 0;
+    if (__any(past != 0)) {
+      constexpr int n = 4 * kQuads;
+#pragma unroll
+      for (int by = 4; by >= 1; by /= 2) {  // (elements)
+        const bool move = past & by;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+          uint32_t to;
+          if (sizeof(T) == 4) {
+            to = i + by < n ? d[i + by] : 0u;
+          } else if (by > 1) {
+            to = i + by / 2 < n ? d[i + by / 2] : 0u;
+          } else {
+            to = __builtin_amdgcn_alignbit(i + 1 < n ? d[i + 1] : 0u, d[i], 16);
+          }
+          d[i] = move ? to : d[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < n; i++) d[i] = past >= 8 ? 0u : d[i];
+    }
+    struct Values {
+      T e[8];
+    };
+    struct Words {
+      uint32_t d[4 * kQuads];
+    } w;
+#pragma unroll
+    for (int i = 0; i < 4 * kQuads; i++) w.d[i] = d[i];
+    const Values e = __builtin_bit_cast(Values, w);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = (float)e.e[j];
+  }
+};
+// kN groups of eight, group i of rows(i) from column cols_of(i) on; rows shorter than eight element by element.
+template <uint32_t kType, int kN, typename Row, typename Col>
+__device__ __forceinline__ void load_eights(uint32_t cols, Row row, Col col, float v[kN][8]) {
+  if (cols >= 8) {
+    Eight<kType> e[kN];
+#pragma unroll
+    for (int i = 0; i < kN; i++) e[i].load(row(i), col(i), cols);
+#pragma unroll
+    for (int i = 0; i < kN; i++) e[i].values(col(i), cols, v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kN; i++)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; j++) {
+        const float x = (float)row(i)[min(j, cols - 1)];
+        v[i][j] = col(i) + j < cols ? x : 0.0f;
+      }
+  }
+}
+
 // c += a b^T on 16 rows each over k = 64: lane l gives row l % 16, bytes 16 (l / 16) and on; it receives c of a's rows
 // 4 (l / 16) + i, b's row l % 16.
 __device__ __forceinline__ mx_i4 i8_mfma16(mx_i4 a, mx_i4 b, mx_i4 c) {

@@ -24,8 +24,7 @@ __global__ void __launch_bounds__(kThreads < 256 ? 256 : kThreads)
     float v[kAhead][8];
     uint32_t most = 0;
     for (uint32_t g0 = tid; g0 < (kLong ? ng : tid + 1); g0 += kSpan) {
-#pragma unroll
-      for (int i = 0; i < kAhead; i++) load8<kType>(row, (g0 + i * kThreads) * 8, cols, v[i]);
+      load_eights<kType, kAhead>(cols, [&](int) { return row; }, [&](int i) { return (g0 + i * kThreads) * 8; }, v);
 #pragma unroll
       for (int i = 0; i < kAhead; i++) most = max(most, most_of8(v[i]));
     }
@@ -39,10 +38,10 @@ __global__ void __launch_bounds__(kThreads < 256 ? 256 : kThreads)
     }
     const float s = i8_scale_of(most);
     for (uint32_t g0 = tid; g0 < (kLong ? ng : tid + 1); g0 += kSpan) {
+      if (kLong) load_eights<kType, kAhead>(cols, [&](int) { return row; }, [&](int i) { return (g0 + i * kThreads) * 8; }, v);
 #pragma unroll
       for (int i = 0; i < kAhead; i++) {
         const uint32_t g = g0 + i * kThreads;
-        if (kLong) load8<kType>(row, g * 8, cols, v[i]);
         if (g < ng) *(uint2 *)(codes + (uint64_t)r * ng * 8 + g * 8) = i8_codes8(v[i], s);
       }
     }

@@ -114,227 +114,343 @@ __global__ void __launch_bounds__(256) i8_down_tiles(I8Experts p, const int8_t *
     }
 }
 
-// ---- few assignments (at most kFew): no sorting, two launches. Bound by latency and by reading the experts' weights, which
-// go to LDS as whole rows: all that a work-group needs is on its way at once.
+// ---- few assignments (at most kFew of at most 16 tokens): no sorting, two or three launches. Bound by latency and by reading the experts'
+// weights, which go to LDS as whole rows, always some of them on their way.
 
 constexpr uint32_t kFew = 160;
 
-// A work-group: an expert and 16 columns of h, for the tokens that use the expert, kTok at a time: the assignment that is the
-// first with its expert does the work, the others' work-groups leave. Quantises x itself (while the weights come) and writes the
-// assignments' rows of h, `pitch` apart. Four waves share the k axis, kSteps steps of 128 at a time (all of n_embd, where it is
-// not longer); the sums are joined in LDS.
-template <uint32_t kX, int kSteps>
-__global__ void __launch_bounds__(256) i8_gate_up_few(I8Experts p, const typename Elem<kX>::T *x, uint64_t stride,
-                                                      const int32_t *ids, uint32_t A, float *h, uint32_t pitch) {
-  constexpr uint32_t kTok = 6, kPitch = kSteps * kI8Row, kXPitch = kPitch + 16;
-  static_assert(kSteps % 2 == 0, "rows of 16 pieces");
-  __shared__ __align__(16) uint8_t wc[32 * kPitch];  // gate's 16 rows, up's; a row's 16-byte pieces exchanged by r % 16
-  __shared__ __align__(16) uint8_t xc[kTok * kXPitch];
-  __shared__ int sums[4][32][kTok];
-  __shared__ uint32_t most[kTok];
-  __shared__ uint16_t member[kFew];
-  __shared__ uint32_t counts[4];
-  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 16, r = lane % 16;
-  const uint32_t steps = i8_steps(p.H), blocks = (p.F + 15) / 16;
-  const uint32_t first = blockIdx.x / blocks, f0 = blockIdx.x % blocks * 16;
-  const uint32_t e = (uint32_t)ids[first];
-  if (e >= p.E) return;
-  const bool mine = threadIdx.x < A && (uint32_t)ids[threadIdx.x] == e;
-  const uint64_t row = (uint64_t)e * p.F + f0, rest = (uint64_t)p.E * p.F - row;
-  const __amdgpu_buffer_rsrc_t w = mx_buffer((const uint8_t *)(wave < 2 ? p.gc : p.uc) + row * steps * kI8Row, rest * steps * kI8Row);
-  // The members, in order; an earlier one: its work-group has this expert.
-  const uint64_t ballot = __ballot(mine);
-  if (lane == 0) counts[wave] = (uint32_t)__popcll(ballot);
-  if (__syncthreads_or(mine && threadIdx.x < first)) return;
-  uint32_t n = 0, at = lanes_below(ballot);
-  for (uint32_t v = 0; v < 4; v++) {
-    if (v < wave) at += counts[v];
-    n += counts[v];
-  }
-  if (mine) member[at] = (uint16_t)threadIdx.x;
-  for (uint32_t m0 = 0; m0 < n; m0 += kTok) {
-    const uint32_t nm = min(n - m0, kTok);
-    mx_i4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    for (uint32_t s0 = 0; s0 < steps; s0 += kSteps) {
-      const uint32_t ns = min(steps - s0, (uint32_t)kSteps);
-      __syncthreads();  // (member; the LDS of the pass before)
-      if (m0 == 0 || steps > kSteps) {
-        // 64 pieces of a row a load: wave w has eight rows, of gate or of up.
-#pragma unroll 4
-        for (uint32_t i = 0; i < 8; i++) {
-          const uint32_t lr = wave * 8 + i, from = (lr % 16 * steps + s0) * kI8Row;
-#pragma unroll
-          for (uint32_t j = 0; j < (kPitch + 1023) / 1024; j++) {
-            const uint32_t piece = j * 64 + lane;
-            if (piece < kPitch / 16 && piece < (ns + 1) / 2 * 16)
-              lds_dma16(w, from + min((piece ^ (lr % 16)) * 16, ns * kI8Row - 16), wc + lr * kPitch + j * 1024);
-          }
-        }
-      }
-      const auto row_of = [&](uint32_t i) { return x + member[m0 + i] / p.K * stride; };
-      if (s0 == 0) {  // the rows' largest
-        if (threadIdx.x < kTok) most[threadIdx.x] = 0;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < nm * steps * 16; i += 256) {
-          float v[8];
-          load8<kX>(row_of(i / (steps * 16)), i % (steps * 16) * 8, p.H, v);
-          uint32_t m = most_of8(v);
-          m = max(m, dpp_u32<kDppXor1>(m));
-          m = max(m, dpp_u32<kDppXor2>(m));
-          m = max(m, dpp_u32<kDppHalfMirror>(m));
-          m = max(m, dpp_u32<kDppMirror>(m));
-          if (lane % 16 == 0) atomicMax(most + i / (steps * 16), m);
-        }
-        __syncthreads();
-      }
-      for (uint32_t i = threadIdx.x; i < nm * ns * 16; i += 256) {
-        const uint32_t xr = i / (ns * 16), gr = i - xr * (ns * 16);
-        float v[8];
-        load8<kX>(row_of(xr), (s0 * 16 + gr) * 8, p.H, v);
-        *(uint2 *)(xc + xr * kXPitch + gr * 8) = i8_codes8(v, i8_scale_of(most[xr]));
-      }
-      dma_barrier();
-      const uint32_t xr = min(r, nm - 1);
-      for (uint32_t k = wave; k < 2 * ns; k += 4) {
-        const mx_i4 b = *(const mx_i4 *)(xc + xr * kXPitch + k * 64 + q * 16);
-#pragma unroll
-        for (uint32_t i = 0; i < 2; i++)
-          acc[i] = i8_mfma16(*(const mx_i4 *)(wc + (16 * i + r) * kPitch + ((4 * k + q) ^ r) * 16), b, acc[i]);
-      }
-    }
-    if (r < kTok)
-#pragma unroll
-      for (uint32_t i = 0; i < 2; i++)
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++) sums[wave][16 * i + 4 * q + j][r] = acc[i][j];
-    __syncthreads();
-    const uint32_t col = threadIdx.x % 16, t = threadIdx.x / 16;
-    if (t < nm && f0 + col < p.F) {
-      int gv = 0, uv = 0;
-#pragma unroll
-      for (uint32_t v = 0; v < 4; v++) gv += sums[v][col][t], uv += sums[v][16 + col][t];
-      const float s = i8_scale_of(most[t]);
-      h[(uint64_t)member[m0 + t] * pitch + f0 + col] =
-          expert_swiglu(i8_value(gv, s, p.gs[row + col]), i8_value(uv, s, p.us[row + col]), p.limit);
-    }
-    __syncthreads();  // (sums and most)
-  }
-}
-
-// A work-group: 16 rows of down for all assignments, and y's 16 columns. It quantises the assignments' rows of h; a wave takes
-// every eighth of the experts that are used (its assignments 16 at a time), 256 bytes of 16 rows a load, two loads of its own on
-// their way.
-constexpr uint32_t kFewHq = 56 * 1024;  // the assignments' rows of h in LDS
-
-template <uint32_t kType>
-__global__ void __launch_bounds__(512) i8_down_few(I8Experts p, const float *h, uint32_t hpitch, const int32_t *ids, const float *w,
-                                                   uint32_t ntok, typename Elem<kType>::T *y, uint64_t stride) {
-  struct Slot {
-    alignas(16) uint8_t c[16 * 256];  // 16 rows, their 16-byte pieces exchanged by the row
-  };
-  __shared__ Slot slot0[8];
-  __shared__ Slot slot1[8];
-  __shared__ __align__(16) uint8_t hq[kFewHq];
-  __shared__ __align__(16) int o[kFew * 16];
-  __shared__ uint32_t first[512], most[kFew];
-  __shared__ uint16_t id[kFew], used[kFew], member[8][kFew];
-  __shared__ uint32_t counts[8];
-  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 16, r = lane % 16, A = ntok * p.K;
-  const uint32_t pitch = i8_pitch(p.F), r0 = blockIdx.x * 16, lpitch = pitch + 16;
-  first[threadIdx.x] = ~0u;
-  uint32_t e = p.E;
+// The ids (at most kFew; past the experts: E) and the experts they name, each by its first assignment; all 512 threads. The number
+// of experts.
+struct Named {
+  uint32_t first[512];  // an expert's first assignment, then which of those in `used` it is
+  uint16_t id[kFew], used[kFew];
+  uint32_t counts[8];
+};
+__device__ __forceinline__ uint32_t name_experts(Named &s, const int32_t *ids, uint32_t A, uint32_t E) {
+  const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
+  s.first[threadIdx.x] = ~0u;
+  uint32_t e = E;
   if (threadIdx.x < A) {
-    e = min((uint32_t)ids[threadIdx.x], p.E);
-    id[threadIdx.x] = (uint16_t)e;
+    e = min((uint32_t)ids[threadIdx.x], E);
+    s.id[threadIdx.x] = (uint16_t)e;
   }
   __syncthreads();
-  if (e < p.E) atomicMin(first + e, threadIdx.x);
+  if (e < E) atomicMin(s.first + e, threadIdx.x);
   __syncthreads();
-  const bool owner = e < p.E && first[e] == threadIdx.x;
+  const bool owner = e < E && s.first[e] == threadIdx.x;
   const uint64_t ballot = __ballot(owner);
-  if (lane == 0) counts[wave] = (uint32_t)__popcll(ballot);
+  if (lane == 0) s.counts[wave] = (uint32_t)__popcll(ballot);
   __syncthreads();
   uint32_t n = 0, at = lanes_below(ballot);
   for (uint32_t v = 0; v < 8; v++) {
-    if (v < wave) at += counts[v];
-    n += counts[v];
+    if (v < wave) at += s.counts[v];
+    n += s.counts[v];
   }
-  if (owner) used[at] = (uint16_t)threadIdx.x;
+  if (owner) s.used[at] = (uint16_t)threadIdx.x, s.first[e] = at;
   __syncthreads();
-  const uint32_t chunks = (pitch + 255) / 256, units = wave < n ? ((n - 1 - wave) / 8 + 1) * chunks : 0;
-  const auto load = [&](Slot &s, uint32_t unit) {
-    const uint32_t ex = (uint32_t)__builtin_amdgcn_readfirstlane(id[used[wave + unit / chunks * 8]]), k = unit % chunks * 256;
-    const uint64_t row = (uint64_t)ex * p.H + r0, rest = (uint64_t)p.E * p.H - row;
-    const __amdgpu_buffer_rsrc_t c = mx_buffer((const uint8_t *)p.dc + row * pitch, rest * pitch);
+  return n;
+}
+
+// The first rank of assignment a's token that names a's expert: its row of h is a's too.
+__device__ __forceinline__ uint32_t row_of(const Named &s, uint32_t a, uint32_t K) {
+  uint32_t first = a / K * K;
+  while (s.id[first] != s.id[a]) first++;
+  return first;
+}
+
+// This wave's loads but the last kLeft have arrived. (No fence, which would wait for all of them.)
+template <int kLeft>
+__device__ __forceinline__ void unit_ready() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | kLeft);  // vmcnt(kLeft) lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+// All loads have arrived (LDS is another work-group's after the last wave).
+__device__ __forceinline__ void loads_done() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  asm volatile("" ::: "memory");
+}
+
+// A unit: 256 bytes of 16 rows, a row's 16-byte pieces exchanged by the row; the operand of four matrix instructions. Each wave has
+// three of its own in use or on their way, and needs no barrier for them. Loads past a wave's last unit read nowhere, so that the
+// waits count the same everywhere; up to two units that are not there follow the last (with a way out between them the compiler,
+// which then no longer tells the buffers' loads apart, waits for all).
+constexpr uint32_t kUnit = 256;
+constexpr int kUnitLoads = 4;
+struct Unit {
+  alignas(16) uint8_t c[16 * kUnit];
+  __device__ __forceinline__ void read(mx_i4 (&a)[4]) const {
+    const uint32_t lane = threadIdx.x & 63, q = lane / 16, r = lane % 16;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) a[j] = *(const mx_i4 *)(c + r * kUnit + ((4 * j + q) ^ r) * 16);
+  }
+  // Rows 8 which .. 8 which + 7: those of `from`, `pitch` apart, `bytes` (up to 256) from byte k on.
+  __device__ __forceinline__ void load(uint32_t which, __amdgpu_buffer_rsrc_t from, uint32_t pitch, uint32_t k, uint32_t bytes) {
+    const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+    for (uint32_t j = 0; j < 2; j++) {
+      const uint32_t row = which * 8 + 4 * j + lane / 16, at = ((lane % 16) ^ row) * 16;
+      lds_dma16(from, at < bytes ? row % 8 * pitch + k + at : kNowhere, c + which * 2048 + j * 1024);
+    }
+  }
+};
+
+// An item: an expert and eight columns of h (eight rows of gate and eight of up: the 16 rows of a matrix instruction, whose 16
+// columns are the tokens, whether they use the expert or not). A wave has every so manieth item, or 1 / kSplit of the k axis of one,
+// joined in LDS. Each work-group quantises all tokens' x. Writes the rows of h (`pitch` apart, a multiple of 4) of the assignments
+// that are their token's first with their expert.
+constexpr uint32_t kFewXq = 48 * 1024;  // the tokens' rows of x in LDS
+
+template <uint32_t kX, uint32_t kSplit>
+__global__ void __launch_bounds__(512) i8_gate_up_few(I8Experts p, const typename Elem<kX>::T *x, uint64_t stride, uint32_t ntok,
+                                                      const int32_t *ids, float *h, uint32_t pitch) {
+  __shared__ Unit unit0[8];
+  __shared__ Unit unit1[8];
+  __shared__ Unit unit2[8];
+  __shared__ __align__(16) uint8_t xq[kFewXq + kUnit];  // (a last row's last unit)
+  __shared__ int sums[kSplit > 1 ? 8 : 1][16][17];
+  __shared__ Named named;
+  __shared__ uint32_t most[16], ranks[kFew * 4];  // ranks: [expert][token], a byte: the token's first rank with the expert
+  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 16, r = lane % 16, A = ntok * p.K;
+  const uint32_t kpitch = i8_pitch(p.H), lpitch = kpitch + 16, blocks = (p.F + 7) / 8;
+  for (uint32_t i = threadIdx.x; i < kFew * 4; i += 512) ranks[i] = ~0u;
+  const uint32_t items = name_experts(named, ids, A, p.E) * blocks;
+  if (threadIdx.x < A && named.id[threadIdx.x] < p.E && row_of(named, threadIdx.x, p.K) == threadIdx.x)
+    ((uint8_t *)ranks)[named.first[named.id[threadIdx.x]] * 16 + threadIdx.x / p.K] = (uint8_t)(threadIdx.x % p.K);
+  const uint32_t per = (kpitch + kSplit * kUnit - 1) / (kSplit * kUnit) * kUnit;  // bytes of k a wave
+  const uint32_t kfirst = min(wave % kSplit * per, kpitch), kend = min(kfirst + per, kpitch), groups = gridDim.x * 8 / kSplit;
+  const auto expert_of = [&](uint32_t item) { return (uint32_t)__builtin_amdgcn_readfirstlane(named.id[named.used[item / blocks]]); };
+  uint32_t next = (blockIdx.x * 8 + wave) / kSplit, next_k = kfirst;
+  uint32_t item = next, k = kfirst;
+  const auto load = [&](Unit &s) {
+    const bool real = next < items;
+    const uint64_t row = real ? (uint64_t)expert_of(next) * p.F + next % blocks * 8 : 0, rest = ((uint64_t)p.E * p.F - row) * kpitch;
+    const uint32_t bytes = real ? min(kend - next_k, kUnit) : 0;
+    s.load(0, mx_buffer((const uint8_t *)p.gc + row * kpitch, rest), kpitch, next_k, bytes);
+    s.load(1, mx_buffer((const uint8_t *)p.uc + row * kpitch, rest), kpitch, next_k, bytes);
+    next_k += kUnit;
+    if (next_k >= kend) next_k = kfirst, next += groups;
+  };
+  float scales[4];  // of the item's four columns that the lane has: gate's in lanes 0 .. 31, up's in the others
+  const auto load_scales = [&] {
+    if (item >= items) return;
+    const float *const from = (q < 2 ? p.gs : p.us) + (uint64_t)expert_of(item) * p.F;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) scales[j] = from[min(item % blocks * 8 + q % 2 * 4 + j, p.F - 1)];
+  };
+  load_scales();
+  load(unit0[wave]);
+  load(unit1[wave]);
+  load(unit2[wave]);
+  quantize_rows<kX>(ntok, kpitch, p.H, [&](uint32_t i) { return x + i * stride; },
+                    [&](uint32_t i, uint32_t c) { return xq + i * lpitch + c; }, most);
+  const uint8_t *const xr = xq + min(r, ntok - 1) * lpitch + q * 16;
+  // An item's values: lanes 0 .. 31 have gate's sums, lanes 32 on up's, of token r.
+  const auto finish = [&](mx_i4 c) {
+    const uint32_t f0 = item % blocks * 8 + q % 2 * 4, rank = ((const uint8_t *)ranks)[item / blocks * 16 + r];
+    const float sx = i8_scale_of(most[min(r, ntok - 1)]);
+    float v[4];
 #pragma unroll
     for (uint32_t j = 0; j < 4; j++) {
-      const uint32_t lr = 4 * j + lane / 16;
-      lds_dma16(c, lr * pitch + k + min(((lane % 16) ^ lr) * 16, min(pitch - k, 256u) - 16), s.c + j * 1024);
+      const float own = i8_value(c[j], sx, scales[j]);
+      v[j] = expert_swiglu(own, __shfl_xor(own, 32, 64), p.limit);  // (of use in the lower half)
     }
+    if (q < 2 && r < ntok && rank != 255 && f0 < p.F)
+      *(float4 *)(h + (uint64_t)(r * p.K + rank) * pitch + f0) = make_float4(v[0], v[1], v[2], v[3]);
   };
-  if (units > 0) load(slot0[wave], 0);
-  if (units > 1) load(slot1[wave], 1);
-  // (Rows of assignments without an expert hold whatever the buffer held: codes that nobody reads.)
-  quantize_rows<QT_F32, kFewHq / 8 / 512>(A, pitch, p.F, [&](uint32_t i) { return h + (uint64_t)i * hpitch; }, hq, lpitch, most);
-  uint32_t nm = 0;
-  const auto use = [&](const Slot &s, uint32_t unit, bool more) {
-    // This unit's load has arrived; the next one's four may be outstanding.
-    asm volatile("" ::: "memory");
-    if (more)
-      __builtin_amdgcn_s_waitcnt(0x0f74);
-    else
-      __builtin_amdgcn_s_waitcnt(0x0f70);
-    asm volatile("" ::: "memory");
-    const uint32_t k = unit % chunks * 4, ns = min(pitch / 64 - k, 4u);
-    if (k == 0) {  // the expert's assignments
-      const uint32_t ex = id[used[wave + unit / chunks * 8]];
-      nm = 0;
-      for (uint32_t a0 = 0; a0 < A; a0 += 64) {
-        const bool is = a0 + lane < A && id[a0 + lane] == ex;
-        const uint64_t bal = __ballot(is);
-        if (is) member[wave][nm + lanes_below(bal)] = (uint16_t)(a0 + lane);
-        nm += (uint32_t)__popcll(bal);
+  mx_i4 acc = {0, 0, 0, 0};
+  const auto use = [&](Unit &s) {
+    unit_ready<2 * kUnitLoads>();
+    mx_i4 a[4], b[4];
+    s.read(a);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) b[j] = *(const mx_i4 *)(xr + k + j * 64);  // (past a row's end: times zeros)
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) acc = i8_mfma16(a[j], b[j], acc);
+    load(s);
+    k += kUnit;
+    if (k < kend) return;
+    if (kSplit == 1) {
+      if (item < items) finish(acc);
+      acc = mx_i4{0, 0, 0, 0};
+    }
+    k = kfirst, item += groups;
+    if (kSplit == 1) load_scales();
+  };
+  if (kSplit == 1) {
+#pragma unroll 1
+    while (item < items) {
+      use(unit0[wave]);
+      use(unit1[wave]);
+      use(unit2[wave]);
+    }
+    loads_done();
+  } else {  // (one item a wave at most)
+    const uint32_t mine = item;
+    if (kfirst < kend) {
+#pragma unroll 1
+      while (item == mine && item < items) {
+        use(unit0[wave]);
+        use(unit1[wave]);
+        use(unit2[wave]);
+      }
+    }
+    loads_done();
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) sums[wave][4 * q + j][r] = acc[j];
+    __syncthreads();
+    if (wave % kSplit != 0 || mine >= items) return;
+#pragma unroll
+    for (uint32_t s = 1; s < kSplit; s++)
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) acc[j] += sums[wave + s][4 * q + j][r];
+    item = mine;
+    finish(acc);
+  }
+}
+
+// A work-group takes every gridDim-th eight rows of down, y's eight columns, for all assignments. A wave has every eighth pair of the
+// experts that are named, whose eight rows each are the 16 rows of a matrix instruction; its columns are eight assignments of the
+// one and eight of the other, of which half of the products count. kOwn: it quantises the rows of h itself, at most kFewOwn values
+// (a launch for that is 3 us; more values take each work-group as long).
+constexpr uint32_t kFewHq = 48 * 1024;  // the assignments' rows of h in LDS
+constexpr uint32_t kFewOwn = 512 * kAtOnce;
+constexpr uint32_t kTerms = (kFew * 8 + 511) / 512;
+
+template <uint32_t kType, bool kOwn>
+__global__ void __launch_bounds__(512) i8_down_few(I8Experts p, const float *h, uint32_t hpitch, const int8_t *hc, const float *hs,
+                                                   const int32_t *ids, const float *w, uint32_t ntok, typename Elem<kType>::T *y,
+                                                   uint64_t stride) {
+  __shared__ Unit unit0[8];
+  __shared__ Unit unit1[8];
+  __shared__ Unit unit2[8];
+  __shared__ __align__(16) uint8_t hq[kFewHq + 1024];  // a row's 16-byte pieces exchanged by the row
+  __shared__ __align__(16) int o[kFew * 8];
+  __shared__ Named named;
+  __shared__ uint16_t member[8][2][kFew], row[kFew];
+  __shared__ float weight[kFew];
+  __shared__ uint32_t most[kFew];
+  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 16, r = lane % 16, A = ntok * p.K;
+  const uint32_t pitch = i8_pitch(p.F), blocks = (p.H + 7) / 8;
+  const uint32_t n = name_experts(named, ids, A, p.E), pairs = (n + 1) / 2;
+  // The two experts of a pair (the second one may be none: n is odd).
+  const auto expert_of = [&](uint32_t pair, uint32_t which) {
+    const uint32_t i = pair * 2 + which;
+    return i < n ? (uint32_t)__builtin_amdgcn_readfirstlane(named.id[named.used[i]]) : p.E;
+  };
+  uint32_t next_pair = 0, next_k = 0, r0 = 0;
+  const auto load = [&](Unit &s) {
+#pragma unroll
+    for (uint32_t which = 0; which < 2; which++) {
+      const uint32_t e = expert_of(next_pair, which);
+      const uint64_t first = (uint64_t)min(e, p.E - 1) * p.H + r0, rest = (uint64_t)p.E * p.H - first;
+      s.load(which, mx_buffer((const uint8_t *)p.dc + first * pitch, rest * pitch), pitch, next_k,
+             e < p.E ? min(pitch - next_k, kUnit) : 0);
+    }
+    next_k += kUnit;
+    if (next_k >= pitch) next_k = 0, next_pair += 8;
+  };
+  uint32_t pair = 0, k = 0, nm[2] = {0, 0};
+  const auto use = [&](Unit &s) {
+    unit_ready<2 * kUnitLoads>();
+    if (k == 0) {  // the experts' assignments
+#pragma unroll
+      for (uint32_t which = 0; which < 2; which++) {
+        const uint32_t ex = expert_of(pair, which);
+        nm[which] = 0;
+#pragma unroll 1
+        for (uint32_t a0 = 0; a0 < A; a0 += 64) {
+          const bool is = a0 + lane < A && named.id[min(a0 + lane, A - 1)] == ex && ex < p.E;
+          const uint64_t bal = __ballot(is);
+          if (is) member[wave][which][nm[which] + lanes_below(bal)] = (uint16_t)(a0 + lane);
+          nm[which] += (uint32_t)__popcll(bal);
+        }
       }
       __builtin_amdgcn_s_waitcnt(0xc07f);
       __builtin_amdgcn_wave_barrier();
     }
     mx_i4 a[4];
-#pragma unroll
-    for (uint32_t j = 0; j < 4; j++) a[j] = *(const mx_i4 *)(s.c + r * 256 + ((4 * j + q) ^ r) * 16);
-    for (uint32_t m0 = 0; m0 < nm; m0 += 16) {
-      const uint32_t as = member[wave][min(m0 + r, nm - 1)];
+    s.read(a);
+    const uint32_t mine = r / 8, many = mine ? nm[1] : nm[0];
+#pragma unroll 1
+    for (uint32_t m0 = 0; m0 < max(nm[0], nm[1]); m0 += 8) {
+      const bool there = m0 + r % 8 < many;
+      const uint32_t as = there ? member[wave][mine][m0 + r % 8] : 0;
+      const bool counts = there && q / 2 == mine;  // (the other rows are the other expert's)
+      const uint32_t hr = row[as];
+      const uint8_t *const from = hq + hr * pitch + k;
       mx_i4 c = {0, 0, 0, 0};
-      int4 *to = (int4 *)(o + as * 16 + 4 * q);
-      if (k != 0) {
+      int4 *to = (int4 *)(o + as * 8 + q % 2 * 4);
+      if (k != 0 && counts) {
         const int4 v = *to;
         c = mx_i4{v.x, v.y, v.z, v.w};
       }
 #pragma unroll
-      for (uint32_t j = 0; j < 4; j++) {
-        if (j >= ns) break;
-        c = i8_mfma16(a[j], *(const mx_i4 *)(hq + as * lpitch + (k + j) * 64 + q * 16), c);
-      }
-      if (m0 + r < nm) *to = make_int4(c[0], c[1], c[2], c[3]);
+      for (uint32_t j = 0; j < 4; j++) c = i8_mfma16(a[j], *(const mx_i4 *)(from + ((4 * j + q) ^ (hr % 8)) * 16), c);  // (past a row's end: times zeros)
+      if (counts) *to = make_int4(c[0], c[1], c[2], c[3]);
     }
+    load(s);
+    k += kUnit;
+    if (k >= pitch) k = 0, pair += 8;
   };
-  for (uint32_t i = 0; i < units; i += 2) {
-    use(slot0[wave], i, i + 1 < units);
-    if (i + 2 < units) load(slot0[wave], i + 2);
-    if (i + 1 >= units) break;
-    use(slot1[wave], i + 1, i + 2 < units);
-    if (i + 3 < units) load(slot1[wave], i + 3);
-  }
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < ntok * 16; i += 512) {
-    const uint32_t t = i / 16, c = i % 16;
-    if (r0 + c >= p.H) continue;
-    float s = 0.0f;
-    for (uint32_t k = 0; k < p.K; k++) {
-      const uint32_t a = t * p.K + k, ex = id[a];
-      if (ex < p.E)
-        s = __builtin_fmaf(w[a], i8_value(o[a * 16 + c], i8_scale_of(most[a]), p.ds[(uint64_t)ex * p.H + r0 + c]), s);
+  for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    r0 = b * 8, next_pair = pair = wave, next_k = k = 0;
+    // (Rows of assignments without an expert, or not their token's first with it, hold what nobody reads.)
+    if (!kOwn && b == blockIdx.x)
+      for (uint32_t i = wave * 1024; i < A * pitch; i += 8 * 1024) {
+        const uint32_t at = i + lane * 16, hr = at / pitch, piece = (at - hr * pitch) / 16;
+        lds_dma16(mx_buffer((const uint8_t *)hc, A * pitch), hr * pitch + (piece ^ (hr % 8)) * 16, hq + i);
+      }
+    load(unit0[wave]);
+    load(unit1[wave]);
+    load(unit2[wave]);
+    if (b == blockIdx.x) {
+      if (threadIdx.x < A) {
+        const bool on = named.id[threadIdx.x] < p.E;
+        row[threadIdx.x] = (uint16_t)row_of(named, threadIdx.x, p.K), weight[threadIdx.x] = on ? w[threadIdx.x] : 0.0f;
+      }
+      if (kOwn) {
+        quantize_rows<QT_F32>(A, pitch, p.F, [&](uint32_t i) { return h + (uint64_t)i * hpitch; },
+                              [&](uint32_t i, uint32_t c) { return hq + i * pitch + ((c / 16) ^ (i % 8)) * 16 + c % 16; }, most);
+      } else {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070 | 3 * kUnitLoads);  // (all but the units: the rows of h)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
     }
-    y[(uint64_t)t * stride + r0 + c] = (typename Elem<kType>::T)s;
+    // The scales of the sums that the thread turns into values.
+    float hscale[kTerms], dscale[kTerms];
+#pragma unroll
+    for (uint32_t j = 0; j < kTerms; j++) {
+      const uint32_t i = min(threadIdx.x + j * 512, A * 8 - 1), a = i / 8, ex = min((uint32_t)named.id[a], p.E - 1);
+      hscale[j] = kOwn ? i8_scale_of(most[row[a]]) : hs[row[a]];
+      dscale[j] = p.ds[min((uint64_t)ex * p.H + r0 + i % 8, (uint64_t)p.E * p.H - 1)];
+    }
+    asm volatile("" ::: "memory");
+#pragma unroll 1
+    while (pair < pairs) {
+      use(unit0[wave]);
+      use(unit1[wave]);
+      use(unit2[wave]);
+    }
+    loads_done();
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < kTerms; j++) {
+      const uint32_t i = threadIdx.x + j * 512;
+      if (i < A * 8) o[i] = named.id[i / 8] < p.E ? __float_as_int(i8_value(o[i], hscale[j], dscale[j])) : 0;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < ntok * 8; i += 512) {
+      const uint32_t t = i / 8, c = i % 8;
+      float s = 0.0f;
+#pragma unroll 8
+      for (uint32_t a = t * p.K; a < (t + 1) * p.K; a++) s = __builtin_fmaf(weight[a], __int_as_float(o[a * 8 + c]), s);
+      if (r0 + c < p.H) y[(uint64_t)t * stride + r0 + c] = (typename Elem<kType>::T)s;
+    }
+    __syncthreads();  // (o)
   }
 }
 
@@ -360,6 +476,7 @@ void check_experts(const moe_i8_experts *e, uint32_t ntok) {
 
 // How a call runs. Few assignments, whose rows of h fit LDS, without sorting them.
 constexpr uint64_t kChunkBytes = 256 << 20;
+constexpr uint32_t kCus = 256;  // work-groups that fill the device where LDS holds one a CU
 
 struct Plan {
   uint32_t A, rows, hpitch, pitch, chunk, max_tiles;
@@ -368,7 +485,7 @@ struct Plan {
 
   Plan(const moe_i8_experts &e, uint32_t T) {
     A = T * e.n_used;
-    few = A <= (e.n_expert <= 32 ? kFew : 96) && A * (i8_pitch(e.n_ff) + 16) <= kFewHq;
+    few = !A || (T <= 16 && A <= kFew && e.n_embd >= 8 && T * (i8_pitch(e.n_embd) + 16) <= kFewXq && A * i8_pitch(e.n_ff) <= kFewHq);
     // Tiles of 32, 64 or 128 positions: the more an expert has on average, the fewer times its weights are read.
     const uint32_t mean = A / e.n_expert;
     rows = mean < 24 ? 32 : mean < 96 ? 64 : 128;
@@ -383,10 +500,9 @@ struct Plan {
       at += (n + 255) / 256 * 256;
       return was;
     };
-    h = part((uint64_t)A * hpitch * 4);
+    h = part((uint64_t)A * hpitch * 4), hc = part(i8_bytes(A, e.n_ff)), hs = part((uint64_t)A * 4);
     if (!few) {
       xc = part(i8_bytes(T, e.n_embd)), xs = part((uint64_t)T * 4);
-      hc = part(i8_bytes(A, e.n_ff)), hs = part((uint64_t)A * 4);
       o = part((uint64_t)A * chunk * 4);
       sort = part(sort_bytes(A, e.n_expert)), order = part((uint64_t)A * 4), places = part((uint64_t)A * 4);
       offsets = part((e.n_expert + 1) * 4ull);
@@ -426,22 +542,35 @@ MOE_API moe_status moe_i8_experts_async(const moe_i8_experts *e, const void *x, 
     const I8Experts p{e->gate.codes, e->up.codes, e->down.codes, e->gate.scales, e->up.scales, e->down.scales, E, K, H, F,
                       e->swiglu_limit};
     float *h = (float *)(b + at.h);
+    const moe_i8_matrix hq{(int8_t *)(b + at.hc), (float *)(b + at.hs), A, F};
     if (at.few) {
+      // The k axis is split where the items leave half of the waves or more without one.
+      const uint32_t items = std::min(A, E) * ((F + 7) / 8), waves = kCus * 8;
       op_by_type(e->x_type, [&](auto t) {
         constexpr uint32_t kX = decltype(t)::value;
-        const auto run = [&](auto kernel) {
-          op_launch(kernel, (uint64_t)A * ((F + 15) / 16), 256, stream, p, (const typename Elem<kX>::T *)x, x_stride, ids, A, h,
-                    at.hpitch);
+        const auto run = [&](auto kernel, uint32_t split) {
+          op_launch(kernel, std::min((items * split + 7) / 8, kCus), 512, stream, p, (const typename Elem<kX>::T *)x, x_stride, ntok,
+                    ids, h, at.hpitch);
         };
-        if (i8_steps(H) <= 16)
-          run(i8_gate_up_few<kX, 16>);
+        if (items * 4 <= waves)
+          run(i8_gate_up_few<kX, 4>, 4);
+        else if (items * 2 <= waves)
+          run(i8_gate_up_few<kX, 2>, 2);
         else
-          run(i8_gate_up_few<kX, 20>);
+          run(i8_gate_up_few<kX, 1>, 1);
       });
+      const bool own = F >= 8 && A * i8_pitch(F) <= kFewOwn;
+      if (!own) i8_quantize_launch(QT_F32, h, at.hpitch, hq, nullptr, stream);
       op_by_type(e->y_type, [&](auto t) {
         constexpr uint32_t kY = decltype(t)::value;
-        op_launch(i8_down_few<kY>, (H + 15) / 16, 512, stream, p, (const float *)h, at.hpitch, ids, w, ntok, (typename Elem<kY>::T *)y,
-                  y_stride);
+        const auto run = [&](auto kernel) {
+          op_launch(kernel, std::min((H + 7) / 8, kCus), 512, stream, p, (const float *)h, at.hpitch, (const int8_t *)hq.codes,
+                    (const float *)hq.scales, ids, w, ntok, (typename Elem<kY>::T *)y, y_stride);
+        };
+        if (own)
+          run(i8_down_few<kY, true>);
+        else
+          run(i8_down_few<kY, false>);
       });
       return;
     }
@@ -449,7 +578,7 @@ MOE_API moe_status moe_i8_experts_async(const moe_i8_experts *e, const void *x, 
     uint32_t *offsets = (uint32_t *)(b + at.offsets), *nt = (uint32_t *)(b + at.n_tiles);
     MoeTile *tiles = (MoeTile *)(b + at.tiles);
     float *o = (float *)(b + at.o);
-    const moe_i8_matrix xq{(int8_t *)(b + at.xc), (float *)(b + at.xs), ntok, H}, hq{(int8_t *)(b + at.hc), (float *)(b + at.hs), A, F};
+    const moe_i8_matrix xq{(int8_t *)(b + at.xc), (float *)(b + at.xs), ntok, H};
     sort_launch(ids, A, E, SortOut{order, places, offsets, tiles, nt, at.rows}, b + at.sort, stream);
     i8_quantize_launch(e->x_type, x, x_stride, xq, nullptr, stream);
     const auto run = [&](auto gate_up, auto down, uint32_t bn) {

@@ -5,43 +5,60 @@
 
 namespace c0ven {
 
-// Rows 0 .. n - 1 (row_of(i): a pointer to i's values; at most kGroups groups of eight of them a thread) to codes at lc, `lpitch`
-// bytes apart, and the bits of their largest |x| at most_of: all threads, each group loaded once. A barrier before it if LDS was
-// in use; it ends with one.
-template <uint32_t kX, int kGroups, typename F>
-__device__ __forceinline__ void quantize_rows(uint32_t n, uint32_t pitch, uint32_t cols, F row_of, uint8_t *lc, uint32_t lpitch,
-                                              uint32_t *most_of) {
-  const uint32_t per = pitch / 8, all = n * per;  // (16 neighbouring groups are of one row)
-  float v[kGroups][8];
-#pragma unroll
-  for (int j = 0; j < kGroups; j++) {
-    const uint32_t i = threadIdx.x + j * blockDim.x;
-    if (j * blockDim.x >= all) break;
-    if (i < all) load8<kX>(row_of(i / per), i % per * 8, cols, v[j]);
-  }
+// Every wave is here, and what they wrote to and read from LDS is done; loads into LDS may be on their way (a fence would wait).
+__device__ __forceinline__ void all_waves() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Rows 0 .. n - 1 of at least eight values (row_of(i): a pointer to i's) to codes, eight at a time to to(i, column), and the bits of
+// their largest |x| to most_of; all threads. Four groups of eight values a thread at a time; more than that are read twice, the second
+// time from the cache. It ends with a barrier. Little code: a work-group that comes this way once waits for its code as long as for
+// its data (unrolled over twelve groups, 35 KB in all, one token's experts took 26 us).
+constexpr uint32_t kAtOnce = 4 * 8;  // values a thread that are read once
+template <uint32_t kX, typename Row, typename To>
+__device__ __forceinline__ void quantize_rows(uint32_t n, uint32_t pitch, uint32_t cols, Row row_of, To to, uint32_t *most_of) {
+  constexpr int kAhead = kAtOnce / 8;
+  const uint32_t per = pitch / 8, all = n * per, round = kAhead * blockDim.x;  // (16 neighbouring groups are of one row)
+  float v[kAhead][8];
   if (threadIdx.x < n) most_of[threadIdx.x] = 0;
-  __syncthreads();
+  all_waves();
+#pragma unroll 1
+  for (uint32_t pass = 0; pass < 2; pass++) {
+#pragma unroll 1
+    for (uint32_t i0 = threadIdx.x; i0 < all; i0 += round) {
+      uint32_t r[kAhead], c[kAhead];
 #pragma unroll
-  for (int j = 0; j < kGroups; j++) {
-    const uint32_t i = threadIdx.x + j * blockDim.x;
-    if (j * blockDim.x >= all) break;
-    if (i < all) {
-      uint32_t m = most_of8(v[j]);
-      m = max(m, dpp_u32<kDppXor1>(m));
-      m = max(m, dpp_u32<kDppXor2>(m));
-      m = max(m, dpp_u32<kDppHalfMirror>(m));
-      m = max(m, dpp_u32<kDppMirror>(m));
-      if (threadIdx.x % 16 == 0) atomicMax(most_of + i / per, m);
+      for (int j = 0; j < kAhead; j++) {
+        const uint32_t i = min(i0 + j * blockDim.x, all - 1);
+        r[j] = i / per, c[j] = (i - r[j] * per) * 8;
+      }
+      if (pass == 0 || all > round) {
+        Eight<kX> e[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) e[j].load(row_of(r[j]), c[j], cols);
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) e[j].values(c[j], cols, v[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) {
+        if (i0 + j * blockDim.x >= all) break;
+        if (pass == 0) {
+          uint32_t m = most_of8(v[j]);
+          m = max(m, dpp_u32<kDppXor1>(m));
+          m = max(m, dpp_u32<kDppXor2>(m));
+          m = max(m, dpp_u32<kDppHalfMirror>(m));
+          m = max(m, dpp_u32<kDppMirror>(m));
+          if (threadIdx.x % 16 == 0) atomicMax(most_of + r[j], m);
+        } else {
+          *(uint2 *)to(r[j], c[j]) = i8_codes8(v[j], i8_scale_of(most_of[r[j]]));
+        }
+      }
     }
+    all_waves();
   }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kGroups; j++) {
-    const uint32_t i = threadIdx.x + j * blockDim.x;
-    if (j * blockDim.x >= all) break;
-    if (i < all) *(uint2 *)(lc + i / per * lpitch + i % per * 8) = i8_codes8(v[j], i8_scale_of(most_of[i / per]));
-  }
-  __syncthreads();
 }
 
 }  // namespace c0ven

@@ -44,8 +44,8 @@ __global__ void __launch_bounds__(64 * kWaves)
   load(one, k0);
   if constexpr (kFloats) {
     typedef typename Elem<kX>::T X;
-    quantize_rows<kX, kFewLds / 8 / (64 * kWaves)>(M, pitch, cols, [&](uint32_t i) { return (const X *)x + i * x_stride; }, lc,
-                                                   pitch + 16, ls);
+    quantize_rows<kX>(M, pitch, cols, [&](uint32_t i) { return (const X *)x + i * x_stride; },
+                      [&](uint32_t i, uint32_t c) { return lc + i * (pitch + 16) + c; }, ls);
   }
   mx_i4 c = {0, 0, 0, 0};
   const auto use = [&](Ahead &v, uint32_t k) {
@@ -259,8 +259,8 @@ void op_results(uint64_t M, uint64_t N) { op_require(M * N <= 1ull << 38, "y of 
 
 // x's rows quantised, in a work buffer.
 uint64_t quantised_bytes(uint32_t rows, uint32_t cols) { return i8_bytes(rows, cols) + ((uint64_t)rows * 4 + 15) / 16 * 16; }
-// The rows that the few-rows kernel quantises for itself.
-bool quantises_itself(uint32_t M, uint32_t cols) { return M <= kFewRows && M * i8_pitch(cols) <= kFewLds; }
+// The rows that the few-rows kernel quantises for itself (it takes eight values at a time).
+bool quantises_itself(uint32_t M, uint32_t cols) { return !M || (M <= kFewRows && cols >= 8 && M * i8_pitch(cols) <= kFewLds); }
 
 }  // namespace
 

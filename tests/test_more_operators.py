@@ -183,8 +183,8 @@ def test_empty_batches():
     moe.i8_matmul_async(none, w, moe.QT_F32, None)
     moe.i8_linear_async(moe.QT_F32, None, 0, w, moe.QT_F32, None, None, 0)
     moe.i8_linear_async(moe.QT_F32, P, 4, none, moe.QT_F32, None, P, moe.i8_linear_work_bytes(none, 4))
-    for E in (8, 512):
-        assert experts(E=E).work_bytes(0) == 0
+    for E, H in ((8, 256), (512, 256), (8, 5)):
+        assert experts(E=E, H=H).work_bytes(0) == 0
         experts(E=E).forward_async(None, 0, None, None, None, None, 0)
     refused(lambda: moe.i8_matmul_async(none, mat(codes=None), moe.QT_F32, None))
     refused(lambda: moe.i8_linear_async(moe.QT_F32, None, 4, none, moe.QT_F32, None, None, 0))
