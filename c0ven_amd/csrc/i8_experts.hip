@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(512) i8_gate_up_few(I8Experts p, const typenam
   load(unit0[wave]);
   load(unit1[wave]);
   load(unit2[wave]);
-  quantize_rows<kX>(ntok, kpitch, p.H, [&](uint32_t i) { return x + i * stride; },
+  quantize_rows<kX, 4>(ntok, kpitch, p.H, [&](uint32_t i) { return x + i * stride; },
                     [&](uint32_t i, uint32_t c) { return xq + i * lpitch + c; }, most);
   const uint8_t *const xr = xq + min(r, ntok - 1) * lpitch + q * 16;
   // An item's values: lanes 0 .. 31 have gate's sums, lanes 32 on up's, of token r.
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(512) i8_gate_up_few(I8Experts p, const typenam
 // one and eight of the other, of which half of the products count. kOwn: it quantises the rows of h itself, at most kFewOwn values
 // (a launch for that is 3 us; more values take each work-group as long).
 constexpr uint32_t kFewHq = 48 * 1024;  // the assignments' rows of h in LDS
-constexpr uint32_t kFewOwn = 512 * kAtOnce;
+constexpr uint32_t kFewOwn = 512 * 4 * 8;
 constexpr uint32_t kTerms = (kFew * 8 + 511) / 512;
 
 template <uint32_t kType, bool kOwn>
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(512) i8_down_few(I8Experts p, const float *h, 
         row[threadIdx.x] = (uint16_t)row_of(named, threadIdx.x, p.K), weight[threadIdx.x] = on ? w[threadIdx.x] : 0.0f;
       }
       if (kOwn) {
-        quantize_rows<QT_F32>(A, pitch, p.F, [&](uint32_t i) { return h + (uint64_t)i * hpitch; },
+        quantize_rows<QT_F32, 4>(A, pitch, p.F, [&](uint32_t i) { return h + (uint64_t)i * hpitch; },
                               [&](uint32_t i, uint32_t c) { return hq + i * pitch + ((c / 16) ^ (i % 8)) * 16 + c % 16; }, most);
       } else {
         asm volatile("" ::: "memory");

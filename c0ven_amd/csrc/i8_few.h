@@ -14,13 +14,11 @@ __device__ __forceinline__ void all_waves() {
 }
 
 // Rows 0 .. n - 1 of at least eight values (row_of(i): a pointer to i's) to codes, eight at a time to to(i, column), and the bits of
-// their largest |x| to most_of; all threads. Four groups of eight values a thread at a time; more than that are read twice, the second
+// their largest |x| to most_of; all threads. kAhead groups of eight values a thread at a time; more than that are read twice, the second
 // time from the cache. It ends with a barrier. Little code: a work-group that comes this way once waits for its code as long as for
 // its data (unrolled over twelve groups, 35 KB in all, one token's experts took 26 us).
-constexpr uint32_t kAtOnce = 4 * 8;  // values a thread that are read once
-template <uint32_t kX, typename Row, typename To>
+template <uint32_t kX, int kAhead, typename Row, typename To>
 __device__ __forceinline__ void quantize_rows(uint32_t n, uint32_t pitch, uint32_t cols, Row row_of, To to, uint32_t *most_of) {
-  constexpr int kAhead = kAtOnce / 8;
   const uint32_t per = pitch / 8, all = n * per, round = kAhead * blockDim.x;  // (16 neighbouring groups are of one row)
   float v[kAhead][8];
   if (threadIdx.x < n) most_of[threadIdx.x] = 0;

@@ -26,54 +26,57 @@ __global__ void __launch_bounds__(64 * kWaves)
   __shared__ int sums[kWaves][16][17];
   const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 16, r = lane % 16, pitch = i8_pitch(cols);
   const uint32_t steps = pitch / 64, n0 = blockIdx.x * 16, per = (steps / 2 + kWaves - 1) / kWaves * 2;  // (whole lines)
-  const uint32_t k0 = min(wave * per, steps), k1 = min(k0 + per, steps);
-  const int8_t *row = wc + (uint64_t)min(n0 + r, N - 1) * pitch + q * 16;
-  const uint32_t m = min(r, M - 1);
-  constexpr int kAhead = 4;
+  const uint32_t k0 = min(wave * per, steps), k1 = min(k0 + per, steps), m = min(r, M - 1);
+  // Rows of w past the last and steps past the wave's are zeros, so that every load is there and none waits for a branch's.
+  const __amdgpu_buffer_rsrc_t w = mx_buffer((const uint8_t *)wc + (uint64_t)n0 * pitch, (uint64_t)(N - n0) * pitch);
+  constexpr int kAhead = kWaves == 16 ? 2 : 4;
   struct Ahead {
     mx_i4 a[kAhead], b[kAhead];
   } one, two;
   const auto load = [&](Ahead &to, uint32_t k) {
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
-      if (k + j >= k1) break;
-      to.a[j] = *(const mx_i4 *)(row + (k + j) * 64);
-      if constexpr (!kFloats) to.b[j] = *(const mx_i4 *)(xc + (uint64_t)m * pitch + (k + j) * 64 + q * 16);
+      to.a[j] = __builtin_bit_cast(mx_i4, __builtin_amdgcn_raw_buffer_load_b128(w, k + j < k1 ? r * pitch + q * 16 + (k + j) * 64 : kNowhere, 0, 0));
+      if constexpr (!kFloats) to.b[j] = *(const mx_i4 *)(xc + (uint64_t)m * pitch + min(k + j, steps - 1) * 64 + q * 16);
     }
   };
   load(one, k0);
+  load(two, k0 + kAhead);
+  static_assert(kFewRows * 16 <= 64 * kWaves, "a value of y a thread");
+  const uint32_t col = threadIdx.x % 16, row = threadIdx.x / 16;
+  const float sw = ws[min(n0 + col, N - 1)];
+  float sx = 0.0f;
   if constexpr (kFloats) {
     typedef typename Elem<kX>::T X;
-    quantize_rows<kX>(M, pitch, cols, [&](uint32_t i) { return (const X *)x + i * x_stride; },
+    quantize_rows<kX, kWaves == 16 ? 2 : 4>(M, pitch, cols, [&](uint32_t i) { return (const X *)x + i * x_stride; },
                       [&](uint32_t i, uint32_t c) { return lc + i * (pitch + 16) + c; }, ls);
+  } else {
+    sx = xs[min(row, M - 1)];
   }
   mx_i4 c = {0, 0, 0, 0};
   const auto use = [&](Ahead &v, uint32_t k) {
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
-      if (k + j >= k1) break;
-      if constexpr (kFloats) v.b[j] = *(const mx_i4 *)(lc + m * (pitch + 16) + (k + j) * 64 + q * 16);
+      if constexpr (kFloats) v.b[j] = *(const mx_i4 *)(lc + m * (pitch + 16) + min(k + j, steps - 1) * 64 + q * 16);
       c = i8_mfma16(v.a[j], v.b[j], c);
     }
   };
+#pragma unroll 1
   for (uint32_t k = k0; k < k1; k += 2 * kAhead) {
-    if (k + kAhead < k1) load(two, k + kAhead);
     use(one, k);
-    if (k + 2 * kAhead < k1) load(one, k + 2 * kAhead);
+    load(one, k + 2 * kAhead);
     use(two, k + kAhead);
+    load(two, k + 3 * kAhead);
   }
 #pragma unroll
   for (int i = 0; i < 4; i++) sums[wave][r][4 * q + i] = c[i];
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < M * 16; i += 64 * kWaves) {
+  if (row < M && n0 + col < N) {
     int s = 0;
 #pragma unroll
-    for (int v = 0; v < kWaves; v++) s += sums[v][i / 16][i % 16];
-    const uint32_t n = n0 + i % 16;
-    if (n < N) {
-      const float sx = kFloats ? i8_scale_of(ls[i / 16]) : xs[i / 16];
-      y[(uint64_t)(i / 16) * stride + n] = (typename Elem<kType>::T)i8_value(s, sx, ws[n]);
-    }
+    for (int v = 0; v < kWaves; v++) s += sums[v][row][col];
+    if (kFloats) sx = i8_scale_of(ls[row]);
+    y[(uint64_t)row * stride + n0 + col] = (typename Elem<kType>::T)i8_value(s, sx, sw);
   }
 }
 
@@ -220,7 +223,11 @@ void launch_few(const void *x, uint64_t x_stride, const int8_t *xc, const float 
       op_launch(kernel, blocks, 64 * waves, stream, x, x_stride, xc, xs, (const int8_t *)w->codes, (const float *)w->scales, M, N,
                 w->cols, (typename Elem<kType>::T *)y, stride);
     };
-    const bool many = kX == kQuantised ? i8_steps(w->cols) >= 64 : M * i8_pitch(w->cols) >= 4096;
+    // Sixteen waves a work-group where there are few of them, for a long k (1 x 512 x 16384 quantised 11.7 us, with four 13.8; x
+    // 8192 with 2048 rows 7.9 and 8.1; 16 x 4096 x 4096 7.4 and 6.6) and for many values to quantise (8 x 2048 x 2048 5.5, with
+    // four 8.0; 4 x 2048 x 2048 5.0 and 5.3; 1 x 2048 x 2048 4.4 and 4.2). With more work-groups four hide each other's latency
+    // (1 x 16384 x 8192 25.6, with sixteen 27.5).
+    const bool many = kX == kQuantised ? i8_steps(w->cols) >= 64 : M * i8_pitch(w->cols) >= 8192;
     if (blocks <= 512 && many)
       run(i8_few<kX, kType, 16>, 16);
     else
