@@ -37,48 +37,77 @@ __global__ void __launch_bounds__(1024) sort_count(const int32_t *ids, uint32_t 
 
 // The places of a slice's assignments: an expert's start, its assignments in the slices before, those of the waves before (each
 // has a sixteenth of the slice) and, 64 ids at a time, those of the lanes before. Equal ids keep their order, so equal calls
-// give equal places.
-__global__ void __launch_bounds__(64 * kSortWaves) sort_place(const int32_t *ids, uint32_t A, uint32_t E, uint32_t slice,
-                                                              const uint32_t *counts, SortOut out) {
-  __shared__ uint32_t at[kSortWaves][kMostExperts];
+// give equal places. kOnce: a slice of kSlice ids, which stay in registers with their ranks within the wave (3996 ids 6.5 us with
+// a pass of atomics for the counts and the ids loaded again one step at a time).
+template <bool kOnce>
+__device__ __forceinline__ void place_slice(const int32_t *ids, uint32_t A, uint32_t E, uint32_t slice, uint32_t slices,
+                                            const uint32_t *counts, const SortOut &out) {
+  __shared__ __align__(16) uint32_t at[kSortWaves][kMostExperts];
   __shared__ uint32_t half[2][kMostExperts];
   __shared__ uint32_t sums[2][8];
   __shared__ uint32_t total;
+  constexpr uint32_t kSteps = kSlice / kSortWaves / 64;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64, bits = 32 - (uint32_t)__clz((int)((E - 1) | 1));
   const uint32_t first = blockIdx.x * slice, end = min(A, first + slice);
   const uint32_t run = slice / kSortWaves, from = min(first + wave * run, end), to = min(from + run, end);
-  for (uint32_t i = tid; i < kSortWaves * kMostExperts; i += 64 * kSortWaves) at[0][i] = 0;
-  __syncthreads();
-  for (uint32_t i0 = from + lane; i0 < to; i0 += 4 * 64) {
-    uint32_t id[4];
+  uint32_t id[kSteps], rank[kSteps];
+  if (kOnce)
 #pragma unroll
-    for (uint32_t j = 0; j < 4; j++) id[j] = i0 + j * 64 < to ? (uint32_t)ids[i0 + j * 64] : ~0u;
-#pragma unroll
-    for (uint32_t j = 0; j < 4; j++)
-      if (id[j] < E) atomicAdd(&at[wave][id[j]], 1u);
-  }
+    for (uint32_t j = 0; j < kSteps; j++) id[j] = from + j * 64 + lane < to ? (uint32_t)ids[from + j * 64 + lane] : ~0u;
+  for (uint32_t i = tid; i < kSortWaves * kMostExperts / 4; i += 64 * kSortWaves) ((uint4 *)at)[i] = make_uint4(0, 0, 0, 0);
   // An expert's assignments in all slices and in those before: two threads an expert, every second slice each.
   const uint32_t e = tid % kMostExperts, h = tid / kMostExperts;
   uint32_t all = 0, before = 0;
-  if (gridDim.x > 1 && e < E)
-    for (uint32_t s0 = h; s0 < gridDim.x; s0 += 16) {
+  if (slices > 1 && e < E)
+    for (uint32_t s0 = h; s0 < slices; s0 += 16) {
       uint32_t c[8];
 #pragma unroll
-      for (uint32_t j = 0; j < 8; j++) c[j] = s0 + 2 * j < gridDim.x ? counts[(s0 + 2 * j) * E + e] : 0;
+      for (uint32_t j = 0; j < 8; j++) c[j] = counts[min(s0 + 2 * j, slices - 1) * E + e];
 #pragma unroll
-      for (uint32_t j = 0; j < 8; j++) all += c[j], before += s0 + 2 * j < blockIdx.x ? c[j] : 0;
+      for (uint32_t j = 0; j < 8; j++) {
+        const uint32_t n = s0 + 2 * j < slices ? c[j] : 0;
+        all += n, before += s0 + 2 * j < blockIdx.x ? n : 0;
+      }
     }
   if (h == 1) half[0][e] = all, half[1][e] = before;
   __syncthreads();
-  uint32_t own = 0, tiles = 0;
+  // 64 ids: what was counted of each one's expert before it; the counts go on.
+  const auto count = [&](uint32_t x) {
+    const bool in = x < E;
+    uint64_t same = __ballot(in);
+    for (uint32_t b = 0; b < bits; b++) {
+      const uint64_t set = __ballot(x >> b & 1);
+      same &= x >> b & 1 ? set : ~set;
+    }
+    uint32_t p = 0;
+    if (in) {
+      const uint32_t under = lanes_below(same);
+      p = at[wave][x] + under;
+      if (under == 0) at[wave][x] = p + (uint32_t)__popcll(same);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (the counts before the next ids')
+    __builtin_amdgcn_wave_barrier();
+    return p;
+  };
+  if (kOnce) {
+#pragma unroll
+    for (uint32_t j = 0; j < kSteps; j++) rank[j] = count(id[j]);
+  } else {
+    for (uint32_t i0 = from; i0 < to; i0 += 64) (void)count(i0 + lane < to ? (uint32_t)ids[i0 + lane] : ~0u);
+  }
+  __syncthreads();
+  uint32_t own = 0, tiles = 0, n[kSortWaves];
   if (h == 0) {
     all += half[0][e], before += half[1][e];
+#pragma unroll
+    for (uint32_t v = 0; v < kSortWaves; v++) n[v] = at[v][e];
+#pragma unroll
     for (uint32_t v = 0; v < kSortWaves; v++) {
-      const uint32_t n = at[v][e];
-      at[v][e] = own;
-      own += n;
+      const uint32_t m = n[v];
+      n[v] = own;
+      own += m;
     }
-    if (gridDim.x == 1) all = own;
+    if (slices == 1) all = own;
     if (out.tiles) tiles = (all + out.rows - 1) / out.rows;
   }
   uint32_t place = all, tile = tiles;  // their sums up to this expert
@@ -90,39 +119,43 @@ __global__ void __launch_bounds__(64 * kSortWaves) sort_place(const int32_t *ids
   __syncthreads();
   if (h == 0) {
     for (uint32_t v = 0; v < wave; v++) place += sums[0][v], tile += sums[1][v];
-    for (uint32_t v = 0; v < kSortWaves; v++) at[v][e] += place - all + before;
+#pragma unroll
+    for (uint32_t v = 0; v < kSortWaves; v++) at[v][e] = n[v] + place - all + before;
     if (e == kMostExperts - 1) total = place;
-    if (blockIdx.x == 0) {
-      if (e < E) out.offsets[e] = place - all;
-      if (e == E - 1) out.offsets[E] = place;
-      if (out.tiles) {
-        for (uint32_t j = 0; j < tiles; j++)
-          out.tiles[tile - tiles + j] = MoeTile{e, e, place - all + j * out.rows, min(out.rows, all - j * out.rows)};
-        if (e == kMostExperts - 1) *out.n_tiles = tile;
-      }
-    }
   }
   __syncthreads();
-  for (uint32_t i0 = from; i0 < to; i0 += 64) {
-    const uint32_t i = i0 + lane, id = i < to ? (uint32_t)ids[i] : ~0u;
-    const bool in = id < E;
-    uint64_t same = __ballot(in);
-    for (uint32_t b = 0; b < bits; b++) {
-      const uint64_t set = __ballot(id >> b & 1);
-      same &= id >> b & 1 ? set : ~set;
-    }
-    if (in) {
-      const uint32_t under = lanes_below(same), p = at[wave][id] + under;
-      if (under == 0) at[wave][id] = p + (uint32_t)__popcll(same);
+  const auto put = [&](uint32_t i, uint32_t x, uint32_t p) {
+    if (x < E) {
       out.order[p] = (int32_t)i;
       out.places[i] = (int32_t)p;
     } else if (i < to) {
       out.places[i] = -1;
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (the counts before the next ids')
-    __builtin_amdgcn_wave_barrier();
+  };
+  if (kOnce) {
+#pragma unroll
+    for (uint32_t j = 0; j < kSteps; j++) put(from + j * 64 + lane, id[j], rank[j] + (id[j] < E ? at[wave][id[j]] : 0));
+  } else {
+    for (uint32_t i0 = from; i0 < to; i0 += 64) {
+      const uint32_t x = i0 + lane < to ? (uint32_t)ids[i0 + lane] : ~0u;
+      put(i0 + lane, x, count(x));
+    }
   }
   for (uint32_t i = max(first, total) + tid; i < end; i += 64 * kSortWaves) out.order[i] = -1;
+  if (blockIdx.x == 0 && h == 0) {
+    if (e < E) out.offsets[e] = place - all;
+    if (e == E - 1) out.offsets[E] = place;
+    if (out.tiles) {
+      for (uint32_t j = 0; j < tiles; j++)
+        out.tiles[tile - tiles + j] = MoeTile{e, e, place - all + j * out.rows, min(out.rows, all - j * out.rows)};
+      if (e == kMostExperts - 1) *out.n_tiles = tile;
+    }
+  }
+}
+template <bool kOnce>
+__global__ void __launch_bounds__(64 * kSortWaves) sort_place(const int32_t *ids, uint32_t A, uint32_t E, uint32_t slice,
+                                                              const uint32_t *counts, SortOut out) {
+  place_slice<kOnce>(ids, A, E, slice, gridDim.x, counts, out);
 }
 
 // ---- rows
@@ -220,11 +253,11 @@ __global__ void __launch_bounds__(256) dispatch_rows(const typename Elem<kType>:
   });
 }
 
-// At most kFewIds ids: the sort and the rows in one launch, each wave counting its token's places itself (those of lower ids and
-// of equal ones before), the last work-group the offsets. cols 0: no rows.
+// At most kFewIds ids: the sort and the rows in one launch, a work-group 256 pieces of a token, whose places its waves count
+// themselves (lower ids, and equal ones before), and the last work-group the offsets. cols 0: no rows.
 constexpr uint32_t kFewIds = 1024;
 template <uint32_t kType, uint32_t kN>
-__global__ void __launch_bounds__(256) dispatch_few(const int32_t *ids, uint32_t ntok, uint32_t K, uint32_t E,
+__global__ void __launch_bounds__(256) dispatch_few(const int32_t *__restrict__ ids, uint32_t ntok, uint32_t K, uint32_t E,
                                                     const typename Elem<kType>::T *x, uint64_t x_stride, uint32_t cols,
                                                     typename Elem<kType>::T *xs, uint64_t xs_stride, SortOut out) {
   const uint32_t A = ntok * K, lane = threadIdx.x & 63;
@@ -255,31 +288,50 @@ __global__ void __launch_bounds__(256) dispatch_few(const int32_t *ids, uint32_t
     for (uint32_t i = total + threadIdx.x; i < A; i += 256) out.order[i] = -1;
     return;
   }
-  uint32_t id[kFewIds / 64];
-#pragma unroll
-  for (uint32_t j = 0; j < kFewIds / 64; j++) id[j] = j * 64 + lane < A ? min((uint32_t)ids[j * 64 + lane], E) : E;
-  const uint32_t pieces = (cols + kN - 1) / kN, runs = max((pieces + 63) / 64, 1u);
-  const uint32_t wave = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint32_t t = wave / runs, run = wave - t * runs, piece = run * 64 + lane;
-  if (t >= ntok) return;
+  __shared__ uint32_t places[16];
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64), pieces = (cols + kN - 1) / kN;
+  const uint32_t parts = max((pieces + 255) / 256, 1u), t = blockIdx.x / parts, piece = (blockIdx.x - t * parts) * 256 + threadIdx.x;
   const bool there = piece < pieces;
   const uint32_t c = there ? min(piece * kN, cols - kN) : 0;
+  uint32_t id[kFewIds / 64], of[4];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; j++) of[j] = (uint32_t)ids[t * K + min(wave + 4 * j, K - 1)];
+#pragma unroll
+  for (uint32_t j = 0; j < kFewIds / 64; j++) {
+    if (j * 64 >= A) break;
+    id[j] = (uint32_t)ids[min(j * 64 + lane, A - 1)];
+  }
   Few<kType, kN> v;
   if (there) v.load(x + t * x_stride + c);
-  for (uint32_t k = 0; k < K; k++) {
-    const uint32_t a = t * K + k, e = min((uint32_t)ids[a], E);
+#pragma unroll
+  for (uint32_t j = 0; j < 4; j++) loaded<true>(of[j]);
+#pragma unroll
+  for (uint32_t i = 0; i < 4; i++) {
+    const uint32_t k = wave + 4 * i, a = t * K + k, e = min(of[i], E);
+    if (k >= K) break;
     uint32_t place = 0;
 #pragma unroll
     for (uint32_t j = 0; j < kFewIds / 64; j++) {
       if (j * 64 >= A) break;
-      place += (uint32_t)__popcll(__ballot(id[j] < e || (id[j] == e && j * 64 + lane < a)));
+      const uint32_t b = j * 64 + lane;  // (past the last id: not before any)
+      place += (uint32_t)__popcll(__ballot(b < A && (id[j] < e || (id[j] == e && b < a))));
     }
-    if (run == 0 && lane == 0) {
-      out.places[a] = e < E ? (int32_t)place : -1;
-      if (e < E) out.order[place] = (int32_t)a;
+    if (lane == 0) {
+      places[k] = e < E ? place : ~0u;
+      if (blockIdx.x - t * parts == 0) {
+        out.places[a] = e < E ? (int32_t)place : -1;
+        if (e < E) out.order[place] = (int32_t)a;
+      }
     }
-    if (e < E && there) v.store(xs + (uint64_t)place * xs_stride + c);
   }
+  __syncthreads();
+  uint32_t to[16];
+#pragma unroll
+  for (uint32_t k = 0; k < 16; k++) to[k] = (uint32_t)__builtin_amdgcn_readfirstlane((int)places[k]);
+  if (there)
+#pragma unroll
+    for (uint32_t k = 0; k < 16; k++)
+      if (k < K && to[k] != ~0u) v.store(xs + (uint64_t)to[k] * xs_stride + c);
 }
 
 // A token's rows, eight ranks' loads on their way at a time; each rank's product is fused into the sum, in rank order. A: rows of o.
@@ -422,7 +474,10 @@ void sort_launch(const int32_t *ids, uint32_t A, uint32_t E, const SortOut &out,
   const uint32_t slice = slice_of(A), slices = slices_of(A);
   uint32_t *counts = (uint32_t *)work;
   if (slices > 1) op_launch(sort_count, slices, 1024, stream, ids, A, E, slice, counts);
-  op_launch(sort_place, slices, 64 * kSortWaves, stream, ids, A, E, slice, (const uint32_t *)counts, out);
+  if (slice == kSlice)
+    op_launch(sort_place<true>, slices, 64 * kSortWaves, stream, ids, A, E, slice, (const uint32_t *)counts, out);
+  else
+    op_launch(sort_place<false>, slices, 64 * kSortWaves, stream, ids, A, E, slice, (const uint32_t *)counts, out);
 }
 
 void combine_launch(uint32_t type, const void *o, uint64_t o_stride, uint32_t ntok, uint32_t K, uint32_t cols,
@@ -504,8 +559,8 @@ MOE_API moe_status moe_dispatch_async(const moe_dispatch_config *cfg, const void
         constexpr uint32_t kN = decltype(piece)::value;
         if (A <= kFewIds) {
           const uint32_t cols = xs ? H : 0;
-          const uint64_t waves = (uint64_t)ntok * std::max(((cols + kN - 1) / kN + 63) / 64, 1u);
-          return op_launch(dispatch_few<kType, kN>, (waves + 3) / 4 + 1, 256, stream, ids, ntok, K, E, from, x_stride, cols, to,
+          const uint64_t parts = std::max(((cols + kN - 1) / kN + 255) / 256, 1u);
+          return op_launch(dispatch_few<kType, kN>, ntok * parts + 1, 256, stream, ids, ntok, K, E, from, x_stride, cols, to,
                            xs_stride, out);
         }
         if (!xs) return;
