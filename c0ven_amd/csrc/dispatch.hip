@@ -293,28 +293,33 @@ __global__ void __launch_bounds__(256) dispatch_few(const int32_t *__restrict__ 
   const uint32_t parts = max((pieces + 255) / 256, 1u), t = blockIdx.x / parts, piece = (blockIdx.x - t * parts) * 256 + threadIdx.x;
   const bool there = piece < pieces;
   const uint32_t c = there ? min(piece * kN, cols - kN) : 0;
-  uint32_t id[kFewIds / 64], of[4];
+  uint32_t key[kFewIds / 64], of[4];
 #pragma unroll
   for (uint32_t j = 0; j < 4; j++) of[j] = (uint32_t)ids[t * K + min(wave + 4 * j, K - 1)];
 #pragma unroll
   for (uint32_t j = 0; j < kFewIds / 64; j++) {
     if (j * 64 >= A) break;
-    id[j] = (uint32_t)ids[min(j * 64 + lane, A - 1)];
+    key[j] = (uint32_t)ids[min(j * 64 + lane, A - 1)];
   }
   Few<kType, kN> v;
   if (there) v.load(x + t * x_stride + c);
 #pragma unroll
   for (uint32_t j = 0; j < 4; j++) loaded<true>(of[j]);
+  // An assignment's place: how many keys (expert, then assignment; past the last id the largest) are below its own.
+#pragma unroll
+  for (uint32_t j = 0; j < kFewIds / 64; j++) {
+    if (j * 64 >= A) break;
+    key[j] = j * 64 + lane < A ? min(key[j], E) * kFewIds + j * 64 + lane : ~0u;
+  }
 #pragma unroll
   for (uint32_t i = 0; i < 4; i++) {
-    const uint32_t k = wave + 4 * i, a = t * K + k, e = min(of[i], E);
+    const uint32_t k = wave + 4 * i, a = t * K + k, e = min(of[i], E), own = e * kFewIds + a;
     if (k >= K) break;
     uint32_t place = 0;
 #pragma unroll
     for (uint32_t j = 0; j < kFewIds / 64; j++) {
       if (j * 64 >= A) break;
-      const uint32_t b = j * 64 + lane;  // (past the last id: not before any)
-      place += (uint32_t)__popcll(__ballot(b < A && (id[j] < e || (id[j] == e && b < a))));
+      place += (uint32_t)__popcll(__ballot(key[j] < own));
     }
     if (lane == 0) {
       places[k] = e < E ? place : ~0u;
