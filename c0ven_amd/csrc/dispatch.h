@@ -18,6 +18,8 @@ struct SortOut {
 // Bytes of work the sort of A ids takes, and the sort, on the current device.
 uint64_t sort_bytes(uint32_t A, uint32_t E);
 void sort_launch(const int32_t *ids, uint32_t A, uint32_t E, const SortOut &out, void *work, void *stream);
+// Its last launch alone: the slices' counts, if there are several, are in work.
+void sort_place_launch(const int32_t *ids, uint32_t A, uint32_t E, const SortOut &out, void *work, void *stream);
 
 // y[t] = sum over t's ranks of w o[place], in rank order in fp32, rounded once to y_type: `cols` values a row from y on, rows
 // of o (of type, o_stride apart); a place outside 0 .. A - 1 adds nothing; w null: ones.

@@ -9,6 +9,8 @@
 #include "i8_api.h"
 #include "i8_few.h"
 #include "i8_gemm.h"
+#include "i8_quant.h"
+#include "sort.h"
 
 #include <algorithm>
 
@@ -20,6 +22,21 @@ struct I8Experts {
   uint32_t E, K, H, F;
   float limit;
 };
+
+// The first `slices` work-groups sort (kCount: count their slices' experts), the others quantise x's rows, 16 at a time or (kLong,
+// more than 2048 values) one: two launches' work in one (30 tokens 57.7 us, 54.4).
+template <uint32_t kX, bool kLong, bool kCount>
+__global__ void __launch_bounds__(1024) i8_prepare(const int32_t *ids, uint32_t A, uint32_t E, uint32_t slices, uint32_t *counts,
+                                                   SortOut out, const typename Elem<kX>::T *x, uint64_t stride, uint32_t ntok, uint32_t H,
+                                                   int8_t *xc, float *xs) {
+  if (blockIdx.x >= slices)
+    quantize_block<kX, 1024, kLong ? 1024 : 64, kLong ? 2 : 4, false>(blockIdx.x - slices, gridDim.x - slices, x, stride, ntok, H, nullptr,
+                                                                      xc, xs);
+  else if (kCount)
+    count_slice(ids, A, E, kSlice, counts);
+  else
+    place_slice<true>(ids, A, E, kSlice, 1, nullptr, out);
+}
 
 // An item: a tile and 32 WN columns of h (their rows of gate and of up). Writes the positions' rows of h, `pitch` apart: a lane
 // has a column of 16 rows, so that a store is of whole lines.
@@ -486,9 +503,13 @@ struct Plan {
   Plan(const moe_i8_experts &e, uint32_t T) {
     A = T * e.n_used;
     few = !A || (T <= 16 && A <= kFew && e.n_embd >= 8 && T * (i8_pitch(e.n_embd) + 16) <= kFewXq && A * i8_pitch(e.n_ff) <= kFewHq);
-    // Tiles of 32, 64 or 128 positions: the more an expert has on average, the fewer times its weights are read.
+    // Tiles of 32, 64 or 128 positions: the more an expert has on average, the fewer times its weights are read, as long as the
+    // tiles are enough for the CUs. 30 tokens of 10 of 512 experts (half of one each) 58, 59 and 65 us; 301 (6, 2560 x 640) 159,
+    // 150 and 171; 2048 (40) 440, 404 and 438; 4096 (80) 618, 564 and 532, with skewed experts 511, 434 and 436; 4096 of 4 of 8
+    // (2048) 222, 172 and 163, 1000 of them (500) 64, 56 and 58. (Of 256, with i8_gemm's five buffers: 178 and 79; h and the
+    // values go out after 4 or 16 stages.)
     const uint32_t mean = A / e.n_expert;
-    rows = mean < 24 ? 32 : mean < 96 ? 64 : 128;
+    rows = mean < 3 ? 32 : mean < 72 || (uint64_t)A / 128 * ((e.n_ff + 63) / 64) < 768 ? 64 : 128;
     hpitch = (e.n_ff + 3) / 4 * 4;
     pitch = (e.n_embd + 255) / 256 * 256;
     // The values of all assignments at once, or of as many columns at a time as 256 MB hold, about the last-level cache.
@@ -579,8 +600,21 @@ MOE_API moe_status moe_i8_experts_async(const moe_i8_experts *e, const void *x, 
     MoeTile *tiles = (MoeTile *)(b + at.tiles);
     float *o = (float *)(b + at.o);
     const moe_i8_matrix xq{(int8_t *)(b + at.xc), (float *)(b + at.xs), ntok, H};
-    sort_launch(ids, A, E, SortOut{order, places, offsets, tiles, nt, at.rows}, b + at.sort, stream);
-    i8_quantize_launch(e->x_type, x, x_stride, xq, nullptr, stream);
+    const SortOut sorted{order, places, offsets, tiles, nt, at.rows};
+    const uint32_t slices = slices_of(A);  // (of kSlice ids: A is at most 2^18)
+    op_by_type(e->x_type, [&](auto t) {
+      constexpr uint32_t kX = decltype(t)::value;
+      const bool wide = H > 2048;
+      const auto run = [&](auto kernel) {
+        op_launch(kernel, slices + (wide ? ntok : (ntok + 15) / 16), 1024, stream, ids, A, E, slices, (uint32_t *)(b + at.sort), sorted,
+                  (const typename Elem<kX>::T *)x, x_stride, ntok, H, xq.codes, xq.scales);
+      };
+      if (slices == 1)
+        wide ? run(i8_prepare<kX, true, false>) : run(i8_prepare<kX, false, false>);
+      else
+        wide ? run(i8_prepare<kX, true, true>) : run(i8_prepare<kX, false, true>);
+    });
+    if (slices > 1) sort_place_launch(ids, A, E, sorted, b + at.sort, stream);
     const auto run = [&](auto gate_up, auto down, uint32_t bn) {
       const uint64_t cols = bn / 2, parts = (F + cols - 1) / cols;
       op_launch(gate_up, item_blocks(at.max_tiles * parts, parts), 256, stream, p, (const int8_t *)xq.codes, (const float *)xq.scales,
