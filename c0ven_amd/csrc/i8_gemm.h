@@ -6,6 +6,15 @@
 
 namespace c0ven {
 
+// A barrier at which all but the wave's last kLoads loads have arrived (no fence: it would wait for all).
+template <int kLoads>
+__device__ __forceinline__ void dma_barrier_but() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | kLoads % 16 | kLoads / 16 << 14);  // vmcnt(kLoads) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // A stage of k = 128, its eight 16-byte pieces of a row exchanged as in MxStage.
 template <int kRows>
 struct I8Rows {
@@ -29,9 +38,10 @@ struct I8Source {
     for (int i = 0; i < kLoads; i++)
       at[i] = row_of((wave + kWaves * i) * 8 + lane / 8) * steps * kI8Row + ((lane % 8) ^ (wave % 2 * 4 + lane / 16)) * 16;
   }
-  __device__ __forceinline__ void load(uint32_t k, uint8_t *to) const {
+  // Stage k, zeros unless k < end.
+  __device__ __forceinline__ void load(uint32_t k, uint8_t *to, uint32_t end = ~0u) const {
     const uint32_t off = k * kI8Row;
-    const auto from = mx_buffer(codes + off, bytes > off ? bytes - off : 0);
+    const auto from = mx_buffer(codes + off, k < end && bytes > off ? bytes - off : 0);
 #pragma unroll
     for (int i = 0; i < kLoads; i++) lds_dma16(from, at[i], to + (mx_wave() + kWaves * i) * 1024);
   }
@@ -123,6 +133,32 @@ struct I8Tile {
     }
     if (k < n) stage(x0, w0, x1, w1, dma_barrier, [] {});
   }
+  // The same with four buffers each, so that a stage's loads have three stages' time: a barrier waits for all but the last two
+  // stages' loads, kLoads a wave and stage.
+  template <int kLoads, typename LoadX, typename LoadW>
+  __device__ __forceinline__ void run8(X &x0, X &x1, X &x2, X &x3, W &w0, W &w1, W &w2, W &w3, uint32_t n, LoadX load_x,
+                                       LoadW load_w) {
+    clear();
+    // (Loads without conditions, past the last stage of nothing, so that the compiler knows which are outstanding where.)
+    load_w(w0, 0), load_x(x0, 0);
+    load_w(w1, 1), load_x(x1, 1);
+    load_w(w2, 2), load_x(x2, 2);
+    load_w(w3, 3), load_x(x3, 3);
+    dma_barrier_but<3 * kLoads>();
+    read<0>(x0, w0);
+    uint32_t k = 0;
+    for (; k + 4 <= n; k += 4) {
+      stage(x0, w0, x1, w1, dma_barrier_but<2 * kLoads>, [&] { load_w(w0, k + 4), load_x(x0, k + 4); });
+      stage(x1, w1, x2, w2, dma_barrier_but<2 * kLoads>, [&] { load_w(w1, k + 5), load_x(x1, k + 5); });
+      stage(x2, w2, x3, w3, dma_barrier_but<2 * kLoads>, [&] { load_w(w2, k + 6), load_x(x2, k + 6); });
+      stage(x3, w3, x0, w0, dma_barrier_but<2 * kLoads>, [&] { load_w(w3, k + 7), load_x(x3, k + 7); });
+    }
+    const auto none = [] {};
+    if (k < n) stage(x0, w0, x1, w1, dma_barrier_but<2 * kLoads>, none);
+    if (k + 1 < n) stage(x1, w1, x2, w2, dma_barrier_but<kLoads>, none);
+    if (k + 2 < n) stage(x2, w2, x3, w3, dma_barrier, none);
+    dma_barrier();
+  }
   // The same with three buffers of x and two of w (all of LDS with tiles of 256): x is loaded two stages ahead, so that half of a
   // stage's bytes have two stages' time, and a barrier waits for w's (and the older x's) alone: all but the last kXLoads loads of
   // a wave, which are one buffer of x's.
@@ -148,12 +184,7 @@ struct I8Tile {
       six([&](X &x, W &w, const X &next_x, const W &next_w, uint32_t i) {
         stage(
             x, w, next_x, next_w,
-            [] {  // (no fence: it would wait for all loads)
-              asm volatile("" ::: "memory");
-              __builtin_amdgcn_s_waitcnt(0x0070 | kXLoads);  // vmcnt(kXLoads) lgkmcnt(0)
-              __builtin_amdgcn_s_barrier();
-              asm volatile("" ::: "memory");
-            },
+            dma_barrier_but<kXLoads>,
             [&] { load_w(w, i + 2), load_x(x, i + 3); });
       });
     const auto last = [&](X &x, W &w, const X &next_x, const W &next_w, uint32_t i) {

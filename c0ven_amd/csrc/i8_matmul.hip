@@ -80,29 +80,56 @@ __global__ void __launch_bounds__(64 * kWaves)
   }
 }
 
-// The sums of `parts` parts, each M x N, and their scales.
+// Four elements at whatever address.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Four {
+  T e[4];
+};
+
+// The sums of `parts` parts, each M x N (fewer than 2^31), and their scales: four columns a thread.
 template <uint32_t kType>
 __global__ void __launch_bounds__(256) i8_join(const int *sums, uint32_t parts, const float *xs, const float *ws, uint32_t M,
                                                uint32_t N, typename Elem<kType>::T *y, uint64_t stride) {
-  const uint64_t n = (uint64_t)M * N, i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  int s = 0;
-  for (uint32_t p = 0; p < parts; p++) s += sums[p * n + i];
-  y[i / N * stride + i % N] = (typename Elem<kType>::T)i8_value(s, xs[i / N], ws[i % N]);
+  typedef typename Elem<kType>::T T;
+  const uint32_t across = (N + 3) / 4, i = blockIdx.x * 256 + threadIdx.x, m = i / across, n0 = i % across * 4;
+  if (m >= M) return;
+  const uint64_t size = (uint64_t)M * N;
+  const int *from = sums + (uint64_t)m * N + n0;
+  T *to = y + m * stride + n0;
+  const float sx = xs[m];
+  if (n0 + 4 <= N) {
+    int s[4] = {0, 0, 0, 0};
+    const Four<float> sw = *(const Four<float> *)(ws + n0);
+#pragma unroll 4
+    for (uint32_t p = 0; p < parts; p++) {
+      const Four<int> v = *(const Four<int> *)(from + p * size);
+#pragma unroll
+      for (int j = 0; j < 4; j++) s[j] += v.e[j];
+    }
+    Four<T> o;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o.e[j] = (T)i8_value(s[j], sx, sw.e[j]);
+    *(Four<T> *)to = o;
+  } else {
+    for (uint32_t j = 0; n0 + j < N; j++) {
+      int s = 0;
+      for (uint32_t p = 0; p < parts; p++) s += from[p * size + j];
+      to[j] = (T)i8_value(s, sx, ws[n0 + j]);
+    }
+  }
 }
 
 // A tile of y a work-group, k split into parts of `span` stages; kSums: the sums themselves, part p's to y + p M N, else y's
-// values. Work-groups to tiles so that an XCD has neighbours: eight tiles down, then across. The 256 tile has eight waves and
-// five buffers. 4096 x 8192 x 8192 on a layer's codes: 247 us, 2.2 POPS, and 254 to 300 with two buffers of each; the clock gives
+// values. Work-groups to tiles so that an XCD has neighbours: eight tiles down, then across. kBuffers: two of x and two of w,
+// four of each, or three of x and two of w (the 256 tile's, which has eight waves). 4096 x 8192 x 8192 on a layer's codes: 247 us, 2.2 POPS, and 254 to 300 with two buffers of each; the clock gives
 // way under such codes (on zeros 183 us, 3.0 POPS, and 202 with two buffers), and the matrix instructions alone, on operands
 // that stay in registers, take 185 on random ones. Four waves of 128 x 128 each read a third less of LDS but leave a SIMD one wave: 265.
-template <uint32_t kType, bool kSums, int TM, int TN, int kWaves>
+template <uint32_t kType, bool kSums, int TM, int TN, int kWaves, int kBuffers>
 __global__ void __launch_bounds__(64 * kWaves, 2)
     i8_gemm(const int8_t *xc, const float *xs, const int8_t *wc, const float *ws, uint32_t M, uint32_t N, uint32_t steps,
             uint32_t span, typename Elem<kType>::T *y, uint64_t stride) {
   typedef I8Tile<TM, TN, 2, false, false, kWaves> Tile;
   constexpr int BM = Tile::BM, BN = Tile::BN;
-  constexpr bool kFive = BM == 256;
   typedef typename Elem<kType>::T T;
   static_assert(!kSums || sizeof(T) == 4, "sums are 32 bits");
   __shared__ typename Tile::X x0;
@@ -121,8 +148,26 @@ __global__ void __launch_bounds__(64 * kWaves, 2)
   const I8Source<BN, kWaves> sw(wc + (uint64_t)n0 * steps * kI8Row, N - n0, steps, same);
   const auto load_x = [&](typename Tile::X &s, uint32_t k) { sx.load(k0 + k, s.b); };
   const auto load_w = [&](typename Tile::W &s, uint32_t k) { sw.load(k0 + k, s.b); };
+  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32, r = lane % 32;
+  constexpr uint32_t kWide = 32 * TN, kPitch = kWide + 4, kFour = kWaves / 4;
+  const uint32_t wm = m0 + Tile::x_row(), gn = n0 + Tile::w_row() + lane % (kWide / 4) * 4;
+  // The scales: a lane's four columns' and one of each 32 rows' (before any store, which a load would wait for).
+  float scale[4], row_scale[TM];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; j++) scale[j] = kSums ? 0.0f : ws[min(gn + j, N - 1)];
+#pragma unroll
+  for (int m = 0; m < TM; m++) row_scale[m] = kSums ? 0.0f : xs[min(wm + 32 * m + r, M - 1)];
   Tile c;
-  if constexpr (kFive) {
+  if constexpr (kBuffers == 8) {
+    __shared__ typename Tile::X x2;
+    __shared__ typename Tile::X x3;
+    __shared__ typename Tile::W w2;
+    __shared__ typename Tile::W w3;
+    const auto within_x = [&](typename Tile::X &s, uint32_t k) { sx.load(k0 + k, s.b, k1); };
+    const auto within_w = [&](typename Tile::W &s, uint32_t k) { sw.load(k0 + k, s.b, k1); };
+    constexpr int kLoads = I8Source<BM, kWaves>::kLoads + I8Source<BN, kWaves>::kLoads;
+    c.template run8<kLoads>(x0, x1, x2, x3, w0, w1, w2, w3, k1 - k0, within_x, within_w);
+  } else if constexpr (kBuffers == 5) {
     __shared__ typename Tile::X x2;
     c.template run5<I8Source<BM, kWaves>::kLoads>(x0, x1, x2, w0, w1, k1 - k0, load_x, load_w);
   } else {
@@ -131,18 +176,11 @@ __global__ void __launch_bounds__(64 * kWaves, 2)
   __builtin_amdgcn_s_barrier();  // (the stages' LDS is used again)
   // Each wave's 32 rows at a time through its part of LDS, so that a row's neighbours are stored together: a lane has four
   // columns, the same of every row.
-  const uint32_t lane = threadIdx.x & 63, wave = mx_wave(), q = lane / 32, r = lane % 32;
-  constexpr uint32_t kWide = 32 * TN, kPitch = kWide + 4, kFour = kWaves / 4;
   static_assert(64 % (kWide / 4) == 0, "a lane's columns");
   static_assert(kWaves % 4 == 0 && kFour * 32 * kPitch * 4 <= sizeof(x0) && BM == BN, "a quarter of the waves' rows in a buffer");
   const uint32_t b = wave / kFour;
   int *mine = (int *)(b == 0 ? x0.b : b == 1 ? x1.b : b == 2 ? w0.b : w1.b) + wave % kFour * 32 * kPitch;
-  const uint32_t wm = m0 + Tile::x_row(), gn = n0 + Tile::w_row() + lane % (kWide / 4) * 4;
   if (kSums) y += (uint64_t)p * M * N;
-  const bool whole = gn + 4 <= N && stride % 4 == 0 && ((uintptr_t)y & (4 * sizeof(T) - 1)) == 0;
-  float scale[4];
-#pragma unroll
-  for (uint32_t j = 0; j < 4; j++) scale[j] = kSums || gn + j >= N ? 0.0f : ws[gn + j];
 #pragma unroll
   for (int m = 0; m < TM; m++) {
 #pragma unroll
@@ -153,30 +191,32 @@ __global__ void __launch_bounds__(64 * kWaves, 2)
             make_int4(c.acc[n][m][4 * j], c.acc[n][m][4 * j + 1], c.acc[n][m][4 * j + 2], c.acc[n][m][4 * j + 3]);
     __builtin_amdgcn_s_waitcnt(0xc07f);
     __builtin_amdgcn_wave_barrier();
-#pragma unroll 4
-    for (uint32_t row = lane / (kWide / 4); row < 32; row += 64 / (kWide / 4)) {
+    constexpr uint32_t kRows = 64 / (kWide / 4);  // at a time
+    const auto value = [&](uint32_t i) {
+      const uint32_t row = lane / (kWide / 4) + kRows * i;
       const int4 v = *(const int4 *)(mine + row * kPitch + lane % (kWide / 4) * 4);
-      const uint32_t gm = wm + 32 * m + row;
-      if (gm >= M) continue;
-      const int s[4] = {v.x, v.y, v.z, v.w};
-      const float f = kSums ? 0.0f : xs[gm];
-      T e[4];
+      const float f = kSums ? 0.0f : __shfl(row_scale[m], row);
+      if constexpr (kSums)
+        return Four<T>{{__int_as_float(v.x), __int_as_float(v.y), __int_as_float(v.z), __int_as_float(v.w)}};
+      else
+        return Four<T>{{(T)i8_value(v.x, f, scale[0]), (T)i8_value(v.y, f, scale[1]), (T)i8_value(v.z, f, scale[2]),
+                        (T)i8_value(v.w, f, scale[3])}};
+    };
+    T *const to = y + (uint64_t)(wm + 32 * m + lane / (kWide / 4)) * stride + gn;
+    if (wm + 32 * m + 32 <= M && n0 + Tile::w_row() + kWide <= N) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if constexpr (kSums)
-          e[j] = (T)__int_as_float(s[j]);
-        else
-          e[j] = (T)i8_value(s[j], f, scale[j]);
-      }
-      T *to = y + (uint64_t)gm * stride + gn;
-      if (whole) {
-        struct alignas(4 * sizeof(T)) Four {
-          T e[4];
-        };
-        *(Four *)to = Four{{e[0], e[1], e[2], e[3]}};
-      } else {
-        for (uint32_t j = 0; j < 4; j++)
-          if (gn + j < N) to[j] = e[j];
+      for (uint32_t i = 0; i < 32 / kRows; i++) *(Four<T> *)(to + kRows * i * stride) = value(i);
+    } else {
+#pragma unroll 1
+      for (uint32_t i = 0; i < 32 / kRows; i++) {
+        const Four<T> v = value(i);
+        if (wm + 32 * m + lane / (kWide / 4) + kRows * i < M) {
+          if (gn + 4 <= N)
+            *(Four<T> *)(to + kRows * i * stride) = v;
+          else
+            for (uint32_t j = 0; j < 4; j++)
+              if (gn + j < N) to[kRows * i * stride + j] = v.e[j];
+        }
       }
     }
     __builtin_amdgcn_s_waitcnt(0xc07f);
@@ -190,28 +230,48 @@ using namespace c0ven;
 
 namespace {
 
-// How a product of M rows with N rows runs: tiles of 64 t by 64 t, k in parts of span stages of 128. The largest tile that still
-// gives most CUs one; if even the smallest leaves CUs without one, the k axis is split.
+// How a product of M rows with N rows runs: tiles of 64 t by 64 t, k in parts of span stages of 128. Up to 512 tiles of 64 (two a
+// CU with four buffers each) wait for memory's latency: four buffers (128 x 8192 x 8192 23.8 us, with two 50; 512 x 4096 x 4096
+// 17.4 and 20.4), and with few tiles parts of k, by what their sums' way through memory costs: a stage takes 220 ns, a part's sums
+// are written and read at 310 to the nanosecond, a launch is 1.5 us (17 x 4096 x 4096 in four parts 7.7 us, in one 10.0, in eight
+// 9.3; 128 x 2048 x 2048 7.5, in two 8.0). More are fewer loads in larger tiles, if those still fill the 256 CUs: tiles of 256
+// where their rounds are three quarters full (2048 x 8192 x 8192 120 us, tiles of 128 145; 2500 x 5120 x 4096, 200 tiles, 55 and
+// 63; but 2678 x 6333 x 4096, 275 tiles, 106 and 91; 4096 x 6144 x 4096, 384, 110 and 109), else tiles of 128, one to a CU with
+// four buffers (512 x 8192 x 8192 46.5, with two 63.8, tiles of 64 66) or two with two (1024 x 8192 x 8192 75, with four 89), else
+// tiles of 64 with two (1500 x 1500 x 512 6.5, with four 8.1, tiles of 128 8.7).
 struct Plan {
-  uint32_t tile = 1, span, parts = 1;
+  uint32_t tile, buffers, span, parts = 1;
   uint64_t tiles;
   Plan(uint32_t M, uint32_t N, uint32_t steps) {
     const auto count = [&](uint64_t t) { return ((M + 64 * t - 1) / (64 * t)) * ((N + 64 * t - 1) / (64 * t)); };
-    for (uint32_t t : {4u, 2u})
-      if (count(t) >= 200) {
-        tile = t;
-        break;
-      }
-    tiles = count(tile);
     span = steps;
-    if (tile == 1 && tiles < 200) {
-      const uint32_t want = (uint32_t)std::min<uint64_t>(400 / tiles, steps / 4);
-      if (want > 1) span = (steps + want - 1) / want;
+    if (count(1) <= 512) {
+      tile = 1, buffers = 8;
+      uint64_t least = ~0ull;
+      for (uint32_t p = 1; p <= std::max<uint64_t>(1, std::min<uint64_t>(512 / count(1), steps)); p++) {
+        const uint32_t of = (steps + p - 1) / p;
+        const uint64_t ns = of * 220ull + (p > 1 ? 1500 + (uint64_t)p * M * N / 310 : 0);
+        if (ns < least) least = ns, span = of;
+      }
+      parts = (steps + span - 1) / span;
+    } else if (count(4) * 4 >= (count(4) + 255) / 256 * 256 * 3) {
+      tile = 4, buffers = 5;
+    } else if (count(2) >= 200) {
+      tile = 2, buffers = count(2) <= 256 ? 8 : 4;
+    } else {
+      tile = 1, buffers = 4;
     }
-    parts = (steps + span - 1) / span;
+    tiles = count(tile);
   }
   uint64_t bytes(uint32_t M, uint32_t N) const { return parts > 1 ? (uint64_t)parts * M * N * 4 : 0; }
 };
+
+// Quantised rows that the few-rows kernel takes, else the tiles do. Above eight, on weights of 32 MB and more, every line of w's is
+// worth more than a launch, and the tiles have more of them on their way (16 x 8192 x 8192 16.4 us and 19.2,
+// 16 x 16384 x 4096 16.3 and 20.4; 8 x 8192 x 8192 15.7 and 16.8, 16 x 4096 x 4096 7.5 and 6.2).
+bool few_rows(uint32_t M, const moe_i8_matrix &w) {
+  return M <= 8 || (M <= kFewRows && (uint64_t)w.rows * i8_pitch(w.cols) < 32u << 20);
+}
 
 template <uint32_t kX>
 void launch_few(const void *x, uint64_t x_stride, const int8_t *xc, const float *xs, uint32_t M, const moe_i8_matrix *w,
@@ -238,7 +298,7 @@ void launch_few(const void *x, uint64_t x_stride, const int8_t *xc, const float 
 void launch_matmul(const int8_t *xc, const float *xs, uint32_t M, const moe_i8_matrix *w, uint32_t y_type, void *y,
                    uint64_t stride, void *work, void *stream) {
   const uint32_t N = w->rows, steps = i8_steps(w->cols);
-  if (M <= kFewRows) return launch_few<kQuantised>(nullptr, 0, xc, xs, M, w, y_type, y, stride, stream);
+  if (few_rows(M, *w)) return launch_few<kQuantised>(nullptr, 0, xc, xs, M, w, y_type, y, stride, stream);
   const Plan p(M, N, steps);
   const auto tiles = [&](auto t, auto sums, void *to, uint64_t to_stride) {
     constexpr uint32_t kType = decltype(t)::value;
@@ -248,16 +308,17 @@ void launch_matmul(const int8_t *xc, const float *xs, uint32_t M, const moe_i8_m
                 (const float *)w->scales, M, N, steps, p.span, (typename Elem<kType>::T *)to, to_stride);
     };
     if constexpr (!kSums) {
-      if (p.tile == 4) run(i8_gemm<kType, kSums, 4, 2, 8>, 8);
-      if (p.tile == 2) run(i8_gemm<kType, kSums, 2, 2, 4>, 4);
+      if (p.tile == 4) return run(i8_gemm<kType, kSums, 4, 2, 8, 5>, 8);
+      if (p.tile == 2) return p.buffers == 8 ? run(i8_gemm<kType, kSums, 2, 2, 4, 8>, 4) : run(i8_gemm<kType, kSums, 2, 2, 4, 4>, 4);
+      if (p.buffers == 4) return run(i8_gemm<kType, kSums, 1, 1, 4, 4>, 4);
     }
-    if (p.tile == 1) run(i8_gemm<kType, kSums, 1, 1, 4>, 4);
+    run(i8_gemm<kType, kSums, 1, 1, 4, 8>, 4);
   };
   if (p.parts == 1) return op_by_type(y_type, [&](auto t) { tiles(t, std::false_type(), y, stride); });
   tiles(std::integral_constant<uint32_t, QT_F32>(), std::true_type(), work, N);
   op_by_type(y_type, [&](auto t) {
     constexpr uint32_t kType = decltype(t)::value;
-    op_launch(i8_join<kType>, ((uint64_t)M * N + 255) / 256, 256, stream, (const int *)work, p.parts, xs, (const float *)w->scales, M, N,
+    op_launch(i8_join<kType>, ((uint64_t)M * ((N + 3) / 4) + 255) / 256, 256, stream, (const int *)work, p.parts, xs, (const float *)w->scales, M, N,
               (typename Elem<kType>::T *)y, stride);
   });
 }
@@ -274,7 +335,7 @@ bool quantises_itself(uint32_t M, uint32_t cols) { return !M || (M <= kFewRows &
 extern "C" {
 
 MOE_API uint64_t moe_i8_matmul_work_bytes(const moe_i8_matrix *w, uint32_t ntok) {
-  if (!w || !i8_sizes(*w) || ntok <= kFewRows || ntok > kI8MostRows || !w->rows) return 0;
+  if (!w || !i8_sizes(*w) || ntok > kI8MostRows || !w->rows || few_rows(ntok, *w)) return 0;
   return Plan(ntok, w->rows, i8_steps(w->cols)).bytes(ntok, w->rows);
 }
 
