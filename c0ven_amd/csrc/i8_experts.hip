@@ -23,6 +23,20 @@ struct I8Experts {
   float limit;
 };
 
+// expert_swiglu for the epilogue of a tile, whose time its arithmetic is a part of: one reciprocal, good to a unit of the last
+// place, for the division's ten instructions. Below g = -87.3, where the reciprocal would be a denormal number, 0 (expert_swiglu
+// from -88.7 on). NaNs and infinities as there: g is a factor of the result.
+__device__ __forceinline__ float i8_swiglu(float g, float u, float limit) {
+  if (limit > 0.0f) {
+    g = g > limit ? limit : g;
+    u = u > limit ? limit : u < -limit ? -limit : u;
+  }
+  const float x = __builtin_amdgcn_fmed3f(-g, -104.0f, 89.0f), hi = x * 1.4426950216e+0f;  // (as exp_f32)
+  const float lo = __builtin_fmaf(x, 1.9259629911e-8f, __builtin_fmaf(x, 1.4426950216e+0f, -hi));
+  const float e = __builtin_amdgcn_exp2f(hi) * __builtin_fmaf(lo, 0.69314718f, 1.0f);
+  return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
+
 // The first `slices` work-groups sort (kCount: count their slices' experts), the others quantise x's rows, 16 at a time or (kLong,
 // more than 2048 values) one: two launches' work in one (30 tokens 57.7 us, 54.4).
 template <uint32_t kX, bool kLong, bool kCount>
@@ -62,29 +76,36 @@ __global__ void __launch_bounds__(256) i8_gate_up_tiles(I8Experts p, const int8_
   const I8Source<kCols> g(p.gc + row * steps * kI8Row, rest, steps, same);
   const I8Source<kCols> u(p.uc + row * steps * kI8Row, rest, steps, same);
   if (threadIdx.x < Tile::BM) sx[threadIdx.x] = threadIdx.x < tile.count ? xs[token(threadIdx.x)] : 0.0f;
+  const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = Tile::w_row() + lane % 32;
+  const bool in = f0 + col < p.F;
+  const float sg = in ? p.gs[row + col] : 0.0f, su = in ? p.us[row + col] : 0.0f;
   Tile c;
   c.run2(
       x0, x1, w0, w1, steps, [&](typename Tile::X &s, uint32_t k) { x.load(k, s.b); },
       [&](typename Tile::W &s, uint32_t k) { g.load(k, s.b), u.load(k, s.b + kCols * kI8Row); });
-  const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = Tile::w_row() + lane % 32;
-  const bool in = f0 + col < p.F;
-  const float sg = in ? p.gs[row + col] : 0.0f, su = in ? p.us[row + col] : 0.0f;
   const __amdgpu_buffer_rsrc_t to =
       mx_buffer((const uint8_t *)(h + (uint64_t)tile.start * pitch), (uint64_t)tile.count * pitch * 4);
+  const uint32_t first = Tile::x_row() + 4 * q, at = in ? (first * pitch + f0 + col) * 4 : kNowhere;
+  const auto rows = [&](auto limited) {
+    const float limit = decltype(limited)::value ? p.limit : 0.0f;
 #pragma unroll
-  for (int m = 0; m < TM; m++)
+    for (int m = 0; m < TM; m++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const uint32_t r = Tile::x_row() + 32 * m + 8 * j + 4 * q;
-      const float4 v = *(const float4 *)(sx + r);
-      const float s[4] = {v.x, v.y, v.z, v.w};
+      for (int j = 0; j < 4; j++) {
+        const float4 v = *(const float4 *)(sx + first + 32 * m + 8 * j);
+        const float s[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float gv = i8_value(c.acc[0][m][4 * j + i], s[i], sg), uv = i8_value(c.acc[1][m][4 * j + i], s[i], su);
-        const uint32_t at = in ? ((r + i) * pitch + f0 + col) * 4 : kNowhere;
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(expert_swiglu(gv, uv, p.limit)), to, at, 0, 0);
+        for (int i = 0; i < 4; i++) {
+          const float gv = i8_value(c.acc[0][m][4 * j + i], s[i], sg), uv = i8_value(c.acc[1][m][4 * j + i], s[i], su);
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(i8_swiglu(gv, uv, limit)), to, at + (32 * m + 8 * j + i) * pitch * 4, 0,
+                                                0);
+        }
       }
-    }
+  };
+  if (p.limit > 0.0f)
+    rows(std::true_type());
+  else
+    rows(std::false_type());
 }
 
 // An item: a tile and BN of the `cols` rows of down from r0 on. Writes the positions' rows of o, `cols` apart (a multiple of 256).
@@ -106,28 +127,28 @@ __global__ void __launch_bounds__(256) i8_down_tiles(I8Experts p, const int8_t *
   const I8Source<Tile::BM> x(hc + (uint64_t)tile.start * steps * kI8Row, tile.count, steps, same);
   const I8Source<Tile::BN> w(p.dc + row * steps * kI8Row, all - row, steps, same);
   if (threadIdx.x < Tile::BM) sh[threadIdx.x] = threadIdx.x < tile.count ? hs[tile.start + threadIdx.x] : 0.0f;
-  Tile c;
-  c.run2(
-      x0, x1, w0, w1, steps, [&](typename Tile::X &s, uint32_t k) { x.load(k, s.b); },
-      [&](typename Tile::W &s, uint32_t k) { w.load(k, s.b); });
   const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = Tile::w_row() + lane % 32;
   float sd[2];
 #pragma unroll
   for (int f = 0; f < 2; f++) sd[f] = row + col + f * Tile::kStep < all ? p.ds[row + col + f * Tile::kStep] : 0.0f;
+  Tile c;
+  c.run2(
+      x0, x1, w0, w1, steps, [&](typename Tile::X &s, uint32_t k) { x.load(k, s.b); },
+      [&](typename Tile::W &s, uint32_t k) { w.load(k, s.b); });
   const __amdgpu_buffer_rsrc_t to = mx_buffer((const uint8_t *)(o + (uint64_t)tile.start * cols), (uint64_t)tile.count * cols * 4);
+  const uint32_t first = Tile::x_row() + 4 * q, at = (first * cols + c0 + col) * 4;
 #pragma unroll
   for (int m = 0; m < TM; m++)
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const uint32_t r = Tile::x_row() + 32 * m + 8 * j + 4 * q;
-      const float4 v = *(const float4 *)(sh + r);
+      const float4 v = *(const float4 *)(sh + first + 32 * m + 8 * j);
       const float s[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int f = 0; f < 2; f++)
           __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(i8_value(c.acc[f][m][4 * j + i], s[i], sd[f])), to,
-                                                ((r + i) * cols + c0 + col) * 4, f * Tile::kStep * 4, 0);
+                                                at + (32 * m + 8 * j + i) * cols * 4, f * Tile::kStep * 4, 0);
     }
 }
 
@@ -271,7 +292,7 @@ __global__ void __launch_bounds__(512) i8_gate_up_few(I8Experts p, const typenam
 #pragma unroll
     for (uint32_t j = 0; j < 4; j++) {
       const float own = i8_value(c[j], sx, scales[j]);
-      v[j] = expert_swiglu(own, __shfl_xor(own, 32, 64), p.limit);  // (of use in the lower half)
+      v[j] = i8_swiglu(own, __shfl_xor(own, 32, 64), p.limit);  // (of use in the lower half)
     }
     if (q < 2 && r < ntok && rank != 255 && f0 < p.F)
       *(float4 *)(h + (uint64_t)(r * p.K + rank) * pitch + f0) = make_float4(v[0], v[1], v[2], v[3]);
