@@ -23,8 +23,8 @@ __device__ __forceinline__ uint32_t lanes_below(uint64_t ballot) {
 // tiles: an expert's tiles share its weights in that L2, while the experts with one tile are dealt over all of them (MX4, 4096
 // tokens of 10 of 512 experts 392 us, with the items in order 430; of 4 of 16 experts 114 and 119). ~0: none.
 constexpr uint32_t kTileRun = 4;
-__device__ __forceinline__ uint32_t item_of(uint32_t all, uint32_t parts) {
-  const uint32_t run = kTileRun * parts, j = blockIdx.x / 8, id = (j / run * 8 + blockIdx.x % 8) * run + j % run;
+__device__ __forceinline__ uint32_t item_of(uint32_t all, uint32_t parts, uint32_t j = blockIdx.x / 8) {
+  const uint32_t run = kTileRun * parts, id = (j / run * 8 + blockIdx.x % 8) * run + j % run;
   return id < all ? id : ~0u;
 }
 // The work-groups that cover `all` items.

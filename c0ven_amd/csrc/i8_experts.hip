@@ -52,9 +52,16 @@ __global__ void __launch_bounds__(1024) i8_prepare(const int32_t *ids, uint32_t 
     place_slice<true>(ids, A, E, kSlice, 1, nullptr, out);
 }
 
+// A tile as scalars (a launch only reads them).
+__device__ __forceinline__ MoeTile tile_at(const MoeTile *tiles, uint32_t i) {
+  typedef uint32_t __attribute__((ext_vector_type(4))) Four;
+  const Four v = *(const __attribute__((address_space(4))) Four *)(uint64_t)(tiles + i);
+  return MoeTile{v[0], v[1], v[2], v[3]};
+}
+
 // An item: a tile and 32 WN columns of h (their rows of gate and of up). Writes the positions' rows of h, `pitch` apart: a lane
 // has a column of 16 rows, so that a store is of whole lines.
-template <int TM, int WM>
+template <int TM, int WM, bool kLimit>
 __global__ void __launch_bounds__(256) i8_gate_up_tiles(I8Experts p, const int8_t *xc, const float *xs, uint32_t ntok,
                                                         const int32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
                                                         float *h, uint32_t pitch) {
@@ -64,48 +71,79 @@ __global__ void __launch_bounds__(256) i8_gate_up_tiles(I8Experts p, const int8_
   __shared__ typename Tile::X x1;
   __shared__ typename Tile::W w0;
   __shared__ typename Tile::W w1;
-  __shared__ __align__(16) float sx[Tile::BM];
-  const uint32_t steps = i8_steps(p.H), parts = (p.F + kCols - 1) / kCols, item = item_of(*n_tiles * parts, parts);
+  __shared__ __align__(16) float sx[2][Tile::BM];
+  typedef I8Source<Tile::BM> Rows;
+  const uint32_t steps = i8_steps(p.H), parts = (p.F + kCols - 1) / kCols, all = *n_tiles * parts;
+  uint32_t j = blockIdx.x / 8, item = item_of(all, parts, j), ahead, now = 0;
   if (item == ~0u) return;
-  const MoeTile tile = tiles[item / parts];
-  const uint32_t f0 = item % parts * kCols;
-  const uint64_t row = (uint64_t)tile.expert * p.F + f0, rest = (uint64_t)p.E * p.F - row;
+  const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = Tile::w_row() + lane % 32, first = Tile::x_row() + 4 * q;
   const auto same = [](uint32_t r) { return r; };
-  const auto token = [&](uint32_t r) { return (uint32_t)order[tile.start + r] / p.K; };
-  const I8Source<Tile::BM> x(xc, ntok, steps, [&](uint32_t r) { return r < tile.count ? token(r) : ntok; });
-  const I8Source<kCols> g(p.gc + row * steps * kI8Row, rest, steps, same);
-  const I8Source<kCols> u(p.uc + row * steps * kI8Row, rest, steps, same);
-  if (threadIdx.x < Tile::BM) sx[threadIdx.x] = threadIdx.x < tile.count ? xs[token(threadIdx.x)] : 0.0f;
-  const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = Tile::w_row() + lane % 32;
-  const bool in = f0 + col < p.F;
-  const float sg = in ? p.gs[row + col] : 0.0f, su = in ? p.us[row + col] : 0.0f;
+  const uint64_t experts = (uint64_t)p.E * p.F;
+  Rows x(xc, ntok, steps, same);
+  I8Source<kCols> g(p.gc, experts, steps, same), u(p.uc, experts, steps, same);
+  MoeTile tile = tiles[item / parts], next, after;
+  uint32_t f0 = item % parts * kCols, next_f0, id[Rows::kLoads], my_id;
+  float sg, su, s;
+  // The tile after the next.
+  const auto look = [&] {
+    j += gridDim.x / 8, ahead = item_of(all, parts, j);
+    after = tile_at(tiles, ahead != ~0u ? ahead / parts : 0);
+    if (ahead == ~0u) after.count = 0;
+  };
+  // The next tile's ids; then its rows as the source.
+  const auto name = [&] {
+#pragma unroll
+    for (int i = 0; i < Rows::kLoads; i++) id[i] = order[next.start + (Rows::row(i) < next.count ? Rows::row(i) : 0)];
+    my_id = order[next.start + (threadIdx.x < next.count ? threadIdx.x : 0)];
+  };
+  const auto turn = [&] {
+#pragma unroll
+    for (int i = 0; i < Rows::kLoads; i++) x.aim(i, Rows::row(i) < next.count ? id[i] / p.K : ntok, steps);
+    const uint64_t row = next.count ? (uint64_t)next.expert * p.F + next_f0 : experts;
+    g.move(p.gc + row * steps * kI8Row, experts - row, steps);
+    u.move(p.uc + row * steps * kI8Row, experts - row, steps);
+    s = xs[my_id / p.K];
+  };
+  next = tile, next_f0 = f0;
+  look();
+  name();
+  turn();
+  if (threadIdx.x < Tile::BM) sx[0][threadIdx.x] = s;
   Tile c;
-  c.run2(
-      x0, x1, w0, w1, steps, [&](typename Tile::X &s, uint32_t k) { x.load(k, s.b); },
-      [&](typename Tile::W &s, uint32_t k) { g.load(k, s.b), u.load(k, s.b + kCols * kI8Row); });
-  const __amdgpu_buffer_rsrc_t to =
-      mx_buffer((const uint8_t *)(h + (uint64_t)tile.start * pitch), (uint64_t)tile.count * pitch * 4);
-  const uint32_t first = Tile::x_row() + 4 * q, at = in ? (first * pitch + f0 + col) * 4 : kNowhere;
-  const auto rows = [&](auto limited) {
-    const float limit = decltype(limited)::value ? p.limit : 0.0f;
+  const auto begin = [&] {
+    const bool in = f0 + col < p.F;
+    const uint64_t row = (uint64_t)tile.expert * p.F + f0 + col;
+    sg = in ? p.gs[row] : 0.0f, su = in ? p.us[row] : 0.0f;
+    next = after, next_f0 = ahead % parts * kCols, item = ahead;
+    look();
+    name();
+  };
+  const auto done = [&] {
+    const __amdgpu_buffer_rsrc_t to =
+        mx_buffer((const uint8_t *)(h + (uint64_t)tile.start * pitch), (uint64_t)tile.count * pitch * 4);
+    const uint32_t at = f0 + col < p.F ? (first * pitch + f0 + col) * 4 : kNowhere;
+    const float limit = kLimit ? p.limit : 0.0f;
 #pragma unroll
     for (int m = 0; m < TM; m++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const float4 v = *(const float4 *)(sx + first + 32 * m + 8 * j);
-        const float s[4] = {v.x, v.y, v.z, v.w};
+        const float4 v = *(const float4 *)(sx[now] + first + 32 * m + 8 * j);
+        const float r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const float gv = i8_value(c.acc[0][m][4 * j + i], s[i], sg), uv = i8_value(c.acc[1][m][4 * j + i], s[i], su);
+          const float gv = i8_value(c.acc[0][m][4 * j + i], r[i], sg), uv = i8_value(c.acc[1][m][4 * j + i], r[i], su);
           __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(i8_swiglu(gv, uv, limit)), to, at + (32 * m + 8 * j + i) * pitch * 4, 0,
                                                 0);
         }
       }
+    now ^= 1;
+    if (threadIdx.x < Tile::BM) sx[now][threadIdx.x] = s;
+    tile = next, f0 = next_f0;
+    return item != ~0u;
   };
-  if (p.limit > 0.0f)
-    rows(std::true_type());
-  else
-    rows(std::false_type());
+  c.template run_items<16 * TM>(
+      x0, x1, w0, w1, (steps + 1) / 2 * 2, [&](typename Tile::X &b, uint32_t k) { x.load(k, b.b, steps); },
+      [&](typename Tile::W &b, uint32_t k) { g.load(k, b.b, steps), u.load(k, b.b + kCols * kI8Row, steps); }, begin, turn, done);
 }
 
 // An item: a tile and BN of the `cols` rows of down from r0 on. Writes the positions' rows of o, `cols` apart (a multiple of 256).
@@ -117,39 +155,66 @@ __global__ void __launch_bounds__(256) i8_down_tiles(I8Experts p, const int8_t *
   __shared__ typename Tile::X x1;
   __shared__ typename Tile::W w0;
   __shared__ typename Tile::W w1;
-  __shared__ __align__(16) float sh[Tile::BM];
-  const uint32_t steps = i8_steps(p.F), parts = cols / Tile::BN, item = item_of(*n_tiles * parts, parts);
+  __shared__ __align__(16) float sh[2][Tile::BM];
+  const uint32_t steps = i8_steps(p.F), parts = cols / Tile::BN, n_items = *n_tiles * parts;
+  uint32_t j = blockIdx.x / 8, item = item_of(n_items, parts, j), ahead, now = 0;
   if (item == ~0u) return;
-  const MoeTile tile = tiles[item / parts];
-  const uint32_t c0 = item % parts * Tile::BN;
-  const uint64_t all = (uint64_t)p.E * p.H, row = min((uint64_t)tile.expert * p.H + r0 + c0, all);
+  const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = Tile::w_row() + lane % 32, first = Tile::x_row() + 4 * q;
   const auto same = [](uint32_t r) { return r; };
-  const I8Source<Tile::BM> x(hc + (uint64_t)tile.start * steps * kI8Row, tile.count, steps, same);
-  const I8Source<Tile::BN> w(p.dc + row * steps * kI8Row, all - row, steps, same);
-  if (threadIdx.x < Tile::BM) sh[threadIdx.x] = threadIdx.x < tile.count ? hs[tile.start + threadIdx.x] : 0.0f;
-  const uint32_t lane = threadIdx.x & 63, q = lane / 32, col = Tile::w_row() + lane % 32;
-  float sd[2];
-#pragma unroll
-  for (int f = 0; f < 2; f++) sd[f] = row + col + f * Tile::kStep < all ? p.ds[row + col + f * Tile::kStep] : 0.0f;
+  const uint64_t all = (uint64_t)p.E * p.H;
+  I8Source<Tile::BM> x(hc, 0, steps, same);
+  I8Source<Tile::BN> w(p.dc, 0, steps, same);
+  MoeTile tile = tiles[item / parts], next, after;
+  uint32_t c0 = item % parts * Tile::BN, next_c0;
+  float sd[2], s;
+  // The tile after the next.
+  const auto look = [&] {
+    j += gridDim.x / 8, ahead = item_of(n_items, parts, j);
+    after = tile_at(tiles, ahead != ~0u ? ahead / parts : 0);
+    if (ahead == ~0u) after.count = 0;
+  };
+  const auto turn = [&] {
+    x.move(hc + (uint64_t)next.start * steps * kI8Row, next.count, steps);
+    const uint64_t row = next.count ? min((uint64_t)next.expert * p.H + r0 + next_c0, all) : all;
+    w.move(p.dc + row * steps * kI8Row, all - row, steps);
+    s = hs[next.start + (threadIdx.x < next.count ? threadIdx.x : 0)];
+  };
+  next = tile, next_c0 = c0;
+  look();
+  turn();
+  if (threadIdx.x < Tile::BM) sh[0][threadIdx.x] = s;
   Tile c;
-  c.run2(
-      x0, x1, w0, w1, steps, [&](typename Tile::X &s, uint32_t k) { x.load(k, s.b); },
-      [&](typename Tile::W &s, uint32_t k) { w.load(k, s.b); });
-  const __amdgpu_buffer_rsrc_t to = mx_buffer((const uint8_t *)(o + (uint64_t)tile.start * cols), (uint64_t)tile.count * cols * 4);
-  const uint32_t first = Tile::x_row() + 4 * q, at = (first * cols + c0 + col) * 4;
+  const auto begin = [&] {
+    const uint64_t row = (uint64_t)tile.expert * p.H + r0 + c0 + col;
 #pragma unroll
-  for (int m = 0; m < TM; m++)
+    for (int f = 0; f < 2; f++) sd[f] = row + f * Tile::kStep < all ? p.ds[row + f * Tile::kStep] : 0.0f;
+    next = after, next_c0 = ahead % parts * Tile::BN, item = ahead;
+    look();
+  };
+  const auto done = [&] {
+    const __amdgpu_buffer_rsrc_t to = mx_buffer((const uint8_t *)(o + (uint64_t)tile.start * cols), (uint64_t)tile.count * cols * 4);
+    const uint32_t at = (first * cols + c0 + col) * 4;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float4 v = *(const float4 *)(sh + first + 32 * m + 8 * j);
-      const float s[4] = {v.x, v.y, v.z, v.w};
+    for (int m = 0; m < TM; m++)
 #pragma unroll
-      for (int i = 0; i < 4; i++)
+      for (int j = 0; j < 4; j++) {
+        const float4 v = *(const float4 *)(sh[now] + first + 32 * m + 8 * j);
+        const float r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int f = 0; f < 2; f++)
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(i8_value(c.acc[f][m][4 * j + i], s[i], sd[f])), to,
-                                                at + (32 * m + 8 * j + i) * cols * 4, f * Tile::kStep * 4, 0);
-    }
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int f = 0; f < 2; f++)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(i8_value(c.acc[f][m][4 * j + i], r[i], sd[f])), to,
+                                                  at + (32 * m + 8 * j + i) * cols * 4, f * Tile::kStep * 4, 0);
+      }
+    now ^= 1;
+    if (threadIdx.x < Tile::BM) sh[now][threadIdx.x] = s;
+    tile = next, c0 = next_c0;
+    return item != ~0u;
+  };
+  c.template run_items<32 * TM>(
+      x0, x1, w0, w1, (steps + 1) / 2 * 2, [&](typename Tile::X &b, uint32_t k) { x.load(k, b.b, steps); },
+      [&](typename Tile::W &b, uint32_t k) { w.load(k, b.b, steps); }, begin, turn, done);
 }
 
 // ---- few assignments (at most kFew of at most 16 tokens): no sorting, two or three launches. Bound by latency and by reading the experts'
@@ -636,22 +701,26 @@ MOE_API moe_status moe_i8_experts_async(const moe_i8_experts *e, const void *x, 
         wide ? run(i8_prepare<kX, true, true>) : run(i8_prepare<kX, false, true>);
     });
     if (slices > 1) sort_place_launch(ids, A, E, sorted, b + at.sort, stream);
-    const auto run = [&](auto gate_up, auto down, uint32_t bn) {
+    const auto run = [&](auto gate_up, auto down, uint32_t bn, uint32_t at_once) {
       const uint64_t cols = bn / 2, parts = (F + cols - 1) / cols;
-      op_launch(gate_up, item_blocks(at.max_tiles * parts, parts), 256, stream, p, (const int8_t *)xq.codes, (const float *)xq.scales,
+      op_launch(gate_up, std::min<uint64_t>(item_blocks(at.max_tiles * parts, parts), at_once), 256, stream, p, (const int8_t *)xq.codes, (const float *)xq.scales,
                 ntok, (const int32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, h, at.hpitch);
       i8_quantize_launch(QT_F32, h, at.hpitch, hq, offsets + E, stream);
       for (uint32_t c = 0; c < at.pitch; c += at.chunk) {
         const uint32_t n = std::min(at.chunk, at.pitch - c);
-        op_launch(down, item_blocks((uint64_t)at.max_tiles * (n / bn), n / bn), 256, stream, p, (const int8_t *)hq.codes,
+        op_launch(down, std::min<uint64_t>(item_blocks((uint64_t)at.max_tiles * (n / bn), n / bn), at_once), 256, stream, p, (const int8_t *)hq.codes,
                   (const float *)hq.scales, (const MoeTile *)tiles, (const uint32_t *)nt, c, n, o);
         combine_launch(QT_F32, o, n, ntok, K, std::min(n, H - c), places, w, e->y_type, (uint8_t *)y + (uint64_t)c * op_size(e->y_type),
                        y_stride, stream);
       }
     };
-    if (at.rows == 32) run(i8_gate_up_tiles<1, 1>, i8_down_tiles<1, 1>, 256);
-    if (at.rows == 64) run(i8_gate_up_tiles<1, 2>, i8_down_tiles<1, 2>, 128);
-    if (at.rows == 128) run(i8_gate_up_tiles<2, 2>, i8_down_tiles<2, 2>, 128);
+    const auto tiles_of = [&](auto limit) {
+      constexpr bool kLimit = decltype(limit)::value;
+      if (at.rows == 32) run(i8_gate_up_tiles<1, 1, kLimit>, i8_down_tiles<1, 1>, 256, 2 * kCus);
+      if (at.rows == 64) run(i8_gate_up_tiles<1, 2, kLimit>, i8_down_tiles<1, 2>, 128, 3 * kCus);
+      if (at.rows == 128) run(i8_gate_up_tiles<2, 2, kLimit>, i8_down_tiles<2, 2>, 128, 2 * kCus);
+    };
+    e->swiglu_limit > 0.0f ? tiles_of(std::true_type()) : tiles_of(std::false_type());
   });
 }
 

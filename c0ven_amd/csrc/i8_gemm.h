@@ -30,13 +30,20 @@ struct I8Source {
   uint64_t bytes;
   uint32_t at[kLoads];
 
+  // The row of a stage that this lane's load i is of.
+  static __device__ __forceinline__ uint32_t row(int i) { return (mx_wave() + kWaves * i) * 8 + (threadIdx.x & 63) / 8; }
+  __device__ __forceinline__ void aim(int i, uint32_t r, uint32_t steps) {
+    const uint32_t lane = threadIdx.x & 63;
+    at[i] = r * steps * kI8Row + ((lane % 8) ^ (mx_wave() % 2 * 4 + lane / 16)) * 16;
+  }
+  __device__ __forceinline__ void move(const int8_t *c, uint64_t rows, uint32_t steps) {
+    codes = (const uint8_t *)c, bytes = rows * steps * kI8Row;
+  }
   template <typename F>
-  __device__ __forceinline__ I8Source(const int8_t *c, uint64_t rows, uint32_t steps, F row_of)
-      : codes((const uint8_t *)c), bytes(rows * steps * kI8Row) {
-    const uint32_t lane = threadIdx.x & 63, wave = mx_wave();
+  __device__ __forceinline__ I8Source(const int8_t *c, uint64_t rows, uint32_t steps, F row_of) {
+    move(c, rows, steps);
 #pragma unroll
-    for (int i = 0; i < kLoads; i++)
-      at[i] = row_of((wave + kWaves * i) * 8 + lane / 8) * steps * kI8Row + ((lane % 8) ^ (wave % 2 * 4 + lane / 16)) * 16;
+    for (int i = 0; i < kLoads; i++) aim(i, row_of(row(i)), steps);
   }
   // Stage k, zeros unless k < end.
   __device__ __forceinline__ void load(uint32_t k, uint8_t *to, uint32_t end = ~0u) const {
@@ -132,6 +139,37 @@ struct I8Tile {
       });
     }
     if (k < n) stage(x0, w0, x1, w1, dma_barrier, [] {});
+  }
+  // Products of n stages (n even) one after another, the next one's first two loaded in the last two of this: begin() at a
+  // product's first stage, turn() from where the loads are the next product's, done() when its sums are there; false ends it.
+  // done()'s kStores stores (a wave's) go on beside the first stage: its barrier waits for what was loaded before them.
+  template <int kStores, typename LoadX, typename LoadW, typename Begin, typename Turn, typename Done>
+  __device__ __forceinline__ void run_items(X &x0, X &x1, W &w0, W &w1, uint32_t n, LoadX load_x, LoadW load_w, Begin begin, Turn turn,
+                                            Done done) {
+    constexpr int kBefore = kStores < 62 ? kStores : 62;  // (63 is no wait)
+    const auto load0 = [&](uint32_t k) { load_w(w0, k), load_x(x0, k); };
+    const auto load1 = [&](uint32_t k) { load_w(w1, k), load_x(x1, k); };
+    const auto pair = [&](auto barrier, uint32_t k) {
+      stage(x0, w0, x1, w1, barrier, [&] { load0(k); });
+      stage(x1, w1, x0, w0, dma_barrier, [&] { load1(k + 1); });
+    };
+    load0(0);
+    dma_barrier();
+    load1(1);
+    read<0>(x0, w0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0) (no store is before the first)
+    do {
+      clear();
+      begin();
+      if (n == 2) turn();
+      pair(dma_barrier_but<kBefore>, n == 2 ? 0 : 2);
+      if (n > 2) {
+        for (uint32_t k = 4; k < n; k += 2) pair(dma_barrier, k);
+        turn();
+        pair(dma_barrier, 0);
+      }
+    } while (done());
+    dma_barrier_but<kBefore>();  // (LDS is another work-group's after this one)
   }
   // The same with four buffers each, so that a stage's loads have three stages' time: a barrier waits for all but the last two
   // stages' loads, kLoads a wave and stage.
