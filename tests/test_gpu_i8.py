@@ -126,7 +126,9 @@ def check(got, x, w, out):
 # Few rows, each tile size, split k, sizes on and off every border.
 SHAPES = [(1, 1, 1), (1, 16, 128), (1, 17, 129), (2, 100, 1000), (5, 33, 64), (16, 2048, 1024), (16, 600, 9000), (1, 9000, 300), (3, 50, 8192),
           (17, 64, 128), (17, 1, 1), (33, 65, 127), (64, 64, 1000), (100, 130, 8200), (65, 1000, 257), (301, 2565, 1000), (128, 128, 65536),
-          (700, 2100, 384), (2000, 1950, 200), (1800, 1804, 513), (3330, 4100, 640), (4096, 3329, 130), (20, 40, 5000)]
+          (700, 2100, 384), (2000, 1950, 200), (1800, 1804, 513), (3330, 4100, 640), (4096, 3329, 130), (20, 40, 5000),
+          (40, 20000, 100), (40, 20000, 300), (40, 20000, 500), (40, 20000, 700), (512, 8192, 200), (520, 8000, 900), (1500, 1500, 130),
+          (2688, 2048, 260), (3500, 3500, 1100), (3500, 3499, 1300), (16, 4096, 8192), (9, 5000, 8190), (17, 1500, 4100), (60, 3, 20000)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)

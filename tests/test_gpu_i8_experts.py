@@ -89,6 +89,21 @@ def test_many(T, H, F, E, K, skew):
     check(Model(E, H, F, 5), x, ids, w, rows=np.r_[0:20, T // 2:T // 2 + 20, T - 20:T])
 
 
+@pytest.mark.parametrize("T,H,F,E,K,limit", [(600, 600, 640, 100, 4, 0.0), (600, 520, 640, 100, 4, 0.1), (2500, 260, 640, 100, 4, 0.0),
+                                             (2500, 100, 640, 100, 4, 0.1), (2500, 1300, 130, 100, 4, 0.0), (250, 1030, 260, 250, 2, 0.0)])
+def test_several_items_a_work_group(T, H, F, E, K, limit):
+    """More pieces of tiles than work-groups, with 32, 64 and 128 rows, of one stage to eleven."""
+    say("items", T, H, F, E, K, limit)
+    check(Model(E, H, F, 4), *tokens(T, H, E, K, 8, 0.05), limit=limit, rows=np.r_[0:16, T // 2:T // 2 + 16, T - 16:T])
+
+
+@pytest.mark.parametrize("T", [2, 40])
+def test_large_gates(T):
+    """Gates of hundreds to both sides: the SiLU at its ends."""
+    say("large gates", T)
+    check(Model(6, 512, 96, 8, sigma=5.0), *tokens(T, 512, 6, 3, 5))
+
+
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("T", [1, 6, 50])
@@ -259,6 +274,34 @@ def test_columns_in_parts(T, H, F, E, K):
     1792 and 512; n_embd ends inside the last."""
     say("columns in parts", T, H, F, E, K)
     check(Model(E, H, F, 6), *tokens(T, H, E, K, 9, 0.05), rows=np.r_[0:16, T // 2:T // 2 + 16, T - 16:T])
+
+
+@pytest.mark.parametrize("T", [8, 90])
+def test_graphs_that_share_a_work_buffer(T):
+    """Two captured calls on one work buffer, replayed in turn on one stream, with eager calls and waits between."""
+    say("shared work", T)
+    model, K = Model(12, 512, 128, 4), 4
+    op, s = model.op(K), hip.stream()
+    n = op.work_bytes(T)
+    work, other = room(n), room(n)
+    sets = []
+    for seed in (6, 7):
+        x, ids, w = tokens(T, 512, 12, K, seed, 0.2)
+        b = [hip.put(x), hip.put(ids.astype(np.int32)), hip.put(w.astype(np.float32)), hip.full((T, 512), 7.0)]
+
+        def call(y, room, stream, b=b):
+            op.forward_async(b[0].ptr, T, b[1].ptr, b[2].ptr, y.ptr, room.ptr, n, stream=stream)
+
+        sets.append((b, call, hip.capture(s, lambda call=call, b=b: call(b[3], work, s))))
+    r, eager = np.random.default_rng(3), hip.full((T, 512), 0)
+    for _ in range(3):
+        for b, _, _ in sets:
+            b[0].put(r.normal(size=(T, 512)).astype(np.float32))
+        for _, _, launch in sets:
+            launch()
+        for b, call, _ in sets:
+            call(eager, other, None)
+            assert np.array_equal(b[3].get(), eager.get())
 
 
 def test_no_tokens():
