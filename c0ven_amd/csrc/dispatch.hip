@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(256) dispatch_rows(const typename Elem<kType>:
 // themselves (lower ids, and equal ones before), and the last work-group the offsets. cols 0: no rows.
 constexpr uint32_t kFewIds = 1024;
 template <uint32_t kType, uint32_t kN>
-__global__ void __launch_bounds__(256) dispatch_few(const int32_t *__restrict__ ids, uint32_t ntok, uint32_t K, uint32_t E,
+__global__ void __launch_bounds__(256) dispatch_few(const int32_t *ids, uint32_t ntok, uint32_t K, uint32_t E,
                                                     const typename Elem<kType>::T *x, uint64_t x_stride, uint32_t cols,
                                                     typename Elem<kType>::T *xs, uint64_t xs_stride, SortOut out) {
   const uint32_t A = ntok * K, lane = threadIdx.x & 63;
