@@ -2,7 +2,10 @@
 //
 // Many tokens: the assignments are sorted by expert and cut into MoeTiles; x's rows are quantised; gate and up of a tile are one
 // product whose epilogue applies the SwiGLU; the rows of h (fp32: a row's scale needs all of it) are quantised; down follows, its
-// values in fp32 by position, and each token's are summed in rank order.
+// values in fp32 by position, and each token's are summed in rank order (in fp32: a value rounded to y's type there would be rounded
+// twice). Of 512 experts of 2048 x 512 with a skewed router, 10 a token: 4096 tokens 386 us (gate and up 183, 0.9 POPS with a quarter
+// of the tiles' rows empty; h quantised 19; down 150, for 0.3 GB of values; their sum 56; the sort and x 17), 1024 166, 30 54, where the
+// weights' bytes bound it (301 tokens of 2560 x 640: gate and up at 4.7 TB/s).
 #include "../../include/c0ven_moe_tile.h"
 #include "dispatch.h"
 #include "experts.h"
@@ -23,8 +26,8 @@ struct I8Experts {
   float limit;
 };
 
-// expert_swiglu for the epilogue of a tile, whose time its arithmetic is a part of: one reciprocal, good to a unit of the last
-// place, for the division's ten instructions. Below g = -87.3, where the reciprocal would be a denormal number, 0 (expert_swiglu
+// expert_swiglu for the epilogue of a tile, a sixth of whose time it was: one reciprocal, good to a unit of the last place, for the
+// division's ten instructions. Below g = -87.3, where the reciprocal would be a denormal number, 0 (expert_swiglu
 // from -88.7 on). NaNs and infinities as there: g is a factor of the result.
 __device__ __forceinline__ float i8_swiglu(float g, float u, float limit) {
   if (limit > 0.0f) {
@@ -59,13 +62,14 @@ __device__ __forceinline__ MoeTile tile_at(const MoeTile *tiles, uint32_t i) {
   return MoeTile{v[0], v[1], v[2], v[3]};
 }
 
-// An item: a tile and 32 WN columns of h (their rows of gate and of up). Writes the positions' rows of h, `pitch` apart: a lane
-// has a column of 16 rows, so that a store is of whole lines.
-template <int TM, int WM, bool kLimit>
+// An item: a tile and 64 columns of h (their rows of gate and of up). Writes the positions' rows of h, `pitch` apart: a lane has a
+// column of 16 rows, so that a store is of whole lines. A work-group has every gridDim-th item: the next one's tile, ids and first
+// two stages are there when it begins (4096 tokens of 10 of 512 experts: 194 us with a work-group an item, 183; down 162 and 150).
+template <int TM, bool kLimit>
 __global__ void __launch_bounds__(256) i8_gate_up_tiles(I8Experts p, const int8_t *xc, const float *xs, uint32_t ntok,
                                                         const int32_t *order, const MoeTile *tiles, const uint32_t *n_tiles,
                                                         float *h, uint32_t pitch) {
-  typedef I8Tile<TM, 2, WM, true, true> Tile;
+  typedef I8Tile<TM, 2, 2, true, true> Tile;
   constexpr uint32_t kCols = Tile::BN / 2;
   __shared__ typename Tile::X x0;
   __shared__ typename Tile::X x1;
@@ -146,11 +150,11 @@ __global__ void __launch_bounds__(256) i8_gate_up_tiles(I8Experts p, const int8_
       [&](typename Tile::W &b, uint32_t k) { g.load(k, b.b, steps), u.load(k, b.b + kCols * kI8Row, steps); }, begin, turn, done);
 }
 
-// An item: a tile and BN of the `cols` rows of down from r0 on. Writes the positions' rows of o, `cols` apart (a multiple of 256).
-template <int TM, int WM>
+// An item: a tile and 128 of the `cols` rows of down from r0 on. Writes the positions' rows of o, `cols` apart (a multiple of 256).
+template <int TM>
 __global__ void __launch_bounds__(256) i8_down_tiles(I8Experts p, const int8_t *hc, const float *hs, const MoeTile *tiles,
                                                      const uint32_t *n_tiles, uint32_t r0, uint32_t cols, float *o) {
-  typedef I8Tile<TM, 2, WM, true, true> Tile;
+  typedef I8Tile<TM, 2, 2, true, true> Tile;
   __shared__ typename Tile::X x0;
   __shared__ typename Tile::X x1;
   __shared__ typename Tile::W w0;
@@ -217,8 +221,9 @@ __global__ void __launch_bounds__(256) i8_down_tiles(I8Experts p, const int8_t *
       [&](typename Tile::W &b, uint32_t k) { w.load(k, b.b, steps); }, begin, turn, done);
 }
 
-// ---- few assignments (at most kFew of at most 16 tokens): no sorting, two or three launches. Bound by latency and by reading the experts'
-// weights, which go to LDS as whole rows, always some of them on their way.
+// ---- few assignments (at most kFew of at most 16 tokens): no sorting, two or three launches. Bound by latency and by reading the
+// experts' weights, which go to LDS as whole rows, always some of them on their way: 8 tokens of 10 of 512 experts of 2048 x 512 32
+// us (gate and up 17, 3.5 TB/s of the weights; h's quantisation 3; down 14), one token 19.5.
 
 constexpr uint32_t kFew = 160;
 
@@ -490,7 +495,8 @@ __global__ void __launch_bounds__(512) i8_down_few(I8Experts p, const float *h, 
         c = mx_i4{v.x, v.y, v.z, v.w};
       }
 #pragma unroll
-      for (uint32_t j = 0; j < 4; j++) c = i8_mfma16(a[j], *(const mx_i4 *)(from + ((4 * j + q) ^ (hr % 8)) * 16), c);  // (past a row's end: times zeros)
+      for (uint32_t j = 0; j < 4; j++)  // (past a row's end: times zeros)
+        c = i8_mfma16(a[j], *(const mx_i4 *)(from + ((4 * j + q) ^ (hr % 8)) * 16), c);
       if (counts) *to = make_int4(c[0], c[1], c[2], c[3]);
     }
     load(s);
@@ -589,13 +595,12 @@ struct Plan {
   Plan(const moe_i8_experts &e, uint32_t T) {
     A = T * e.n_used;
     few = !A || (T <= 16 && A <= kFew && e.n_embd >= 8 && T * (i8_pitch(e.n_embd) + 16) <= kFewXq && A * i8_pitch(e.n_ff) <= kFewHq);
-    // Tiles of 32, 64 or 128 positions: the more an expert has on average, the fewer times its weights are read, as long as the
-    // tiles are enough for the CUs. 30 tokens of 10 of 512 experts (half of one each) 58, 59 and 65 us; 301 (6, 2560 x 640) 159,
-    // 150 and 171; 2048 (40) 440, 404 and 438; 4096 (80) 618, 564 and 532, with skewed experts 511, 434 and 436; 4096 of 4 of 8
-    // (2048) 222, 172 and 163, 1000 of them (500) 64, 56 and 58. (Of 256, with i8_gemm's five buffers: 178 and 79; h and the
-    // values go out after 4 or 16 stages.)
-    const uint32_t mean = A / e.n_expert;
-    rows = mean < 3 ? 32 : mean < 72 || (uint64_t)A / 128 * ((e.n_ff + 63) / 64) < 768 ? 64 : 128;
+    // Tiles of 64 or 128 positions: the more an expert has on average, the fewer times its weights are read, as long as the tiles
+    // are enough for the CUs. 2048 tokens of 10 of 512 experts (40 each) 399 and 410 us, 1024 of 8 of 128 (64) 136 and 141; 4096 (80)
+    // 545 and 501, with skewed experts 411 and 388; 1000 tokens of 4 of 8 (500, 250 pieces) 50 and 52, 2000 (500 pieces) 81 and 79,
+    // 4096 159 and 149. (Of 32, 30 of 10 of 512 take 53.6 and with 64 53.7, 300 both 310, 301 of a skewed router 153 and 138. Of
+    // 256, with i8_gemm's five buffers, 4096 of 4 of 8 were 178 and with 128 163: h and the values go out after 4 or 16 stages.)
+    rows = A / e.n_expert < 72 || (uint64_t)A / 128 * ((e.n_ff + 63) / 64) < 400 ? 64 : 128;
     hpitch = (e.n_ff + 3) / 4 * 4;
     pitch = (e.n_embd + 255) / 256 * 256;
     // The values of all assignments at once, or of as many columns at a time as 256 MB hold, about the last-level cache.
@@ -701,24 +706,24 @@ MOE_API moe_status moe_i8_experts_async(const moe_i8_experts *e, const void *x, 
         wide ? run(i8_prepare<kX, true, true>) : run(i8_prepare<kX, false, true>);
     });
     if (slices > 1) sort_place_launch(ids, A, E, sorted, b + at.sort, stream);
-    const auto run = [&](auto gate_up, auto down, uint32_t bn, uint32_t at_once) {
-      const uint64_t cols = bn / 2, parts = (F + cols - 1) / cols;
-      op_launch(gate_up, std::min<uint64_t>(item_blocks(at.max_tiles * parts, parts), at_once), 256, stream, p, (const int8_t *)xq.codes, (const float *)xq.scales,
-                ntok, (const int32_t *)order, (const MoeTile *)tiles, (const uint32_t *)nt, h, at.hpitch);
+    const auto run = [&](auto gate_up, auto down, uint32_t at_once) {
+      const uint64_t bn = 128, parts = (F + bn / 2 - 1) / (bn / 2);
+      const auto blocks = [&](uint64_t n) { return std::min<uint64_t>(item_blocks(at.max_tiles * n, n), at_once); };
+      op_launch(gate_up, blocks(parts), 256, stream, p, (const int8_t *)xq.codes, (const float *)xq.scales, ntok, (const int32_t *)order,
+                (const MoeTile *)tiles, (const uint32_t *)nt, h, at.hpitch);
       i8_quantize_launch(QT_F32, h, at.hpitch, hq, offsets + E, stream);
       for (uint32_t c = 0; c < at.pitch; c += at.chunk) {
         const uint32_t n = std::min(at.chunk, at.pitch - c);
-        op_launch(down, std::min<uint64_t>(item_blocks((uint64_t)at.max_tiles * (n / bn), n / bn), at_once), 256, stream, p, (const int8_t *)hq.codes,
-                  (const float *)hq.scales, (const MoeTile *)tiles, (const uint32_t *)nt, c, n, o);
+        op_launch(down, blocks(n / bn), 256, stream, p, (const int8_t *)hq.codes, (const float *)hq.scales, (const MoeTile *)tiles,
+                  (const uint32_t *)nt, c, n, o);
         combine_launch(QT_F32, o, n, ntok, K, std::min(n, H - c), places, w, e->y_type, (uint8_t *)y + (uint64_t)c * op_size(e->y_type),
                        y_stride, stream);
       }
     };
     const auto tiles_of = [&](auto limit) {
       constexpr bool kLimit = decltype(limit)::value;
-      if (at.rows == 32) run(i8_gate_up_tiles<1, 1, kLimit>, i8_down_tiles<1, 1>, 256, 2 * kCus);
-      if (at.rows == 64) run(i8_gate_up_tiles<1, 2, kLimit>, i8_down_tiles<1, 2>, 128, 3 * kCus);
-      if (at.rows == 128) run(i8_gate_up_tiles<2, 2, kLimit>, i8_down_tiles<2, 2>, 128, 2 * kCus);
+      if (at.rows == 64) run(i8_gate_up_tiles<1, kLimit>, i8_down_tiles<1>, 3 * kCus);
+      if (at.rows == 128) run(i8_gate_up_tiles<2, kLimit>, i8_down_tiles<2>, 2 * kCus);
     };
     e->swiglu_limit > 0.0f ? tiles_of(std::true_type()) : tiles_of(std::false_type());
   });

@@ -10,7 +10,8 @@
 namespace c0ven {
 
 // Few rows of x (at most 16): y = x w^T is bound by reading w. A work-group has 16 rows of w, its kWaves waves each a run of their
-// k, four steps of 64 in use and four more on their way; the waves' sums are added in LDS. kX kQuantised: x is quantised already
+// k, four steps of 64 in use and four more on their way; the waves' sums are added in LDS. 1 x 16384 x 8192 25.6 us (5.2 TB/s),
+// 8 x 2048 x 2048 with x's quantisation 5.5. kX kQuantised: x is quantised already
 // (xc, xs); else x are floats of that type, which the work-group quantises into LDS while its first loads of w are on their way.
 constexpr uint32_t kQuantised = ~0u;
 constexpr uint32_t kFewRows = 16;
@@ -36,7 +37,8 @@ __global__ void __launch_bounds__(64 * kWaves)
   const auto load = [&](Ahead &to, uint32_t k) {
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
-      to.a[j] = __builtin_bit_cast(mx_i4, __builtin_amdgcn_raw_buffer_load_b128(w, k + j < k1 ? r * pitch + q * 16 + (k + j) * 64 : kNowhere, 0, 0));
+      const uint32_t at = k + j < k1 ? r * pitch + q * 16 + (k + j) * 64 : kNowhere;
+      to.a[j] = __builtin_bit_cast(mx_i4, __builtin_amdgcn_raw_buffer_load_b128(w, at, 0, 0));
       if constexpr (!kFloats) to.b[j] = *(const mx_i4 *)(xc + (uint64_t)m * pitch + min(k + j, steps - 1) * 64 + q * 16);
     }
   };
@@ -121,9 +123,12 @@ __global__ void __launch_bounds__(256) i8_join(const int *sums, uint32_t parts, 
 
 // A tile of y a work-group, k split into parts of `span` stages; kSums: the sums themselves, part p's to y + p M N, else y's
 // values. Work-groups to tiles so that an XCD has neighbours: eight tiles down, then across. kBuffers: two of x and two of w,
-// four of each, or three of x and two of w (the 256 tile's, which has eight waves). 4096 x 8192 x 8192 on a layer's codes: 247 us, 2.2 POPS, and 254 to 300 with two buffers of each; the clock gives
-// way under such codes (on zeros 183 us, 3.0 POPS, and 202 with two buffers), and the matrix instructions alone, on operands
-// that stay in registers, take 185 on random ones. Four waves of 128 x 128 each read a third less of LDS but leave a SIMD one wave: 265.
+// four of each, or three of x and two of w (the 256 tile's, which has eight waves).
+// 4096 x 8192 x 8192 on a layer's codes: 237 us, 2.3 POPS. Bound by power there: the clock gives way under such codes (on zeros 183
+// us, 3.0 POPS), and the matrix instructions alone, on operands that stay in registers, take 185 on random ones. Before the values
+// went out as below it was 247, with two buffers of each 254 to 300, and with four waves of 128 x 128, which read a third less of
+// LDS but leave a SIMD one wave, 265. Small products are bound by latency and by w (17 x 8192 x 8192 14.5 us, 4.7 TB/s), wide ones of a
+// short k by the values' way out (4096 x 8192 x 1024 47 us).
 template <uint32_t kType, bool kSums, int TM, int TN, int kWaves, int kBuffers>
 __global__ void __launch_bounds__(64 * kWaves, 2)
     i8_gemm(const int8_t *xc, const float *xs, const int8_t *wc, const float *ws, uint32_t M, uint32_t N, uint32_t steps,
@@ -175,7 +180,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2)
   }
   __builtin_amdgcn_s_barrier();  // (the stages' LDS is used again)
   // Each wave's 32 rows at a time through its part of LDS, so that a row's neighbours are stored together: a lane has four
-  // columns, the same of every row.
+  // columns, the same of every row; whole tiles without a branch (4096 x 8192 x 128 22 us; 36 with a test and a scale's load a row).
   static_assert(64 % (kWide / 4) == 0, "a lane's columns");
   static_assert(kWaves % 4 == 0 && kFour * 32 * kPitch * 4 <= sizeof(x0) && BM == BN, "a quarter of the waves' rows in a buffer");
   const uint32_t b = wave / kFour;
@@ -318,8 +323,8 @@ void launch_matmul(const int8_t *xc, const float *xs, uint32_t M, const moe_i8_m
   tiles(std::integral_constant<uint32_t, QT_F32>(), std::true_type(), work, N);
   op_by_type(y_type, [&](auto t) {
     constexpr uint32_t kType = decltype(t)::value;
-    op_launch(i8_join<kType>, ((uint64_t)M * ((N + 3) / 4) + 255) / 256, 256, stream, (const int *)work, p.parts, xs, (const float *)w->scales, M, N,
-              (typename Elem<kType>::T *)y, stride);
+    op_launch(i8_join<kType>, ((uint64_t)M * ((N + 3) / 4) + 255) / 256, 256, stream, (const int *)work, p.parts, xs,
+              (const float *)w->scales, M, N, (typename Elem<kType>::T *)y, stride);
   });
 }
 

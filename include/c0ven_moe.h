@@ -448,7 +448,7 @@ MOE_API moe_status moe_mx4_experts_async(const moe_mx4_experts *e, const void *x
  * most 2^27 rows of 1 to 65536 cols. Quantisation writes codes of -127 .. 127; a matrix from elsewhere may hold -128. */
 typedef struct {
   int8_t *codes;
-  float *scales; /* rows of them */
+  float *scales; /* rows of them, not negative (NaN: the row's values are) */
   uint32_t rows;
   uint32_t cols;
 } moe_i8_matrix;
