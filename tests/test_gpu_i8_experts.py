@@ -270,8 +270,8 @@ def test_far_experts():
 
 @pytest.mark.parametrize("T,H,F,E,K", [(4096, 2300, 40, 20, 16), (4200, 2300, 8, 400, 8)])
 def test_columns_in_parts(T, H, F, E, K):
-    """More values than down takes at a time: parts of 1024, 1024 and 256 columns (256 MB hold 1024 of 65536 assignments), and of
-    1792 and 512; n_embd ends inside the last."""
+    """More values than down takes at a time: three parts of 768 columns (2304 of 65536 assignments are 604 MB), and parts of 1280
+    and 1024; n_embd ends inside the last."""
     say("columns in parts", T, H, F, E, K)
     check(Model(E, H, F, 6), *tokens(T, H, E, K, 9, 0.05), rows=np.r_[0:16, T // 2:T // 2 + 16, T - 16:T])
 
