@@ -239,16 +239,19 @@ namespace {
 // CU with four buffers each) wait for memory's latency: four buffers (128 x 8192 x 8192 23.8 us, with two 50; 512 x 4096 x 4096
 // 17.4 and 20.4), and with few tiles parts of k, by what their sums' way through memory costs: a stage takes 220 ns, a part's sums
 // are written and read at 310 to the nanosecond, a launch is 1.5 us (17 x 4096 x 4096 in four parts 7.7 us, in one 10.0, in eight
-// 9.3; 128 x 2048 x 2048 7.5, in two 8.0). More are fewer loads in larger tiles, if those still fill the 256 CUs: tiles of 256
-// where their rounds are three quarters full (2048 x 8192 x 8192 120 us, tiles of 128 145; 2500 x 5120 x 4096, 200 tiles, 55 and
-// 63; but 2678 x 6333 x 4096, 275 tiles, 106 and 91; 4096 x 6144 x 4096, 384, 110 and 109), else tiles of 128, one to a CU with
-// four buffers (512 x 8192 x 8192 46.5, with two 63.8, tiles of 64 66) or two with two (1024 x 8192 x 8192 75, with four 89), else
-// tiles of 64 with two (1500 x 1500 x 512 6.5, with four 8.1, tiles of 128 8.7).
+// 9.3; 128 x 2048 x 2048 7.5, in two 8.0). More are fewer loads in larger tiles, if those still fill the 256 CUs and are not half
+// empty to a side: tiles of 256 where their rounds are three quarters full (2048 x 8192 x 8192 120 us, tiles of 128 145; 2500 x
+// 5120 x 4096, 200 tiles, 55 and 63; but 2678 x 6333 x 4096, 275 tiles, 106 and 91; 4096 x 6144 x 4096, 384, 110 and 109; 100 x
+// 100000 x 4096 131 and 114), else tiles of 128, one to a CU with four buffers (512 x 8192 x 8192 46.5, with two 63.8, tiles of 64
+// 66) or two with two (1024 x 8192 x 8192 75, with four 89), else tiles of 64 with two (1500 x 1500 x 512 6.5, with four 8.1,
+// tiles of 128 8.7; 40 x 40000 x 1024 11.6, 12.8 and 14.6) or, for a long k, four (17 x 100000 x 4096 87, with two 100, tiles of
+// 128 105).
 struct Plan {
   uint32_t tile, buffers, span, parts = 1;
   uint64_t tiles;
   Plan(uint32_t M, uint32_t N, uint32_t steps) {
     const auto count = [&](uint64_t t) { return ((M + 64 * t - 1) / (64 * t)) * ((N + 64 * t - 1) / (64 * t)); };
+    const uint32_t side = std::min(M, N);
     span = steps;
     if (count(1) <= 512) {
       tile = 1, buffers = 8;
@@ -259,12 +262,12 @@ struct Plan {
         if (ns < least) least = ns, span = of;
       }
       parts = (steps + span - 1) / span;
-    } else if (count(4) * 4 >= (count(4) + 255) / 256 * 256 * 3) {
+    } else if (side > 128 && count(4) * 4 >= (count(4) + 255) / 256 * 256 * 3) {
       tile = 4, buffers = 5;
-    } else if (count(2) >= 200) {
+    } else if (side > 64 && count(2) >= 200) {
       tile = 2, buffers = count(2) <= 256 ? 8 : 4;
     } else {
-      tile = 1, buffers = 4;
+      tile = 1, buffers = steps >= 24 ? 8 : 4;
     }
     tiles = count(tile);
   }

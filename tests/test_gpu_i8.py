@@ -128,7 +128,8 @@ SHAPES = [(1, 1, 1), (1, 16, 128), (1, 17, 129), (2, 100, 1000), (5, 33, 64), (1
           (17, 64, 128), (17, 1, 1), (33, 65, 127), (64, 64, 1000), (100, 130, 8200), (65, 1000, 257), (301, 2565, 1000), (128, 128, 65536),
           (700, 2100, 384), (2000, 1950, 200), (1800, 1804, 513), (3330, 4100, 640), (4096, 3329, 130), (20, 40, 5000),
           (40, 20000, 100), (40, 20000, 300), (40, 20000, 500), (40, 20000, 700), (512, 8192, 200), (520, 8000, 900), (1500, 1500, 130),
-          (2688, 2048, 260), (3500, 3500, 1100), (3500, 3499, 1300), (16, 4096, 8192), (9, 5000, 8190), (17, 1500, 4100), (60, 3, 20000)]
+          (2688, 2048, 260), (3500, 3500, 1100), (3500, 3499, 1300), (16, 4096, 8192), (9, 5000, 8190), (17, 1500, 4100), (60, 3, 20000),
+          (40, 40000, 130), (33000, 20, 129), (17, 33000, 3200), (100, 30000, 200)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
