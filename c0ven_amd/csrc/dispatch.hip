@@ -4,7 +4,7 @@
 // a lane, a wave a run of 64 such pieces of one token, whose places are then the wave's (scalar loads). 16384 tokens of 10 ranks and
 // rows of 4 KB: dispatched in 152 us (24 of them the sort's; 4.9 TB/s of a copy's 5.0), combined in 122 (6.0; reads are cheaper), the
 // gradients of 4096 in 97 (5.5). A few hundred tokens are bound by launches and the sort's steps: 999 of 4 ranks and rows of 10 KB
-// 18.9, 100 of 10 ranks 6.6, 8 combined 3.9.
+// 18.7, 100 of 10 ranks 6.0, 8 combined 3.9.
 #include "dispatch.h"
 #include "experts.h"
 #include "mx4_api.h"
@@ -120,13 +120,16 @@ __global__ void __launch_bounds__(256) dispatch_rows(const typename Elem<kType>:
   });
 }
 
-// At most kFewIds ids: the sort and the rows in one launch (100 tokens of 10 ranks 6.6 us, in two launches 12.7), a work-group 256 pieces of a token, whose places its waves count
-// themselves (lower ids, and equal ones before), and the last work-group the offsets. cols 0: no rows.
-constexpr uint32_t kFewIds = 1024;
+// At most kFewIds ids: the sort and the rows in one launch, a work-group every parts-th 256 pieces of a token, whose places its waves
+// count themselves (lower ids, and equal ones before), and the last work-group the offsets. cols 0: no rows. 100 tokens of 10 ranks
+// 6.0 us, in two launches 9.8; 250 9.3 and 11; 400 12.8 and 12.5: each token's work-group reads all ids.
+constexpr uint32_t kFewIds = 2560;
 template <uint32_t kType, uint32_t kN>
 __global__ void __launch_bounds__(256) dispatch_few(const int32_t *ids, uint32_t ntok, uint32_t K, uint32_t E,
                                                     const typename Elem<kType>::T *x, uint64_t x_stride, uint32_t cols,
-                                                    typename Elem<kType>::T *xs, uint64_t xs_stride, SortOut out) {
+                                                    typename Elem<kType>::T *xs, uint64_t xs_stride, uint32_t parts, SortOut out) {
+  constexpr uint32_t kKeys = 16, kKey = 4096;  // (ids a lane at a time; above an assignment)
+  static_assert(kFewIds <= kKey, "an assignment in a key");
   const uint32_t A = ntok * K, lane = threadIdx.x & 63;
   if (blockIdx.x == gridDim.x - 1) {
     __shared__ uint32_t n[kMostExperts];
@@ -157,42 +160,52 @@ __global__ void __launch_bounds__(256) dispatch_few(const int32_t *ids, uint32_t
   }
   __shared__ uint32_t places[16];
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / 64), pieces = (cols + kN - 1) / kN;
-  const uint32_t parts = max((pieces + 255) / 256, 1u), t = blockIdx.x / parts, piece = (blockIdx.x - t * parts) * 256 + threadIdx.x;
-  const bool there = piece < pieces;
-  const uint32_t c = there ? min(piece * kN, cols - kN) : 0;
-  uint32_t key[kFewIds / 64], of[4];
+  const uint32_t t = blockIdx.x / parts, part = blockIdx.x - t * parts, first = part * 256 + threadIdx.x;
+  uint32_t key[kKeys], of[4], place[4] = {0, 0, 0, 0};
 #pragma unroll
   for (uint32_t j = 0; j < 4; j++) of[j] = (uint32_t)ids[t * K + min(wave + 4 * j, K - 1)];
+  const auto keys = [&](uint32_t i0) {
 #pragma unroll
-  for (uint32_t j = 0; j < kFewIds / 64; j++) {
-    if (j * 64 >= A) break;
-    key[j] = (uint32_t)ids[min(j * 64 + lane, A - 1)];
-  }
+    for (uint32_t j = 0; j < kKeys; j++) {
+      if (i0 + j * 64 >= A) break;
+      key[j] = (uint32_t)ids[min(i0 + j * 64 + lane, A - 1)];
+    }
+  };
+  keys(0);
   Few<kType, kN> v;
-  if (there) v.load(x + t * x_stride + c);
+  if (first < pieces) v.load(x + t * x_stride + min(first * kN, cols - kN));
 #pragma unroll
   for (uint32_t j = 0; j < 4; j++) loaded<true>(of[j]);
   // An assignment's place: how many keys (expert, then assignment; past the last id the largest) are below its own.
+#pragma unroll 1
+  for (uint32_t i0 = 0; i0 < A; i0 += 64 * kKeys) {
 #pragma unroll
-  for (uint32_t j = 0; j < kFewIds / 64; j++) {
-    if (j * 64 >= A) break;
-    key[j] = j * 64 + lane < A ? min(key[j], E) * kFewIds + j * 64 + lane : ~0u;
+    for (uint32_t j = 0; j < kKeys; j++) {
+      if (i0 + j * 64 >= A) break;
+      key[j] = i0 + j * 64 + lane < A ? min(key[j], E) * kKey + i0 + j * 64 + lane : ~0u;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++) {
+      if (wave + 4 * i >= K) break;
+      const uint32_t own = min(of[i], E) * kKey + t * K + wave + 4 * i;
+#pragma unroll
+      for (uint32_t j = 0; j < kKeys; j++) {
+        if (i0 + j * 64 >= A) break;
+        place[i] += (uint32_t)__popcll(__ballot(key[j] < own));
+      }
+    }
+    keys(i0 + 64 * kKeys);
   }
 #pragma unroll
   for (uint32_t i = 0; i < 4; i++) {
-    const uint32_t k = wave + 4 * i, a = t * K + k, e = min(of[i], E), own = e * kFewIds + a;
+    const uint32_t k = wave + 4 * i, a = t * K + k;
     if (k >= K) break;
-    uint32_t place = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < kFewIds / 64; j++) {
-      if (j * 64 >= A) break;
-      place += (uint32_t)__popcll(__ballot(key[j] < own));
-    }
     if (lane == 0) {
-      places[k] = e < E ? place : ~0u;
-      if (blockIdx.x - t * parts == 0) {
-        out.places[a] = e < E ? (int32_t)place : -1;
-        if (e < E) out.order[place] = (int32_t)a;
+      const bool there = of[i] < E;
+      places[k] = there ? place[i] : ~0u;
+      if (part == 0) {
+        out.places[a] = there ? (int32_t)place[i] : -1;
+        if (there) out.order[place[i]] = (int32_t)a;
       }
     }
   }
@@ -200,10 +213,14 @@ __global__ void __launch_bounds__(256) dispatch_few(const int32_t *ids, uint32_t
   uint32_t to[16];
 #pragma unroll
   for (uint32_t k = 0; k < 16; k++) to[k] = (uint32_t)__builtin_amdgcn_readfirstlane((int)places[k]);
-  if (there)
+#pragma unroll 1
+  for (uint32_t piece = first; piece < pieces; piece += parts * 256) {
+    const uint32_t c = min(piece * kN, cols - kN);
+    if (piece != first) v.load(x + t * x_stride + c);
 #pragma unroll
     for (uint32_t k = 0; k < 16; k++)
       if (k < K && to[k] != ~0u) v.store(xs + (uint64_t)to[k] * xs_stride + c);
+  }
 }
 
 // A token's rows, eight ranks' loads on their way at a time; each rank's product is fused into the sum, in rank order. A: rows of o.
@@ -431,9 +448,11 @@ MOE_API moe_status moe_dispatch_async(const moe_dispatch_config *cfg, const void
         constexpr uint32_t kN = decltype(piece)::value;
         if (A <= kFewIds) {
           const uint32_t cols = xs ? H : 0;
-          const uint64_t parts = std::max(((cols + kN - 1) / kN + 255) / 256, 1u);
-          return op_launch(dispatch_few<kType, kN>, ntok * parts + 1, 256, stream, ids, ntok, K, E, from, x_stride, cols, to,
-                           xs_stride, out);
+          // (More than 1024 work-groups would only read the ids more often.)
+          const uint32_t most = std::max(((cols + kN - 1) / kN + 255) / 256, 1u);
+          const uint32_t parts = std::min(most, std::max(1024 / std::max(ntok, 1u), 1u));
+          return op_launch(dispatch_few<kType, kN>, (uint64_t)ntok * parts + 1, 256, stream, ids, ntok, K, E, from, x_stride, cols, to,
+                           xs_stride, parts, out);
         }
         if (!xs) return;
         by_tokens(ntok, kWide, (H + kN - 1) / kN, [&](uint32_t t0, uint32_t n, uint64_t blocks) {

@@ -71,7 +71,8 @@ class Call:
 # One token to several slices of ids; rows of one value, of fewer and of more than 32 pieces, of whole pieces and not.
 @pytest.mark.parametrize("T,K,E,H", [(1, 1, 1, 1), (1, 10, 512, 2048), (3, 4, 7, 33), (8, 10, 512, 100), (16, 16, 64, 515),
                                      (64, 16, 8, 260), (65, 16, 8, 129), (200, 7, 2, 17), (255, 16, 512, 64), (300, 14, 100, 1000),
-                                     (1025, 4, 511, 250), (2000, 10, 60, 40), (5000, 3, 512, 7), (17, 2, 5, 20000)])
+                                     (1025, 4, 511, 250), (2000, 10, 60, 40), (5000, 3, 512, 7), (17, 2, 5, 20000), (160, 16, 40, 2700), (161, 16, 40, 130), (2560, 1, 33, 9),
+                                     (700, 3, 512, 5000), (2, 16, 20, 70001)])
 def test_dispatch(T, K, E, H):
     for type, extra, dropped, skew in (("f32", 0, 0.0, 0.0), ("bf16", 3, 0.2, 0.7), ("f16", 0, 0.1, 0.0)):
         say("dispatch", T, K, E, H, type)
@@ -81,7 +82,7 @@ def test_dispatch(T, K, E, H):
         c.check(ids)
 
 
-@pytest.mark.parametrize("T,K", [(5, 3), (70, 16), (400, 16)])
+@pytest.mark.parametrize("T,K", [(5, 3), (70, 16), (150, 16), (400, 16)])
 def test_edges_of_ids(T, K):
     """All on the first, on the last, on no expert; the same one in each rank; all in order and in reverse."""
     say("ids", T, K)
