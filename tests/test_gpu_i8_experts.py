@@ -268,6 +268,13 @@ def test_far_experts():
         within(got[rows], *ref.i8_experts(values[rows], np.zeros((len(rows), 1), int), w[rows].astype(np.float32).astype(np.float64), *model.v))
 
 
+def test_far_positions():
+    """The most tokens and ranks: rows of h past 2^32 bytes, their codes past 2^30."""
+    say("far positions")
+    T, H, F, E, K = 16384, 64, 5000, 20, 16
+    check(Model(E, H, F, 6), *tokens(T, H, E, K, 9, 0.01), rows=np.r_[0:8, T // 2:T // 2 + 8, T - 24:T])
+
+
 @pytest.mark.parametrize("T,H,F,E,K", [(4096, 2300, 40, 20, 16), (4200, 2300, 8, 400, 8)])
 def test_columns_in_parts(T, H, F, E, K):
     """More values than down takes at a time: three parts of 768 columns (2304 of 65536 assignments are 604 MB), and parts of 1280
