@@ -421,19 +421,20 @@ __global__ void __launch_bounds__(512) i8_gate_up_few(I8Experts p, const typenam
 // A work-group takes every gridDim-th eight rows of down, y's eight columns, for all assignments. A wave has every eighth pair of the
 // experts that are named, whose eight rows each are the 16 rows of a matrix instruction; its columns are eight assignments of the
 // one and eight of the other, of which half of the products count. kOwn: it quantises the rows of h itself, at most kFewOwn values
-// (a launch for that is 3 us; more values take each work-group as long).
-constexpr uint32_t kFewHq = 48 * 1024;  // the assignments' rows of h in LDS
+// (a launch for that is 3 us; more values take each work-group as long: 8 tokens of 10 ranks 38 us so, 32 with the launch). kUnits:
+// the units of a wave in LDS, three if h's rows leave them room.
+constexpr uint32_t few_hq(int units) { return (units == 3 ? 48 : 80) * 1024; }  // the assignments' rows of h in LDS
 constexpr uint32_t kFewOwn = 512 * 4 * 8;
 constexpr uint32_t kTerms = (kFew * 8 + 511) / 512;
 
-template <uint32_t kType, bool kOwn>
+template <uint32_t kType, bool kOwn, int kUnits>
 __global__ void __launch_bounds__(512) i8_down_few(I8Experts p, const float *h, uint32_t hpitch, const int8_t *hc, const float *hs,
                                                    const int32_t *ids, const float *w, uint32_t ntok, typename Elem<kType>::T *y,
                                                    uint64_t stride) {
   __shared__ Unit unit0[8];
   __shared__ Unit unit1[8];
-  __shared__ Unit unit2[8];
-  __shared__ __align__(16) uint8_t hq[kFewHq + 1024];  // a row's 16-byte pieces exchanged by the row
+  __shared__ Unit unit2[kUnits == 3 ? 8 : 1];
+  __shared__ __align__(16) uint8_t hq[few_hq(kUnits) + 1024];  // a row's 16-byte pieces exchanged by the row
   __shared__ __align__(16) int o[kFew * 8];
   __shared__ Named named;
   __shared__ uint16_t member[8][2][kFew], row[kFew];
@@ -461,7 +462,7 @@ __global__ void __launch_bounds__(512) i8_down_few(I8Experts p, const float *h, 
   };
   uint32_t pair = 0, k = 0, nm[2] = {0, 0};
   const auto use = [&](Unit &s) {
-    unit_ready<2 * kUnitLoads>();
+    unit_ready<(kUnits - 1) * kUnitLoads>();
     if (k == 0) {  // the experts' assignments
 #pragma unroll
       for (uint32_t which = 0; which < 2; which++) {
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(512) i8_down_few(I8Experts p, const float *h, 
       }
     load(unit0[wave]);
     load(unit1[wave]);
-    load(unit2[wave]);
+    if constexpr (kUnits == 3) load(unit2[wave]);
     if (b == blockIdx.x) {
       if (threadIdx.x < A) {
         const bool on = named.id[threadIdx.x] < p.E;
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(512) i8_down_few(I8Experts p, const float *h, 
                               [&](uint32_t i, uint32_t c) { return hq + i * pitch + ((c / 16) ^ (i % 8)) * 16 + c % 16; }, most);
       } else {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070 | 3 * kUnitLoads);  // (all but the units: the rows of h)
+        __builtin_amdgcn_s_waitcnt(0x0070 | kUnits * kUnitLoads);  // (all but the units: the rows of h)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       }
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__(512) i8_down_few(I8Experts p, const float *h, 
     while (pair < pairs) {
       use(unit0[wave]);
       use(unit1[wave]);
-      use(unit2[wave]);
+      if constexpr (kUnits == 3) use(unit2[wave]);
     }
     loads_done();
     __syncthreads();
@@ -583,7 +584,8 @@ void check_experts(const moe_i8_experts *e, uint32_t ntok) {
   op_require(op_float(e->x_type) && op_float(e->y_type), "the element type must be QT_F32, QT_F16 or QT_BF16");
 }
 
-// How a call runs. Few assignments, whose rows of h fit LDS, without sorting them.
+// How a call runs. Few assignments, whose rows of h fit LDS, without sorting them: 16 tokens of 10 of 512 experts of 2048 x 512 44
+// us, sorted 49; of 16 experts 28 and 35; but 12 of 512 of 2560 x 640 64 and 63.
 constexpr uint64_t kTurnBytes = 256 << 20;
 constexpr uint32_t kCus = 256;  // work-groups that fill the device where LDS holds one a CU
 
@@ -594,7 +596,7 @@ struct Plan {
 
   Plan(const moe_i8_experts &e, uint32_t T) {
     A = T * e.n_used;
-    few = !A || (T <= 16 && A <= kFew && e.n_embd >= 8 && T * (i8_pitch(e.n_embd) + 16) <= kFewXq && A * i8_pitch(e.n_ff) <= kFewHq);
+    few = !A || (T <= 16 && A <= kFew && e.n_embd >= 8 && T * (i8_pitch(e.n_embd) + 16) <= kFewXq && A * i8_pitch(e.n_ff) <= few_hq(2));
     // Tiles of 64 or 128 positions: the more an expert has on average, the fewer times its weights are read, as long as the tiles
     // are enough for the CUs. 2048 tokens of 10 of 512 experts (40 each) 399 and 410 us, 1024 of 8 of 128 (64) 136 and 141; 4096 (80)
     // 545 and 501, with skewed experts 411 and 388; 1000 tokens of 4 of 8 (500, 250 pieces) 50 and 52, 2000 (500 pieces) 81 and 79,
@@ -682,9 +684,11 @@ MOE_API moe_status moe_i8_experts_async(const moe_i8_experts *e, const void *x, 
                     (const float *)hq.scales, ids, w, ntok, (typename Elem<kY>::T *)y, y_stride);
         };
         if (own)
-          run(i8_down_few<kY, true>);
+          run(i8_down_few<kY, true, 3>);
+        else if (A * i8_pitch(F) <= few_hq(3))
+          run(i8_down_few<kY, false, 3>);
         else
-          run(i8_down_few<kY, false>);
+          run(i8_down_few<kY, false, 2>);
       });
       return;
     }

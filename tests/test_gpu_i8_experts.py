@@ -71,7 +71,8 @@ def tokens(T, H, E, K, seed, dropped=0.0, repeat=False):
                                        (9, 2560, 640, 6, 4), (300, 130, 129, 40, 5),
                                        (16, 256, 600, 12, 10), (23, 256, 64, 12, 7), (16, 200, 700, 12, 10),
                                        (3, 2100, 64, 4, 2), (20, 3200, 96, 2, 2), (200, 640, 640, 64, 2), (90, 384, 300, 4, 2),
-                                       (2, 2700, 129, 3, 3), (13, 5200, 24, 2, 2), (1, 300, 5000, 3, 2)])
+                                       (2, 2700, 129, 3, 3), (13, 5200, 24, 2, 2), (1, 300, 5000, 3, 2), (16, 256, 500, 200, 10),
+                                       (16, 2100, 500, 40, 10), (12, 300, 640, 8, 8), (11, 128, 899, 100, 7)])
 def test_experts(T, H, F, E, K):
     say("experts", T, H, F, E, K)
     model = Model(E, H, F, T + H)
