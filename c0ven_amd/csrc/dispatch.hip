@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(256) combine_rows(const typename Elem<kIn>::T 
 }
 
 // A wave an assignment: do = w dy (rounded once) and dw = <dy, o>, four pieces of both rows on their way at a time; a lane's
-// products are added in column order, the lanes' sums by halves. dw or dout may be null.
+// products are added in column order by their place in a piece, these sums and the lanes' by halves. dw or dout may be null.
 template <uint32_t kType, uint32_t kN>
 __global__ void __launch_bounds__(256) combine_gradient(const typename Elem<kType>::T *__restrict__ dy, uint64_t dy_stride, uint32_t A,
                                                         uint32_t K, uint32_t cols, const int32_t *__restrict__ places,
@@ -293,7 +293,9 @@ __global__ void __launch_bounds__(256) combine_gradient(const typename Elem<kTyp
   dy += a / K * dy_stride;
   if (dw) o += p * o_stride;
   if (dout) dout += p * do_stride;
-  float s = 0.0f;
+  float s[kN];
+#pragma unroll
+  for (uint32_t n = 0; n < kN; n++) s[n] = 0.0f;
   for (uint32_t c0 = lane * kN; c0 < cols; c0 += 4 * kRun) {
     Few<kType, kN> d[4], v[4];
 #pragma unroll
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(256) combine_gradient(const typename Elem<kTyp
       if (dw)
 #pragma unroll
         for (uint32_t n = 0; n < kN; n++)
-          if (at + n >= c) s = __builtin_fmaf(d[j][n], v[j][n], s);  // (the others are the piece before's)
+          if (at + n >= c) s[n] = __builtin_fmaf(d[j][n], v[j][n], s[n]);  // (the others are the piece before's)
       if (dout) {
         float e[kN];
 #pragma unroll
@@ -321,8 +323,12 @@ __global__ void __launch_bounds__(256) combine_gradient(const typename Elem<kTyp
   }
   if (dw) {
 #pragma unroll
-    for (uint32_t m = 32; m >= 1; m /= 2) s += __shfl_xor(s, (int)m, 64);
-    if (lane == 0) dw[a] = s;
+    for (uint32_t m = kN / 2; m >= 1; m /= 2)
+#pragma unroll
+      for (uint32_t n = 0; n < m; n++) s[n] += s[n + m];
+#pragma unroll
+    for (uint32_t m = 32; m >= 1; m /= 2) s[0] += __shfl_xor(s[0], (int)m, 64);
+    if (lane == 0) dw[a] = s[0];
   }
 }
 
