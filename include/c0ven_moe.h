@@ -374,9 +374,10 @@ MOE_API moe_status moe_combine_async(const moe_dispatch_config *cfg, const void 
  * dxs[place], as moe_combine_async with weights of one. */
 MOE_API moe_status moe_dispatch_backward_async(const moe_dispatch_config *cfg, const void *dxs, uint64_t dxs_stride, uint32_t ntok,
                                                const int32_t *places, void *dx, uint64_t dx_stride, void *stream);
-/* The gradients of moe_combine_async with regard to o and w, from dy, that with regard to y: dout[place] = w dy[t], rounded once
- * (rows without an assignment are left as they were); dw = <dy[t], o[place]> in fp32, in an order that goes by n_embd and type
- * alone (0 for an assignment without a place). dout or dw may be null (not formed; without dw, o too); w null: ones. */
+/* The gradients of moe_combine_async with regard to o and w, from dy, that with regard to y: dout[place] = w dy[t], the product in
+ * fp32 and then rounded to type (rows without an assignment are left as they were); dw = <dy[t], o[place]> in fp32, in an order that
+ * goes by n_embd and type alone (0 for an assignment without a place). dout or dw may be null (not formed; without dw, o too); w
+ * null: ones. */
 MOE_API moe_status moe_combine_backward_async(const moe_dispatch_config *cfg, const void *dy, uint64_t dy_stride, uint32_t ntok,
                                               const int32_t *places, const void *o, uint64_t o_stride, const float *w, void *dout,
                                               uint64_t dout_stride, float *dw, void *stream);
@@ -458,7 +459,7 @@ MOE_API uint64_t moe_i8_code_bytes(uint32_t rows, uint32_t cols);
  * gets the scale NaN and codes 0. */
 MOE_API moe_status moe_i8_quantize_async(int32_t device, uint32_t type, const void *x, uint64_t stride, const moe_i8_matrix *m,
                                          void *stream);
-/* m's values, rounded to type, into out (rows stride apart). */
+/* m's values, each in fp32 (rounded) and then rounded to type, into out (rows stride apart). */
 MOE_API moe_status moe_i8_dequantize_async(int32_t device, const moe_i8_matrix *m, uint32_t type, void *out, uint64_t stride,
                                            void *stream);
 
