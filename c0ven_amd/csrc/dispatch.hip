@@ -2,9 +2,9 @@
 //
 // All of it moves rows: bound by memory. The sort is a stable counting sort of the ids; the rows are read and written 16 bytes
 // a lane, a wave a run of 64 such pieces of one token, whose places are then the wave's (scalar loads). 16384 tokens of 10 ranks and
-// rows of 4 KB: dispatched in 152 us (24 of them the sort's; 4.9 TB/s of a copy's 5.0), combined in 122 (6.0; reads are cheaper), the
-// gradients of 4096 in 97 (5.5). A few hundred tokens are bound by launches and the sort's steps: 999 of 4 ranks and rows of 10 KB
-// 18.7, 100 of 10 ranks 6.0, 8 combined 3.9.
+// rows of 4 KB: dispatched in 153 us (15 of them the sort's, the rows at 5.2 TB/s), combined in 123 (5.9, mostly read), the gradients
+// of 4096 in 97 (5.5); wide accesses alone read 7.1 TB/s and write 6.8. A few hundred tokens are bound by launches and the sort's
+// steps: 999 of 4 ranks and rows of 10 KB 17.9, 100 of 10 ranks 6.1, 8 combined 3.9.
 #include "dispatch.h"
 #include "experts.h"
 #include "mx4_api.h"
@@ -28,8 +28,8 @@ __global__ void __launch_bounds__(1024) sort_place(const int32_t *ids, uint32_t 
 // ---- rows
 
 // kN neighbouring elements: 16 bytes at whatever address, or one element (rows shorter than 16 bytes). Rows pass through once and
-// are far more than a cache holds, so they are loaded and stored past it (16384 x 10 rows of 4 KB: dispatched in 128 us, 150
-// without; combined in 126, 144).
+// are far more than a cache holds, so they are loaded and stored past it (16384 x 10 rows of 4 KB: dispatched in 153 us, 157
+// through the caches; combined in 123, 140; both gradients of 4096 x 10 in 98, 112).
 typedef uint32_t Quad __attribute__((ext_vector_type(4), aligned(2)));
 template <uint32_t kType, uint32_t kN>
 struct Few {
@@ -273,8 +273,10 @@ __global__ void __launch_bounds__(256) combine_rows(const typename Elem<kIn>::T 
   });
 }
 
-// A wave an assignment: do = w dy (rounded once) and dw = <dy, o>, four pieces of both rows on their way at a time; a lane's
-// products are added in column order by their place in a piece, these sums and the lanes' by halves. dw or dout may be null.
+// A wave an assignment: do = w dy (in fp32, then rounded to the type) and dw = <dy, o>, four pieces of both rows on their way at a
+// time; a lane's products are added in column order by their place in a piece, these sums and the lanes' by halves. dw or dout may be
+// null. A row is one wave's whatever its length and the number of rows: 10 x 4096 of 64 bf16 values 17.4 us with the dispatch's
+// gradient, one of 16384 fp32 values 22 us, one of 2^20 1.4 ms.
 template <uint32_t kType, uint32_t kN>
 __global__ void __launch_bounds__(256) combine_gradient(const typename Elem<kType>::T *__restrict__ dy, uint64_t dy_stride, uint32_t A,
                                                         uint32_t K, uint32_t cols, const int32_t *__restrict__ places,

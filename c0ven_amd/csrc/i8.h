@@ -143,8 +143,9 @@ __device__ __forceinline__ i8_i16 i8_mfma32(mx_i4 a, mx_i4 b, i8_i16 c) {
 }
 
 // A sum of codes' products as a value: the smaller scale first, so that what is between leaves fp32's range only where the value
-// does (a scale is at least 2^-100, a sum at most 2^30). A scale that is NaN stays: scales are not
-// negative, so that their bits are ordered as they are, with NaN above all.
+// does (a quantised row's scale is at least 2^-100, a sum at most 2^30; of a smaller scale from elsewhere the first product may be a
+// denormal number, rounded as one). A scale that is NaN stays: scales are not negative, so that their bits are ordered as they
+// are, with NaN above all.
 __device__ __forceinline__ float i8_value(int sum, float sx, float sw) {
   const uint32_t a = __float_as_uint(sx), b = __float_as_uint(sw);
   return (float)sum * __uint_as_float(min(a, b)) * __uint_as_float(max(a, b));

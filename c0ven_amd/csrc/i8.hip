@@ -14,7 +14,8 @@ __global__ void __launch_bounds__(kThreads < 256 ? 256 : kThreads)
                                                                                  codes, scales);
 }
 
-// Eight values a thread.
+// Eight values a thread: code * scale in fp32, then rounded to the type. Bound by memory: 4096 x 8192 to bf16 19.7 us, 5.1 TB/s, 16384 x
+// 8192 70, 5.8; 25915 x 100 3.9.
 template <uint32_t kType>
 __global__ void __launch_bounds__(256) i8_dequantize(const int8_t *codes, const float *scales, uint32_t rows, uint32_t cols,
                                                      typename Elem<kType>::T *out, uint64_t stride) {

@@ -3,9 +3,10 @@
 // Many tokens: the assignments are sorted by expert and cut into MoeTiles; x's rows are quantised; gate and up of a tile are one
 // product whose epilogue applies the SwiGLU; the rows of h (fp32: a row's scale needs all of it) are quantised; down follows, its
 // values in fp32 by position, and each token's are summed in rank order (in fp32: a value rounded to y's type there would be rounded
-// twice). Of 512 experts of 2048 x 512 with a skewed router, 10 a token: 4096 tokens 386 us (gate and up 183, 0.9 POPS with a quarter
-// of the tiles' rows empty; h quantised 19; down 150, for 0.3 GB of values; their sum 56; the sort and x 17), 1024 166, 30 54, where the
-// weights' bytes bound it (301 tokens of 2560 x 640: gate and up at 4.7 TB/s).
+// twice). Of 512 experts of 2048 x 512 with a skewed router, 10 a token: 4096 tokens 403 us a call in a row (traced one launch at a time
+// 447: gate and up 194, 0.9 POPS with a third of the tiles' rows empty; h quantised 20; down 155, for 0.34 GB of values; their sum 56;
+// the sort and x 22), 30 54; 1024 tokens of 8 of 128 experts 144; 301 of 10 of 512 of 2560 x 640 135, where the weights' bytes bound
+// it (gate and up 72 us, 4.6 TB/s).
 #include "../../include/c0ven_moe_tile.h"
 #include "dispatch.h"
 #include "experts.h"
@@ -27,8 +28,9 @@ struct I8Experts {
 };
 
 // expert_swiglu for the epilogue of a tile, a sixth of whose time it was: one reciprocal, good to a unit of the last place, for the
-// division's ten instructions. Below g = -87.3, where the reciprocal would be a denormal number, 0 (expert_swiglu
-// from -88.7 on). NaNs and infinities as there: g is a factor of the result.
+// division's ten instructions. What that loses: on 2^24 normal g the result is off by 5.6e-8 of itself (root of the mean square) and
+// 2.6e-7 at most, expert_swiglu's by 4.9e-8 and 2.3e-7, beside the three roundings of g and of u. Below g = -87.3, where the
+// reciprocal would be a denormal number, 0 (expert_swiglu from -88.7 on). NaNs and infinities as there: g is a factor of the result.
 __device__ __forceinline__ float i8_swiglu(float g, float u, float limit) {
   if (limit > 0.0f) {
     g = g > limit ? limit : g;
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(256) i8_down_tiles(I8Experts p, const int8_t *
 
 // ---- few assignments (at most kFew of at most 16 tokens): no sorting, two or three launches. Bound by latency and by reading the
 // experts' weights, which go to LDS as whole rows, always some of them on their way: 8 tokens of 10 of 512 experts of 2048 x 512 32
-// us (gate and up 17, 3.5 TB/s of the weights; h's quantisation 3; down 14), one token 19.5.
+// us (gate and up 17, 3.8 TB/s of the weights; h's quantisation 4; down 14), one token 19.3 (10 and 11), two 21.8, 16 44.5.
 
 constexpr uint32_t kFew = 160;
 

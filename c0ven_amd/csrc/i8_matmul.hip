@@ -124,11 +124,11 @@ __global__ void __launch_bounds__(256) i8_join(const int *sums, uint32_t parts, 
 // A tile of y a work-group, k split into parts of `span` stages; kSums: the sums themselves, part p's to y + p M N, else y's
 // values. Work-groups to tiles so that an XCD has neighbours: eight tiles down, then across. kBuffers: two of x and two of w,
 // four of each, or three of x and two of w (the 256 tile's, which has eight waves).
-// 4096 x 8192 x 8192 on a layer's codes: 237 us, 2.3 POPS. Bound by power there: the clock gives way under such codes (on zeros 183
-// us, 3.0 POPS), and the matrix instructions alone, on operands that stay in registers, take 185 on random ones. Before the values
-// went out as below it was 247, with two buffers of each 254 to 300, and with four waves of 128 x 128, which read a third less of
-// LDS but leave a SIMD one wave, 265. Small products are bound by latency and by w (17 x 8192 x 8192 14.5 us, 4.7 TB/s), wide ones of a
-// short k by the values' way out (4096 x 8192 x 1024 47 us).
+// 4096 x 8192 x 8192 on a layer's codes: 250 us, 2.2 POPS (traced 290, from 248 to 339; 228 on another card). Bound by power there: the
+// clock gives way under such codes (on zeros 184 us, 3.0 POPS), and the matrix instructions alone, on operands that stay in registers,
+// take 168 to 182 on random ones. On a card where it took 237 it was 247 before the values went out as below, with two buffers of each
+// 254 to 300, and with four waves of 128 x 128, which read a third less of LDS but leave a SIMD one wave, 265. Small products are bound
+// by latency and by w (17 x 8192 x 8192 14.5 us, 4.7 TB/s), wide ones of a short k by the values' way out (4096 x 8192 x 1024 47 us).
 template <uint32_t kType, bool kSums, int TM, int TN, int kWaves, int kBuffers>
 __global__ void __launch_bounds__(64 * kWaves, 2)
     i8_gemm(const int8_t *xc, const float *xs, const int8_t *wc, const float *ws, uint32_t M, uint32_t N, uint32_t steps,

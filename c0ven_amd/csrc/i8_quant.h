@@ -8,7 +8,7 @@ namespace c0ven {
 // Rows of x to codes and scales, by work-group `block` of `blocks` of kBlock threads: kThreads threads a row (64, or all), kAhead
 // groups of eight values a thread at a time. A row of that many is in registers, read once, so that the scale (the row's
 // largest) is known before the codes are formed; kLong: longer rows, read again for their codes. Bound by memory: 4096 x 8192 of
-// bf16 21 us, 4.8 TB/s.
+// bf16 21.6 us, 4.7 TB/s, 16384 x 8192 71, 5.7; short rows, a wave each, by their number: 25915 x 100 9.1.
 template <uint32_t kType, int kBlock, int kThreads, int kAhead, bool kLong>
 __device__ __forceinline__ void quantize_block(uint32_t block, uint32_t blocks, const typename Elem<kType>::T *x, uint64_t stride,
                                                uint32_t rows, uint32_t cols, const uint32_t *n_rows, int8_t *codes, float *scales) {
