@@ -608,7 +608,7 @@ struct Plan {
     hpitch = (e.n_ff + 3) / 4 * 4;
     pitch = (e.n_embd + 255) / 256 * 256;
     // The values of all assignments at once, or in turns of about 256 MB each, the last-level cache's size (4096 tokens of 10 of 512
-    // experts in two turns 378 us; before the tiles' last steps all at once 438, in turns of 256 MB 437, of 128 450, of 64 495).
+    // experts in two turns 378 us, on another card 403; before the tiles' last steps all at once 438, in turns of 256 MB 437, of 128 450, of 64 495).
     const uint64_t turns = (4ull * A * pitch + kTurnBytes - 1) / kTurnBytes;
     chunk = few ? pitch : (uint32_t)((pitch / 256 + turns - 1) / turns * 256);
     max_tiles = std::min(A, e.n_expert + A / rows);
