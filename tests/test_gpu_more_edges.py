@@ -154,3 +154,83 @@ def test_scales_that_are_no_numbers(T, which):
     else:
         assert np.isnan(got[hit]).all()
     assert np.array_equal(got[~hit], clean[~hit]) and not hit[1]
+
+
+def replayed(inputs, results, call):
+    """call(results, stream) captured and replayed on new inputs, between eager calls on other results: the same bytes. inputs: (buffer,
+    maker of its contents); results: twice the same buffers."""
+    s1, s2 = hip.stream(), hip.stream()
+    launch = hip.capture(s1, lambda: call(results[0], s1))
+    for i in range(3):
+        for b, make in inputs:
+            b.put(make(i))
+        launch()
+        call(results[1], s2)
+        for a, b in zip(*results):  # (work, where it is among them, too)
+            assert np.array_equal(a.get(), b.get())
+
+
+def test_graph_of_many_tokens():
+    """The dispatch of several slices of ids and the ways back, captured."""
+    say("graph of many tokens")
+    T, K, E, H = 1500, 8, 60, 300
+    d = moe.Dispatch(E, K, H)
+    x, ids, w = hip.full((T, H), 0, np.uint16), hip.full((T, K), 0, np.int32), hip.full((T, K), 0)
+    n = d.work_bytes(T)
+    assert n > 0
+
+    def results():
+        return [hip.full((T * K, H), 0, np.uint16), hip.full(T * K, 0, np.int32), hip.full((T, K), 0, np.int32), hip.full(E + 1, 0, np.int32),
+                hip.full((T, H), 0, np.uint16), hip.full((T * K, H), 0, np.uint16), hip.full((T, K), 0), hip.full((T, H), 0, np.uint16),
+                hip.full(n, 0xA5, np.uint8)]
+
+    def call(b, s):
+        d.dispatch_async(x.ptr, T, ids.ptr, b[0].ptr, b[1].ptr, b[2].ptr, b[3].ptr, b[8].ptr, n, stream=s)
+        d.combine_async(b[0].ptr, T, b[2].ptr, b[4].ptr, w.ptr, stream=s)
+        d.combine_backward_async(x.ptr, T, b[2].ptr, b[0].ptr, b[5].ptr, b[6].ptr, w.ptr, stream=s)
+        d.dispatch_backward_async(b[5].ptr, T, b[2].ptr, b[7].ptr, stream=s)
+
+    replayed([(x, lambda i: encode(np.random.default_rng(i).normal(size=(T, H)), "bf16")), (ids, lambda i: draw_ids(T, K, E, i, 0.0)),
+              (w, lambda i: np.random.default_rng(i).normal(size=(T, K)).astype(np.float32))], [results(), results()], call)
+
+
+@pytest.mark.parametrize("M,N,K", [(17, 100, 3000), (1500, 1500, 130), (700, 8192, 200), (3500, 3500, 200)])
+def test_graph_of_products(M, N, K):
+    """Parts of k and each size of tiles, captured."""
+    say("graph of products", M, N, K)
+    w, s = operand(N, K, 3)
+    codes, scales = hip.put(ref.i8_padded(w)), hip.put(s.astype(np.float32))
+    wm, x = moe.I8Matrix(codes.ptr, scales.ptr, N, K), hip.full((M, K), 0)
+    n = moe.i8_linear_work_bytes(wm, M)
+    results = [[hip.full((M, N), 0), hip.full(n, v, np.uint8)] for v in (0, 0xA5)]
+
+    def call(b, s):
+        moe.i8_linear_async(moe.QT_F32, x.ptr, M, wm, moe.QT_F32, b[0].ptr, b[1].ptr, n, stream=s)
+
+    replayed([(x, lambda i: np.random.default_rng(i).normal(size=(M, K)).astype(np.float32))], [r[:1] for r in results],
+             lambda b, s: call(results[0] if b[0] is results[0][0] else results[1], s))
+
+
+@pytest.mark.parametrize("T,H,F,E,K", [(1100, 256, 100, 12, 4), (4200, 2300, 8, 400, 8)])
+def test_graph_of_experts(T, H, F, E, K):
+    """Several slices of ids; values in several turns; captured."""
+    say("graph of experts", T, H, F, E, K)
+    model = Model(E, H, F, 6)
+    op = model.op(K)
+    n = op.work_bytes(T)
+    x, ids, w = hip.full((T, H), 0), hip.full((T, K), 0, np.int32), hip.full((T, K), 0)
+    results = [[hip.full((T, H), 0)] for _ in range(2)]
+    work = [hip.full(n, v, np.uint8) for v in (0, 0xA5)]
+
+    def call(b, s):
+        op.forward_async(x.ptr, T, ids.ptr, w.ptr, b[0].ptr, work[0 if b is results[0] else 1].ptr, n, stream=s)
+
+    made = {}
+
+    def make(i, j):
+        if i not in made:
+            a = tokens(T, H, E, K, i, 0.1, True)
+            made[i] = (a[0], a[1].astype(np.int32), a[2].astype(np.float32))
+        return made[i][j]
+
+    replayed([(b, lambda i, j=j: make(i, j)) for j, b in enumerate((x, ids, w))], results, call)
